@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-import torch  # noqa: F401  (loads the HIP runtime the library binds to)
+import torch  # (loads the HIP runtime the library binds to)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CVN_LIB", os.path.join(_HERE, "lib", "libcvn_hip.so"))
@@ -27,12 +27,16 @@ COLS_SINGLE, COLS_LINES, COLS_PLANNED = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 64 << 20  # CVN_NOALLOC_SCRATCH_BYTES
 ACT_NONE = 0
 ACT_GELU = 1
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # CVN_F32, CVN_BF16, CVN_F16
+GATE_NONE, GATE_SAMPLE, GATE_FULL = 0, 1, 2
+NORM_2, NORM_INF = 0, 1
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
 _ptr = ctypes.c_void_p
 _size = ctypes.c_size_t
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/converse2d.h
 SIGNATURES = {
@@ -81,6 +85,14 @@ SIGNATURES = {
     "cvn_conv_ln_mlp_head_f32": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _f32,
                                         _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _f32, _ptr, _ptr,
                                         _ptr, _ptr]),
+    "cvn_residual_norm_fwd": (_int, [_ptr, _int, _ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _int, _ptr, _ptr, _f32, _ptr,
+                                     _ptr, _f32, _ptr, _ptr, _ptr, _ptr]),
+    "cvn_residual_norm_bwd_workspace": (_size, [_i64, _i64, _i64, _int]),
+    "cvn_residual_norm_bwd": (_int, [_ptr, _ptr, _ptr, _int, _ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _int, _ptr, _ptr,
+                                     _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _size, _ptr]),
+    "cvn_grad_norm_workspace": (_size, [_ptr, _i64]),
+    "cvn_grad_norm": (_int, [_ptr, _ptr, _ptr, _i64, _int, _ptr, _ptr, _size, _ptr]),
+    "cvn_clip_grads": (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _int, _f64, _ptr, _ptr, _size, _ptr]),
     "cvn_copy_f32": (_int, [_ptr, _ptr, _i64, _ptr]),
 }
 

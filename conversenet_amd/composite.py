@@ -93,3 +93,21 @@ def converse2d_module(x, weight, bias, scale, padding, padding_mode, eps):
         ps = padding * scale
         out = out[..., ps:-ps, ps:-ps]
     return out
+
+
+def layernorm_cf(x, weight, bias, eps):
+    """LayerNorm(data_format='channels_first') (util_converse.py:63-68), over any trailing dimensions."""
+    u = x.mean(1, keepdim=True)
+    s = (x - u).pow(2).mean(1, keepdim=True)
+    cf = (-1,) + (1,) * (x.dim() - 2)
+    return weight.view(cf) * ((x - u) / torch.sqrt(s + eps)) + bias.view(cf)
+
+
+def residual_branch(h, res_scale=None, gate=None, post=None):
+    """res_scale * gate * P(h) in float32 or wider (functional.residual_norm)."""
+    u = h.to(torch.promote_types(h.dtype, torch.float32))
+    if post is not None:
+        u = layernorm_cf(u, *post)
+    if gate is not None:
+        u = u * (gate if gate.shape == h.shape else gate.reshape(gate.shape[:2] + (1,) * (h.dim() - 2)))
+    return u if res_scale is None else res_scale.reshape((-1,) + (1,) * (h.dim() - 2)) * u

@@ -1,0 +1,200 @@
+// C entry points of residual_norm.h, and the last step of its sums over pixels.
+#include <algorithm>
+
+#include "residual_norm.h"
+
+namespace cvn {
+
+// Up to a block per 4 tiles and CU-filling at least: each keeps its own partial sums, one row of 5 C.
+int64_t rn_bwd_blocks(int64_t ntiles) { return std::min<int64_t>(ntiles, 2048); }
+
+namespace {
+
+// out[k][c] = sum over blocks of part[k][c][:], and the per-sample gates' gradients from their tiles' sums: a wave per
+// sum, in 64 bits, in the same order on every call.
+struct RnSumArgs {
+  const float *part, *dgpart;
+  float* out[kRnSums];
+  void* dg;  // (B C) of type dg_type, or null
+  int dg_type;
+  int C, G, tps;
+  int64_t rows;  // kRnSums C, and B C for the gates
+};
+
+__global__ void __launch_bounds__(256) k_rn_sums(RnSumArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int64_t ns = (int64_t)kRnSums * a.C;
+  const float* p;
+  int n;
+  if (row < ns) {
+    if (!a.out[row / a.C]) return;
+    p = a.part + row * a.G;
+    n = a.G;
+  } else {
+    p = a.dgpart + (row - ns) * a.tps;
+    n = a.tps;
+  }
+  double s = 0.;
+  for (int i = lane; i < n; i += 64) s += p[i];
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+  if (lane) return;
+  if (row < ns) a.out[row / a.C][row % a.C] = (float)s;
+  else if (a.dg_type == CVN_F32) ((float*)a.dg)[row - ns] = (float)s;
+  else if (a.dg_type == CVN_BF16) ((__bf16*)a.dg)[row - ns] = (__bf16)(float)s;
+  else ((_Float16*)a.dg)[row - ns] = (_Float16)(float)s;
+}
+
+bool rn_kernels(int x_type, int h_type, RnKernels* k) {
+  if (x_type == CVN_F32 && h_type == CVN_F32) *k = rn_f32_f32();
+  else if (x_type == CVN_F32 && h_type == CVN_BF16) *k = rn_f32_bf16();
+  else if (x_type == CVN_F32 && h_type == CVN_F16) *k = rn_f32_f16();
+  else if (x_type == CVN_BF16 && h_type == CVN_BF16) *k = rn_bf16_bf16();
+  else if (x_type == CVN_F16 && h_type == CVN_F16) *k = rn_f16_f16();
+  else return false;
+  return true;
+}
+
+int rn_shape_ok(int64_t B, int64_t C, int64_t HW, int x_type, int h_type, RnKernels* k) {
+  if (B < 0 || C < 1 || HW < 0) return fail(CVN_ERR_ARG, "bad shape");
+  if (!rn_kernels(x_type, h_type, k))
+    return fail(CVN_ERR_ARG, "types %d and %d: x and h of one type, or a 16-bit h on a float32 x", x_type, h_type);
+  // pixel and tile numbers are held in 32 bits; offsets of elements in 64
+  if (C > 65536 || B > INT32_MAX || HW > INT32_MAX || B * HW > INT32_MAX)
+    return fail(CVN_ERR_UNSUPPORTED, "more than 65536 channels or 2^31 - 1 pixels");
+  return CVN_OK;
+}
+
+int rn_branch_ok(const void* h, const float* s, const void* gate, int gate_kind, const float* pw, const float* pb) {
+  if (gate_kind != CVN_GATE_NONE && gate_kind != CVN_GATE_SAMPLE && gate_kind != CVN_GATE_FULL)
+    return fail(CVN_ERR_ARG, "bad gate kind");
+  if ((gate != nullptr) != (gate_kind != CVN_GATE_NONE)) return fail(CVN_ERR_ARG, "gate and its kind do not match");
+  if ((pw != nullptr) != (pb != nullptr)) return fail(CVN_ERR_ARG, "the branch norm needs weight and bias");
+  if (!h && (s || gate || pw)) return fail(CVN_ERR_ARG, "scale, gate or branch norm without a branch");
+  return CVN_OK;
+}
+
+}  // namespace
+}  // namespace cvn
+
+using namespace cvn;
+
+extern "C" int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, int h_type, int64_t B, int64_t C,
+                                     int64_t HW, const float* res_scale, const void* gate, int gate_kind,
+                                     const float* post_w, const float* post_b, float post_eps, const float* norm_w,
+                                     const float* norm_b, float norm_eps, void* r, void* y, float* stats,
+                                     cvn_stream_t stream) {
+  RnKernels k;
+  int rc = rn_shape_ok(B, C, HW, x_type, h ? h_type : x_type, &k);
+  if (rc == CVN_OK && B * HW == 0) return CVN_OK;  // empty tensors have no addresses to check
+  if (rc == CVN_OK) rc = rn_branch_ok(h, res_scale, gate, gate_kind, post_w, post_b);
+  if (rc != CVN_OK) return rc;
+  if (!x || (h && !r) || (norm_w && (!norm_b || !y)) || (!h && !norm_w)) return fail(CVN_ERR_ARG, "null pointer");
+  RnArgs a = {};
+  a.x = x;
+  a.h = h;
+  a.gate = gate;
+  a.gate_full = gate_kind == CVN_GATE_FULL;
+  a.s = res_scale;
+  a.nw = norm_w;
+  a.nb = norm_b;
+  a.pw = post_w;
+  a.pb = post_b;
+  a.neps = norm_eps;
+  a.peps = post_eps;
+  a.r = h ? r : nullptr;
+  a.y = y;
+  a.stats = stats;
+  a.C = C;
+  a.HW = HW;
+  a.total = B * HW;
+  const RnTiles t = rn_tiles(B, HW, false);
+  a.ntiles = t.n;
+  a.tps = t.tps;
+  return k.fwd(a, B, (hipStream_t)stream);
+}
+
+extern "C" size_t cvn_residual_norm_bwd_workspace(int64_t B, int64_t C, int64_t HW, int gate_kind) {
+  RnKernels k;
+  if (rn_shape_ok(B, C, HW, CVN_F32, CVN_F32, &k) != CVN_OK) return 0;
+  const bool sample = gate_kind == CVN_GATE_SAMPLE;
+  const RnTiles t = rn_tiles(B, HW, sample);
+  const size_t part = align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)rn_bwd_blocks(t.n));
+  return part + (sample ? sizeof(float) * (size_t)(B * C) * (size_t)t.tps : 0) + 256;
+}
+
+extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, const void* base, int x_type, const void* h,
+                                     int h_type, int64_t B, int64_t C, int64_t HW, const float* res_scale,
+                                     const void* gate, int gate_kind, const float* post_w, const float* post_b,
+                                     const float* norm_w, const float* stats, void* grad_x, void* grad_h, void* grad_gate,
+                                     float* grad_scale, float* grad_norm_w, float* grad_norm_b, float* grad_post_w,
+                                     float* grad_post_b, void* workspace, size_t workspace_bytes, cvn_stream_t stream) {
+  RnKernels k;
+  int rc = rn_shape_ok(B, C, HW, x_type, h || grad_h ? h_type : x_type, &k);
+  const bool empty = B == 0 || HW == 0;
+  if (rc == CVN_OK && !empty) rc = rn_branch_ok(h, res_scale, gate, gate_kind, post_w, post_b);
+  if (rc != CVN_OK) return rc;
+  if ((grad_gate && !gate) || (grad_scale && !res_scale) || ((grad_norm_w || grad_norm_b) && !norm_w) ||
+      ((grad_post_w || grad_post_b) && !post_w))
+    return fail(CVN_ERR_ARG, "a gradient of an argument that was not given");
+  if (!empty && ((!grad_r && !grad_y) || (grad_y && !norm_w) || (norm_w && !base) ||
+                 (((norm_w && grad_y) || post_w) && !stats)))
+    return fail(CVN_ERR_ARG, "null pointer");
+  if (!empty && !grad_y && (grad_norm_w || grad_norm_b))
+    return fail(CVN_ERR_ARG, "gradients of the norm's parameters without a gradient of y");
+  const bool sample = gate_kind == CVN_GATE_SAMPLE;
+  const RnTiles t = rn_tiles(B, HW, sample);
+  if (!workspace || workspace_bytes < cvn_residual_norm_bwd_workspace(B, C, HW, gate_kind))
+    return fail(CVN_ERR_WORKSPACE, "residual_norm backward workspace missing or too small");
+  const int64_t G = rn_bwd_blocks(t.n);
+  hipStream_t st = (hipStream_t)stream;
+  RnArgs a = {};
+  a.part = (float*)align_up((size_t)workspace);
+  a.dgpart = (float*)((char*)a.part + align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)G));
+  a.x = base;
+  a.h = h;
+  a.gate = gate;
+  a.gate_full = gate_kind == CVN_GATE_FULL;
+  a.s = res_scale;
+  a.nw = norm_w;
+  a.pw = post_w;
+  a.pb = post_b;
+  a.stats = const_cast<float*>(stats);
+  a.gr = grad_r;
+  a.gy = grad_y;
+  a.dx = grad_x;
+  a.dh = grad_h;
+  a.dg = grad_gate;
+  a.C = C;
+  a.HW = HW;
+  a.total = B * HW;
+  a.ntiles = t.n;
+  a.tps = t.tps;
+  if (!empty) {
+    rc = k.bwd(a, B, st);
+    if (rc != CVN_OK) return rc;
+  }
+  RnSumArgs s = {};
+  s.part = a.part;
+  s.dgpart = a.dgpart;
+  s.C = (int)C;
+  s.G = (int)G;
+  s.out[0] = grad_norm_w;
+  s.out[1] = grad_norm_b;
+  s.out[2] = grad_scale;
+  s.out[3] = grad_post_w;
+  s.out[4] = grad_post_b;
+  if (sample && grad_gate) {
+    s.dg = grad_gate;
+    s.dg_type = h_type;
+    s.tps = t.tps;
+  }
+  s.rows = kRnSums * C + (s.dg ? B * C : 0);
+  bool any = s.dg && B > 0;
+  for (int i = 0; i < kRnSums; ++i) any = any || s.out[i];
+  if (!any) return CVN_OK;
+  hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, s);
+  return check_launch("residual_norm sums");
+}

@@ -7,9 +7,12 @@ kernels on torch's current stream.  No CPU fallback exists here: a missing libra
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 import os
 import threading
+from array import array
 
 import torch
 from torch.multiprocessing.reductions import StorageWeakRef
@@ -614,6 +617,364 @@ def conv_ln_mlp_residual(t, x, w0, b0, ln_w, ln_b, ln_eps, w1, b1, w2, b2, res_s
     _lib.check(lib.cvn_conv_ln_mlp_head_f32(*common, hw_, hb_, float(heps), wh_, bh_, tn.data_ptr(), _stream(x.device)),
                "conv_ln_mlp_head")
     return y, tn
+
+
+def _on(dev):
+    """Makes a tensor's device current for the launches on its stream."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _param32(keep, t, C, what):
+    """Address of a parameter's C values in float32 (None for None); copies go to `keep`, as in _ptrs."""
+    if t is None:
+        return None
+    if not t.is_cuda or t.numel() != C or t.dtype not in _lib.TYPES:
+        raise RuntimeError(f"{what} must hold {C} values on the HIP device")
+    if t.dtype != torch.float32 or not t.is_contiguous():
+        t = t.to(torch.float32).contiguous()
+        keep.append(t)
+    return t.data_ptr()
+
+
+def _gate_kind(h, gate):
+    if gate is None:
+        return _lib.GATE_NONE
+    if gate.shape == h.shape:
+        return _lib.GATE_FULL
+    if tuple(gate.shape) in (tuple(h.shape[:2]), tuple(h.shape[:2]) + (1,) * (h.dim() - 2)):
+        return _lib.GATE_SAMPLE
+    raise RuntimeError("gate must have the branch's shape, or (B,C) or (B,C,1,..) for a factor per sample and channel")
+
+
+def _norm_shape(x, h, res_scale, gate, post, norm):
+    """Checks a residual_norm call: (B, C, HW)."""
+    for t in (x, h, gate):
+        if t is not None and not (t.is_cuda and t.dtype in _lib.TYPES and t.device == x.device):
+            raise RuntimeError("residual_norm needs float32, bfloat16 or float16 tensors on one HIP device")
+    if x.dim() < 2:
+        raise RuntimeError("x must be (B,C,*)")
+    if h is None:
+        if res_scale is not None or gate is not None or post is not None or norm is None:
+            raise RuntimeError("without a branch there is only the norm of x")
+    else:
+        if h.shape != x.shape:
+            raise RuntimeError("x and the branch must have one shape")
+        if h.dtype != x.dtype and x.dtype != torch.float32:
+            raise RuntimeError("x and the branch must have one type, or x float32 and the branch a 16-bit type")
+        if gate is not None and gate.dtype != h.dtype:
+            raise RuntimeError("gate must have the branch's type")
+    for t in (res_scale, *(post or ())[:2], *(norm or ())[:2]):
+        if t is not None and t.device != x.device:
+            raise RuntimeError("tensors on same device")
+    if x.shape[1] < 1:
+        raise RuntimeError("x must have channels")
+    return x.shape[0], x.shape[1], math.prod(x.shape[2:])
+
+
+def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
+    """The launch behind residual_norm: (r or None, y or None, stats or None), on contiguous x, h and gate."""
+    lib = _lib.load()
+    B, C, HW = _norm_shape(x, h, res_scale, gate, post, norm)
+    keep = []
+    s, nw, nb = (_param32(keep, t, C, n) for t, n in zip((res_scale, *(norm or (None, None))[:2]),
+                                                         ("res_scale", "norm weight", "norm bias")))
+    pw, pb = (_param32(keep, t, C, "branch norm") for t in (post or (None, None))[:2])
+    kind = _gate_kind(h, gate)
+    r = torch.empty_like(x) if h is not None else None
+    y = torch.empty_like(x) if norm is not None else None
+    stats = None
+    if need_stats and (norm is not None or post is not None):
+        stats = torch.empty((4 if post is not None else 2, B * HW), dtype=torch.float32, device=x.device)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with _on(x.device):
+        rc = lib.cvn_residual_norm_fwd(x.data_ptr(), _lib.TYPES[x.dtype], ptr(h), 0 if h is None else _lib.TYPES[h.dtype],
+                                       B, C, HW, s, ptr(gate), kind, pw, pb, float(post[2]) if post else 0.0, nw, nb,
+                                       float(norm[2]) if norm else 0.0, ptr(r), ptr(y), ptr(stats), _stream(x.device))
+    _lib.check(rc, "residual_norm")
+    return r, y, stats
+
+
+def _contiguous(*ts):
+    return [t if t is None else t.contiguous() for t in ts]
+
+
+def residual_norm(x, h, norm=None, res_scale=None, gate=None, post=None):
+    """A block's scaled residual and the norms before and after its branch, in one pass:
+    r = x + res_scale * gate * P(h), y = N(r); returns (r, y), y None without norm.
+
+    x, h (B,C,*), channels first, of one type, or a 16-bit branch h on a float32 x; r and y have x's type.
+    norm, post: (weight, bias, eps) of channels-first LayerNorms of r and of the branch (P(h) = h without post);
+    res_scale: C values (ConverseBlockAlphaVariant's alphas, util_converse.py:321-322); gate: a factor per element
+    (h's shape) or per sample and channel ((B,C) or (B,C,1,1)), of h's type.  Computed in float32, each output
+    rounded once: y is the norm of r before its rounding.  For gradients see residual_norm_train."""
+    if h is None:
+        raise RuntimeError("residual_norm needs a branch")
+    x, h, gate = _contiguous(x, h, gate)
+    return _residual_norm(x, h, norm, res_scale, gate, post, False)[:2]
+
+
+def residual_norm_backward(grad_r, grad_y, base, h, stats, norm_weight=None, res_scale=None, gate=None, post=None,
+                           h_dtype=None, need=(True,) * 8):
+    """Gradients of residual_norm in one call and its sums: (x, h, res_scale, gate, post weight, post bias, norm
+    weight, norm bias), None where not asked for by `need` or not given.
+
+    grad_r, grad_y: gradients of r and y (None: zero).  base: the forward's r where x is float32, x itself where it
+    is a 16-bit type (there the norm is that of r before its rounding).  h may be None where base is r and there is
+    no scale, gate and post: its gradient is x's, of type h_dtype.  stats: what the forward kept, (2 or 4, B HW)."""
+    lib = _lib.load()
+    norm = None if norm_weight is None else (norm_weight, norm_weight, 0.0)
+    if h is not None:
+        h_dtype = h.dtype
+    ref = base if base is not None else grad_r
+    base, h, gate, grad_r, grad_y = _contiguous(base, h, gate, grad_r, grad_y)
+    for t in (grad_r, grad_y):
+        if t is not None and (t.shape != ref.shape or t.dtype != ref.dtype or t.device != ref.device):
+            raise RuntimeError("gradients must match r and y")
+    if h is not None or norm is not None:
+        _norm_shape(ref, h, res_scale, gate, post, norm)
+    B, C, HW = ref.shape[0], ref.shape[1], math.prod(ref.shape[2:])
+    if stats is not None and (tuple(stats.shape) != (4 if post is not None else 2, B * HW) or not stats.is_contiguous()
+                              or stats.dtype != torch.float32 or stats.device != ref.device):
+        raise RuntimeError("stats must be the forward's")
+    nx, nh, ns, ng, npw, npb, nnw, nnb = need
+    keep = []
+    s = _param32(keep, res_scale, C, "res_scale")
+    nw = _param32(keep, norm_weight, C, "norm weight")
+    pw, pb = (_param32(keep, t, C, "branch norm") for t in (post or (None, None))[:2])
+    dev = ref.device
+    has_norm = norm is not None and grad_y is not None
+    plain = res_scale is None and gate is None and post is None  # then the branch's gradient is x's
+    gx = None
+    if has_norm and (nx or (nh and plain and h_dtype == ref.dtype)):
+        gx = torch.empty(ref.shape, dtype=ref.dtype, device=dev)
+    elif nx or (nh and plain):
+        gx = grad_r if grad_r is not None else torch.zeros(ref.shape, dtype=ref.dtype, device=dev)
+    gh = None
+    if nh and h_dtype is not None:
+        if plain and h_dtype == ref.dtype:
+            gh = gx
+        elif plain and not has_norm:
+            gh = gx.to(h_dtype)
+        else:
+            gh = torch.empty(ref.shape, dtype=h_dtype, device=dev)
+    f32 = lambda want: torch.empty(C, dtype=torch.float32, device=dev) if want else None  # noqa: E731
+    gs = f32(ns and res_scale is not None)
+    gg = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if ng and gate is not None else None
+    gpw, gpb = f32(npw and post is not None), f32(npb and post is not None)
+    gnw, gnb = f32(nnw and has_norm), f32(nnb and has_norm)
+    out_x = gx if has_norm else None
+    out_h = None if gh is gx or (plain and not has_norm) else gh
+    if any(t is not None for t in (out_x, out_h, gs, gg, gpw, gpb, gnw, gnb)):
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        kind = _lib.GATE_NONE if gate is None else _gate_kind(h, gate)
+        nbytes = lib.cvn_residual_norm_bwd_workspace(B, C, HW, kind)
+        st = _stream(dev)
+        ws = _scratch(dev, st)
+        with _on(dev), ws.lock:
+            rc = lib.cvn_residual_norm_bwd(ptr(grad_r), ptr(grad_y) if has_norm else None, ptr(base),
+                                           _lib.TYPES[ref.dtype], ptr(h),
+                                           _lib.TYPES[h_dtype or ref.dtype], B, C, HW, s, ptr(gate), kind, pw, pb,
+                                           nw if has_norm else None, ptr(stats), ptr(out_x), ptr(out_h), ptr(gg), ptr(gs),
+                                           ptr(gnw), ptr(gnb), ptr(gpw), ptr(gpb), ws.ptr(nbytes), nbytes, st)
+        _lib.check(rc, "residual_norm_backward")
+    if norm is not None and not has_norm:  # y was not used
+        gnw, gnb = (torch.zeros(C, dtype=torch.float32, device=dev) if w else None for w in (nnw, nnb))
+    return (gx if nx else None), gh, gs, gg, gpw, gpb, gnw, gnb
+
+
+class ResidualNormFunction(torch.autograd.Function):
+    """residual_norm (h None: LayerNorm alone) with the library's forward and backward kernels.  A backward that is
+    itself to be differentiated runs as a composition of torch operations."""
+
+    @staticmethod
+    def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps):
+        ctx.set_materialize_grads(False)
+        x, h, gate = _contiguous(x, h, gate)
+        post = None if post_w is None else (post_w, post_b, post_eps)
+        norm = None if norm_w is None else (norm_w, norm_b, norm_eps)
+        r, y, stats = _residual_norm(x, h, norm, res_scale, gate, post, True)
+        half = x.dtype != torch.float32
+        keep_h = h is not None and (half or res_scale is not None or gate is not None or post is not None)
+        base = None if norm is None else (r if h is not None and not half else x)
+        ctx.save_for_backward(base, h if keep_h else None, res_scale, gate, post_w, post_b, norm_w, norm_b, stats)
+        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype)
+        return tuple(t for t in (r, y) if t is not None)
+
+    @staticmethod
+    def backward(ctx, *gos):
+        base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = ctx.saved_tensors
+        post_eps, norm_eps, h_dtype, x_dtype = ctx.cfg
+        gr = gos[0] if h_dtype is not None else None
+        gy = gos[-1] if norm_w is not None else None
+        n = ctx.needs_input_grad
+        if (gr is None and gy is None) or not any(n[:8]):
+            return (None,) * 10
+        post = None if post_w is None else (post_w, post_b, post_eps)
+        if torch.is_grad_enabled():
+            return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
+                                                     h_dtype, x_dtype, n) + (None, None)
+        if norm_w is None:
+            base = None
+        gx, gh, gs, gg, gpw, gpb, gnw, gnb = residual_norm_backward(
+            gr, gy, base, h, stats, norm_w, res_scale, gate, post, h_dtype, n[:8])
+        like = lambda g, t: None if g is None else g.to(t.dtype).reshape(t.shape)  # noqa: E731
+        return (gx, gh, like(gs, res_scale), gg, like(gpw, post_w), like(gpb, post_b), like(gnw, norm_w),
+                like(gnb, norm_b), None, None)
+
+
+def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy, h_dtype, x_dtype,
+                                      need):
+    """The same gradients from differentiable torch operations."""
+    branch = composite.residual_branch(h, res_scale, gate, post) if h is not None else None
+    dr = None if gr is None else gr.float()
+    gnw = gnb = None
+    if gy is not None:
+        r = base.float()
+        if x_dtype != torch.float32 and branch is not None:
+            r = r + branch  # base is x
+        if not r.requires_grad:
+            r = r.detach().requires_grad_()
+        y = composite.layernorm_cf(r, norm_w.float(), norm_b.float(), norm_eps)
+        ts = [r] + [t for t, k in ((norm_w, need[6]), (norm_b, need[7])) if k]
+        got = list(torch.autograd.grad(y, ts, gy.float(), create_graph=True))
+        d = got.pop(0)
+        dr = d if dr is None else dr + d
+        gnw = got.pop(0) if need[6] else None
+        gnb = got.pop(0) if need[7] else None
+    gx = dr.to(x_dtype) if need[0] else None
+    gh = gs = gg = gpw = gpb = None
+    if branch is None:
+        gh = dr.to(h_dtype) if need[1] else None
+    else:
+        ts = [h, res_scale, gate, *(post or (None, None))[:2]]
+        ask = [i for i in range(5) if need[1 + i] and ts[i] is not None]
+        if ask:
+            got = dict(zip(ask, torch.autograd.grad(branch, [ts[i] for i in ask], dr, create_graph=True)))
+            gh, gs, gg, gpw, gpb = (got.get(i) for i in range(5))
+    return gx, gh, gs, gg, gpw, gpb, gnw, gnb
+
+
+def residual_norm_train(x, h, norm=None, res_scale=None, gate=None, post=None):
+    """Differentiable residual_norm on the HIP kernels (forward and backward): (r, y)."""
+    if h is None:
+        raise RuntimeError("residual_norm needs a branch")
+    pw, pb, pe = post or (None, None, 0.0)
+    nw, nb, ne = norm or (None, None, 0.0)
+    out = ResidualNormFunction.apply(x, h, res_scale, gate, pw, pb, nw, nb, pe, ne)
+    return out if norm is not None else (out[0], None)
+
+
+def layernorm_cf_train(x, weight, bias, eps):
+    """Differentiable layernorm_cf on the HIP kernels (forward and backward)."""
+    return ResidualNormFunction.apply(x, None, None, None, None, None, weight, bias, 0.0, eps)[0]
+
+
+def _grad_list(ts):
+    """The device of a list of gradients, and its host tables for the library: addresses come per call."""
+    devs = {t.device for t in ts}
+    if len(devs) != 1 or not next(iter(devs)).type == "cuda":
+        raise RuntimeError("gradients must be on one HIP device")
+    if not all(t.layout == torch.strided for t in ts):
+        raise RuntimeError("gradients must be dense")
+    try:
+        types = array("i", [_lib.TYPES[t.dtype] for t in ts])
+    except KeyError as e:
+        raise RuntimeError(f"gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
+    return devs.pop(), types, array("q", [t.numel() for t in ts])
+
+
+def _norm_kind(norm_type):
+    kind = {2.0: _lib.NORM_2, math.inf: _lib.NORM_INF}.get(float(norm_type))
+    if kind is None:
+        raise RuntimeError("norm_type must be 2 or inf")
+    return kind
+
+
+def _addresses(ts):
+    return array("Q", [t.data_ptr() for t in ts])
+
+
+def _clip(grads, out, max_norm, norm_type):
+    """The norm of contiguous grads, and (out not None) their clipped values into contiguous out."""
+    kind = _norm_kind(norm_type)
+    max_norm = 0.0 if out is None else float(max_norm)
+    if not max_norm >= 0.0:
+        raise RuntimeError("max_norm must be at least 0")
+    if not grads:
+        return torch.tensor(0.0)
+    lib = _lib.load()
+    dev, types, sizes = _grad_list(grads)
+    n = len(grads)
+    src = _addresses(grads)
+    at = lambda a: a.buffer_info()[0]  # noqa: E731
+    nbytes = lib.cvn_grad_norm_workspace(at(sizes), n)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    st = _stream(dev)
+    ws = _scratch(dev, st)
+    with _on(dev), ws.lock:
+        if out is None:
+            rc = lib.cvn_grad_norm(at(src), at(sizes), at(types), n, kind, norm.data_ptr(), ws.ptr(nbytes), nbytes, st)
+        else:
+            dst = src if out is grads else _addresses(out)
+            rc = lib.cvn_clip_grads(at(src), at(dst), at(sizes), at(types), n, kind, max_norm, norm.data_ptr(),
+                                    ws.ptr(nbytes), nbytes, st)
+    _lib.check(rc, "grad_norm" if out is None else "clip_grads")
+    return norm
+
+
+def _tensors(ts):
+    return [ts] if isinstance(ts, torch.Tensor) else list(ts)
+
+
+def grad_norm(grads, norm_type=2.0):
+    """The norm over all elements of many tensors (2, or math.inf for the largest magnitude): a float32 scalar on their
+    device, accumulated in 64 bits.  grads: tensors of any shapes, float32, bfloat16 or float16, on one device."""
+    return _clip([t.contiguous() for t in _tensors(grads)], None, None, norm_type)
+
+
+def _written(ts):
+    """The library wrote these tensors: autograd sees it as it sees torch's in-place operations."""
+    ts = [t for t in ts if not t.is_inference()]
+    if ts:
+        torch.autograd.graph.increment_version(ts)
+
+
+def clip_grads(grads, max_norm, norm_type=2.0, out=None):
+    """(grads scaled by min(1, max_norm / (norm + 1e-6)), norm).  The scaled gradients go to new tensors, or to `out`:
+    contiguous tensors of the same types and shapes, each its own gradient or memory apart from all others."""
+    grads = _tensors(grads)
+    if out is None:
+        out = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in grads]
+    else:
+        out = _tensors(out)
+        if len(out) != len(grads):
+            raise RuntimeError("out must hold a tensor for each gradient")
+        for g, o in zip(grads, out):
+            if o.shape != g.shape or o.dtype != g.dtype or o.device != g.device or not o.is_contiguous():
+                raise RuntimeError("out must be contiguous, with the gradients' shapes and types, on their device")
+    norm = _clip([g.contiguous() for g in grads], out, max_norm, norm_type)
+    _written(out)
+    return out, norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scales the parameters' .grad in place so that their norm is at most max_norm; returns the norm they had.  As
+    torch.nn.utils.clip_grad_norm_; error_if_nonfinite waits for the norm and raises before any gradient changes."""
+    grads = [p.grad for p in _tensors(parameters) if p.grad is not None]
+    if error_if_nonfinite and grads:
+        norm = grad_norm(grads, norm_type)
+        if not math.isfinite(norm.item()):
+            raise RuntimeError(f"the norm of the gradients is {norm.item()}")
+    for g in grads:
+        if 0 in g.stride() and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+            raise RuntimeError("a gradient's elements share memory")
+    dense = [g.contiguous() for g in grads]
+    norm = _clip(dense, dense, max_norm, norm_type)
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+    _written([g for g, d in zip(grads, dense) if d is g])
+    return norm
 
 
 def copy_(dst, src):

@@ -263,6 +263,48 @@ int cvn_conv_ln_mlp_head_f32(const float* t, int t_act, int64_t B, int64_t Ct, i
                              const float* head_ln_b, float head_ln_eps, const float* head_w,
                              const float* head_b, float* t_next, cvn_stream_t stream);
 
+/* Types of tensors, where an entry point takes more than fp32. */
+enum { CVN_F32 = 0, CVN_BF16 = 1, CVN_F16 = 2 };
+/* A gate of a branch: none, a factor per sample and channel (B,C), or a factor per element (B,C,HW). */
+enum { CVN_GATE_NONE = 0, CVN_GATE_SAMPLE = 1, CVN_GATE_FULL = 2 };
+/* Norms over many tensors. */
+enum { CVN_NORM_2 = 0, CVN_NORM_INF = 1 };
+
+/* A block's scaled residual and the norms before and after its branch (util_converse.py:285-293, 314-323):
+ *   r = x + res_scale[c] * gate * P(h),  y = N(r)
+ * P: LayerNorm over the channels of h with (post_w, post_b, post_eps), or h itself where post_w is NULL; N: the same
+ * of r with (norm_w, norm_b, norm_eps), or no y where norm_w is NULL; res_scale (C) and gate may be NULL.  h NULL:
+ * y = N(x) alone, r is not written.  x, r, y: (B,C,HW) of x_type; h, gate: of h_type, which is x_type or, on a float32
+ * x, a 16-bit type; the parameters fp32.  Computed in fp32 and rounded once, r before its norm not at all.
+ * stats: NULL, or fp32 (4,B HW), which the backward reads: mean and 1/deviation of r, then of h (rows of norms that
+ * are not there are not written).  Up to 65536 channels and 2^31 - 1 pixels. */
+int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, int h_type, int64_t B, int64_t C, int64_t HW,
+                          const float* res_scale, const void* gate, int gate_kind, const float* post_w,
+                          const float* post_b, float post_eps, const float* norm_w, const float* norm_b,
+                          float norm_eps, void* r, void* y, float* stats, cvn_stream_t stream);
+/* Its gradients from those of r and y (either may be NULL: zero).  base: the forward's r where x is float32; x itself
+ * where x is a 16-bit type (the rounded r would not give r's norm), and then h is read too wherever the forward had
+ * one.  Otherwise h may be NULL without scale, gate and post_w.  Outputs may each be NULL; grad_h without scale, gate
+ * and post_w is grad_x rounded to h_type.  The sums over pixels are added up in the same order on every call. */
+size_t cvn_residual_norm_bwd_workspace(int64_t B, int64_t C, int64_t HW, int gate_kind);
+int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, const void* base, int x_type, const void* h,
+                          int h_type, int64_t B, int64_t C, int64_t HW, const float* res_scale, const void* gate,
+                          int gate_kind, const float* post_w, const float* post_b, const float* norm_w,
+                          const float* stats, void* grad_x, void* grad_h, void* grad_gate, float* grad_scale,
+                          float* grad_norm_w, float* grad_norm_b, float* grad_post_w, float* grad_post_b,
+                          void* workspace, size_t workspace_bytes, cvn_stream_t stream);
+
+/* The norm over all elements of n tensors (grads, numel, types: host arrays, read before the call returns), in 64 bits
+ * and rounded once into *norm (device memory).  0 for no elements. */
+size_t cvn_grad_norm_workspace(const int64_t* numel, int64_t n);
+int cvn_grad_norm(const void* const* grads, const int64_t* numel, const int* types, int64_t n, int norm_kind,
+                  float* norm, void* workspace, size_t workspace_bytes, cvn_stream_t stream);
+/* The norm, and out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)).  out[i] may be grads[i]; otherwise no output may
+ * share memory with a gradient or another output (CVN_ERR_ARG).  A norm that is NaN makes every output NaN. */
+int cvn_clip_grads(const void* const* grads, void* const* out, const int64_t* numel, const int* types, int64_t n,
+                   int norm_kind, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                   cvn_stream_t stream);
+
 /* Plain device copy of n floats (bandwidth calibration). */
 int cvn_copy_f32(const float* src, float* dst, int64_t n, cvn_stream_t stream);
 
