@@ -33,7 +33,8 @@ struct RnArgs {
 };
 
 // The launches of one pair of types (residual_norm_f32.hip, residual_norm_half.hip).
-typedef int (*RnLaunch)(const RnArgs&, int64_t B, hipStream_t);
+struct RnShape;
+typedef int (*RnLaunch)(const RnArgs&, const RnShape&, hipStream_t);
 struct RnKernels {
   RnLaunch fwd, bwd;
 };
@@ -43,21 +44,37 @@ RnKernels rn_f32_f16();
 RnKernels rn_bf16_bf16();
 RnKernels rn_f16_f16();
 
-// Blocks of the backward, which each keep a row of partial sums.
-int64_t rn_bwd_blocks(int64_t ntiles);
-
-struct RnTiles {
-  int64_t n;
-  int tps;
+// How a call runs: pixels of a lane (0: the kernels of any channel count), channels of a wave, and its tiles of 64 px
+// pixels.
+struct RnShape {
+  int px, ch;
+  int64_t ntiles;
+  int tps;  // tiles per sample, or 0: tiles of consecutive pixels of any samples
 };
-// Tiles of 64 pixels.  A gate per sample and channel has its gradient summed tile by tile, so its tiles end with their
-// sample; others do where a sample's last tile is a small part of it.
-inline RnTiles rn_tiles(int64_t B, int64_t HW, bool gate_sample) {
-  if (gate_sample || HW >= 1024) {
-    const int64_t tps = (HW + 63) / 64;
-    return {B * tps, (int)tps};
+
+inline RnShape rn_shape(int64_t B, int64_t C, int64_t HW, bool gate_sample) {
+  RnShape s = {1, 16, 0, 0};
+  // A gate per sample and channel has its gradient summed tile by tile, so its tiles end with their sample; others do
+  // where a sample's last tile is a small part of it, and only then may a lane take several pixels.
+  const bool per_sample = gate_sample || HW >= 1024;
+  if (C > 256) s.px = 0;
+  else if (HW >= 1024 && C <= 128 && C % 8 == 0) s = {2, 8, 0, 0};
+  const int64_t tile = 64 * (s.px ? s.px : 1);
+  if (per_sample) {
+    s.tps = (int)((HW + tile - 1) / tile);
+    s.ntiles = B * s.tps;
+  } else {
+    s.ntiles = (B * HW + tile - 1) / tile;
   }
-  return {(B * HW + 63) / 64, 0};
+  return s;
+}
+
+// Blocks of the backward, which each keep a row of partial sums: as many tiles for each as can be.
+inline int64_t rn_bwd_blocks(const RnShape& s) {
+  const int64_t most = s.px ? 1024 : 2048;
+  if (s.ntiles <= most) return s.ntiles;
+  const int64_t per = (s.ntiles + most - 1) / most;
+  return (s.ntiles + per - 1) / per;
 }
 
 }  // namespace cvn

@@ -5,9 +5,6 @@
 
 namespace cvn {
 
-// Up to a block per 4 tiles and CU-filling at least: each keeps its own partial sums, one row of 5 C.
-int64_t rn_bwd_blocks(int64_t ntiles) { return std::min<int64_t>(ntiles, 2048); }
-
 namespace {
 
 // out[k][c] = sum over blocks of part[k][c][:], and the per-sample gates' gradients from their tiles' sums: a wave per
@@ -110,18 +107,18 @@ extern "C" int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, i
   a.C = C;
   a.HW = HW;
   a.total = B * HW;
-  const RnTiles t = rn_tiles(B, HW, false);
-  a.ntiles = t.n;
+  const RnShape t = rn_shape(B, C, HW, false);
+  a.ntiles = t.ntiles;
   a.tps = t.tps;
-  return k.fwd(a, B, (hipStream_t)stream);
+  return k.fwd(a, t, (hipStream_t)stream);
 }
 
 extern "C" size_t cvn_residual_norm_bwd_workspace(int64_t B, int64_t C, int64_t HW, int gate_kind) {
   RnKernels k;
   if (rn_shape_ok(B, C, HW, CVN_F32, CVN_F32, &k) != CVN_OK) return 0;
   const bool sample = gate_kind == CVN_GATE_SAMPLE;
-  const RnTiles t = rn_tiles(B, HW, sample);
-  const size_t part = align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)rn_bwd_blocks(t.n));
+  const RnShape t = rn_shape(B, C, HW, sample);
+  const size_t part = align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)rn_bwd_blocks(t));
   return part + (sample ? sizeof(float) * (size_t)(B * C) * (size_t)t.tps : 0) + 256;
 }
 
@@ -145,10 +142,10 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   if (!empty && !grad_y && (grad_norm_w || grad_norm_b))
     return fail(CVN_ERR_ARG, "gradients of the norm's parameters without a gradient of y");
   const bool sample = gate_kind == CVN_GATE_SAMPLE;
-  const RnTiles t = rn_tiles(B, HW, sample);
+  const RnShape t = rn_shape(B, C, HW, sample);
   if (!workspace || workspace_bytes < cvn_residual_norm_bwd_workspace(B, C, HW, gate_kind))
     return fail(CVN_ERR_WORKSPACE, "residual_norm backward workspace missing or too small");
-  const int64_t G = rn_bwd_blocks(t.n);
+  const int64_t G = rn_bwd_blocks(t);
   hipStream_t st = (hipStream_t)stream;
   RnArgs a = {};
   a.part = (float*)align_up((size_t)workspace);
@@ -170,10 +167,10 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   a.C = C;
   a.HW = HW;
   a.total = B * HW;
-  a.ntiles = t.n;
+  a.ntiles = t.ntiles;
   a.tps = t.tps;
   if (!empty) {
-    rc = k.bwd(a, B, st);
+    rc = k.bwd(a, t, st);
     if (rc != CVN_OK) return rc;
   }
   RnSumArgs s = {};

@@ -195,18 +195,470 @@ __global__ void __launch_bounds__(64) k_rn_bwd_any(RnArgs a) {
   }
 }
 
-template <class T, class TH>
-int rn_launch_fwd(const RnArgs& a, int64_t, hipStream_t st) {
-  auto k = a.pw ? k_rn_fwd_any<T, TH, true> : k_rn_fwd_any<T, TH, false>;
-  hipLaunchKernelGGL(k, dim3((unsigned)a.ntiles), dim3(64), 0, st, a);
-  return check_launch("residual_norm");
+// ------------------------------------------------------------------------------------------------
+// Up to 256 channels: a block per tile of 64 V pixels, its channels spread over the waves, NC to a wave, so that a
+// tensor's part of a tile is read once, V pixels of a channel to a lane, and stays in registers.
+// ------------------------------------------------------------------------------------------------
+
+// A lane's V pixels of a tile.  The last lanes of a sample's last tile move back to its last V pixels: they compute
+// what their neighbours do, store the same, and leave the pixels before `dup` out of their sums.
+template <int V>
+struct RnLane {
+  int64_t base, q, b;  // element of the tile's first pixel at channel 0; index of the lane's first pixel; its sample
+  int off, dup;
+
+  __device__ __forceinline__ RnLane(const RnArgs& a, int64_t tile, int lane) {
+    if (V == 1) {
+      const RnPx p = rn_px(a, tile, lane);
+      base = p.base;
+      q = p.q;
+      b = p.b;
+      off = p.off;
+      dup = p.ok ? 0 : 1;
+      return;
+    }
+    b = (uint32_t)tile / (uint32_t)a.tps;
+    const int64_t p0 = (tile - b * a.tps) * (64 * V);
+    off = (int)min((int64_t)(lane * V), a.HW - V - p0);
+    dup = lane * V - off;
+    base = b * a.C * a.HW + p0;
+    q = b * a.HW + p0 + off;
+  }
+  __device__ __forceinline__ bool any() const { return dup < V; }
+  __device__ __forceinline__ bool counts(int j) const { return j >= dup; }
+};
+
+// Addresses need only be multiples of the type's size: a lane's V pixels start anywhere in rows of odd length.
+template <class T, int V>
+struct RnVec {
+  typedef T v __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+
+template <class T, int V>
+__device__ __forceinline__ void rn_load(float (&o)[V], const T* p) {
+  if constexpr (V == 1) {
+    o[0] = (float)*p;
+  } else {
+    const typename RnVec<T, V>::v t = *(const typename RnVec<T, V>::v*)p;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = (float)t[j];
+  }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void rn_store(T* p, const float (&o)[V]) {
+  if constexpr (V == 1) {
+    *p = (T)o[0];
+  } else {
+    typename RnVec<T, V>::v t;
+#pragma unroll
+    for (int j = 0; j < V; ++j) t[j] = (T)o[j];
+    *(typename RnVec<T, V>::v*)p = t;
+  }
+}
+
+// A wave's channels of a tensor, from channel c0 on; those behind the n of this wave repeat its last.
+template <class T, int V, int NC>
+__device__ __forceinline__ void rn_load_all(float (&o)[NC][V], const void* p, const RnLane<V>& px, int64_t HW, int c0, int n) {
+  const T* t = (const T*)p + px.base + c0 * HW;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) rn_load<T, V>(o[i], t + min(i, n - 1) * HW + px.off);
+}
+
+// Sums of K values per pixel over the waves of a block, in the order of the waves.  red: two buffers of nw K V 64
+// floats, taken in turn, so that one barrier a time is enough: a buffer is written again only after the barrier of the
+// other, which a wave reaches after its reads.
+template <int K, int V>
+__device__ __forceinline__ void rn_exchange(float* red, int& turn, int nw, int wave, int lane, const float (&v)[K][V]) {
+  float* o = red + (turn * nw + wave) * (K * V * 64) + lane;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[(k * V + j) * 64] = v[k][j];
+  __syncthreads();
+}
+
+template <int V>
+__device__ __forceinline__ void rn_block_sums(float* red, int& turn, int nw, int wave, int lane, float (&v)[2][V]) {
+  if (nw == 1) return;
+  rn_exchange<2, V>(red, turn, nw, wave, lane, v);
+  const float* o = red + turn * nw * (2 * V * 64) + lane;
+  turn ^= 1;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float s = 0.f;
+      for (int w = 0; w < nw; ++w) s += o[(w * 2 * V + k * V + j) * 64];
+      v[k][j] = s;
+    }
+}
+
+// mu and rho of a pixel's channels: each wave's mean and sum of squares about it, joined by the means' spread, so that
+// no large mean cancels.
+template <int V, int NC>
+__device__ __forceinline__ void rn_block_moments(float* red, int& turn, int nw, int wave, int lane, int C, int n, float eps,
+                                                 const float (&x)[NC][V], float (&mu)[V], float (&rho)[V]) {
+  float m[2][V];
+  const float rn = 1.f / (float)n;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) s += i < n ? x[i][j] : 0.f;
+    const float u = s * rn;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const float d = i < n ? x[i][j] - u : 0.f;
+      q = fmaf(d, d, q);
+    }
+    m[0][j] = u;
+    m[1][j] = q;
+  }
+  if (nw > 1) {
+    rn_exchange<2, V>(red, turn, nw, wave, lane, m);
+    const float* o = red + turn * nw * (2 * V * 64) + lane;
+    turn ^= 1;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float s = 0.f;
+      for (int w = 0; w < nw; ++w) s = fmaf((float)min(NC, C - w * NC), o[(w * 2 * V + j) * 64], s);
+      const float u = s / (float)C;
+      float q = 0.f;
+      for (int w = 0; w < nw; ++w) {
+        const float d = o[(w * 2 * V + j) * 64] - u;
+        q += fmaf((float)min(NC, C - w * NC) * d, d, o[(w * 2 * V + V + j) * 64]);
+      }
+      m[0][j] = u;
+      m[1][j] = q;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    mu[j] = m[0][j];
+    rho[j] = 1.f / sqrtf(m[1][j] / (float)C + eps);
+  }
+}
+
+// Sums over a wave's lanes of NC values at a time: each step halves the values a lane holds, sending the other half to
+// the lane it is kept in, so NC sums take about NC + 6 operations; lane l ends with value l NC / 64.
+__device__ __forceinline__ float rn_swap_add32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float rn_swap_add16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float rn_dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// from lane l ^ 8, l ^ 7, l ^ 2, l ^ 1: together they reach all 16 lanes of a row
+constexpr int kXor8 = 0x128, kXor7 = 0x141, kXor2 = 0x4e, kXor1 = 0xb1;
+template <int CTRL>
+__device__ __forceinline__ float rn_swap_add(float a, float b, bool upper) {
+  return (upper ? b : a) + rn_dpp<CTRL>(upper ? a : b);
+}
+
+template <int NC>
+__device__ __forceinline__ float rn_lane_sums(float (&v)[NC], int lane) {
+  static_assert(NC == 8 || NC == 16 || NC == 32, "");
+#pragma unroll
+  for (int i = 0; i < NC / 2; ++i) v[i] = rn_swap_add32(v[i], v[i + NC / 2]);
+#pragma unroll
+  for (int i = 0; i < NC / 4; ++i) v[i] = rn_swap_add16(v[i], v[i + NC / 4]);
+#pragma unroll
+  for (int i = 0; i < NC / 8; ++i) v[i] = rn_swap_add<kXor8>(v[i], v[i + NC / 8], lane & 8);
+  if constexpr (NC >= 16) {
+#pragma unroll
+    for (int i = 0; i < NC / 16; ++i) v[i] = rn_swap_add<kXor7>(v[i], v[i + NC / 16], lane & 4);
+  } else {
+    v[0] += rn_dpp<kXor7>(v[0]);
+  }
+  if constexpr (NC >= 32) v[0] = rn_swap_add<kXor2>(v[0], v[1], lane & 2);
+  else v[0] += rn_dpp<kXor2>(v[0]);
+  return v[0] + rn_dpp<kXor1>(v[0]);
+}
+
+template <class T, class TH, int V, int NC, bool FULL, bool POST, bool FG>
+__global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
+  extern __shared__ float red[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+  const int C = (int)a.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
+  const RnLane<V> px(a, blockIdx.x, lane);
+  const int64_t HW = a.HW, at = px.base + c0 * HW + px.off;
+  int turn = 0;
+  float x[NC][V], h[NC][V], g[FG ? NC : 1][V];
+  rn_load_all<T, V, NC>(x, a.x, px, HW, c0, n);
+  if (a.h) rn_load_all<TH, V, NC>(h, a.h, px, HW, c0, n);
+  if constexpr (FG) rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
+  if constexpr (POST) {
+    float mu[V], rho[V];
+    rn_block_moments<V, NC>(red, turn, nw, wave, lane, C, n, a.peps, h, mu, rho);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = c0 + min(i, n - 1);
+      const float w = a.pw[c], b = a.pb[c];
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[i][j] = fmaf((h[i][j] - mu[j]) * rho[j], w, b);
+    }
+    if (a.stats && wave == 0 && px.any()) {
+      rn_store<float, V>(a.stats + 2 * a.total + px.q, mu);
+      rn_store<float, V>(a.stats + 3 * a.total + px.q, rho);
+    }
+  }
+  if (a.h) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = c0 + min(i, n - 1);
+      const float s = a.s ? a.s[c] : 1.f;
+      const float gs = !FG && a.gate ? rn_ld<TH>(a.gate, px.b * C + c) : 1.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[i][j] = fmaf(s, h[i][j] * (FG ? g[FG ? i : 0][j] : gs), x[i][j]);
+    }
+    if (px.any())
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (i < n) rn_store<T, V>((T*)a.r + at + i * HW, x[i]);
+  }
+  if (!a.nw) return;
+  float mu[V], rho[V];
+  rn_block_moments<V, NC>(red, turn, nw, wave, lane, C, n, a.neps, x, mu, rho);
+  if (!px.any()) return;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    if (i >= n) break;
+    const float w = a.nw[c0 + i], b = a.nb[c0 + i];
+    float y[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) y[j] = fmaf((x[i][j] - mu[j]) * rho[j], w, b);
+    rn_store<T, V>((T*)a.y + at + i * HW, y);
+  }
+  if (a.stats && wave == 0) {
+    rn_store<float, V>(a.stats + px.q, mu);
+    rn_store<float, V>(a.stats + a.total + px.q, rho);
+  }
+}
+
+// Values that depend on v are computed in the loop they stand in: held for all channels over all tiles, parameters and
+// offsets would not fit the scalar registers.
+template <class P>
+__device__ __forceinline__ void rn_in_loop(P& v) {
+  asm volatile("" : "+s"(v));
+}
+
+template <class T, class TH, int V, int NC, bool FULL, bool POST, bool FG>
+__global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
+  extern __shared__ float red[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+  const int C = (int)a0.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
+  const float rC = 1.f / (float)C;
+  const bool norm = a0.nw && a0.gy, branch = a0.dh || a0.dg || a0.s || POST;
+  int turn = 0;
+  float acc[kRnSums] = {};  // lane l: the sums of channel c0 + l NC / 64
+  for (int64_t tile = blockIdx.x; tile < a0.ntiles; tile += gridDim.x) {
+    RnArgs a = a0;
+    rn_in_loop(a.HW);
+    rn_in_loop(a.s);
+    rn_in_loop(a.nw);
+    rn_in_loop(a.pw);
+    rn_in_loop(a.pb);
+    const int64_t HW = a.HW;
+    const RnLane<V> px(a, tile, lane);
+    const int64_t at = px.base + c0 * HW + px.off;
+    float r[NC][V], d[NC][V], e[NC][V], h[NC][V], g[FG ? NC : 1][V];
+    if (norm) {
+      rn_load_all<T, V, NC>(r, a.x, px, HW, c0, n);
+      rn_load_all<T, V, NC>(d, a.gy, px, HW, c0, n);
+    }
+    if (a.gr) rn_load_all<T, V, NC>(e, a.gr, px, HW, c0, n);
+    if (a.h) rn_load_all<TH, V, NC>(h, a.h, px, HW, c0, n);
+    if constexpr (FG) rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
+    float mh[V], rh[V];
+    if constexpr (POST) {
+      rn_load<float, V>(mh, a.stats + 2 * a.total + px.q);
+      rn_load<float, V>(rh, a.stats + 3 * a.total + px.q);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mh[j]) * rh[j];  // hhat
+    }
+    float gs[NC];  // a gate per sample
+    if constexpr (!FG) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) gs[i] = a.gate ? rn_ld<TH>(a.gate, px.b * C + c0 + min(i, n - 1)) : 1.f;
+    }
+    auto gate = [&](int i, int j) { return FG ? g[FG ? i : 0][j] : gs[i]; };
+    auto nv = [&](int i, int j, int c) { return POST ? fmaf(h[i][j], a.pw[c], a.pb[c]) : h[i][j]; };
+    float t[NC];
+    if (norm) {
+      float mu[V], rho[V], s[2][V] = {};
+      rn_load<float, V>(mu, a.stats + px.q);
+      rn_load<float, V>(rho, a.stats + a.total + px.q);
+      if (sizeof(T) < 4 && a.h) {  // x: r as the forward had it
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int c = c0 + min(i, n - 1);
+          const float sc = a.s ? a.s[c] : 1.f;
+#pragma unroll
+          for (int j = 0; j < V; ++j) r[i][j] = fmaf(sc, nv(i, j, c) * gate(i, j), r[i][j]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const float w = a.nw[c0 + min(i, n - 1)];
+        float tw = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          r[i][j] = (r[i][j] - mu[j]) * rho[j];  // rhat
+          tw += px.counts(j) ? d[i][j] * r[i][j] : 0.f;
+          const float gw = i < n ? d[i][j] * w : 0.f;
+          s[0][j] += gw;
+          s[1][j] = fmaf(gw, i < n ? r[i][j] : 0.f, s[1][j]);
+        }
+        t[i] = tw;
+      }
+      acc[0] += rn_lane_sums<NC>(t, lane);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[i] += px.counts(j) ? d[i][j] : 0.f;
+      }
+      acc[1] += rn_lane_sums<NC>(t, lane);
+      rn_block_sums<V>(red, turn, nw, wave, lane, s);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const float w = a.nw[c0 + min(i, n - 1)];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float v = rho[j] * (d[i][j] * w - s[0][j] * rC - r[i][j] * (s[1][j] * rC));
+          d[i][j] = a.gr ? e[i][j] + v : v;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] = e[i][j];
+    }
+    if (a.dx && px.any())
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (i < n) rn_store<T, V>((T*)a.dx + at + i * HW, d[i]);
+    if (!branch) continue;
+    if (a.s) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = c0 + min(i, n - 1);
+        const float sc = a.s[c];
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          t[i] += px.counts(j) ? d[i][j] * (nv(i, j, c) * gate(i, j)) : 0.f;
+          d[i][j] *= sc;
+        }
+      }
+      acc[2] += rn_lane_sums<NC>(t, lane);
+    }
+    if (a.dg) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = c0 + min(i, n - 1);
+        float dg[V];
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          dg[j] = d[i][j] * nv(i, j, c);
+          t[i] += px.counts(j) ? dg[j] : 0.f;
+        }
+        if (FG && i < n && px.any()) rn_store<TH, V>((TH*)a.dg + at + i * HW, dg);
+      }
+      if constexpr (!FG) {
+        const float v = rn_lane_sums<NC>(t, lane);
+        const int i = lane / (64 / NC);
+        if (lane % (64 / NC) == 0 && i < n) a.dgpart[(px.b * C + c0 + i) * a.tps + tile % a.tps] = v;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[i][j] *= gate(i, j);  // dn
+    if constexpr (POST) {
+      float s[2][V] = {};
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[i] += px.counts(j) ? d[i][j] * h[i][j] : 0.f;
+      }
+      acc[3] += rn_lane_sums<NC>(t, lane);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const float w = a.pw[c0 + min(i, n - 1)];
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          t[i] += px.counts(j) ? d[i][j] : 0.f;
+          d[i][j] *= w;
+          const float gw = i < n ? d[i][j] : 0.f;
+          s[0][j] += gw;
+          s[1][j] = fmaf(gw, i < n ? h[i][j] : 0.f, s[1][j]);
+        }
+      }
+      acc[4] += rn_lane_sums<NC>(t, lane);
+      rn_block_sums<V>(red, turn, nw, wave, lane, s);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] = rh[j] * (d[i][j] - s[0][j] * rC - h[i][j] * (s[1][j] * rC));
+    }
+    if (a.dh && px.any())
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (i < n) rn_store<TH, V>((TH*)a.dh + at + i * HW, d[i]);
+  }
+  const int i = lane / (64 / NC);
+  if (lane % (64 / NC) == 0 && i < n)
+#pragma unroll
+    for (int k = 0; k < kRnSums; ++k) a0.part[((int64_t)k * C + c0 + i) * gridDim.x + blockIdx.x] = acc[k];
+}
+
+template <class T, class TH, int V, int NC, bool FULL>
+int rn_launch_tile(const RnArgs& a, int64_t blocks, bool bwd, hipStream_t st) {
+  const int nw = (int)((a.C + NC - 1) / NC);
+  const size_t lds = nw == 1 ? 0 : sizeof(float) * 2 * nw * 2 * V * 64;
+  const bool fg = a.gate && a.gate_full;
+  auto k = bwd ? (a.pw ? (fg ? k_rn_bwd<T, TH, V, NC, FULL, true, true> : k_rn_bwd<T, TH, V, NC, FULL, true, false>)
+                       : (fg ? k_rn_bwd<T, TH, V, NC, FULL, false, true> : k_rn_bwd<T, TH, V, NC, FULL, false, false>))
+               : (a.pw ? (fg ? k_rn_fwd<T, TH, V, NC, FULL, true, true> : k_rn_fwd<T, TH, V, NC, FULL, true, false>)
+                       : (fg ? k_rn_fwd<T, TH, V, NC, FULL, false, true> : k_rn_fwd<T, TH, V, NC, FULL, false, false>));
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * nw), lds, st, a);
+  return check_launch(bwd ? "residual_norm backward" : "residual_norm");
 }
 
 template <class T, class TH>
-int rn_launch_bwd(const RnArgs& a, int64_t, hipStream_t st) {
-  auto k = a.pw ? k_rn_bwd_any<T, TH, true> : k_rn_bwd_any<T, TH, false>;
-  hipLaunchKernelGGL(k, dim3((unsigned)rn_bwd_blocks(a.ntiles)), dim3(64), 0, st, a);
-  return check_launch("residual_norm backward");
+int rn_launch(const RnArgs& a, const RnShape& s, int64_t blocks, bool bwd, hipStream_t st) {
+  switch (s.px) {
+    case 2: return rn_launch_tile<T, TH, 2, 8, true>(a, blocks, bwd, st);
+    case 1: return rn_launch_tile<T, TH, 1, 16, false>(a, blocks, bwd, st);
+  }
+  auto k = bwd ? (a.pw ? k_rn_bwd_any<T, TH, true> : k_rn_bwd_any<T, TH, false>)
+               : (a.pw ? k_rn_fwd_any<T, TH, true> : k_rn_fwd_any<T, TH, false>);
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64), 0, st, a);
+  return check_launch(bwd ? "residual_norm backward" : "residual_norm");
+}
+
+template <class T, class TH>
+int rn_launch_fwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
+  return rn_launch<T, TH>(a, s, s.ntiles, false, st);
+}
+
+template <class T, class TH>
+int rn_launch_bwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
+  return rn_launch<T, TH>(a, s, rn_bwd_blocks(s), true, st);
 }
 
 }  // namespace
