@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import operator
 import os
 import threading
 from array import array
@@ -621,16 +622,23 @@ def conv_ln_mlp_residual(t, x, w0, b0, ln_w, ln_b, ln_eps, w1, b1, w2, b2, res_s
 
 def _on(dev):
     """Makes a tensor's device current for the launches on its stream."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _NO_SWITCH if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
-def _param32(keep, t, C, what):
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _param32(keep, t, C, index, what):
     """Address of a parameter's C values in float32 (None for None); copies go to `keep`, as in _ptrs."""
     if t is None:
         return None
-    if not t.is_cuda or t.numel() != C or t.dtype not in _lib.TYPES:
-        raise RuntimeError(f"{what} must hold {C} values on the HIP device")
-    if t.dtype != torch.float32 or not t.is_contiguous():
+    if t.get_device() != index or t.numel() != C or t.dtype not in _lib.TYPES:
+        raise RuntimeError(f"{what} must hold {C} values on the device of x")
+    if t.dtype is not torch.float32 or not t.is_contiguous():
         t = t.to(torch.float32).contiguous()
         keep.append(t)
     return t.data_ptr()
@@ -646,56 +654,57 @@ def _gate_kind(h, gate):
     raise RuntimeError("gate must have the branch's shape, or (B,C) or (B,C,1,..) for a factor per sample and channel")
 
 
-def _norm_shape(x, h, res_scale, gate, post, norm):
-    """Checks a residual_norm call: (B, C, HW)."""
+def _norm_args(x, h, gate):
+    """Checks the large arguments of a residual_norm call: ((B, C, HW, kind of gate), device index)."""
+    index = x.get_device()
     for t in (x, h, gate):
-        if t is not None and not (t.is_cuda and t.dtype in _lib.TYPES and t.device == x.device):
+        if t is not None and (t.get_device() != index or index < 0 or t.dtype not in _lib.TYPES):
             raise RuntimeError("residual_norm needs float32, bfloat16 or float16 tensors on one HIP device")
-    if x.dim() < 2:
-        raise RuntimeError("x must be (B,C,*)")
-    if h is None:
-        if res_scale is not None or gate is not None or post is not None or norm is None:
-            raise RuntimeError("without a branch there is only the norm of x")
-    else:
-        if h.shape != x.shape:
+    shape = x.shape
+    if len(shape) < 2 or shape[1] < 1:
+        raise RuntimeError("x must be (B,C,*) with channels")
+    if h is not None:
+        if h.shape != shape:
             raise RuntimeError("x and the branch must have one shape")
-        if h.dtype != x.dtype and x.dtype != torch.float32:
+        if h.dtype is not x.dtype and x.dtype is not torch.float32:
             raise RuntimeError("x and the branch must have one type, or x float32 and the branch a 16-bit type")
-        if gate is not None and gate.dtype != h.dtype:
+        if gate is not None and gate.dtype is not h.dtype:
             raise RuntimeError("gate must have the branch's type")
-    for t in (res_scale, *(post or ())[:2], *(norm or ())[:2]):
-        if t is not None and t.device != x.device:
-            raise RuntimeError("tensors on same device")
-    if x.shape[1] < 1:
-        raise RuntimeError("x must have channels")
-    return x.shape[0], x.shape[1], math.prod(x.shape[2:])
+    return (shape[0], shape[1], math.prod(shape[2:]), _gate_kind(h, gate)), index
 
 
 def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
-    """The launch behind residual_norm: (r or None, y or None, stats or None), on contiguous x, h and gate."""
+    """The launch behind residual_norm, on contiguous x, h and gate: (r, y, stats, what _norm_args gave), None for what
+    there is not."""
     lib = _lib.load()
-    B, C, HW = _norm_shape(x, h, res_scale, gate, post, norm)
+    geo, index = _norm_args(x, h, gate)
+    B, C, HW, kind = geo
     keep = []
-    s, nw, nb = (_param32(keep, t, C, n) for t, n in zip((res_scale, *(norm or (None, None))[:2]),
-                                                         ("res_scale", "norm weight", "norm bias")))
-    pw, pb = (_param32(keep, t, C, "branch norm") for t in (post or (None, None))[:2])
-    kind = _gate_kind(h, gate)
-    r = torch.empty_like(x) if h is not None else None
-    y = torch.empty_like(x) if norm is not None else None
-    stats = None
+    s = _param32(keep, res_scale, C, index, "res_scale")
+    nw = nb = pw = pb = r = y = stats = None
+    neps = peps = 0.0
+    if norm is not None:
+        nw, nb = _param32(keep, norm[0], C, index, "norm weight"), _param32(keep, norm[1], C, index, "norm bias")
+        neps = norm[2]
+        y = torch.empty_like(x)
+    if post is not None:
+        pw, pb = _param32(keep, post[0], C, index, "branch norm"), _param32(keep, post[1], C, index, "branch norm")
+        peps = post[2]
+    if h is not None:
+        r = torch.empty_like(x)
+    dev = x.device
     if need_stats and (norm is not None or post is not None):
-        stats = torch.empty((4 if post is not None else 2, B * HW), dtype=torch.float32, device=x.device)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with _on(x.device):
-        rc = lib.cvn_residual_norm_fwd(x.data_ptr(), _lib.TYPES[x.dtype], ptr(h), 0 if h is None else _lib.TYPES[h.dtype],
-                                       B, C, HW, s, ptr(gate), kind, pw, pb, float(post[2]) if post else 0.0, nw, nb,
-                                       float(norm[2]) if norm else 0.0, ptr(r), ptr(y), ptr(stats), _stream(x.device))
+        stats = torch.empty((2 if post is None else 4, B * HW), dtype=torch.float32, device=dev)
+    with _on(dev):
+        rc = lib.cvn_residual_norm_fwd(x.data_ptr(), _lib.TYPES[x.dtype], _ptr(h), _lib.TYPES[(x if h is None else h).dtype],
+                                       B, C, HW, s, _ptr(gate), kind, pw, pb, peps, nw, nb, neps, _ptr(r), _ptr(y),
+                                       _ptr(stats), _stream(dev))
     _lib.check(rc, "residual_norm")
-    return r, y, stats
+    return r, y, stats, geo
 
 
-def _contiguous(*ts):
-    return [t if t is None else t.contiguous() for t in ts]
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def residual_norm(x, h, norm=None, res_scale=None, gate=None, post=None):
@@ -709,77 +718,101 @@ def residual_norm(x, h, norm=None, res_scale=None, gate=None, post=None):
     rounded once: y is the norm of r before its rounding.  For gradients see residual_norm_train."""
     if h is None:
         raise RuntimeError("residual_norm needs a branch")
-    x, h, gate = _contiguous(x, h, gate)
-    return _residual_norm(x, h, norm, res_scale, gate, post, False)[:2]
+    return _residual_norm(_contiguous(x), _contiguous(h), norm, res_scale, _contiguous(gate), post, False)[:2]
 
 
-def residual_norm_backward(grad_r, grad_y, base, h, stats, norm_weight=None, res_scale=None, gate=None, post=None,
-                           h_dtype=None, need=(True,) * 8):
-    """Gradients of residual_norm in one call and its sums: (x, h, res_scale, gate, post weight, post bias, norm
-    weight, norm bias), None where not asked for by `need` or not given.
-
-    grad_r, grad_y: gradients of r and y (None: zero).  base: the forward's r where x is float32, x itself where it
-    is a 16-bit type (there the norm is that of r before its rounding).  h may be None where base is r and there is
-    no scale, gate and post: its gradient is x's, of type h_dtype.  stats: what the forward kept, (2 or 4, B HW)."""
+def _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, post_w, post_b, geo, shape, x_dtype, h_dtype,
+                            need):
+    """The launches behind residual_norm_backward, on arguments that a forward has checked."""
     lib = _lib.load()
-    norm = None if norm_weight is None else (norm_weight, norm_weight, 0.0)
-    if h is not None:
-        h_dtype = h.dtype
-    ref = base if base is not None else grad_r
-    base, h, gate, grad_r, grad_y = _contiguous(base, h, gate, grad_r, grad_y)
-    for t in (grad_r, grad_y):
-        if t is not None and (t.shape != ref.shape or t.dtype != ref.dtype or t.device != ref.device):
-            raise RuntimeError("gradients must match r and y")
-    if h is not None or norm is not None:
-        _norm_shape(ref, h, res_scale, gate, post, norm)
-    B, C, HW = ref.shape[0], ref.shape[1], math.prod(ref.shape[2:])
-    if stats is not None and (tuple(stats.shape) != (4 if post is not None else 2, B * HW) or not stats.is_contiguous()
-                              or stats.dtype != torch.float32 or stats.device != ref.device):
-        raise RuntimeError("stats must be the forward's")
+    B, C, HW, kind = geo
     nx, nh, ns, ng, npw, npb, nnw, nnb = need
+    gr, gy = _contiguous(gr), _contiguous(gy) if norm_w is not None else None
+    dev = (gr if gr is not None else gy).device
+    index = dev.index
     keep = []
-    s = _param32(keep, res_scale, C, "res_scale")
-    nw = _param32(keep, norm_weight, C, "norm weight")
-    pw, pb = (_param32(keep, t, C, "branch norm") for t in (post or (None, None))[:2])
-    dev = ref.device
-    has_norm = norm is not None and grad_y is not None
-    plain = res_scale is None and gate is None and post is None  # then the branch's gradient is x's
-    gx = None
-    if has_norm and (nx or (nh and plain and h_dtype == ref.dtype)):
-        gx = torch.empty(ref.shape, dtype=ref.dtype, device=dev)
-    elif nx or (nh and plain):
-        gx = grad_r if grad_r is not None else torch.zeros(ref.shape, dtype=ref.dtype, device=dev)
-    gh = None
-    if nh and h_dtype is not None:
-        if plain and h_dtype == ref.dtype:
-            gh = gx
-        elif plain and not has_norm:
-            gh = gx.to(h_dtype)
-        else:
-            gh = torch.empty(ref.shape, dtype=h_dtype, device=dev)
-    f32 = lambda want: torch.empty(C, dtype=torch.float32, device=dev) if want else None  # noqa: E731
-    gs = f32(ns and res_scale is not None)
-    gg = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if ng and gate is not None else None
-    gpw, gpb = f32(npw and post is not None), f32(npb and post is not None)
-    gnw, gnb = f32(nnw and has_norm), f32(nnb and has_norm)
-    out_x = gx if has_norm else None
-    out_h = None if gh is gx or (plain and not has_norm) else gh
-    if any(t is not None for t in (out_x, out_h, gs, gg, gpw, gpb, gnw, gnb)):
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        kind = _lib.GATE_NONE if gate is None else _gate_kind(h, gate)
+    f32 = torch.float32
+    plain = res_scale is None and gate is None and post_w is None  # then the branch's gradient is x's
+    gx = gh = gs = gg = gpw = gpb = gnw = gnb = out_x = out_h = None
+    nh = nh and h_dtype is not None
+    same = nh and plain and h_dtype is x_dtype
+    if gy is not None:
+        if nx or same:
+            gx = out_x = torch.empty(shape, dtype=x_dtype, device=dev)
+        if nh and not same:
+            gh = out_h = torch.empty(shape, dtype=h_dtype, device=dev)
+        gnw = torch.empty(norm_w.shape, dtype=f32, device=dev) if nnw else None
+        gnb = torch.empty(norm_w.shape, dtype=f32, device=dev) if nnb else None
+    else:  # x's gradient is r's
+        gx = gr
+        if nh and plain and not same:
+            gh = gr.to(h_dtype)
+        elif nh and not plain:
+            gh = out_h = torch.empty(shape, dtype=h_dtype, device=dev)
+        if norm_w is not None:  # y was not used
+            gnw, gnb = (torch.zeros(norm_w.shape, dtype=f32, device=dev) if w else None for w in (nnw, nnb))
+    if same:
+        gh = gx
+    if ns and res_scale is not None:
+        gs = torch.empty(res_scale.shape, dtype=f32, device=dev)
+    if ng and gate is not None:
+        gg = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    if post_w is not None:
+        gpw = torch.empty(post_w.shape, dtype=f32, device=dev) if npw else None
+        gpb = torch.empty(post_b.shape, dtype=f32, device=dev) if npb else None
+    if gy is not None or out_h is not None or gs is not None or gg is not None or gpw is not None or gpb is not None:
         nbytes = lib.cvn_residual_norm_bwd_workspace(B, C, HW, kind)
         st = _stream(dev)
         ws = _scratch(dev, st)
         with _on(dev), ws.lock:
-            rc = lib.cvn_residual_norm_bwd(ptr(grad_r), ptr(grad_y) if has_norm else None, ptr(base),
-                                           _lib.TYPES[ref.dtype], ptr(h),
-                                           _lib.TYPES[h_dtype or ref.dtype], B, C, HW, s, ptr(gate), kind, pw, pb,
-                                           nw if has_norm else None, ptr(stats), ptr(out_x), ptr(out_h), ptr(gg), ptr(gs),
-                                           ptr(gnw), ptr(gnb), ptr(gpw), ptr(gpb), ws.ptr(nbytes), nbytes, st)
+            rc = lib.cvn_residual_norm_bwd(
+                _ptr(gr), _ptr(gy), None if gy is None else base.data_ptr(), _lib.TYPES[x_dtype], _ptr(h),
+                _lib.TYPES[h_dtype or x_dtype], B, C, HW, _param32(keep, res_scale, C, index, "res_scale"), _ptr(gate), kind,
+                _param32(keep, post_w, C, index, "branch norm"), _param32(keep, post_b, C, index, "branch norm"),
+                None if gy is None else _param32(keep, norm_w, C, index, "norm weight"), _ptr(stats), _ptr(out_x),
+                _ptr(out_h), _ptr(gg), _ptr(gs), *((None, None) if gy is None else (_ptr(gnw), _ptr(gnb))), _ptr(gpw),
+                _ptr(gpb), ws.ptr(nbytes), nbytes, st)
         _lib.check(rc, "residual_norm_backward")
-    if norm is not None and not has_norm:  # y was not used
-        gnw, gnb = (torch.zeros(C, dtype=torch.float32, device=dev) if w else None for w in (nnw, nnb))
     return (gx if nx else None), gh, gs, gg, gpw, gpb, gnw, gnb
+
+
+def residual_norm_backward(grad_r, grad_y, base, h, stats, norm_weight=None, res_scale=None, gate=None, post=None,
+                           h_dtype=None, need=(True,) * 8):
+    """Gradients of residual_norm in one call: (x, h, res_scale, gate, post weight, post bias, norm weight, norm bias),
+    None where not asked for by `need` or not given; those of parameters in float32.
+
+    grad_r, grad_y: gradients of r and y (None: zero).  base: the forward's r where x is float32, x itself where it
+    is a 16-bit type (there the norm is that of r before its rounding), or None without norm_weight.  h may be None
+    where x is float32 and there is no scale, gate and post: its gradient is x's, of type h_dtype.  stats: mean and
+    1 / deviation of r, and with post of h, float32 (2 or 4, B HW), as residual_norm_stats gives them."""
+    ref = next((t for t in (base, grad_r, grad_y) if t is not None), None)
+    if ref is None or (norm_weight is None and grad_r is None) or (norm_weight is not None and base is None):
+        raise RuntimeError("residual_norm_backward needs a gradient, and what its norm was of")
+    if h is not None:
+        h_dtype = h.dtype
+    elif res_scale is not None or gate is not None or post is not None or (ref.dtype != torch.float32 and h_dtype):
+        raise RuntimeError("residual_norm_backward needs the branch")
+    h, gate = _contiguous(h), _contiguous(gate)
+    geo, index = _norm_args(ref, h, gate)
+    for t in (grad_r, grad_y):
+        if t is not None and (t.shape != ref.shape or t.dtype != ref.dtype or t.get_device() != index):
+            raise RuntimeError("gradients must match r and y")
+    if (norm_weight is not None or post is not None) and (
+            stats is None or tuple(stats.shape) != (2 if post is None else 4, geo[0] * geo[2])
+            or not stats.is_contiguous() or stats.dtype != torch.float32 or stats.get_device() != index):
+        raise RuntimeError("stats must be the forward's")
+    if grad_r is None and grad_y is None:
+        raise RuntimeError("residual_norm_backward needs a gradient")
+    pw, pb = (None, None) if post is None else post[:2]
+    return _residual_norm_backward(grad_r, grad_y, _contiguous(base), h, stats, norm_weight, res_scale, gate, pw, pb, geo,
+                                   ref.shape, ref.dtype, h_dtype, need)
+
+
+def residual_norm_stats(x, h, norm=None, res_scale=None, gate=None, post=None):
+    """residual_norm with what residual_norm_backward needs of it: (r, y, stats).  h may be None: y = N(x), r None."""
+    if h is None and (res_scale is not None or gate is not None or post is not None or norm is None):
+        raise RuntimeError("without a branch there is only the norm of x")
+    return _residual_norm(_contiguous(x), _contiguous(h), norm, res_scale, _contiguous(gate), post, True)[:3]
 
 
 class ResidualNormFunction(torch.autograd.Function):
@@ -789,37 +822,34 @@ class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps):
         ctx.set_materialize_grads(False)
-        x, h, gate = _contiguous(x, h, gate)
+        x, h, gate = _contiguous(x), _contiguous(h), _contiguous(gate)
         post = None if post_w is None else (post_w, post_b, post_eps)
         norm = None if norm_w is None else (norm_w, norm_b, norm_eps)
-        r, y, stats = _residual_norm(x, h, norm, res_scale, gate, post, True)
-        half = x.dtype != torch.float32
-        keep_h = h is not None and (half or res_scale is not None or gate is not None or post is not None)
-        base = None if norm is None else (r if h is not None and not half else x)
+        r, y, stats, geo = _residual_norm(x, h, norm, res_scale, gate, post, True)
+        f32 = x.dtype is torch.float32
+        keep_h = h is not None and not (f32 and res_scale is None and gate is None and post is None)
+        base = None if norm is None else (r if h is not None and f32 else x)
         ctx.save_for_backward(base, h if keep_h else None, res_scale, gate, post_w, post_b, norm_w, norm_b, stats)
-        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype)
-        return tuple(t for t in (r, y) if t is not None)
+        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape)
+        return r if y is None else y if r is None else (r, y)
 
     @staticmethod
     def backward(ctx, *gos):
         base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = ctx.saved_tensors
-        post_eps, norm_eps, h_dtype, x_dtype = ctx.cfg
+        post_eps, norm_eps, h_dtype, x_dtype, geo, shape = ctx.cfg
         gr = gos[0] if h_dtype is not None else None
         gy = gos[-1] if norm_w is not None else None
-        n = ctx.needs_input_grad
-        if (gr is None and gy is None) or not any(n[:8]):
+        need = ctx.needs_input_grad[:8]
+        if gr is None and gy is None:
             return (None,) * 10
-        post = None if post_w is None else (post_w, post_b, post_eps)
         if torch.is_grad_enabled():
+            post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
-                                                     h_dtype, x_dtype, n) + (None, None)
-        if norm_w is None:
-            base = None
-        gx, gh, gs, gg, gpw, gpb, gnw, gnb = residual_norm_backward(
-            gr, gy, base, h, stats, norm_w, res_scale, gate, post, h_dtype, n[:8])
-        like = lambda g, t: None if g is None else g.to(t.dtype).reshape(t.shape)  # noqa: E731
-        return (gx, gh, like(gs, res_scale), gg, like(gpw, post_w), like(gpb, post_b), like(gnw, norm_w),
-                like(gnb, norm_b), None, None)
+                                                     h_dtype, x_dtype, need) + (None, None)
+        gx, gh, gs, gg, *gp = _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, post_w, post_b, geo,
+                                                      shape, x_dtype, h_dtype, need)
+        like = lambda g, t: g if g is None or t.dtype is torch.float32 else g.to(t.dtype)  # noqa: E731
+        return (gx, gh, like(gs, res_scale), gg, *map(like, gp, (post_w, post_b, norm_w, norm_b)), None, None)
 
 
 def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy, h_dtype, x_dtype,
@@ -861,26 +891,28 @@ def residual_norm_train(x, h, norm=None, res_scale=None, gate=None, post=None):
     pw, pb, pe = post or (None, None, 0.0)
     nw, nb, ne = norm or (None, None, 0.0)
     out = ResidualNormFunction.apply(x, h, res_scale, gate, pw, pb, nw, nb, pe, ne)
-    return out if norm is not None else (out[0], None)
+    return (out, None) if norm is None else out
 
 
 def layernorm_cf_train(x, weight, bias, eps):
     """Differentiable layernorm_cf on the HIP kernels (forward and backward)."""
-    return ResidualNormFunction.apply(x, None, None, None, None, None, weight, bias, 0.0, eps)[0]
+    return ResidualNormFunction.apply(x, None, None, None, None, None, weight, bias, 0.0, eps)
 
 
 def _grad_list(ts):
-    """The device of a list of gradients, and its host tables for the library: addresses come per call."""
-    devs = {t.device for t in ts}
-    if len(devs) != 1 or not next(iter(devs)).type == "cuda":
+    """What the library takes of a list of gradients: device index, types, sizes and addresses.  (A model has hundreds:
+    the loops run in C.)"""
+    index = ts[0].get_device()
+    if index < 0 or set(map(torch.Tensor.get_device, ts)) != {index}:
         raise RuntimeError("gradients must be on one HIP device")
-    if not all(t.layout == torch.strided for t in ts):
-        raise RuntimeError("gradients must be dense")
     try:
-        types = array("i", [_lib.TYPES[t.dtype] for t in ts])
+        types = array("i", map(_lib.TYPES.__getitem__, map(_DTYPE, ts)))
     except KeyError as e:
         raise RuntimeError(f"gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
-    return devs.pop(), types, array("q", [t.numel() for t in ts])
+    return index, types, array("q", map(torch.Tensor.numel, ts)), array("Q", map(torch.Tensor.data_ptr, ts))
+
+
+_DTYPE = operator.attrgetter("dtype")
 
 
 def _norm_kind(norm_type):
@@ -890,8 +922,8 @@ def _norm_kind(norm_type):
     return kind
 
 
-def _addresses(ts):
-    return array("Q", [t.data_ptr() for t in ts])
+def _all_contiguous(ts):
+    return ts if all(map(torch.Tensor.is_contiguous, ts)) else [t.contiguous() for t in ts]
 
 
 def _clip(grads, out, max_norm, norm_type):
@@ -903,21 +935,27 @@ def _clip(grads, out, max_norm, norm_type):
     if not grads:
         return torch.tensor(0.0)
     lib = _lib.load()
-    dev, types, sizes = _grad_list(grads)
+    index, types, sizes, src = _grad_list(grads)
+    dst = src
+    if out is not None and out is not grads:
+        oi, ot, on, dst = _grad_list(out)
+        if oi != index or ot != types or on != sizes:
+            raise RuntimeError("out must have the gradients' sizes and types, on their device")
     n = len(grads)
-    src = _addresses(grads)
-    at = lambda a: a.buffer_info()[0]  # noqa: E731
-    nbytes = lib.cvn_grad_norm_workspace(at(sizes), n)
+    dev = grads[0].device
+    tables = (src, dst, sizes, types)  # held until the library has read them
+    src_at, dst_at, sizes_at, types_at = (a.buffer_info()[0] for a in tables)
+    nbytes = lib.cvn_grad_norm_workspace(sizes_at, n)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     st = _stream(dev)
     ws = _scratch(dev, st)
     with _on(dev), ws.lock:
         if out is None:
-            rc = lib.cvn_grad_norm(at(src), at(sizes), at(types), n, kind, norm.data_ptr(), ws.ptr(nbytes), nbytes, st)
+            rc = lib.cvn_grad_norm(src_at, sizes_at, types_at, n, kind, norm.data_ptr(), ws.ptr(nbytes), nbytes, st)
         else:
-            dst = src if out is grads else _addresses(out)
-            rc = lib.cvn_clip_grads(at(src), at(dst), at(sizes), at(types), n, kind, max_norm, norm.data_ptr(),
+            rc = lib.cvn_clip_grads(src_at, dst_at, sizes_at, types_at, n, kind, max_norm, norm.data_ptr(),
                                     ws.ptr(nbytes), nbytes, st)
+    del tables
     _lib.check(rc, "grad_norm" if out is None else "clip_grads")
     return norm
 
@@ -929,19 +967,19 @@ def _tensors(ts):
 def grad_norm(grads, norm_type=2.0):
     """The norm over all elements of many tensors (2, or math.inf for the largest magnitude): a float32 scalar on their
     device, accumulated in 64 bits.  grads: tensors of any shapes, float32, bfloat16 or float16, on one device."""
-    return _clip([t.contiguous() for t in _tensors(grads)], None, None, norm_type)
+    return _clip(_all_contiguous(_tensors(grads)), None, None, norm_type)
 
 
 def _written(ts):
     """The library wrote these tensors: autograd sees it as it sees torch's in-place operations."""
-    ts = [t for t in ts if not t.is_inference()]
-    if ts:
-        torch.autograd.graph.increment_version(ts)
+    if any(map(torch.Tensor.is_inference, ts)):
+        ts = [t for t in ts if not t.is_inference()]
+    torch.autograd.graph.increment_version(ts)
 
 
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """(grads scaled by min(1, max_norm / (norm + 1e-6)), norm).  The scaled gradients go to new tensors, or to `out`:
-    contiguous tensors of the same types and shapes, each its own gradient or memory apart from all others."""
+    contiguous tensors of the same types and sizes, each its own gradient or memory apart from all others."""
     grads = _tensors(grads)
     if out is None:
         out = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in grads]
@@ -949,10 +987,9 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         out = _tensors(out)
         if len(out) != len(grads):
             raise RuntimeError("out must hold a tensor for each gradient")
-        for g, o in zip(grads, out):
-            if o.shape != g.shape or o.dtype != g.dtype or o.device != g.device or not o.is_contiguous():
-                raise RuntimeError("out must be contiguous, with the gradients' shapes and types, on their device")
-    norm = _clip([g.contiguous() for g in grads], out, max_norm, norm_type)
+        if not all(map(torch.Tensor.is_contiguous, out)):
+            raise RuntimeError("out must be contiguous")
+    norm = _clip(_all_contiguous(grads), out, max_norm, norm_type)
     _written(out)
     return out, norm
 
@@ -960,20 +997,23 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Scales the parameters' .grad in place so that their norm is at most max_norm; returns the norm they had.  As
     torch.nn.utils.clip_grad_norm_; error_if_nonfinite waits for the norm and raises before any gradient changes."""
-    grads = [p.grad for p in _tensors(parameters) if p.grad is not None]
+    grads = [g for g in [p.grad for p in _tensors(parameters)] if g is not None]
     if error_if_nonfinite and grads:
         norm = grad_norm(grads, norm_type)
         if not math.isfinite(norm.item()):
             raise RuntimeError(f"the norm of the gradients is {norm.item()}")
-    for g in grads:
-        if 0 in g.stride() and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
-            raise RuntimeError("a gradient's elements share memory")
-    dense = [g.contiguous() for g in grads]
+    dense = _all_contiguous(grads)
+    if dense is not grads:
+        for g in grads:
+            if 0 in g.stride() and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+                raise RuntimeError("a gradient's elements share memory")
     norm = _clip(dense, dense, max_norm, norm_type)
-    for g, d in zip(grads, dense):
-        if d is not g:
-            g.copy_(d)
-    _written([g for g, d in zip(grads, dense) if d is g])
+    if dense is not grads:
+        for g, d in zip(grads, dense):
+            if d is not g:
+                g.copy_(d)
+        dense = [d for g, d in zip(grads, dense) if d is g]
+    _written(dense)
     return norm
 
 

@@ -425,8 +425,8 @@ def test_recorded_graphs():
     st = torch.cuda.Stream()
 
     def step(d):
-        r, y, stats = Fh._residual_norm(d["x"], d["h"], (d["w"], d["b"], EPS), d["s"], d["gate"],
-                                        (d["pw"], d["pb"], EPS), True)
+        r, y, stats = Fh.residual_norm_stats(d["x"], d["h"], (d["w"], d["b"], EPS), d["s"], d["gate"],
+                                             (d["pw"], d["pb"], EPS))
         return (r, y) + Fh.residual_norm_backward(d["gr"], d["gy"], r, d["h"], stats, d["w"], d["s"], d["gate"],
                                                   (d["pw"], d["pb"], EPS))
 

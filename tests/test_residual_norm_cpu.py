@@ -1,4 +1,5 @@
 """Host checks of the residual-norm and gradient-norm entry points: what they refuse, before anything reaches a device."""
+import ctypes
 import math
 from array import array
 
@@ -112,3 +113,40 @@ def test_composition_matches_the_definition():
     per_sample = torch.randn(2, 5, generator=g, dtype=torch.float64)
     assert torch.equal(composite.residual_branch(h, None, per_sample), h * per_sample[:, :, None, None])
     assert composite.residual_branch(h.float().half()).dtype == torch.float32
+
+
+def test_tables_live_through_the_call(monkeypatch):
+    """The host tables handed to the library are the lists' own while it reads them, whatever is allocated meanwhile."""
+    ts = [torch.ones(n) for n in (3, 5, 7)]
+    seen = {}
+
+    class Lib:
+        def cvn_grad_norm_workspace(self, sizes, n):
+            seen["churn"] = [array("Q", [1] * 3) for _ in range(200)]
+            return 64
+
+        def _read(self, grads, out, sizes, types, n):
+            seen["src"] = list((ctypes.c_uint64 * n).from_address(grads))
+            seen["dst"] = list((ctypes.c_uint64 * n).from_address(out))
+            seen["sizes"] = list((ctypes.c_int64 * n).from_address(sizes))
+            seen["types"] = list((ctypes.c_int * n).from_address(types))
+            return 0
+
+        def cvn_grad_norm(self, grads, sizes, types, n, *rest):
+            return self._read(grads, grads, sizes, types, n)
+
+        def cvn_clip_grads(self, grads, out, sizes, types, n, *rest):
+            return self._read(grads, out, sizes, types, n)
+
+    index = functional._grad_list
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(functional._lib, "load", lambda: Lib())
+    monkeypatch.setattr(functional, "_stream", lambda dev: 0)
+    monkeypatch.setattr(functional, "_on", lambda dev: functional._NO_SWITCH)
+    assert index(ts)[0] == 0
+    functional.grad_norm(ts)
+    want = {"src": [t.data_ptr() for t in ts], "sizes": [3, 5, 7], "types": [0, 0, 0]}
+    assert {k: seen[k] for k in want} == want
+    out, _ = functional.clip_grads(ts, 1.0)
+    assert {k: seen[k] for k in want} == want and seen["dst"] == [t.data_ptr() for t in out]
+    functional.release_workspace()
