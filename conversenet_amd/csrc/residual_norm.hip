@@ -7,41 +7,59 @@ namespace cvn {
 
 namespace {
 
-// out[k][c] = sum over blocks of part[k][c][:], and the per-sample gates' gradients from their tiles' sums: a wave per
-// sum, in 64 bits, in the same order on every call.
+// The parameters' gradients from the blocks' sums, and the per-sample gates' from their tiles': a wave per channel or
+// gate, in 64 bits, in the same order on every call.
 struct RnSumArgs {
   const float *part, *dgpart;
-  float* out[kRnSums];
+  const float *s, *pw, *pb;
+  float *dw, *db, *ds, *dpw, *dpb;
   void* dg;  // (B C) of type dg_type, or null
   int dg_type;
   int C, G, tps;
-  int64_t rows;  // kRnSums C, and B C for the gates
+  int64_t rows;  // C, and B C for the gates
 };
+
+__device__ __forceinline__ double rn_row_sum(const float* p, int n, int lane) {
+  double s[4] = {0., 0., 0., 0.};
+  int i = lane;
+  for (; i + 192 < n; i += 256) {
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = p[i + 64 * j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += v[j];
+  }
+  for (; i < n; i += 64) s[0] += p[i];
+  double t = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) t += __shfl_xor(t, d);
+  return t;
+}
 
 __global__ void __launch_bounds__(256) k_rn_sums(RnSumArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= a.rows) return;
-  const int64_t ns = (int64_t)kRnSums * a.C;
-  const float* p;
-  int n;
-  if (row < ns) {
-    if (!a.out[row / a.C]) return;
-    p = a.part + row * a.G;
-    n = a.G;
-  } else {
-    p = a.dgpart + (row - ns) * a.tps;
-    n = a.tps;
+  if (row >= a.C) {
+    const int64_t i = row - a.C;
+    const float s = (float)rn_row_sum(a.dgpart + i * a.tps, a.tps, lane);
+    if (lane) return;
+    if (a.dg_type == CVN_F32) ((float*)a.dg)[i] = s;
+    else if (a.dg_type == CVN_BF16) ((__bf16*)a.dg)[i] = (__bf16)s;
+    else ((_Float16*)a.dg)[i] = (_Float16)s;
+    return;
   }
-  double s = 0.;
-  for (int i = lane; i < n; i += 64) s += p[i];
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+  const int c = (int)row;
+  auto sum = [&](int k) { return rn_row_sum(a.part + ((int64_t)k * a.C + c) * a.G, a.G, lane); };
+  const double w = a.dw ? sum(0) : 0., b = a.db ? sum(1) : 0.;
+  const double sa = a.dpb || (a.ds && a.pw) ? sum(2) : 0., sh = a.ds || a.dpw ? sum(3) : 0.;
   if (lane) return;
-  if (row < ns) a.out[row / a.C][row % a.C] = (float)s;
-  else if (a.dg_type == CVN_F32) ((float*)a.dg)[row - ns] = (float)s;
-  else if (a.dg_type == CVN_BF16) ((__bf16*)a.dg)[row - ns] = (__bf16)(float)s;
-  else ((_Float16*)a.dg)[row - ns] = (_Float16)(float)s;
+  const double s = a.s ? a.s[c] : 1.;
+  if (a.dw) a.dw[c] = (float)w;
+  if (a.db) a.db[c] = (float)b;
+  if (a.ds) a.ds[c] = (float)(a.pw ? a.pw[c] * sh + a.pb[c] * sa : sh);
+  if (a.dpw) a.dpw[c] = (float)(s * sh);
+  if (a.dpb) a.dpb[c] = (float)(s * sa);
 }
 
 bool rn_kernels(int x_type, int h_type, RnKernels* k) {
@@ -107,7 +125,7 @@ extern "C" int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, i
   a.C = C;
   a.HW = HW;
   a.total = B * HW;
-  const RnShape t = rn_shape(B, C, HW, false);
+  const RnShape t = rn_shape(false, B, C, HW, false);
   a.ntiles = t.ntiles;
   a.tps = t.tps;
   return k.fwd(a, t, (hipStream_t)stream);
@@ -117,7 +135,7 @@ extern "C" size_t cvn_residual_norm_bwd_workspace(int64_t B, int64_t C, int64_t 
   RnKernels k;
   if (rn_shape_ok(B, C, HW, CVN_F32, CVN_F32, &k) != CVN_OK) return 0;
   const bool sample = gate_kind == CVN_GATE_SAMPLE;
-  const RnShape t = rn_shape(B, C, HW, sample);
+  const RnShape t = rn_shape(true, B, C, HW, sample);
   const size_t part = align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)rn_bwd_blocks(t));
   return part + (sample ? sizeof(float) * (size_t)(B * C) * (size_t)t.tps : 0) + 256;
 }
@@ -142,7 +160,7 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   if (!empty && !grad_y && (grad_norm_w || grad_norm_b))
     return fail(CVN_ERR_ARG, "gradients of the norm's parameters without a gradient of y");
   const bool sample = gate_kind == CVN_GATE_SAMPLE;
-  const RnShape t = rn_shape(B, C, HW, sample);
+  const RnShape t = rn_shape(true, B, C, HW, sample);
   if (!workspace || workspace_bytes < cvn_residual_norm_bwd_workspace(B, C, HW, gate_kind))
     return fail(CVN_ERR_WORKSPACE, "residual_norm backward workspace missing or too small");
   const int64_t G = rn_bwd_blocks(t);
@@ -178,20 +196,21 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   s.dgpart = a.dgpart;
   s.C = (int)C;
   s.G = (int)G;
-  s.out[0] = grad_norm_w;
-  s.out[1] = grad_norm_b;
-  s.out[2] = grad_scale;
-  s.out[3] = grad_post_w;
-  s.out[4] = grad_post_b;
+  s.s = res_scale;
+  s.pw = post_w;
+  s.pb = post_b;
+  s.dw = grad_norm_w;
+  s.db = grad_norm_b;
+  s.ds = grad_scale;
+  s.dpw = grad_post_w;
+  s.dpb = grad_post_b;
   if (sample && grad_gate) {
     s.dg = grad_gate;
     s.dg_type = h_type;
     s.tps = t.tps;
   }
-  s.rows = kRnSums * C + (s.dg ? B * C : 0);
-  bool any = s.dg && B > 0;
-  for (int i = 0; i < kRnSums; ++i) any = any || s.out[i];
-  if (!any) return CVN_OK;
+  s.rows = C + (s.dg ? B * C : 0);
+  if (!s.dw && !s.db && !s.ds && !s.dpw && !s.dpb && !s.dg) return CVN_OK;
   hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, s);
   return check_launch("residual_norm sums");
 }

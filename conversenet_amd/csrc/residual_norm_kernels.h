@@ -161,23 +161,25 @@ __global__ void __launch_bounds__(64) k_rn_bwd_any(RnArgs a) {
       }
       if (a.dx && px.ok) ((T*)a.dx)[e.at(c)] = (T)d;
       if (!branch) continue;
+      if (!a.h) {  // no scale, gate and norm: dh is dr in its own type
+        if (px.ok) ((TH*)a.dh)[e.at(c)] = (TH)d;
+        continue;
+      }
       const float gt = e.gate(c), du = a.s ? a.s[c] * d : d, dn = du * gt;
-      if (a.s || a.dg) {
+      const float hh = POST ? e.hhat(c) : rn_ld<TH>(a.h, e.at(c));
+      if (POST) add(2, c, d * gt);
+      add(3, c, d * gt * hh);
+      if (a.dg) {
         const float n = e.n(c);
-        if (a.s) add(2, c, d * (n * gt));
-        if (a.dg) {
-          if (a.gate_full) {
-            if (px.ok) ((TH*)a.dg)[e.at(c)] = (TH)(du * n);
-          } else {
-            const float v = wave_sum(px.ok ? du * n : 0.f);
-            if (lane == 0) a.dgpart[(px.b * a.C + c) * a.tps + tile % a.tps] = v;
-          }
+        if (a.gate_full) {
+          if (px.ok) ((TH*)a.dg)[e.at(c)] = (TH)(du * n);
+        } else {
+          const float v = wave_sum(px.ok ? du * n : 0.f);
+          if (lane == 0) a.dgpart[(px.b * a.C + c) * a.tps + tile % a.tps] = v;
         }
       }
       if (POST) {
-        const float hh = e.hhat(c), g = dn * a.pw[c];
-        add(3, c, dn * hh);
-        add(4, c, dn);
+        const float g = dn * a.pw[c];
         s3 += g;
         s4 = fmaf(g, hh, s4);
       } else if (a.dh && px.ok) {
@@ -200,12 +202,14 @@ __global__ void __launch_bounds__(64) k_rn_bwd_any(RnArgs a) {
 // tensor's part of a tile is read once, V pixels of a channel to a lane, and stays in registers.
 // ------------------------------------------------------------------------------------------------
 
-// A lane's V pixels of a tile.  The last lanes of a sample's last tile move back to its last V pixels: they compute
-// what their neighbours do, store the same, and leave the pixels before `dup` out of their sums.
+// A lane's V pixels of a tile.  The last lanes of a sample's last tile move back to its last V pixels, of which the
+// first `dup` are other lanes' too; `whole`: no lane of the tile does.
 template <int V>
 struct RnLane {
   int64_t base, q, b;  // element of the tile's first pixel at channel 0; index of the lane's first pixel; its sample
-  int off, dup;
+  uint32_t off;        // the lane's first pixel behind base
+  int dup;
+  bool whole;
 
   __device__ __forceinline__ RnLane(const RnArgs& a, int64_t tile, int lane) {
     if (V == 1) {
@@ -213,19 +217,21 @@ struct RnLane {
       base = p.base;
       q = p.q;
       b = p.b;
-      off = p.off;
+      off = (uint32_t)p.off;
       dup = p.ok ? 0 : 1;
+      whole = a.tps ? (tile % a.tps + 1) * 64 <= a.HW : (tile + 1) * 64 <= a.total;
       return;
     }
     b = (uint32_t)tile / (uint32_t)a.tps;
-    const int64_t p0 = (tile - b * a.tps) * (64 * V);
-    off = (int)min((int64_t)(lane * V), a.HW - V - p0);
-    dup = lane * V - off;
+    const int hw = (int)a.HW, first = (int)(tile - b * a.tps) * (64 * V), p0 = min(first, hw - V);
+    const int l = min(first + lane * V, hw - V) - p0;
+    off = (uint32_t)l;
+    dup = first - p0 + lane * V - l;
+    whole = first + 64 * V <= hw;
     base = b * a.C * a.HW + p0;
-    q = b * a.HW + p0 + off;
+    q = b * a.HW + p0 + l;
   }
   __device__ __forceinline__ bool any() const { return dup < V; }
-  __device__ __forceinline__ bool counts(int j) const { return j >= dup; }
 };
 
 // Addresses need only be multiples of the type's size: a lane's V pixels start anywhere in rows of odd length.
@@ -234,8 +240,10 @@ struct RnVec {
   typedef T v __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
 
+// p is uniform, so that the address is a scalar and a 32-bit offset.
 template <class T, int V>
-__device__ __forceinline__ void rn_load(float (&o)[V], const T* p) {
+__device__ __forceinline__ void rn_load(float (&o)[V], const T* p, uint32_t off) {
+  p += off;
   if constexpr (V == 1) {
     o[0] = (float)*p;
   } else {
@@ -246,7 +254,8 @@ __device__ __forceinline__ void rn_load(float (&o)[V], const T* p) {
 }
 
 template <class T, int V>
-__device__ __forceinline__ void rn_store(T* p, const float (&o)[V]) {
+__device__ __forceinline__ void rn_store(T* p, uint32_t off, const float (&o)[V]) {
+  p += off;
   if constexpr (V == 1) {
     *p = (T)o[0];
   } else {
@@ -257,12 +266,24 @@ __device__ __forceinline__ void rn_store(T* p, const float (&o)[V]) {
   }
 }
 
+// The pixels of a lane that are its own.
+template <class T, int V>
+__device__ __forceinline__ void rn_store_own(T* p, const float (&o)[V], const RnLane<V>& px) {
+  if (px.dup == 0) {
+    rn_store<T, V>(p, px.off, o);
+  } else {
+#pragma unroll
+    for (int j = 1; j < V; ++j)
+      if (j >= px.dup) p[px.off + j] = (T)o[j];
+  }
+}
+
 // A wave's channels of a tensor, from channel c0 on; those behind the n of this wave repeat its last.
 template <class T, int V, int NC>
 __device__ __forceinline__ void rn_load_all(float (&o)[NC][V], const void* p, const RnLane<V>& px, int64_t HW, int c0, int n) {
   const T* t = (const T*)p + px.base + c0 * HW;
 #pragma unroll
-  for (int i = 0; i < NC; ++i) rn_load<T, V>(o[i], t + min(i, n - 1) * HW + px.off);
+  for (int i = 0; i < NC; ++i) rn_load<T, V>(o[i], t + min(i, n - 1) * HW, px.off);
 }
 
 // Sums of K values per pixel over the waves of a block, in the order of the waves.  red: two buffers of nw K V 64
@@ -382,13 +403,21 @@ __device__ __forceinline__ float rn_lane_sums(float (&v)[NC], int lane) {
   return v[0] + rn_dpp<kXor1>(v[0]);
 }
 
+// Blocks go to the 8 XCDs in turn; runs of 8 tiles to each keep the lines that two tiles share, where rows do not start
+// on lines, in one L2 (a photo of 321 x 481, 64 channels: 45 -> 40 us; longer runs slow rows that do: 207 -> 219 us with
+// an eighth of 16 x 64 x 256 x 256 to each XCD, against 202-207 us with runs of 8 or 1).
+__device__ __forceinline__ int64_t rn_order(uint32_t b, uint32_t blocks) {
+  if (b >= blocks / 64 * 64) return b;
+  return b / 64 * 64 + b % 8 * 8 + b % 64 / 8;
+}
+
 template <class T, class TH, int V, int NC, bool FULL, bool POST, bool FG>
 __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
   extern __shared__ float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int C = (int)a.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
-  const RnLane<V> px(a, blockIdx.x, lane);
-  const int64_t HW = a.HW, at = px.base + c0 * HW + px.off;
+  const RnLane<V> px(a, rn_order(blockIdx.x, gridDim.x), lane);
+  const int64_t HW = a.HW, at = px.base + c0 * HW;
   int turn = 0;
   float x[NC][V], h[NC][V], g[FG ? NC : 1][V];
   rn_load_all<T, V, NC>(x, a.x, px, HW, c0, n);
@@ -405,8 +434,8 @@ __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
       for (int j = 0; j < V; ++j) h[i][j] = fmaf((h[i][j] - mu[j]) * rho[j], w, b);
     }
     if (a.stats && wave == 0 && px.any()) {
-      rn_store<float, V>(a.stats + 2 * a.total + px.q, mu);
-      rn_store<float, V>(a.stats + 3 * a.total + px.q, rho);
+      rn_store<float, V>(a.stats + 2 * a.total + px.q, 0, mu);
+      rn_store<float, V>(a.stats + 3 * a.total + px.q, 0, rho);
     }
   }
   if (a.h) {
@@ -421,7 +450,7 @@ __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
     if (px.any())
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (i < n) rn_store<T, V>((T*)a.r + at + i * HW, x[i]);
+        if (i < n) rn_store<T, V>((T*)a.r + at + i * HW, px.off, x[i]);
   }
   if (!a.nw) return;
   float mu[V], rho[V];
@@ -434,11 +463,11 @@ __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
     float y[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) y[j] = fmaf((x[i][j] - mu[j]) * rho[j], w, b);
-    rn_store<T, V>((T*)a.y + at + i * HW, y);
+    rn_store<T, V>((T*)a.y + at + i * HW, px.off, y);
   }
   if (a.stats && wave == 0) {
-    rn_store<float, V>(a.stats + px.q, mu);
-    rn_store<float, V>(a.stats + a.total + px.q, rho);
+    rn_store<float, V>(a.stats + px.q, 0, mu);
+    rn_store<float, V>(a.stats + a.total + px.q, 0, rho);
   }
 }
 
@@ -449,15 +478,28 @@ __device__ __forceinline__ void rn_in_loop(P& v) {
   asm volatile("" : "+s"(v));
 }
 
+__device__ __forceinline__ float rn_uniform(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
+template <int V, int NC>
+__device__ __forceinline__ void rn_drop(float (&v)[NC][V], int dup) {
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] = j < dup ? 0.f : v[i][j];
+}
+
 template <class T, class TH, int V, int NC, bool FULL, bool POST, bool FG>
 __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
   extern __shared__ float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int C = (int)a0.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
   const float rC = 1.f / (float)C;
-  const bool norm = a0.nw && a0.gy, branch = a0.dh || a0.dg || a0.s || POST;
+  const bool norm = a0.nw && a0.gy, branch = a0.dh || a0.dg || a0.s || POST, sample = !FG && a0.gate;
+  const int mine = lane / (64 / NC);  // the channel whose sums this lane ends with
   int turn = 0;
-  float acc[kRnSums] = {};  // lane l: the sums of channel c0 + l NC / 64
+  float acc[kRnSums] = {};  // the sums so far of channel c0 + mine
   for (int64_t tile = blockIdx.x; tile < a0.ntiles; tile += gridDim.x) {
     RnArgs a = a0;
     rn_in_loop(a.HW);
@@ -467,78 +509,95 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     rn_in_loop(a.pb);
     const int64_t HW = a.HW;
     const RnLane<V> px(a, tile, lane);
-    const int64_t at = px.base + c0 * HW + px.off;
+    const int64_t at = px.base + c0 * HW;
     float r[NC][V], d[NC][V], e[NC][V], h[NC][V], g[FG ? NC : 1][V];
+    float mu[V], rho[V], mh[V], rh[V];
     if (norm) {
       rn_load_all<T, V, NC>(r, a.x, px, HW, c0, n);
       rn_load_all<T, V, NC>(d, a.gy, px, HW, c0, n);
+      rn_load<float, V>(mu, a.stats + px.q, 0);
+      rn_load<float, V>(rho, a.stats + a.total + px.q, 0);
     }
     if (a.gr) rn_load_all<T, V, NC>(e, a.gr, px, HW, c0, n);
     if (a.h) rn_load_all<TH, V, NC>(h, a.h, px, HW, c0, n);
-    if constexpr (FG) rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
-    float mh[V], rh[V];
+    if constexpr (FG && sizeof(T) < 4) rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
     if constexpr (POST) {
-      rn_load<float, V>(mh, a.stats + 2 * a.total + px.q);
-      rn_load<float, V>(rh, a.stats + 3 * a.total + px.q);
+      rn_load<float, V>(mh, a.stats + 2 * a.total + px.q, 0);
+      rn_load<float, V>(rh, a.stats + 3 * a.total + px.q, 0);
+    }
+    float k[NC];  // scale and gate of a channel
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = c0 + min(i, n - 1);
+      k[i] = sample ? rn_uniform(rn_ld<TH>(a.gate, px.b * C + c)) : 1.f;
+      if (a.s) k[i] *= a.s[c];
+    }
+    if (!px.whole) {  // pixels of other lanes: gradients of 0, and finite values beside them
+      if (norm) rn_drop<V, NC>(r, px.dup), rn_drop<V, NC>(d, px.dup);
+      if (a.gr) rn_drop<V, NC>(e, px.dup);
+      if (a.h) rn_drop<V, NC>(h, px.dup);
+      if constexpr (FG && sizeof(T) < 4) rn_drop<V, NC>(g, px.dup);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < px.dup) mu[j] = mh[j] = 0.f, rho[j] = rh[j] = 1.f;
+    }
+    if constexpr (POST) {
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mh[j]) * rh[j];  // hhat
     }
-    float gs[NC];  // a gate per sample
-    if constexpr (!FG) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) gs[i] = a.gate ? rn_ld<TH>(a.gate, px.b * C + c0 + min(i, n - 1)) : 1.f;
-    }
-    auto gate = [&](int i, int j) { return FG ? g[FG ? i : 0][j] : gs[i]; };
-    auto nv = [&](int i, int j, int c) { return POST ? fmaf(h[i][j], a.pw[c], a.pb[c]) : h[i][j]; };
-    float t[NC];
-    if (norm) {
-      float mu[V], rho[V], s[2][V] = {};
-      rn_load<float, V>(mu, a.stats + px.q);
-      rn_load<float, V>(rho, a.stats + a.total + px.q);
-      if (sizeof(T) < 4 && a.h) {  // x: r as the forward had it
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int c = c0 + min(i, n - 1);
-          const float sc = a.s ? a.s[c] : 1.f;
-#pragma unroll
-          for (int j = 0; j < V; ++j) r[i][j] = fmaf(sc, nv(i, j, c) * gate(i, j), r[i][j]);
-        }
+    // A gate per element is loaded behind the norm's sums, for a 16-bit stream (whose r needs it too) once more: held
+    // from the start it would not fit the registers of 16 waves on a CU.
+    auto load_gate = [&]() {
+      if constexpr (FG) {
+        asm volatile("" ::: "memory");
+        rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
+        if (!px.whole) rn_drop<V, NC>(g, px.dup);
       }
+    };
+    if (norm) {
+      float s[2][V] = {}, sw[NC], sb[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const float w = a.nw[c0 + min(i, n - 1)];
-        float tw = 0.f;
+        const int c = c0 + min(i, n - 1);
+        const float w = i < n ? a.nw[c] : 0.f;
+        sw[i] = sb[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+          if (sizeof(T) < 4 && a.h) {  // x: r as the forward had it
+            const float nv = POST ? fmaf(h[i][j], a.pw[c], a.pb[c]) : h[i][j];
+            r[i][j] = fmaf(k[i], FG ? nv * g[FG ? i : 0][j] : nv, r[i][j]);
+          }
           r[i][j] = (r[i][j] - mu[j]) * rho[j];  // rhat
-          tw += px.counts(j) ? d[i][j] * r[i][j] : 0.f;
-          const float gw = i < n ? d[i][j] * w : 0.f;
-          s[0][j] += gw;
-          s[1][j] = fmaf(gw, i < n ? r[i][j] : 0.f, s[1][j]);
+          sw[i] = fmaf(d[i][j], r[i][j], sw[i]);
+          sb[i] += d[i][j];
+          d[i][j] *= w;
+          s[0][j] += d[i][j];
+          s[1][j] = fmaf(d[i][j], r[i][j], s[1][j]);
         }
-        t[i] = tw;
       }
-      acc[0] += rn_lane_sums<NC>(t, lane);
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        t[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) t[i] += px.counts(j) ? d[i][j] : 0.f;
-      }
-      acc[1] += rn_lane_sums<NC>(t, lane);
+      acc[0] += rn_lane_sums<NC>(sw, lane);
+      acc[1] += rn_lane_sums<NC>(sb, lane);
+      load_gate();
       rn_block_sums<V>(red, turn, nw, wave, lane, s);
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const float w = a.nw[c0 + min(i, n - 1)];
+      for (int j = 0; j < V; ++j) {
+        s[0][j] *= rC;
+        s[1][j] *= rC;
+      }
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float v = rho[j] * (d[i][j] * w - s[0][j] * rC - r[i][j] * (s[1][j] * rC));
-          d[i][j] = a.gr ? e[i][j] + v : v;
-        }
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] = fmaf(-r[i][j], s[1][j], d[i][j] - s[0][j]) * rho[j];
+      if (a.gr) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[i][j] += e[i][j];
       }
     } else {
+      load_gate();
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -547,118 +606,109 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     if (a.dx && px.any())
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (i < n) rn_store<T, V>((T*)a.dx + at + i * HW, d[i]);
+        if (i < n) rn_store_own<T, V>((T*)a.dx + at + i * HW, d[i], px);
     if (!branch) continue;
-    if (a.s) {
+    if (FG && a.dg && px.any()) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int c = c0 + min(i, n - 1);
-        const float sc = a.s[c];
-        t[i] = 0.f;
+        if (i >= n) break;
+        float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          t[i] += px.counts(j) ? d[i][j] * (nv(i, j, c) * gate(i, j)) : 0.f;
-          d[i][j] *= sc;
-        }
-      }
-      acc[2] += rn_lane_sums<NC>(t, lane);
-    }
-    if (a.dg) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + min(i, n - 1);
-        float dg[V];
-        t[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          dg[j] = d[i][j] * nv(i, j, c);
-          t[i] += px.counts(j) ? dg[j] : 0.f;
-        }
-        if (FG && i < n && px.any()) rn_store<TH, V>((TH*)a.dg + at + i * HW, dg);
-      }
-      if constexpr (!FG) {
-        const float v = rn_lane_sums<NC>(t, lane);
-        const int i = lane / (64 / NC);
-        if (lane % (64 / NC) == 0 && i < n) a.dgpart[(px.b * C + c0 + i) * a.tps + tile % a.tps] = v;
+        for (int j = 0; j < V; ++j) o[j] = k[i] * d[i][j] * (POST ? fmaf(h[i][j], a.pw[c0 + i], a.pb[c0 + i]) : h[i][j]);
+        rn_store_own<TH, V>((TH*)a.dg + at + i * HW, o, px);
       }
     }
+    float s[2][V] = {}, sa[NC], sh[NC];
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+    for (int i = 0; i < NC; ++i) {
+      sa[i] = sh[i] = 0.f;
+      const float kp = i < n ? (POST ? k[i] * a.pw[c0 + i] : k[i]) : 0.f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[i][j] *= gate(i, j);  // dn
+      for (int j = 0; j < V; ++j) {
+        if constexpr (FG) d[i][j] *= g[FG ? i : 0][j];
+        if (POST) sa[i] += d[i][j];
+        if (a.h) sh[i] = fmaf(d[i][j], h[i][j], sh[i]);
+        d[i][j] *= kp;  // dn wp
+        if (POST) {
+          s[0][j] += d[i][j];
+          s[1][j] = fmaf(d[i][j], h[i][j], s[1][j]);
+        }
+      }
+    }
+    if (a.h) {
+      const int c = c0 + min(mine, n - 1);
+      const float va = POST ? rn_lane_sums<NC>(sa, lane) : 0.f, vh = rn_lane_sums<NC>(sh, lane);
+      const float gt = sample ? rn_ld<TH>(a.gate, px.b * C + c) : 1.f;
+      acc[2] = fmaf(gt, va, acc[2]);
+      acc[3] = fmaf(gt, vh, acc[3]);
+      if (sample && a.dg && lane % (64 / NC) == 0 && mine < n) {
+        const float v = POST ? fmaf(a.pw[c], vh, a.pb[c] * va) : vh;
+        a.dgpart[(px.b * C + c) * a.tps + tile % a.tps] = a.s ? a.s[c] * v : v;
+      }
+    }
     if constexpr (POST) {
-      float s[2][V] = {};
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        t[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) t[i] += px.counts(j) ? d[i][j] * h[i][j] : 0.f;
-      }
-      acc[3] += rn_lane_sums<NC>(t, lane);
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const float w = a.pw[c0 + min(i, n - 1)];
-        t[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          t[i] += px.counts(j) ? d[i][j] : 0.f;
-          d[i][j] *= w;
-          const float gw = i < n ? d[i][j] : 0.f;
-          s[0][j] += gw;
-          s[1][j] = fmaf(gw, i < n ? h[i][j] : 0.f, s[1][j]);
-        }
-      }
-      acc[4] += rn_lane_sums<NC>(t, lane);
       rn_block_sums<V>(red, turn, nw, wave, lane, s);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s[0][j] *= rC;
+        s[1][j] *= rC;
+      }
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] = rh[j] * (d[i][j] - s[0][j] * rC - h[i][j] * (s[1][j] * rC));
+        for (int j = 0; j < V; ++j) d[i][j] = fmaf(-h[i][j], s[1][j], d[i][j] - s[0][j]) * rh[j];
     }
     if (a.dh && px.any())
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (i < n) rn_store<TH, V>((TH*)a.dh + at + i * HW, d[i]);
+        if (i < n) rn_store_own<TH, V>((TH*)a.dh + at + i * HW, d[i], px);
   }
-  const int i = lane / (64 / NC);
-  if (lane % (64 / NC) == 0 && i < n)
+  if (lane % (64 / NC) == 0 && mine < n)
 #pragma unroll
-    for (int k = 0; k < kRnSums; ++k) a0.part[((int64_t)k * C + c0 + i) * gridDim.x + blockIdx.x] = acc[k];
+    for (int q = 0; q < kRnSums; ++q) a0.part[((int64_t)q * C + c0 + mine) * gridDim.x + blockIdx.x] = acc[q];
 }
 
-template <class T, class TH, int V, int NC, bool FULL>
-int rn_launch_tile(const RnArgs& a, int64_t blocks, bool bwd, hipStream_t st) {
+template <bool BWD, class T, class TH, int V, int NC, bool FULL>
+int rn_launch_tile(const RnArgs& a, int64_t blocks, hipStream_t st) {
   const int nw = (int)((a.C + NC - 1) / NC);
   const size_t lds = nw == 1 ? 0 : sizeof(float) * 2 * nw * 2 * V * 64;
   const bool fg = a.gate && a.gate_full;
-  auto k = bwd ? (a.pw ? (fg ? k_rn_bwd<T, TH, V, NC, FULL, true, true> : k_rn_bwd<T, TH, V, NC, FULL, true, false>)
-                       : (fg ? k_rn_bwd<T, TH, V, NC, FULL, false, true> : k_rn_bwd<T, TH, V, NC, FULL, false, false>))
-               : (a.pw ? (fg ? k_rn_fwd<T, TH, V, NC, FULL, true, true> : k_rn_fwd<T, TH, V, NC, FULL, true, false>)
-                       : (fg ? k_rn_fwd<T, TH, V, NC, FULL, false, true> : k_rn_fwd<T, TH, V, NC, FULL, false, false>));
+  void (*k)(RnArgs);
+  if constexpr (BWD)
+    k = a.pw ? (fg ? k_rn_bwd<T, TH, V, NC, FULL, true, true> : k_rn_bwd<T, TH, V, NC, FULL, true, false>)
+             : (fg ? k_rn_bwd<T, TH, V, NC, FULL, false, true> : k_rn_bwd<T, TH, V, NC, FULL, false, false>);
+  else
+    k = a.pw ? (fg ? k_rn_fwd<T, TH, V, NC, FULL, true, true> : k_rn_fwd<T, TH, V, NC, FULL, true, false>)
+             : (fg ? k_rn_fwd<T, TH, V, NC, FULL, false, true> : k_rn_fwd<T, TH, V, NC, FULL, false, false>);
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * nw), lds, st, a);
-  return check_launch(bwd ? "residual_norm backward" : "residual_norm");
-}
-
-template <class T, class TH>
-int rn_launch(const RnArgs& a, const RnShape& s, int64_t blocks, bool bwd, hipStream_t st) {
-  switch (s.px) {
-    case 2: return rn_launch_tile<T, TH, 2, 8, true>(a, blocks, bwd, st);
-    case 1: return rn_launch_tile<T, TH, 1, 16, false>(a, blocks, bwd, st);
-  }
-  auto k = bwd ? (a.pw ? k_rn_bwd_any<T, TH, true> : k_rn_bwd_any<T, TH, false>)
-               : (a.pw ? k_rn_fwd_any<T, TH, true> : k_rn_fwd_any<T, TH, false>);
-  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64), 0, st, a);
-  return check_launch(bwd ? "residual_norm backward" : "residual_norm");
+  return check_launch(BWD ? "residual_norm backward" : "residual_norm");
 }
 
 template <class T, class TH>
 int rn_launch_fwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
-  return rn_launch<T, TH>(a, s, s.ntiles, false, st);
+  if (s.px == 0) {
+    auto k = a.pw ? k_rn_fwd_any<T, TH, true> : k_rn_fwd_any<T, TH, false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)s.ntiles), dim3(64), 0, st, a);
+    return check_launch("residual_norm");
+  }
+  if (s.px == 2)
+    return s.ch == 8 ? rn_launch_tile<false, T, TH, 2, 8, true>(a, s.ntiles, st)
+                     : rn_launch_tile<false, T, TH, 2, 16, true>(a, s.ntiles, st);
+  return rn_launch_tile<false, T, TH, 1, 16, false>(a, s.ntiles, st);
 }
 
 template <class T, class TH>
 int rn_launch_bwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
-  return rn_launch<T, TH>(a, s, rn_bwd_blocks(s), true, st);
+  const int64_t blocks = rn_bwd_blocks(s);
+  if (s.px == 0) {
+    auto k = a.pw ? k_rn_bwd_any<T, TH, true> : k_rn_bwd_any<T, TH, false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64), 0, st, a);
+    return check_launch("residual_norm backward");
+  }
+  if (s.px == 2) return rn_launch_tile<true, T, TH, 2, 8, true>(a, blocks, st);
+  if (s.ch == 8) return rn_launch_tile<true, T, TH, 1, 8, false>(a, blocks, st);
+  return a.C % 16 ? rn_launch_tile<true, T, TH, 1, 16, false>(a, blocks, st)
+                  : rn_launch_tile<true, T, TH, 1, 16, true>(a, blocks, st);
 }
 
 }  // namespace
