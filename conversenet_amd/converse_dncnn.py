@@ -7,7 +7,7 @@ checkpoints load with strict=True.  The 1x1 head (1->64) and tail (64->1) run on
 import torch.nn as nn
 
 from . import functional
-from .util_converse import ConverseBlock, _hip_eligible, run_blocks
+from .util_converse import ConverseBlock, _hip_eligible, _plain, run_blocks
 
 
 class ConverseDnCNN(nn.Module):
@@ -34,6 +34,6 @@ class ConverseDnCNN(nn.Module):
             x = run_blocks(self.m_body, x)
             return functional.conv1x1(x, t.weight, t.bias)
         x = self.m_head(x)
-        x = self.m_body(x)
+        x = run_blocks(self.m_body, x) if type(self.m_body) is nn.Sequential and _plain(self.m_body) else self.m_body(x)
         x = self.m_tail(x)
         return x

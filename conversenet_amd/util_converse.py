@@ -13,7 +13,8 @@ Dispatch (mirrors the reference's backend selection, util_converse.py:150-169):
   * $CONVERSE2D_BACKEND overrides the module's backend (:150).
 A forward that autograd must differentiate runs the library's forward and backward kernels
 (functional.Converse2DFunction) where the backward supports the configuration, and the composition
-otherwise; the LayerNorm / 1x1 kernels are forward-only (the composition runs under autograd).
+otherwise.  So do channels-first LayerNorms and the blocks' scaled residuals (functional.residual_norm_train, each
+residual fused with the norm behind it); the 1x1 kernels are forward-only (torch's convolutions run under autograd).
 """
 from __future__ import annotations
 
@@ -21,8 +22,10 @@ import os
 from collections import OrderedDict
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import _lib, composite, functional
 from . import op_registry  # noqa: F401  (registers torch.ops.converse2d)
@@ -74,6 +77,37 @@ def _hip_grad_eligible(x, weight, bias, scale, padding, padding_mode) -> bool:
     return functional.supported(x, weight, scale, padding, x.requires_grad, weight.requires_grad or bias.requires_grad)
 
 
+def _plain(*ms) -> bool:
+    """True when calling these modules runs their forward alone: no hook observes or changes it."""
+    return not _has_any_global_hook() and not any(
+        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in ms)
+
+
+def _norm_grad_eligible(x, *params) -> bool:
+    """True when a norm (and residual) that autograd must differentiate runs on the library's kernels: contiguous fp32
+    (B,C,H,W) HIP tensors within cvn_residual_norm_fwd's limits, a weight per channel, and plain backward: function
+    transforms, forward-mode gradients and tracing see the composition."""
+    ts = (x, *params)
+    if not all(t.is_cuda and t.dtype is torch.float32 for t in ts):
+        return False
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)):
+        return False
+    if type(x) not in _TENSORS or not all(type(p) in _TENSORS for p in params):
+        return False
+    if torch._C._are_functorch_transforms_active() or fwAD._current_level >= 0 or torch.compiler.is_compiling() \
+            or torch.jit.is_tracing():
+        return False
+    if x.dim() != 4 or not x.is_contiguous() or not 0 < x.shape[1] <= 65536 or x.numel() // x.shape[1] >= 1 << 31:
+        return False
+    if any(p.numel() != x.shape[1] or p.device != x.device for p in params):
+        return False
+    _lib.load()
+    return True
+
+
+_TENSORS = (torch.Tensor, nn.Parameter)
+
+
 """
 # --------------------------------------------
 # LayerNorm for Vision Normalization
@@ -99,6 +133,8 @@ class LayerNorm(nn.Module):
             return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
         if _hip_eligible(x, self.weight, self.bias) and x.dim() >= 2:
             return functional.layernorm_cf(x, self.weight, self.bias, self.eps)
+        if _norm_grad_eligible(x, self.weight, self.bias):
+            return functional.layernorm_cf_train(x, self.weight, self.bias, self.eps)
         u = x.mean(1, keepdim=True)
         s = (x - u).pow(2).mean(1, keepdim=True)
         x = (x - u) / torch.sqrt(s + self.eps)
@@ -298,13 +334,56 @@ def _fused_block_forward(blk, x, alpha1=None, alpha2=None):
     return _block_tail(parts, _block_converse(parts, t, None if gin else "gelu"), x, t_act="gelu" if gin else None)[0]
 
 
+def _trainable(blk, x) -> bool:
+    """True when a block's residuals and norms run on the library under autograd (_block_train)."""
+    if type(blk) not in (ConverseBlock, ConverseBlockAlphaVariant):
+        return False
+    seqs = (blk.conv1, blk.conv2)
+    if not all(type(s) is nn.Sequential and len(s) > 1 and type(s[0]) is LayerNorm for s in seqs):
+        return False
+    lns = (blk.conv1[0], blk.conv2[0])
+    params = [p for n in lns for p in (n.weight, n.bias)]
+    if hasattr(blk, "alpha1"):
+        params += [blk.alpha1, blk.alpha2]
+    cv = blk.conv1[3] if len(blk.conv1) > 3 else None
+    return (all(n.data_format == "channels_first" for n in lns) and _plain(*seqs, *lns)
+            and _backend(getattr(cv, "backend", "auto")) != "pytorch" and _norm_grad_eligible(x, *params))
+
+
+def _add_norm(x, h, alpha, ln):
+    """x + alpha * h and its LayerNorm (None without ln), differentiable."""
+    if alpha is None and ln is None or h.shape != x.shape or h.dtype not in _lib.TYPES or type(h) not in _TENSORS:
+        x = (h if alpha is None else alpha * h) + x
+        return x, None if ln is None else ln(x)
+    return functional.residual_norm_train(x, h, None if ln is None else (ln.weight, ln.bias, ln.eps), alpha)
+
+
+def _block_train(blk, x, n=None, next_ln=None):
+    """A block under autograd, each residual fused with the norm behind it: (output, next_ln of it).  n: the block's first
+    norm of x, where the previous block has it."""
+    if n is None:
+        n = functional.layernorm_cf_train(x, blk.conv1[0].weight, blk.conv1[0].bias, blk.conv1[0].eps)
+    a1, a2 = (blk.alpha1, blk.alpha2) if hasattr(blk, "alpha1") else (None, None)
+    for m in list(blk.conv1)[1:]:
+        n = m(n)
+    x, n = _add_norm(x, n, a1, blk.conv2[0])
+    for m in list(blk.conv2)[1:]:
+        n = m(n)
+    return _add_norm(x, n, a2, next_ln)
+
+
 def run_blocks(blocks, x):
     """A chain of ConverseBlocks (util_converse.py:253-323 applied in sequence, as in the bodies of
     converse_dncnn.py:24 and converse_usrnet.py:19-33).  On the HIP path each block's tail kernel
-    also computes the next block's LN -> 1x1 -> GELU, so a block's output is read once; otherwise the
-    blocks run one by one."""
+    also computes the next block's LN -> 1x1 -> GELU, so a block's output is read once; under autograd the last
+    residual of a block and the first norm of the next are one operation; otherwise the blocks run one by one."""
     blocks = list(blocks)
     if not blocks:
+        return x
+    if torch.is_grad_enabled() and all(_trainable(b, x) and _plain(b) for b in blocks):
+        n = None
+        for i, b in enumerate(blocks):
+            x, n = _block_train(b, x, n, blocks[i + 1].conv1[0] if i + 1 < len(blocks) else None)
         return x
     parts = [_block_parts(b) if _hip_eligible(x, *_block_params(b)) else None for b in blocks]
     if any(p is None for p in parts) or not all(_parts_supported(p, x) for p in parts):
@@ -348,6 +427,8 @@ class ConverseBlock(nn.Module):
             y = _fused_block_forward(self, x)
             if y is not None:
                 return y
+        if torch.is_grad_enabled() and _trainable(self, x):
+            return _block_train(self, x)[0]
         x = self.conv1(x) + x
         x = self.conv2(x) + x
         return x
@@ -379,6 +460,8 @@ class ConverseBlockAlphaVariant(nn.Module):
             y = _fused_block_forward(self, x, self.alpha1, self.alpha2)
             if y is not None:
                 return y
+        if torch.is_grad_enabled() and _trainable(self, x):
+            return _block_train(self, x)[0]
         x = self.alpha1 * self.conv1(x) + x
         x = self.alpha2 * self.conv2(x) + x
         return x
