@@ -77,10 +77,11 @@ inline RnShape rn_shape(bool bwd, int64_t B, int64_t C, int64_t HW, bool gate_sa
   return s;
 }
 
-// Blocks of the backward, which each keep a row of partial sums: what the CUs hold at 16 waves, and as even a number of
-// tiles for each as can be.
+// Blocks of the backward, which each keep a row of partial sums: what the CUs hold at once (16 waves of its kernels with
+// 128 registers, 20 of those with 8 channels of one pixel), and as even a number of tiles for each as can be.
 inline int64_t rn_bwd_blocks(const RnShape& s) {
-  const int64_t most = s.px ? 4096 / s.waves : 2048;
+  const int resident = s.px == 1 && s.ch == 8 ? 20 : 16;
+  const int64_t most = s.px ? 256 * (resident / s.waves) : 2048;
   if (s.ntiles <= most) return s.ntiles;
   const int64_t per = (s.ntiles + most - 1) / most;
   return (s.ntiles + per - 1) / per;

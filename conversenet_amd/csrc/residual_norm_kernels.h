@@ -239,6 +239,10 @@ template <class T, int V>
 struct RnVec {
   typedef T v __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
+template <class T>
+struct RnVec<T, 1> {
+  typedef T v;
+};
 
 // p is uniform, so that the address is a scalar and a 32-bit offset.
 template <class T, int V>
@@ -284,6 +288,20 @@ __device__ __forceinline__ void rn_load_all(float (&o)[NC][V], const void* p, co
   const T* t = (const T*)p + px.base + c0 * HW;
 #pragma unroll
   for (int i = 0; i < NC; ++i) rn_load<T, V>(o[i], t + min(i, n - 1) * HW, px.off);
+}
+
+// The same as it was stored.
+template <class T, int V, int NC>
+__device__ __forceinline__ void rn_load_raw(typename RnVec<T, V>::v (&o)[NC], const void* p, const RnLane<V>& px, int64_t HW,
+                                            int c0, int n) {
+  const T* t = (const T*)p + px.base + c0 * HW;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) o[i] = *(const typename RnVec<T, V>::v*)(t + min(i, n - 1) * HW + px.off);
+}
+template <class T, int V>
+__device__ __forceinline__ float rn_at(const typename RnVec<T, V>::v& v, int j) {
+  if constexpr (V == 1) return (float)v;
+  else return (float)v[j];
 }
 
 // Sums of K values per pixel over the waves of a block, in the order of the waves.  red: two buffers of nw K V 64
@@ -510,7 +528,9 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     const int64_t HW = a.HW;
     const RnLane<V> px(a, tile, lane);
     const int64_t at = px.base + c0 * HW;
-    float r[NC][V], d[NC][V], e[NC][V], h[NC][V], g[FG ? NC : 1][V];
+    float r[NC][V], d[NC][V], h[NC][V];
+    typename RnVec<T, V>::v e[NC];             // gr and the gate as they were stored, until they are needed
+    typename RnVec<TH, V>::v g[FG ? NC : 1];
     float mu[V], rho[V], mh[V], rh[V];
     if (norm) {
       rn_load_all<T, V, NC>(r, a.x, px, HW, c0, n);
@@ -518,9 +538,9 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
       rn_load<float, V>(mu, a.stats + px.q, 0);
       rn_load<float, V>(rho, a.stats + a.total + px.q, 0);
     }
-    if (a.gr) rn_load_all<T, V, NC>(e, a.gr, px, HW, c0, n);
+    if (a.gr) rn_load_raw<T, V, NC>(e, a.gr, px, HW, c0, n);
     if (a.h) rn_load_all<TH, V, NC>(h, a.h, px, HW, c0, n);
-    if constexpr (FG && sizeof(T) < 4) rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
+    if constexpr (FG && sizeof(T) < 4) rn_load_raw<TH, V, NC>(g, a.gate, px, HW, c0, n);
     if constexpr (POST) {
       rn_load<float, V>(mh, a.stats + 2 * a.total + px.q, 0);
       rn_load<float, V>(rh, a.stats + 3 * a.total + px.q, 0);
@@ -534,9 +554,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     }
     if (!px.whole) {  // pixels of other lanes: gradients of 0, and finite values beside them
       if (norm) rn_drop<V, NC>(r, px.dup), rn_drop<V, NC>(d, px.dup);
-      if (a.gr) rn_drop<V, NC>(e, px.dup);
       if (a.h) rn_drop<V, NC>(h, px.dup);
-      if constexpr (FG && sizeof(T) < 4) rn_drop<V, NC>(g, px.dup);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (j < px.dup) mu[j] = mh[j] = 0.f, rho[j] = rh[j] = 1.f;
@@ -547,38 +565,43 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
 #pragma unroll
         for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mh[j]) * rh[j];  // hhat
     }
-    // A gate per element is loaded behind the norm's sums, for a 16-bit stream (whose r needs it too) once more: held
-    // from the start it would not fit the registers of 16 waves on a CU.
+    auto gr = [&](int i, int j) { return j < px.dup ? 0.f : rn_at<T, V>(e[i], j); };
+    auto gate = [&](int i, int j) { return j < px.dup ? 0.f : rn_at<TH, V>(g[FG ? i : 0], j); };
+    // With float32 x and r a gate is loaded behind the norm's sums: held from the start it would not fit the registers of
+    // 16 waves on a CU (4 x 128 x 16384, float32 and bfloat16: 57 us, 71 us spilt).
     auto load_gate = [&]() {
-      if constexpr (FG) {
-        asm volatile("" ::: "memory");
-        rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
-        if (!px.whole) rn_drop<V, NC>(g, px.dup);
-      }
+      if constexpr (FG && sizeof(T) == 4) rn_load_raw<TH, V, NC>(g, a.gate, px, HW, c0, n);
     };
     if (norm) {
-      float s[2][V] = {}, sw[NC], sb[NC];
+      float s[2][V] = {}, t[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const int c = c0 + min(i, n - 1);
-        const float w = i < n ? a.nw[c] : 0.f;
-        sw[i] = sb[i] = 0.f;
+        t[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (sizeof(T) < 4 && a.h) {  // x: r as the forward had it
             const float nv = POST ? fmaf(h[i][j], a.pw[c], a.pb[c]) : h[i][j];
-            r[i][j] = fmaf(k[i], FG ? nv * g[FG ? i : 0][j] : nv, r[i][j]);
+            r[i][j] = fmaf(k[i], FG ? nv * gate(i, j) : nv, r[i][j]);
           }
           r[i][j] = (r[i][j] - mu[j]) * rho[j];  // rhat
-          sw[i] = fmaf(d[i][j], r[i][j], sw[i]);
-          sb[i] += d[i][j];
+          t[i] = fmaf(d[i][j], r[i][j], t[i]);
+        }
+      }
+      acc[0] += rn_lane_sums<NC>(t, lane);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const float w = i < n ? a.nw[c0 + min(i, n - 1)] : 0.f;
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          t[i] += d[i][j];
           d[i][j] *= w;
           s[0][j] += d[i][j];
           s[1][j] = fmaf(d[i][j], r[i][j], s[1][j]);
         }
       }
-      acc[0] += rn_lane_sums<NC>(sw, lane);
-      acc[1] += rn_lane_sums<NC>(sb, lane);
+      acc[1] += rn_lane_sums<NC>(t, lane);
       load_gate();
       rn_block_sums<V>(red, turn, nw, wave, lane, s);
 #pragma unroll
@@ -594,14 +617,14 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) d[i][j] += e[i][j];
+          for (int j = 0; j < V; ++j) d[i][j] += gr(i, j);
       }
     } else {
       load_gate();
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] = e[i][j];
+        for (int j = 0; j < V; ++j) d[i][j] = gr(i, j);
     }
     if (a.dx && px.any())
 #pragma unroll
@@ -618,32 +641,50 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
         rn_store_own<TH, V>((TH*)a.dg + at + i * HW, o, px);
       }
     }
-    float s[2][V] = {}, sa[NC], sh[NC];
+    if constexpr (FG) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] *= gate(i, j);
+    }
+    if (a.h) {
+      const int c = c0 + min(mine, n - 1);
+      const float gt = sample ? rn_ld<TH>(a.gate, px.b * C + c) : 1.f;
+      float t[NC], va = 0.f;
+      if constexpr (POST) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          t[i] = 0.f;
+#pragma unroll
+          for (int j = 0; j < V; ++j) t[i] += d[i][j];
+        }
+        va = rn_lane_sums<NC>(t, lane);
+        acc[2] = fmaf(gt, va, acc[2]);
+      }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        t[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[i] = fmaf(d[i][j], h[i][j], t[i]);
+      }
+      const float vh = rn_lane_sums<NC>(t, lane);
+      acc[3] = fmaf(gt, vh, acc[3]);
+      if (sample && a.dg && lane % (64 / NC) == 0 && mine < n) {
+        const float v = POST ? fmaf(a.pw[c], vh, a.pb[c] * va) : vh;
+        a.dgpart[(px.b * C + c) * a.tps + tile % a.tps] = a.s ? a.s[c] * v : v;
+      }
+    }
+    float s[2][V] = {};
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      sa[i] = sh[i] = 0.f;
       const float kp = i < n ? (POST ? k[i] * a.pw[c0 + i] : k[i]) : 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if constexpr (FG) d[i][j] *= g[FG ? i : 0][j];
-        if (POST) sa[i] += d[i][j];
-        if (a.h) sh[i] = fmaf(d[i][j], h[i][j], sh[i]);
         d[i][j] *= kp;  // dn wp
         if (POST) {
           s[0][j] += d[i][j];
           s[1][j] = fmaf(d[i][j], h[i][j], s[1][j]);
         }
-      }
-    }
-    if (a.h) {
-      const int c = c0 + min(mine, n - 1);
-      const float va = POST ? rn_lane_sums<NC>(sa, lane) : 0.f, vh = rn_lane_sums<NC>(sh, lane);
-      const float gt = sample ? rn_ld<TH>(a.gate, px.b * C + c) : 1.f;
-      acc[2] = fmaf(gt, va, acc[2]);
-      acc[3] = fmaf(gt, vh, acc[3]);
-      if (sample && a.dg && lane % (64 / NC) == 0 && mine < n) {
-        const float v = POST ? fmaf(a.pw[c], vh, a.pb[c] * va) : vh;
-        a.dgpart[(px.b * C + c) * a.tps + tile % a.tps] = a.s ? a.s[c] * v : v;
       }
     }
     if constexpr (POST) {
