@@ -199,7 +199,13 @@ __global__ void __launch_bounds__(64) k_rn_bwd_any(RnArgs a) {
 
 // ------------------------------------------------------------------------------------------------
 // Up to 256 channels: a block per tile of 64 V pixels, its channels spread over the waves, NC to a wave, so that a
-// tensor's part of a tile is read once, V pixels of a channel to a lane, and stays in registers.
+// tensor's part of a tile is read once, V pixels of a channel to a lane, and stays in registers (with a thread per
+// pixel and the channels read again, as above, 16 x 64 x 256 x 256 takes 2.7 ms forward and backward).  Memory is the
+// bound: at that size, float32 with a scale, the forward moves 1.07 GB in 198-208 us (5.2 TB/s, a copy's rate) and the
+// backward 1.61 GB in 308-330 us (4.9-5.2).  With 16-bit tensors the joins and conversions show: 8 x 64 x 256 x 256 bf16,
+// per-sample gate and both norms, 64 us forward (4.2 TB/s) and 103 us backward (3.9); without gate and branch norm 54
+// and 91.  At 128 channels a block of the backward is all a CU holds: 4 x 128 x 128 x 128, float32 with a bf16 branch and
+// gate, 28 us forward (4.8 TB/s) and 54 us backward (3.7).
 // ------------------------------------------------------------------------------------------------
 
 // A lane's V pixels of a tile.  The last lanes of a sample's last tile move back to its last V pixels, of which the
@@ -304,48 +310,72 @@ __device__ __forceinline__ float rn_at(const typename RnVec<T, V>::v& v, int j) 
   else return (float)v[j];
 }
 
-// Sums of K values per pixel over the waves of a block, in the order of the waves.  red: two buffers of nw K V 64
-// floats, taken in turn, so that one barrier a time is enough: a buffer is written again only after the barrier of the
+template <int V>
+__device__ __forceinline__ void rn_put(float* p, const float (&v)[V]) {
+  if constexpr (V == 1) *p = v[0];
+  else *(float2*)p = make_float2(v[0], v[1]);
+}
+template <int V>
+__device__ __forceinline__ void rn_get(float (&v)[V], const float* p) {
+  if constexpr (V == 1) {
+    v[0] = *p;
+  } else {
+    const float2 t = *(const float2*)p;
+    v[0] = t.x;
+    v[1] = t.y;
+  }
+}
+
+// Two values per pixel over the waves of a block, which each wave joins in the order of the waves.  red: two buffers of
+// nw 2 V 64 floats, taken in turn, so that one barrier a time is enough: a buffer is written again only after the barrier of the
 // other, which a wave reaches after its reads.
-template <int K, int V>
-__device__ __forceinline__ void rn_exchange(float* red, int& turn, int nw, int wave, int lane, const float (&v)[K][V]) {
-  float* o = red + (turn * nw + wave) * (K * V * 64) + lane;
+template <int V>
+__device__ __forceinline__ const float* rn_exchange(float* red, int& turn, int nw, int wave, int lane, const float (&v)[2][V]) {
+  float* buf = red + turn * nw * (2 * V * 64) + lane * V;
+  turn ^= 1;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[(k * V + j) * 64] = v[k][j];
+  for (int k = 0; k < 2; ++k) rn_put<V>(buf + (2 * wave + k) * (V * 64), v[k]);
   __syncthreads();
+  return buf;
 }
 
 template <int V>
 __device__ __forceinline__ void rn_block_sums(float* red, int& turn, int nw, int wave, int lane, float (&v)[2][V]) {
   if (nw == 1) return;
-  rn_exchange<2, V>(red, turn, nw, wave, lane, v);
-  const float* o = red + turn * nw * (2 * V * 64) + lane;
-  turn ^= 1;
+  const float* o = rn_exchange<V>(red, turn, nw, wave, lane, v);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float s = 0.f;
-      for (int w = 0; w < nw; ++w) s += o[(w * 2 * V + k * V + j) * 64];
-      v[k][j] = s;
+    for (int j = 0; j < V; ++j) v[k][j] = 0.f;
+  for (int w = 0; w < nw; ++w)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float t[V];
+      rn_get<V>(t, o + (2 * w + k) * (V * 64));
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[k][j] += t[j];
     }
 }
 
-// mu and rho of a pixel's channels: each wave's mean and sum of squares about it, joined by the means' spread, so that
-// no large mean cancels.
-template <int V, int NC>
+// s / n, rounded as a division is (rn: 1 / n rounded).
+__device__ __forceinline__ float rn_over(float s, float n, float rn) {
+  const float u = s * rn;
+  return fmaf(fmaf(-u, n, s), rn, u);
+}
+
+// mu and rho of a pixel's channels: each wave's mean and sum of squares about it, joined by the means' spread about the
+// first wave's, so that no large mean cancels.
+template <int V, int NC, bool FULL>
 __device__ __forceinline__ void rn_block_moments(float* red, int& turn, int nw, int wave, int lane, int C, int n, float eps,
                                                  const float (&x)[NC][V], float (&mu)[V], float (&rho)[V]) {
   float m[2][V];
-  const float rn = 1.f / (float)n;
+  const float fn = (float)n, rn = 1.f / fn, fC = (float)C, rC = 1.f / fC;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) s += i < n ? x[i][j] : 0.f;
-    const float u = s * rn;
+    const float u = rn_over(s, fn, rn);
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -356,27 +386,34 @@ __device__ __forceinline__ void rn_block_moments(float* red, int& turn, int nw, 
     m[1][j] = q;
   }
   if (nw > 1) {
-    rn_exchange<2, V>(red, turn, nw, wave, lane, m);
-    const float* o = red + turn * nw * (2 * V * 64) + lane;
-    turn ^= 1;
+    const float* o = rn_exchange<V>(red, turn, nw, wave, lane, m);
+    float u[V], q[V], d[V] = {}, e[V] = {}, t[V];  // d, e: sums over the channels of the means' distances and squares
+    rn_get<V>(u, o);
+    rn_get<V>(q, o + V * 64);
+    for (int w = 1; w < nw; ++w) {
+      const float k = FULL ? (float)NC : (float)min(NC, C - w * NC);
+      rn_get<V>(t, o + 2 * w * (V * 64));
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float v = t[j] - u[j], kv = k * v;
+        d[j] += kv;
+        e[j] = fmaf(kv, v, e[j]);
+      }
+      rn_get<V>(t, o + (2 * w + 1) * (V * 64));
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] += t[j];
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float s = 0.f;
-      for (int w = 0; w < nw; ++w) s = fmaf((float)min(NC, C - w * NC), o[(w * 2 * V + j) * 64], s);
-      const float u = s / (float)C;
-      float q = 0.f;
-      for (int w = 0; w < nw; ++w) {
-        const float d = o[(w * 2 * V + j) * 64] - u;
-        q += fmaf((float)min(NC, C - w * NC) * d, d, o[(w * 2 * V + V + j) * 64]);
-      }
-      m[0][j] = u;
-      m[1][j] = q;
+      const float v = rn_over(d[j], fC, rC), w = fmaf(-d[j], v, e[j]);
+      m[0][j] = u[j] + v;
+      m[1][j] = q[j] + (w < 0.f ? 0.f : w);
     }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     mu[j] = m[0][j];
-    rho[j] = 1.f / sqrtf(m[1][j] / (float)C + eps);
+    rho[j] = rsqrtf(fmaf(m[1][j], rC, eps));
   }
 }
 
@@ -421,9 +458,35 @@ __device__ __forceinline__ float rn_lane_sums(float (&v)[NC], int lane) {
   return v[0] + rn_dpp<kXor1>(v[0]);
 }
 
+// What no kernel here writes, in the constant address space: its loads are scalar and need not wait for stores before
+// them, which may be to the same memory for all the compiler knows (forward at 8 x 64 x 65536 bf16, gate and both norms:
+// 64 us, 75 without).
+template <class P>
+__device__ __forceinline__ float rn_const(const P* p, int64_t i) {
+  typedef const P __attribute__((address_space(4))) C;
+  return (float)((C*)(uintptr_t)p)[i];
+}
+
+// Scale and, for a gate per sample, gate of a wave's channels (one branch for all of them, so that their loads are in
+// flight together).
+template <class TH, int NC, bool SAMPLE>
+__device__ __forceinline__ void rn_factors(float (&k)[NC], const RnArgs& a, int64_t b, int c0, int n) {
+#pragma unroll
+  for (int i = 0; i < NC; ++i) k[i] = 1.f;
+  if (a.s) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) k[i] = rn_const(a.s, c0 + min(i, n - 1));
+  }
+  if (SAMPLE && a.gate) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) k[i] *= rn_const((const TH*)a.gate, b * a.C + c0 + min(i, n - 1));
+  }
+}
+
 // Blocks go to the 8 XCDs in turn; runs of 8 tiles to each keep the lines that two tiles share, where rows do not start
-// on lines, in one L2 (a photo of 321 x 481, 64 channels: 45 -> 40 us; longer runs slow rows that do: 207 -> 219 us with
-// an eighth of 16 x 64 x 256 x 256 to each XCD, against 202-207 us with runs of 8 or 1).
+// on lines, in one L2 (64 channels of a photo of 321 x 481: forward 45 -> 40 us, backward 70 -> 65; 3 x 96 x 201 x 327 with
+// gate and both norms: backward 163 -> 149).  Longer runs slow rows that do start on lines: an eighth of
+// 16 x 64 x 256 x 256 to each XCD takes 219 us forward, against 202-207 us with runs of 8 or 1.
 __device__ __forceinline__ int64_t rn_order(uint32_t b, uint32_t blocks) {
   if (b >= blocks / 64 * 64) return b;
   return b / 64 * 64 + b % 8 * 8 + b % 64 / 8;
@@ -437,47 +500,59 @@ __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
   const RnLane<V> px(a, rn_order(blockIdx.x, gridDim.x), lane);
   const int64_t HW = a.HW, at = px.base + c0 * HW;
   int turn = 0;
-  float x[NC][V], h[NC][V], g[FG ? NC : 1][V];
-  rn_load_all<T, V, NC>(x, a.x, px, HW, c0, n);
-  if (a.h) rn_load_all<TH, V, NC>(h, a.h, px, HW, c0, n);
-  if constexpr (FG) rn_load_all<TH, V, NC>(g, a.gate, px, HW, c0, n);
-  if constexpr (POST) {
-    float mu[V], rho[V];
-    rn_block_moments<V, NC>(red, turn, nw, wave, lane, C, n, a.peps, h, mu, rho);
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + min(i, n - 1);
-      const float w = a.pw[c], b = a.pb[c];
-#pragma unroll
-      for (int j = 0; j < V; ++j) h[i][j] = fmaf((h[i][j] - mu[j]) * rho[j], w, b);
-    }
-    if (a.stats && wave == 0 && px.any()) {
-      rn_store<float, V>(a.stats + 2 * a.total + px.q, 0, mu);
-      rn_store<float, V>(a.stats + 3 * a.total + px.q, 0, rho);
-    }
-  }
+  // all loads first, as stored: a conversion would wait for its own
+  typename RnVec<T, V>::v xr[NC];
+  typename RnVec<TH, V>::v hr[NC], g[FG ? NC : 1];
+  float k[NC];
+  rn_load_raw<T, V, NC>(xr, a.x, px, HW, c0, n);
+  if (a.h) rn_load_raw<TH, V, NC>(hr, a.h, px, HW, c0, n);
+  if constexpr (FG) rn_load_raw<TH, V, NC>(g, a.gate, px, HW, c0, n);
+  rn_factors<TH, NC, !FG>(k, a, px.b, c0, n);
+  float x[NC][V];
   if (a.h) {
+    float h[NC][V];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + min(i, n - 1);
-      const float s = a.s ? a.s[c] : 1.f;
-      const float gs = !FG && a.gate ? rn_ld<TH>(a.gate, px.b * C + c) : 1.f;
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] = fmaf(s, h[i][j] * (FG ? g[FG ? i : 0][j] : gs), x[i][j]);
+      for (int j = 0; j < V; ++j) h[i][j] = rn_at<TH, V>(hr[i], j);
+    if constexpr (POST) {
+      float mu[V], rho[V];
+      rn_block_moments<V, NC, FULL>(red, turn, nw, wave, lane, C, n, a.peps, h, mu, rho);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = c0 + min(i, n - 1);
+        const float w = rn_const(a.pw, c), b = rn_const(a.pb, c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[i][j] = fmaf((h[i][j] - mu[j]) * rho[j], w, b);
+      }
+      if (a.stats && wave == 0 && px.any()) {
+        rn_store<float, V>(a.stats + 2 * a.total + px.q, 0, mu);
+        rn_store<float, V>(a.stats + 3 * a.total + px.q, 0, rho);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        x[i][j] = fmaf(k[i], FG ? h[i][j] * rn_at<TH, V>(g[FG ? i : 0], j) : h[i][j], rn_at<T, V>(xr[i], j));
     if (px.any())
 #pragma unroll
       for (int i = 0; i < NC; ++i)
         if (i < n) rn_store<T, V>((T*)a.r + at + i * HW, px.off, x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[i][j] = rn_at<T, V>(xr[i], j);
   }
   if (!a.nw) return;
   float mu[V], rho[V];
-  rn_block_moments<V, NC>(red, turn, nw, wave, lane, C, n, a.neps, x, mu, rho);
+  rn_block_moments<V, NC, FULL>(red, turn, nw, wave, lane, C, n, a.neps, x, mu, rho);
   if (!px.any()) return;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     if (i >= n) break;
-    const float w = a.nw[c0 + i], b = a.nb[c0 + i];
+    const float w = rn_const(a.nw, c0 + i), b = rn_const(a.nb, c0 + i);
     float y[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) y[j] = fmaf((x[i][j] - mu[j]) * rho[j], w, b);
@@ -518,7 +593,8 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
   const int mine = lane / (64 / NC);  // the channel whose sums this lane ends with
   int turn = 0;
   float acc[kRnSums] = {};  // the sums so far of channel c0 + mine
-  for (int64_t tile = blockIdx.x; tile < a0.ntiles; tile += gridDim.x) {
+  for (int64_t next = blockIdx.x; next < a0.ntiles; next += gridDim.x) {
+    const int64_t tile = rn_order((uint32_t)next, (uint32_t)a0.ntiles);
     RnArgs a = a0;
     rn_in_loop(a.HW);
     rn_in_loop(a.s);
@@ -529,7 +605,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     const RnLane<V> px(a, tile, lane);
     const int64_t at = px.base + c0 * HW;
     float r[NC][V], d[NC][V], h[NC][V];
-    typename RnVec<T, V>::v e[NC];             // gr and the gate as they were stored, until they are needed
+    typename RnVec<T, V>::v e[NC];  // gr and the gate as they were stored, until they are needed
     typename RnVec<TH, V>::v g[FG ? NC : 1];
     float mu[V], rho[V], mh[V], rh[V];
     if (norm) {
@@ -545,13 +621,11 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
       rn_load<float, V>(mh, a.stats + 2 * a.total + px.q, 0);
       rn_load<float, V>(rh, a.stats + 3 * a.total + px.q, 0);
     }
-    float k[NC];  // scale and gate of a channel
+    float k[NC];
+    rn_factors<TH, NC, !FG>(k, a, px.b, c0, n);
+    if (sample)
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + min(i, n - 1);
-      k[i] = sample ? rn_uniform(rn_ld<TH>(a.gate, px.b * C + c)) : 1.f;
-      if (a.s) k[i] *= a.s[c];
-    }
+      for (int i = 0; i < NC; ++i) k[i] = rn_uniform(k[i]);
     if (!px.whole) {  // pixels of other lanes: gradients of 0, and finite values beside them
       if (norm) rn_drop<V, NC>(r, px.dup), rn_drop<V, NC>(d, px.dup);
       if (a.h) rn_drop<V, NC>(h, px.dup);
@@ -581,7 +655,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (sizeof(T) < 4 && a.h) {  // x: r as the forward had it
-            const float nv = POST ? fmaf(h[i][j], a.pw[c], a.pb[c]) : h[i][j];
+            const float nv = POST ? fmaf(h[i][j], rn_const(a.pw, c), rn_const(a.pb, c)) : h[i][j];
             r[i][j] = fmaf(k[i], FG ? nv * gate(i, j) : nv, r[i][j]);
           }
           r[i][j] = (r[i][j] - mu[j]) * rho[j];  // rhat
@@ -591,7 +665,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
       acc[0] += rn_lane_sums<NC>(t, lane);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const float w = i < n ? a.nw[c0 + min(i, n - 1)] : 0.f;
+        const float w = i < n ? rn_const(a.nw, c0 + min(i, n - 1)) : 0.f;
         t[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -637,7 +711,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
         if (i >= n) break;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = k[i] * d[i][j] * (POST ? fmaf(h[i][j], a.pw[c0 + i], a.pb[c0 + i]) : h[i][j]);
+        for (int j = 0; j < V; ++j) o[j] = k[i] * d[i][j] * (POST ? fmaf(h[i][j], rn_const(a.pw, c0 + i), rn_const(a.pb, c0 + i)) : h[i][j]);
         rn_store_own<TH, V>((TH*)a.dg + at + i * HW, o, px);
       }
     }
@@ -677,7 +751,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     float s[2][V] = {};
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const float kp = i < n ? (POST ? k[i] * a.pw[c0 + i] : k[i]) : 0.f;
+      const float kp = i < n ? (POST ? k[i] * rn_const(a.pw, c0 + i) : k[i]) : 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         d[i][j] *= kp;  // dn wp
