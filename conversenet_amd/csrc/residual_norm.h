@@ -46,8 +46,8 @@ RnKernels rn_f32_f16();
 RnKernels rn_bf16_bf16();
 RnKernels rn_f16_f16();
 
-// How a call runs: pixels of a lane (0: the kernels of any channel count), channels of a wave, and its tiles of 64 px
-// pixels.
+// How a call runs: pixels of a lane (0: the kernels for many channels), channels of a wave, and its tiles of 64 px pixels
+// (64 there).
 struct RnShape {
   int px, ch, waves;
   int64_t ntiles;
@@ -62,11 +62,11 @@ inline RnShape rn_shape(bool bwd, int64_t B, int64_t C, int64_t HW, bool gate_sa
   // Few channels to a wave keep the backward's values in registers, more spare the forward waves to join.  Measured at
   // 4 x 128 x 128 x 128 (float32 and bfloat16, gate and both norms): forward 25 us with 16 channels, 38 us with 8;
   // backward 61 with 8, 147 with 16.
-  if (C > 256) s.px = 0;
+  if (C > 256) s.px = 0, s.ch = 16;
   else if (pairs && C <= (bwd ? 128 : 64) && C % 8 == 0) s.px = 2, s.ch = 8;
   else if (pairs && !bwd && C % 16 == 0) s.px = 2, s.ch = 16;
   else s.px = 1, s.ch = bwd && C <= 128 ? 8 : 16;
-  s.waves = s.px ? (int)((C + s.ch - 1) / s.ch) : 1;
+  s.waves = s.px ? (int)((C + s.ch - 1) / s.ch) : 16;
   const int64_t tile = 64 * (s.px ? s.px : 1);
   if (per_sample) {
     s.tps = (int)((HW + tile - 1) / tile);
@@ -81,7 +81,7 @@ inline RnShape rn_shape(bool bwd, int64_t B, int64_t C, int64_t HW, bool gate_sa
 // 128 registers, 20 of those with 8 channels of one pixel), and as even a number of tiles for each as can be.
 inline int64_t rn_bwd_blocks(const RnShape& s) {
   const int resident = s.px == 1 && s.ch == 8 ? 20 : 16;
-  const int64_t most = s.px ? 256 * (resident / s.waves) : 2048;
+  const int64_t most = 256 * (resident / s.waves);
   if (s.ntiles <= most) return s.ntiles;
   const int64_t per = (s.ntiles + most - 1) / most;
   return (s.ntiles + per - 1) / per;

@@ -45,162 +45,10 @@ __device__ __forceinline__ float rn_ld(const void* p, int64_t i) {
   return (float)((const T*)p)[i];
 }
 
-// The sum of v over a wave's lanes, in every lane.
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-  return v;
-}
-
-// Any channel count: a wave per tile of 64 pixels, a pixel per lane, the channels read again for each step of the
-// formulas (from the caches: a tile's channels are 64 C elements).
-template <class T, class TH, bool POST>
-struct RnPixel {
-  const RnArgs& a;
-  const RnPx p;
-  float mh = 0.f, rh = 0.f;  // mu and rho of h
-  __device__ RnPixel(const RnArgs& a_, const RnPx& p_) : a(a_), p(p_) {}
-  __device__ int64_t at(int64_t c) const { return p.base + c * a.HW + p.off; }
-  __device__ float gate(int64_t c) const {
-    if (!a.gate) return 1.f;
-    return rn_ld<TH>(a.gate, a.gate_full ? at(c) : p.b * a.C + c);
-  }
-  __device__ float hhat(int64_t c) const { return (rn_ld<TH>(a.h, at(c)) - mh) * rh; }
-  __device__ float n(int64_t c) const { return POST ? fmaf(hhat(c), a.pw[c], a.pb[c]) : rn_ld<TH>(a.h, at(c)); }
-  __device__ float r(int64_t c) const {
-    const float x = rn_ld<T>(a.x, at(c));
-    if (!a.h) return x;
-    const float u = n(c) * gate(c);
-    return a.s ? fmaf(a.s[c], u, x) : x + u;
-  }
-};
-
-template <class F>
-__device__ __forceinline__ void rn_moments(int64_t C, float eps, float& mu, float& rho, F v) {
-  float s = 0.f;
-  for (int64_t c = 0; c < C; ++c) s += v(c);
-  mu = s / (float)C;
-  float q = 0.f;
-  for (int64_t c = 0; c < C; ++c) {
-    const float d = v(c) - mu;
-    q = fmaf(d, d, q);
-  }
-  rho = 1.f / sqrtf(q / (float)C + eps);
-}
-
-template <class T, class TH, bool POST>
-__global__ void __launch_bounds__(64) k_rn_fwd_any(RnArgs a) {
-  const RnPx px = rn_px(a, blockIdx.x, threadIdx.x);
-  RnPixel<T, TH, POST> e(a, px);
-  if (POST) rn_moments(a.C, a.peps, e.mh, e.rh, [&](int64_t c) { return rn_ld<TH>(a.h, e.at(c)); });
-  float mu = 0.f, rho = 0.f;
-  if (a.nw) rn_moments(a.C, a.neps, mu, rho, [&](int64_t c) { return e.r(c); });
-  if (!px.ok) return;
-  for (int64_t c = 0; c < a.C; ++c) {
-    const float r = e.r(c);
-    if (a.r) ((T*)a.r)[e.at(c)] = (T)r;
-    if (a.nw) ((T*)a.y)[e.at(c)] = (T)fmaf((r - mu) * rho, a.nw[c], a.nb[c]);
-  }
-  if (a.stats) {
-    if (a.nw) {
-      a.stats[px.q] = mu;
-      a.stats[a.total + px.q] = rho;
-    }
-    if (POST) {
-      a.stats[2 * a.total + px.q] = e.mh;
-      a.stats[3 * a.total + px.q] = e.rh;
-    }
-  }
-}
-
-template <class T, class TH, bool POST>
-__global__ void __launch_bounds__(64) k_rn_bwd_any(RnArgs a) {
-  const int lane = threadIdx.x;
-  const int64_t G = gridDim.x;
-  const bool branch = a.dh || a.dg || a.s || POST;
-  for (int64_t tile = blockIdx.x; tile < a.ntiles; tile += G) {
-    const bool first = tile == blockIdx.x;
-    const RnPx px = rn_px(a, tile, lane);
-    RnArgs b = a;
-    if (sizeof(T) == 4) b.h = nullptr;  // x holds r
-    RnPixel<T, TH, POST> e(a, px), f(b, px);
-    if (POST) {
-      e.mh = f.mh = a.stats[2 * a.total + px.q];
-      e.rh = f.rh = a.stats[3 * a.total + px.q];
-    }
-    float mu = 0.f, rho = 0.f, s1 = 0.f, s2 = 0.f;
-    const bool norm = a.nw && a.gy;
-    if (norm) {
-      mu = a.stats[px.q];
-      rho = a.stats[a.total + px.q];
-      for (int64_t c = 0; c < a.C; ++c) {
-        const float g = rn_ld<T>(a.gy, e.at(c)) * a.nw[c];
-        s1 += g;
-        s2 = fmaf(g, (f.r(c) - mu) * rho, s2);
-      }
-      s1 /= (float)a.C;
-      s2 /= (float)a.C;
-    }
-    auto add = [&](int k, int64_t c, float v) {  // a lane's part of a channel's sum
-      v = wave_sum(px.ok ? v : 0.f);
-      float* o = a.part + ((int64_t)k * a.C + c) * G + blockIdx.x;
-      if (lane == 0) *o = first ? v : *o + v;
-    };
-    auto dr = [&](int64_t c, float gy, float rhat) {
-      float d = a.gr ? rn_ld<T>(a.gr, e.at(c)) : 0.f;
-      if (norm) d += rho * (gy * a.nw[c] - s1 - rhat * s2);
-      return d;
-    };
-    float s3 = 0.f, s4 = 0.f;
-    for (int64_t c = 0; c < a.C; ++c) {
-      const float gy = norm ? rn_ld<T>(a.gy, e.at(c)) : 0.f, rhat = norm ? (f.r(c) - mu) * rho : 0.f;
-      const float d = dr(c, gy, rhat);
-      if (norm) {
-        add(0, c, gy * rhat);
-        add(1, c, gy);
-      }
-      if (a.dx && px.ok) ((T*)a.dx)[e.at(c)] = (T)d;
-      if (!branch) continue;
-      if (!a.h) {  // no scale, gate and norm: dh is dr in its own type
-        if (px.ok) ((TH*)a.dh)[e.at(c)] = (TH)d;
-        continue;
-      }
-      const float gt = e.gate(c), du = a.s ? a.s[c] * d : d, dn = du * gt;
-      const float hh = POST ? e.hhat(c) : rn_ld<TH>(a.h, e.at(c));
-      if (POST) add(2, c, d * gt);
-      add(3, c, d * gt * hh);
-      if (a.dg) {
-        const float n = e.n(c);
-        if (a.gate_full) {
-          if (px.ok) ((TH*)a.dg)[e.at(c)] = (TH)(du * n);
-        } else {
-          const float v = wave_sum(px.ok ? du * n : 0.f);
-          if (lane == 0) a.dgpart[(px.b * a.C + c) * a.tps + tile % a.tps] = v;
-        }
-      }
-      if (POST) {
-        const float g = dn * a.pw[c];
-        s3 += g;
-        s4 = fmaf(g, hh, s4);
-      } else if (a.dh && px.ok) {
-        ((TH*)a.dh)[e.at(c)] = (TH)dn;
-      }
-    }
-    if (!POST || !a.dh) continue;
-    s3 /= (float)a.C;
-    s4 /= (float)a.C;
-    for (int64_t c = 0; c < a.C; ++c) {
-      const float gy = norm ? rn_ld<T>(a.gy, e.at(c)) : 0.f, rhat = norm ? (f.r(c) - mu) * rho : 0.f;
-      const float d = dr(c, gy, rhat), dn = (a.s ? a.s[c] * d : d) * e.gate(c);
-      if (px.ok) ((TH*)a.dh)[e.at(c)] = (TH)(e.rh * (dn * a.pw[c] - s3 - e.hhat(c) * s4));
-    }
-  }
-}
-
 // ------------------------------------------------------------------------------------------------
 // Up to 256 channels: a block per tile of 64 V pixels, its channels spread over the waves, NC to a wave, so that a
 // tensor's part of a tile is read once, V pixels of a channel to a lane, and stays in registers (with a thread per
-// pixel and the channels read again, as above, 16 x 64 x 256 x 256 takes 2.7 ms forward and backward).  Memory is the
+// pixel and the channels read again for each step 16 x 64 x 256 x 256 takes 2.7 ms forward and backward).  Memory is the
 // bound: at that size, float32 with a scale, the forward moves 1.07 GB in 198-208 us (5.2 TB/s, a copy's rate) and the
 // backward 1.61 GB in 308-330 us (4.9-5.2).  With 16-bit tensors the joins and conversions show: 8 x 64 x 256 x 256 bf16,
 // per-sample gate and both norms, 64 us forward (4.2 TB/s) and 103 us backward (3.9); without gate and branch norm 54
@@ -363,8 +211,44 @@ __device__ __forceinline__ float rn_over(float s, float n, float rn) {
   return fmaf(fmaf(-u, n, s), rn, u);
 }
 
-// mu and rho of a pixel's channels: each wave's mean and sum of squares about it, joined by the means' spread about the
-// first wave's, so that no large mean cancels.
+// mu and rho of a pixel's channels from each wave's mean and sum of squares about it (m), over count(w) channels: joined
+// by the means' spread about the first wave's, so that no large mean cancels.
+template <int V, class F>
+__device__ __forceinline__ void rn_join(float* red, int& turn, int nw, int wave, int lane, float C, float rC, float eps,
+                                        F count, float (&m)[2][V], float (&mu)[V], float (&rho)[V]) {
+  if (nw > 1) {
+    const float* o = rn_exchange<V>(red, turn, nw, wave, lane, m);
+    float u[V], q[V], d[V] = {}, e[V] = {}, t[V];  // d, e: sums over the channels of the means' distances and squares
+    rn_get<V>(u, o);
+    rn_get<V>(q, o + V * 64);
+    for (int w = 1; w < nw; ++w) {
+      const float k = count(w);
+      rn_get<V>(t, o + 2 * w * (V * 64));
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float v = t[j] - u[j], kv = k * v;
+        d[j] += kv;
+        e[j] = fmaf(kv, v, e[j]);
+      }
+      rn_get<V>(t, o + (2 * w + 1) * (V * 64));
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] += t[j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float v = rn_over(d[j], C, rC), w = fmaf(-d[j], v, e[j]);
+      m[0][j] = u[j] + v;
+      m[1][j] = q[j] + (w < 0.f ? 0.f : w);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    mu[j] = m[0][j];
+    rho[j] = rsqrtf(fmaf(m[1][j], rC, eps));
+  }
+}
+
+// The same from the NC channels (n of them there) that each wave holds.
 template <int V, int NC, bool FULL>
 __device__ __forceinline__ void rn_block_moments(float* red, int& turn, int nw, int wave, int lane, int C, int n, float eps,
                                                  const float (&x)[NC][V], float (&mu)[V], float (&rho)[V]) {
@@ -385,36 +269,8 @@ __device__ __forceinline__ void rn_block_moments(float* red, int& turn, int nw, 
     m[0][j] = u;
     m[1][j] = q;
   }
-  if (nw > 1) {
-    const float* o = rn_exchange<V>(red, turn, nw, wave, lane, m);
-    float u[V], q[V], d[V] = {}, e[V] = {}, t[V];  // d, e: sums over the channels of the means' distances and squares
-    rn_get<V>(u, o);
-    rn_get<V>(q, o + V * 64);
-    for (int w = 1; w < nw; ++w) {
-      const float k = FULL ? (float)NC : (float)min(NC, C - w * NC);
-      rn_get<V>(t, o + 2 * w * (V * 64));
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float v = t[j] - u[j], kv = k * v;
-        d[j] += kv;
-        e[j] = fmaf(kv, v, e[j]);
-      }
-      rn_get<V>(t, o + (2 * w + 1) * (V * 64));
-#pragma unroll
-      for (int j = 0; j < V; ++j) q[j] += t[j];
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float v = rn_over(d[j], fC, rC), w = fmaf(-d[j], v, e[j]);
-      m[0][j] = u[j] + v;
-      m[1][j] = q[j] + (w < 0.f ? 0.f : w);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    mu[j] = m[0][j];
-    rho[j] = rsqrtf(fmaf(m[1][j], rC, eps));
-  }
+  rn_join<V>(red, turn, nw, wave, lane, fC, rC, eps, [&](int w) { return FULL ? fn : (float)min(NC, C - w * NC); }, m, mu,
+             rho);
 }
 
 // Sums over a wave's lanes of NC values at a time: each step halves the values a lane holds, sending the other half to
@@ -470,14 +326,14 @@ __device__ __forceinline__ float rn_const(const P* p, int64_t i) {
 // Scale and, for a gate per sample, gate of a wave's channels (one branch for all of them, so that their loads are in
 // flight together).
 template <class TH, int NC, bool SAMPLE>
-__device__ __forceinline__ void rn_factors(float (&k)[NC], const RnArgs& a, int64_t b, int c0, int n) {
+__device__ __forceinline__ void rn_factors(float (&k)[NC], const RnArgs& a, int64_t b, int c0, int n, bool sample = true) {
 #pragma unroll
   for (int i = 0; i < NC; ++i) k[i] = 1.f;
   if (a.s) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) k[i] = rn_const(a.s, c0 + min(i, n - 1));
   }
-  if (SAMPLE && a.gate) {
+  if (SAMPLE && a.gate && sample) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) k[i] *= rn_const((const TH*)a.gate, b * a.C + c0 + min(i, n - 1));
   }
@@ -783,6 +639,319 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
     for (int q = 0; q < kRnSums; ++q) a0.part[((int64_t)q * C + c0 + mine) * gridDim.x + blockIdx.x] = acc[q];
 }
 
+// ------------------------------------------------------------------------------------------------
+// More channels: a block of 16 waves per tile of 64 pixels, a pixel to a lane, each wave taking 16 channels of every 256
+// in turn.  The channels are read again for each step of the formulas, from the caches (a tile of 512 float32 channels is
+// 128 KB), and the sums over pixels are added to the block's row in memory.
+// ------------------------------------------------------------------------------------------------
+constexpr int kWideWaves = 16, kWideCh = 16;
+
+template <class T, class TH, bool POST>
+struct RnWide {
+  const RnArgs& a;
+  const RnLane<1> px;
+  const int wave, lane, C;
+  float mh[1] = {0.f}, rh[1] = {1.f}, mu[1] = {0.f}, rho[1] = {1.f};  // of h and of r
+
+  __device__ RnWide(const RnArgs& a_, int64_t tile, int wave_, int lane_)
+      : a(a_), px(a_, tile, lane_), wave(wave_), lane(lane_), C((int)a_.C) {}
+
+  // The channels of wave w below C.
+  __device__ float count(int w) const {
+    const int rest = C % (kWideWaves * kWideCh) - w * kWideCh;
+    return (float)(C / (kWideWaves * kWideCh) * kWideCh + (rest < 0 ? 0 : min(rest, kWideCh)));
+  }
+  template <class F>
+  __device__ void groups(F f) const {
+    for (int c0 = wave * kWideCh; c0 < C; c0 += kWideWaves * kWideCh) f(c0, min(kWideCh, C - c0));
+  }
+  template <class P>
+  __device__ void load(float (&o)[kWideCh], const void* p, int c0, int n) const {
+    const P* t = (const P*)p + px.base + c0 * a.HW;
+    if (a.HW == 1 && n == kWideCh) {  // a pixel's channels lie together: 256 rows of 1024, 436 -> 147 us a training pass
+      constexpr int W = 16 / sizeof(P);
+#pragma unroll
+      for (int i = 0; i < kWideCh / W; ++i) {
+        const typename RnVec<P, W>::v v = *(const typename RnVec<P, W>::v*)(t + W * i + px.off);
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[W * i + j] = (float)v[j];
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kWideCh; ++i) o[i] = (float)t[min(i, n - 1) * a.HW + px.off];
+  }
+  template <class P>
+  __device__ void store(void* p, int c0, int n, const float (&v)[kWideCh]) const {
+    if (px.dup) return;
+    P* t = (P*)p + px.base + c0 * a.HW;
+    if (a.HW == 1 && n == kWideCh) {
+      constexpr int W = 16 / sizeof(P);
+#pragma unroll
+      for (int i = 0; i < kWideCh / W; ++i) {
+        typename RnVec<P, W>::v o;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[j] = (P)v[W * i + j];
+        *(typename RnVec<P, W>::v*)(t + W * i + px.off) = o;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kWideCh; ++i)
+      if (i < n) t[i * a.HW + px.off] = (P)v[i];
+  }
+  // h or hhat, and n of it
+  __device__ void branch(float (&h)[kWideCh], int c0, int n) const {
+    load<TH>(h, a.h, c0, n);
+    if (POST)
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) h[i] = (h[i] - mh[0]) * rh[0];
+  }
+  __device__ float value(float h, int c) const { return POST ? fmaf(h, rn_const(a.pw, c), rn_const(a.pb, c)) : h; }
+  // r from x; g: scratch
+  __device__ void residual(float (&r)[kWideCh], int c0, int n) const {
+    load<T>(r, a.x, c0, n);
+    if (!a.h) return;
+    float h[kWideCh], k[kWideCh], g[kWideCh];
+    branch(h, c0, n);
+    rn_factors<TH, kWideCh, true>(k, a, px.b, c0, n, !a.gate_full);
+    if (a.gate && a.gate_full) {
+      load<TH>(g, a.gate, c0, n);
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) k[i] *= g[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kWideCh; ++i) r[i] = fmaf(k[i], value(h[i], c0 + min(i, n - 1)), r[i]);
+  }
+  // Mean and deviation over all channels of what f puts into its array.
+  template <class F>
+  __device__ void moments(float* red, int& turn, float eps, F f, float (&m)[1], float (&s)[1]) const {
+    float cnt = 0.f, v[2][1] = {};
+    groups([&](int c0, int n) {
+      float x[kWideCh];
+      f(x, c0, n);
+      const float fn = (float)n;
+      float u = 0.f, q = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) u += i < n ? x[i] : 0.f;
+      u = rn_over(u, fn, 1.f / fn);
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) {
+        const float d = i < n ? x[i] - u : 0.f;
+        q = fmaf(d, d, q);
+      }
+      const float d = u - v[0][0], part = fn / (cnt + fn);
+      v[0][0] = fmaf(d, part, v[0][0]);
+      v[1][0] += fmaf(d * d, cnt * part, q);
+      cnt += fn;
+    });
+    const float fC = (float)C;
+    rn_join<1>(red, turn, kWideWaves, wave, lane, fC, 1.f / fC, eps, [&](int w) { return count(w); }, v, m, s);
+  }
+};
+
+template <class T, class TH, bool POST>
+__global__ void __launch_bounds__(64 * kWideWaves) k_rn_fwd_wide(RnArgs a) {
+  extern __shared__ float red[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  RnWide<T, TH, POST> e(a, blockIdx.x, wave, lane);
+  int turn = 0;
+  if constexpr (POST) {
+    float mh[1], rh[1];
+    e.moments(red, turn, a.peps, [&](float (&v)[kWideCh], int c0, int n) { e.template load<TH>(v, a.h, c0, n); }, mh, rh);
+    e.mh[0] = mh[0];
+    e.rh[0] = rh[0];
+  }
+  if (a.nw)
+    e.moments(red, turn, a.neps, [&](float (&v)[kWideCh], int c0, int n) { e.residual(v, c0, n); }, e.mu, e.rho);
+  e.groups([&](int c0, int n) {
+    float r[kWideCh];
+    e.residual(r, c0, n);
+    if (a.r) e.template store<T>(a.r, c0, n, r);
+    if (a.nw) {
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) {
+        const int c = c0 + min(i, n - 1);
+        r[i] = fmaf((r[i] - e.mu[0]) * e.rho[0], rn_const(a.nw, c), rn_const(a.nb, c));
+      }
+      e.template store<T>(a.y, c0, n, r);
+    }
+  });
+  if (a.stats && wave == 0 && e.px.any()) {
+    if (a.nw) {
+      a.stats[e.px.q] = e.mu[0];
+      a.stats[a.total + e.px.q] = e.rho[0];
+    }
+    if (POST) {
+      a.stats[2 * a.total + e.px.q] = e.mh[0];
+      a.stats[3 * a.total + e.px.q] = e.rh[0];
+    }
+  }
+}
+
+template <class T, class TH, bool POST>
+__global__ void __launch_bounds__(64 * kWideWaves) k_rn_bwd_wide(RnArgs a) {
+  extern __shared__ float red[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), C = (int)a.C;
+  const int mine = lane / (64 / kWideCh);
+  const float rC = 1.f / (float)C;
+  const bool norm = a.nw && a.gy, branch = a.dh || a.dg || a.s || POST, sample = a.gate && !a.gate_full;
+  int turn = 0;
+  for (int64_t tile = blockIdx.x; tile < a.ntiles; tile += gridDim.x) {
+    RnWide<T, TH, POST> e(a, tile, wave, lane);
+    const bool own = !e.px.dup;
+    if (norm) {
+      e.mu[0] = a.stats[e.px.q];
+      e.rho[0] = a.stats[a.total + e.px.q];
+    }
+    if (POST) {
+      e.mh[0] = a.stats[2 * a.total + e.px.q];
+      e.rh[0] = a.stats[3 * a.total + e.px.q];
+    }
+    // Adds a channel's sum over the tile, which the wave's lane `mine` of it holds, to the block's row.
+    auto add = [&](int k, int c0, int n, float v) {
+      if (lane % (64 / kWideCh) || mine >= n) return;
+      float* o = a.part + ((int64_t)k * C + c0 + mine) * gridDim.x + blockIdx.x;
+      *o = tile == blockIdx.x ? v : *o + v;
+    };
+    // rhat and gy; a lane without a pixel of its own: zeros
+    auto load = [&](float (&r)[kWideCh], float (&g)[kWideCh], int c0, int n) {
+      if (sizeof(T) == 4) e.template load<T>(r, a.x, c0, n);  // r itself
+      else e.residual(r, c0, n);
+      e.template load<T>(g, a.gy, c0, n);
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) {
+        r[i] = own ? (r[i] - e.mu[0]) * e.rho[0] : 0.f;
+        g[i] = own ? g[i] : 0.f;
+      }
+    };
+    float s[2][1] = {};
+    if (norm) {
+      e.groups([&](int c0, int n) {
+        float r[kWideCh], g[kWideCh], t[kWideCh];
+        load(r, g, c0, n);
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) {
+          t[i] = g[i] * r[i];
+          const float w = i < n ? rn_const(a.nw, c0 + min(i, n - 1)) : 0.f;
+          s[0][0] = fmaf(g[i], w, s[0][0]);
+          s[1][0] = fmaf(t[i], w, s[1][0]);
+        }
+        add(0, c0, n, rn_lane_sums<kWideCh>(t, lane));
+        add(1, c0, n, rn_lane_sums<kWideCh>(g, lane));
+      });
+      rn_block_sums<1>(red, turn, kWideWaves, wave, lane, s);
+    }
+    const float s1 = s[0][0] * rC, s2 = s[1][0] * rC;
+    // dr, times a gate per element
+    auto grad = [&](float (&d)[kWideCh], int c0, int n) {
+      float r[kWideCh];
+      if (norm) {
+        load(r, d, c0, n);
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i)
+          d[i] = fmaf(-r[i], s2, fmaf(d[i], rn_const(a.nw, c0 + min(i, n - 1)), -s1)) * e.rho[0];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) d[i] = 0.f;
+      }
+      if (a.gr) {
+        e.template load<T>(r, a.gr, c0, n);
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) d[i] += r[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) d[i] = own ? d[i] : 0.f;
+    };
+    auto hidden = [&](float (&h)[kWideCh], int c0, int n) {
+      e.branch(h, c0, n);
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) h[i] = own ? h[i] : 0.f;
+    };
+    auto gated = [&](float (&d)[kWideCh], int c0, int n) {
+      if (!a.gate || !a.gate_full) return;
+      float g[kWideCh];
+      e.template load<TH>(g, a.gate, c0, n);
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) d[i] *= own ? g[i] : 0.f;
+    };
+    float z[2][1] = {};
+    e.groups([&](int c0, int n) {
+      float d[kWideCh], h[kWideCh], k[kWideCh], t[kWideCh];
+      grad(d, c0, n);
+      if (a.dx) e.template store<T>(a.dx, c0, n, d);
+      if (!branch) return;
+      if (!a.h) {  // no scale, gate and norm: dh is dr in its own type
+        e.template store<TH>(a.dh, c0, n, d);
+        return;
+      }
+      hidden(h, c0, n);
+      rn_factors<TH, kWideCh, true>(k, a, e.px.b, c0, n, sample);
+      if (a.dg && !sample) {
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) t[i] = k[i] * d[i] * e.value(h[i], c0 + min(i, n - 1));
+        e.template store<TH>(a.dg, c0, n, t);
+      }
+      gated(d, c0, n);
+      const int c = c0 + min(mine, n - 1);
+      const float gt = sample ? rn_ld<TH>(a.gate, e.px.b * C + c) : 1.f;
+      float va = 0.f;
+      if (POST) {
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) t[i] = d[i];
+        va = rn_lane_sums<kWideCh>(t, lane);
+        add(2, c0, n, gt * va);
+      }
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) t[i] = d[i] * h[i];
+      const float vh = rn_lane_sums<kWideCh>(t, lane);
+      add(3, c0, n, gt * vh);
+      if (a.dg && sample && lane % (64 / kWideCh) == 0 && mine < n) {
+        const float v = POST ? fmaf(a.pw[c], vh, a.pb[c] * va) : vh;
+        a.dgpart[(e.px.b * C + c) * a.tps + tile % a.tps] = a.s ? a.s[c] * v : v;
+      }
+      if (POST) {
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) {
+          const float v = i < n ? d[i] * (k[i] * rn_const(a.pw, c0 + min(i, n - 1))) : 0.f;
+          z[0][0] += v;
+          z[1][0] = fmaf(v, h[i], z[1][0]);
+        }
+      } else if (a.dh) {
+#pragma unroll
+        for (int i = 0; i < kWideCh; ++i) d[i] *= k[i];
+        e.template store<TH>(a.dh, c0, n, d);
+      }
+    });
+    if (!POST) continue;
+    rn_block_sums<1>(red, turn, kWideWaves, wave, lane, z);
+    if (!a.dh) continue;
+    const float s3 = z[0][0] * rC, s4 = z[1][0] * rC;
+    e.groups([&](int c0, int n) {
+      float d[kWideCh], h[kWideCh], k[kWideCh];
+      grad(d, c0, n);
+      gated(d, c0, n);
+      hidden(h, c0, n);
+      rn_factors<TH, kWideCh, true>(k, a, e.px.b, c0, n, sample);
+#pragma unroll
+      for (int i = 0; i < kWideCh; ++i) {
+        const float v = d[i] * (k[i] * rn_const(a.pw, c0 + min(i, n - 1)));
+        d[i] = fmaf(-h[i], s4, v - s3) * e.rh[0];
+      }
+      e.template store<TH>(a.dh, c0, n, d);
+    });
+  }
+}
+
+template <bool BWD, class T, class TH>
+int rn_launch_wide(const RnArgs& a, int64_t blocks, hipStream_t st) {
+  void (*k)(RnArgs);
+  if constexpr (BWD) k = a.pw ? k_rn_bwd_wide<T, TH, true> : k_rn_bwd_wide<T, TH, false>;
+  else k = a.pw ? k_rn_fwd_wide<T, TH, true> : k_rn_fwd_wide<T, TH, false>;
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * kWideWaves), sizeof(float) * 2 * kWideWaves * 2 * 64, st, a);
+  return check_launch(BWD ? "residual_norm backward" : "residual_norm");
+}
+
 template <bool BWD, class T, class TH, int V, int NC, bool FULL>
 int rn_launch_tile(const RnArgs& a, int64_t blocks, hipStream_t st) {
   const int nw = (int)((a.C + NC - 1) / NC);
@@ -801,11 +970,7 @@ int rn_launch_tile(const RnArgs& a, int64_t blocks, hipStream_t st) {
 
 template <class T, class TH>
 int rn_launch_fwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
-  if (s.px == 0) {
-    auto k = a.pw ? k_rn_fwd_any<T, TH, true> : k_rn_fwd_any<T, TH, false>;
-    hipLaunchKernelGGL(k, dim3((unsigned)s.ntiles), dim3(64), 0, st, a);
-    return check_launch("residual_norm");
-  }
+  if (s.px == 0) return rn_launch_wide<false, T, TH>(a, s.ntiles, st);
   if (s.px == 2)
     return s.ch == 8 ? rn_launch_tile<false, T, TH, 2, 8, true>(a, s.ntiles, st)
                      : rn_launch_tile<false, T, TH, 2, 16, true>(a, s.ntiles, st);
@@ -815,11 +980,7 @@ int rn_launch_fwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
 template <class T, class TH>
 int rn_launch_bwd(const RnArgs& a, const RnShape& s, hipStream_t st) {
   const int64_t blocks = rn_bwd_blocks(s);
-  if (s.px == 0) {
-    auto k = a.pw ? k_rn_bwd_any<T, TH, true> : k_rn_bwd_any<T, TH, false>;
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64), 0, st, a);
-    return check_launch("residual_norm backward");
-  }
+  if (s.px == 0) return rn_launch_wide<true, T, TH>(a, blocks, st);
   if (s.px == 2) return rn_launch_tile<true, T, TH, 2, 8, true>(a, blocks, st);
   if (s.ch == 8) return rn_launch_tile<true, T, TH, 1, 8, false>(a, blocks, st);
   return a.C % 16 ? rn_launch_tile<true, T, TH, 1, 16, false>(a, blocks, st)

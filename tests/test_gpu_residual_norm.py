@@ -189,6 +189,7 @@ def check(a, use_r=True, use_y=True, what=""):
 SHAPES = [(1, 64, 1, 1), (1, 1, 5, 7), (2, 3, 9, 11), (2, 64, 32, 40), (1, 64, 37, 53), (3, 48, 5, 5), (70, 8, 1, 1),
           (2, 128, 17, 16), (1, 100, 33, 32), (2, 200, 12, 13), (1, 256, 20, 20), (1, 257, 9, 9), (1, 600, 8, 33),
           (5, 16, 40, 30), (1, 65, 64, 64)]
+WIDE = [(3, 512, 1, 1), (70, 300, 1, 1), (2, 1040, 3, 5), (1, 2000, 1, 2), (1, 272, 30, 40)]
 TYPES = [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16), (F32, F16)]
 
 
@@ -196,6 +197,13 @@ TYPES = [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16), (F32, F16)]
 @pytest.mark.parametrize("gate,post", [(None, False), ("full", True), ("sample", True), ("sample", False)])
 def test_shapes_f32(shape, gate, post):
     check(make(shape, gate=gate, post=post, seed=sum(shape)), what=str(shape))
+
+
+@pytest.mark.parametrize("shape", WIDE)
+@pytest.mark.parametrize("tx,th", TYPES)
+@pytest.mark.parametrize("scale,gate,post", [(True, None, False), (False, "full", True), (True, "sample", True)])
+def test_many_channels(shape, tx, th, scale, gate, post):
+    check(make(shape, tx, th, scale, gate, post, seed=sum(shape)), what=str((shape, tx, th)))
 
 
 @pytest.mark.parametrize("shape", [(1, 64, 1, 1), (2, 64, 33, 31), (2, 128, 16, 24), (1, 300, 7, 10), (3, 20, 64, 64)])

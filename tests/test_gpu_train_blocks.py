@@ -143,7 +143,7 @@ def test_training_steps_with_clipping():
         assert float(norm64) > 0.1
     for p, q in zip(m.parameters(), ref.parameters()):
         # three steps of at most 0.05 * 0.1, each off by 3.2e-4 of itself
-        assert float((p.detach().double().cpu() - q).norm()) <= 3 * 0.005 * 1e-3 + 1e-6 * float(q.norm())
+        assert float((p.detach().double().cpu() - q.detach()).norm()) <= 3 * 0.005 * 1e-3 + 1e-6 * float(q.detach().norm())
 
 
 def test_hooks_see_their_modules(monkeypatch):
