@@ -95,19 +95,24 @@ def converse2d_module(x, weight, bias, scale, padding, padding_mode, eps):
     return out
 
 
-def layernorm_cf(x, weight, bias, eps):
-    """LayerNorm(data_format='channels_first') (util_converse.py:63-68), over any trailing dimensions."""
-    u = x.mean(1, keepdim=True)
-    s = (x - u).pow(2).mean(1, keepdim=True)
-    cf = (-1,) + (1,) * (x.dim() - 2)
-    return weight.view(cf) * ((x - u) / torch.sqrt(s + eps)) + bias.view(cf)
+def standardised(x, eps):
+    """(x - mean) rho over the channels (dim 1), and rho = 1 / sqrt(var + eps)."""
+    d = x - x.mean(1, keepdim=True)
+    rho = 1 / torch.sqrt(d.pow(2).mean(1, keepdim=True) + eps)
+    return d * rho, rho
+
+
+def standardised_grad(g, hat, rho):
+    """The gradient with respect to x of values standardised(x), from theirs."""
+    return rho * (g - g.mean(1, keepdim=True) - hat * (g * hat).mean(1, keepdim=True))
 
 
 def residual_branch(h, res_scale=None, gate=None, post=None):
     """res_scale * gate * P(h) in float32 or wider (functional.residual_norm)."""
     u = h.to(torch.promote_types(h.dtype, torch.float32))
+    cf = (-1,) + (1,) * (h.dim() - 2)
     if post is not None:
-        u = layernorm_cf(u, *post)
+        u = standardised(u, post[2])[0] * post[0].view(cf) + post[1].view(cf)
     if gate is not None:
         u = u * (gate if gate.shape == h.shape else gate.reshape(gate.shape[:2] + (1,) * (h.dim() - 2)))
-    return u if res_scale is None else res_scale.reshape((-1,) + (1,) * (h.dim() - 2)) * u
+    return u if res_scale is None else res_scale.reshape(cf) * u

@@ -76,9 +76,10 @@ int rn_shape_ok(int64_t B, int64_t C, int64_t HW, int x_type, int h_type, RnKern
   if (B < 0 || C < 1 || HW < 0) return fail(CVN_ERR_ARG, "bad shape");
   if (!rn_kernels(x_type, h_type, k))
     return fail(CVN_ERR_ARG, "types %d and %d: x and h of one type, or a 16-bit h on a float32 x", x_type, h_type);
-  // pixel and tile numbers are held in 32 bits; offsets of elements in 64
-  if (C > 65536 || B > INT32_MAX || HW > INT32_MAX || B * HW > INT32_MAX)
-    return fail(CVN_ERR_UNSUPPORTED, "more than 65536 channels or 2^31 - 1 pixels");
+  // pixel and tile numbers are held in 32 bits, a tile's last pixel behind the last one too; offsets of elements in 64
+  constexpr int64_t kPixels = INT32_MAX - 255;
+  if (C > 65536 || B > kPixels || HW > kPixels || B * HW > kPixels)
+    return fail(CVN_ERR_UNSUPPORTED, "more than 65536 channels or 2^31 - 256 pixels");
   return CVN_OK;
 }
 

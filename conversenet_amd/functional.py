@@ -1,4 +1,5 @@
-"""Tensor-level wrappers over the HIP C ABI (fp32, HIP device tensors only, forward only).
+"""Tensor-level wrappers over the HIP C ABI (HIP device tensors only; fp32, and 16-bit types where a wrapper says so;
+forward only, except for the *_train functions and what they call).
 
 Each wrapper validates shapes the way the reference does (TORCH_CHECK -> RuntimeError,
 Converse2D/torch_converse2d/converse2d.cpp:167-172), makes inputs contiguous like the reference op
@@ -685,11 +686,11 @@ def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
     neps = peps = 0.0
     if norm is not None:
         nw, nb = _param32(keep, norm[0], C, index, "norm weight"), _param32(keep, norm[1], C, index, "norm bias")
-        neps = norm[2]
+        neps = float(norm[2])
         y = torch.empty_like(x)
     if post is not None:
         pw, pb = _param32(keep, post[0], C, index, "branch norm"), _param32(keep, post[1], C, index, "branch norm")
-        peps = post[2]
+        peps = float(post[2])
     if h is not None:
         r = torch.empty_like(x)
     dev = x.device
@@ -815,9 +816,17 @@ def residual_norm_stats(x, h, norm=None, res_scale=None, gate=None, post=None):
     return _residual_norm(_contiguous(x), _contiguous(h), norm, res_scale, _contiguous(gate), post, True)[:3]
 
 
+def _in_memory(t):
+    """Whether a gradient (None: true) is a plain tensor: one that stands for many, or for none yet, has no address."""
+    try:
+        return t is None or type(t) in (torch.Tensor, torch.nn.Parameter) and t.data_ptr() is not None
+    except RuntimeError:
+        return False
+
+
 class ResidualNormFunction(torch.autograd.Function):
     """residual_norm (h None: LayerNorm alone) with the library's forward and backward kernels.  A backward that is
-    itself to be differentiated runs as a composition of torch operations."""
+    itself to be differentiated, or mapped over many gradients at once, runs as a composition of torch operations."""
 
     @staticmethod
     def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps):
@@ -842,7 +851,7 @@ class ResidualNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad[:8]
         if gr is None and gy is None:
             return (None,) * 10
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or not (_in_memory(gr) and _in_memory(gy)):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
                                                      h_dtype, x_dtype, need) + (None, None)
@@ -854,33 +863,56 @@ class ResidualNormFunction(torch.autograd.Function):
 
 def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy, h_dtype, x_dtype,
                                       need):
-    """The same gradients from differentiable torch operations."""
-    branch = composite.residual_branch(h, res_scale, gate, post) if h is not None else None
+    """The same gradients from their formulas in differentiable torch operations."""
+    ref = next(t for t in (base, h, gr, gy) if t is not None)
+    cf = (1, -1) + (1,) * (ref.dim() - 2)
+    pixels = [d for d in range(ref.dim()) if d != 1]
+
+    def like(g, t):
+        return g.reshape(t.shape).to(t.dtype)
+
     dr = None if gr is None else gr.float()
     gnw = gnb = None
     if gy is not None:
         r = base.float()
-        if x_dtype != torch.float32 and branch is not None:
-            r = r + branch  # base is x
-        if not r.requires_grad:
-            r = r.detach().requires_grad_()
-        y = composite.layernorm_cf(r, norm_w.float(), norm_b.float(), norm_eps)
-        ts = [r] + [t for t, k in ((norm_w, need[6]), (norm_b, need[7])) if k]
-        got = list(torch.autograd.grad(y, ts, gy.float(), create_graph=True))
-        d = got.pop(0)
+        if x_dtype != torch.float32 and h is not None:
+            r = r + composite.residual_branch(h, res_scale, gate, post)  # base is x
+        hat, rho = composite.standardised(r, norm_eps)
+        gy = gy.float()
+        d = composite.standardised_grad(gy * norm_w.float().view(cf), hat, rho)
         dr = d if dr is None else dr + d
-        gnw = got.pop(0) if need[6] else None
-        gnb = got.pop(0) if need[7] else None
+        gnw = like((gy * hat).sum(pixels), norm_w) if need[6] else None
+        gnb = like(gy.sum(pixels), norm_b) if need[7] else None
     gx = dr.to(x_dtype) if need[0] else None
     gh = gs = gg = gpw = gpb = None
-    if branch is None:
-        gh = dr.to(h_dtype) if need[1] else None
-    else:
-        ts = [h, res_scale, gate, *(post or (None, None))[:2]]
-        ask = [i for i in range(5) if need[1 + i] and ts[i] is not None]
-        if ask:
-            got = dict(zip(ask, torch.autograd.grad(branch, [ts[i] for i in ask], dr, create_graph=True)))
-            gh, gs, gg, gpw, gpb = (got.get(i) for i in range(5))
+    if h is None:
+        gh = dr.to(h_dtype) if h_dtype is not None and need[1] else None
+        return gx, gh, gs, gg, gpw, gpb, gnw, gnb
+    n = h.float()
+    if post is not None:
+        phat, prho = composite.standardised(n, post[2])
+        n = phat * post[0].float().view(cf) + post[1].float().view(cf)
+    g = None
+    if gate is not None:
+        g = (gate if gate.shape == h.shape else gate.reshape(gate.shape[:2] + (1,) * (h.dim() - 2))).float()
+    u = n if g is None else n * g
+    du = dr
+    if res_scale is not None:
+        gs = like((dr * u).sum(pixels), res_scale) if need[2] else None
+        du = dr * res_scale.float().view(cf)
+    dn = du
+    if gate is not None:
+        if need[3]:
+            gg = du * n
+            if gate.shape != h.shape:
+                gg = gg.flatten(2).sum(2)
+            gg = like(gg, gate)
+        dn = du * g
+    if post is not None:
+        gpw = like((dn * phat).sum(pixels), post[0]) if need[4] else None
+        gpb = like(dn.sum(pixels), post[1]) if need[5] else None
+        dn = composite.standardised_grad(dn * post[0].float().view(cf), phat, prho)
+    gh = dn.to(h_dtype) if need[1] else None
     return gx, gh, gs, gg, gpw, gpb, gnw, gnb
 
 
@@ -966,7 +998,8 @@ def _tensors(ts):
 
 def grad_norm(grads, norm_type=2.0):
     """The norm over all elements of many tensors (2, or math.inf for the largest magnitude): a float32 scalar on their
-    device, accumulated in 64 bits.  grads: tensors of any shapes, float32, bfloat16 or float16, on one device."""
+    device, accumulated in 64 bits.  grads: tensors of any shapes, float32, bfloat16 or float16, on one device.  (Not
+    differentiable; no host wait.)"""
     return _clip(_all_contiguous(_tensors(grads)), None, None, norm_type)
 
 

@@ -97,7 +97,7 @@ def _norm_grad_eligible(x, *params) -> bool:
     if torch._C._are_functorch_transforms_active() or fwAD._current_level >= 0 or torch.compiler.is_compiling() \
             or torch.jit.is_tracing():
         return False
-    if x.dim() != 4 or not x.is_contiguous() or not 0 < x.shape[1] <= 65536 or x.numel() // x.shape[1] >= 1 << 31:
+    if x.dim() != 4 or not x.is_contiguous() or not 0 < x.shape[1] <= 65536 or x.numel() // x.shape[1] > (1 << 31) - 256:
         return False
     if any(p.numel() != x.shape[1] or p.device != x.device for p in params):
         return False

@@ -399,7 +399,7 @@ def test_backward_is_differentiable():
         c = {k: v.double().requires_grad_(k in keys) for k, v in a.items()}
         post = None if plain else (c["pw"], c["pb"], EPS)
         r = c["x"] + composite.residual_branch(c["h"], c.get("s"), c.get("gate"), post)
-        y = composite.layernorm_cf(r, c["w"], c["b"], EPS)
+        y = composite.standardised(r, EPS)[0] * _cf(c["w"], 4) + _cf(c["b"], 4)
         ref = torch.autograd.grad(penalty(c, r, y), [c[k] for k in keys], allow_unused=True)
         # first gradients rounded to 16 bits enter the penalty's own gradient: a relative 2^-8 of its terms
         rel = 1e-4 if tx == th == F32 else 2.0 ** -5
@@ -408,6 +408,46 @@ def test_backward_is_differentiable():
                 assert g is None or float(g.abs().max()) <= rel
                 continue
             assert float((g.double().cpu() - w).norm()) <= rel * float(w.norm()), (k, tx, th)
+
+
+@pytest.mark.parametrize("tx,th,gate,plain", [(F32, F32, "full", False), (BF16, BF16, "sample", False), (F32, F32, None, True),
+                                              (F32, F16, "sample2", False)])
+def test_composed_backward_is_the_same(tx, th, gate, plain):
+    """The composition a differentiated backward runs: within the kernels' bounds too."""
+    a = make((2, 24, 9, 8), tx, th, not plain, gate, not plain, seed=17)
+    val, tol = oracle(a)
+    d = _dev(a)
+    out = call(d)
+    keys = [k for k in ("x", "h", "gate", "s", "pw", "pb", "w", "b") if k in d]
+    g = torch.autograd.grad((out["r"], out["y"]), [d[k] for k in keys], (d["gr"], d["gy"]), create_graph=True)
+    compare({"d" + k: v for k, v in zip(keys, g)}, val, tol, "composed")
+
+
+def test_many_gradients_at_once():
+    a = make((2, 12, 4, 5), gate="full", post=True, seed=18)
+    d = _dev(a)
+    out = call(d)
+    keys = ("x", "h", "gate", "s", "pw", "pb", "w", "b")
+    many = [torch.stack([t, 2 * t, -t]) for t in (d["gr"], d["gy"])]
+    got = torch.autograd.grad((out["r"], out["y"]), [d[k] for k in keys], many, is_grads_batched=True)
+    want = grads(d, call(d))
+    for k, g in zip(keys, got):
+        w = want["d" + k]
+        for i, f in enumerate((1, 2, -1)):
+            assert float((g[i] - f * w).norm()) <= 2e-6 * float(w.norm()) + 1e-12
+
+
+@pytest.mark.parametrize("scale", [False, True])
+def test_one_tensor_as_stream_and_branch(scale):
+    a = make((2, 16, 9, 9), scale=scale, seed=19)
+    a["h"] = a["x"]
+    val, tol = oracle(a)
+    d = _dev(a)
+    d["h"] = d["x"]
+    out = call(d)
+    compare(out, val, tol, "shared")
+    g, = torch.autograd.grad((out["r"], out["y"]), (d["x"],), (d["gr"], d["gy"]))
+    compare({"dx": g}, {"dx": val["dx"] + val["dh"]}, {"dx": tol["dx"] + tol["dh"] + 2 * U * val["dx"].abs()}, "shared")
 
 
 def test_other_stream():
@@ -460,6 +500,38 @@ def test_recorded_graphs():
             torch.cuda.synchronize()
             for t, u in zip(outs[i], want):
                 assert torch.equal(t, u)
+
+
+def test_recorded_training_pass():
+    """Forward and autograd's backward in one graph, replayed on new inputs against eager passes on leaves of their own."""
+    shape = (2, 64, 20, 30)
+    d = _dev(make(shape, gate="full", post=True, seed=30))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            grads(d, call(d))  # nothing of these passes is kept
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        out = call(d)
+        got = grads(d, out)
+    for rep in range(3):
+        new = make(shape, gate="full", post=True, seed=40 + rep)
+        with torch.no_grad():
+            for k, v in new.items():
+                d[k].copy_(v)
+        e = _dev(new)
+        eout = call(e)
+        want = grads(e, eout)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for k in out:
+            assert torch.equal(out[k], eout[k])
+        for k in want:
+            assert torch.equal(got[k], want[k])
 
 
 def test_offsets_beyond_32_bits():

@@ -57,7 +57,7 @@ def _run(m, x, go):
 
 def _close(got, ref, tol, what=""):
     for i, (g, r) in enumerate(zip(got, ref)):
-        r = r.double().cpu()
+        g, r = g.detach(), r.detach().double().cpu()
         assert float((g.double().cpu() - r).norm()) <= tol * float(r.norm()) + 1e-12, (what, i, float((g.double().cpu() - r).norm()), float(r.norm()))
 
 

@@ -27,6 +27,8 @@ def test_forward_argument_errors(kw):
 def test_forward_limits_and_nothing_to_do():
     assert fwd(C=65537) == _lib.CVN_ERR_UNSUPPORTED
     assert fwd(B=1 << 20, HW=1 << 20) == _lib.CVN_ERR_UNSUPPORTED
+    assert fwd(B=1, HW=(1 << 31) - 255) == _lib.CVN_ERR_UNSUPPORTED
+    assert fwd(B=0, HW=(1 << 31) - 256) == _lib.CVN_OK
     assert fwd(B=0) == _lib.CVN_OK and fwd(HW=0) == _lib.CVN_OK
 
 
@@ -97,7 +99,8 @@ def test_cpu_tensors_are_refused():
 
 
 def test_composition_matches_the_definition():
-    """composite.residual_branch and layernorm_cf, which differentiate a backward, against the formulas."""
+    """composite.residual_branch, standardised and its gradient, which a differentiated backward runs, against the
+    formulas."""
     g = torch.Generator().manual_seed(0)
     h, gate = (torch.randn(2, 5, 3, 4, generator=g, dtype=torch.float64) for _ in range(2))
     s, pw, pb = (torch.randn(5, generator=g, dtype=torch.float64) for _ in range(3))
@@ -110,6 +113,10 @@ def test_composition_matches_the_definition():
                 ref[b, :, i, j] = s * gate[b, :, i, j] * (hat * pw + pb)
     got = composite.residual_branch(h, s, gate, (pw, pb, 1e-3))
     assert torch.allclose(got, ref, rtol=0, atol=1e-13)
+    v = h.clone().requires_grad_(True)
+    hat, rho = composite.standardised(v, 1e-3)
+    want, = torch.autograd.grad(hat, v, gate, create_graph=True)
+    assert torch.allclose(composite.standardised_grad(gate, hat, rho), want, rtol=0, atol=1e-12)
     per_sample = torch.randn(2, 5, generator=g, dtype=torch.float64)
     assert torch.equal(composite.residual_branch(h, None, per_sample), h * per_sample[:, :, None, None])
     assert composite.residual_branch(h.float().half()).dtype == torch.float32
