@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import operator
 import os
@@ -675,8 +676,8 @@ def _norm_args(x, h, gate):
 
 
 def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
-    """The launch behind residual_norm, on contiguous x, h and gate: (r, y, stats, what _norm_args gave), None for what
-    there is not."""
+    """The launch behind residual_norm, on contiguous x, h and gate: (r, y, stats, what _norm_args gave, whether the
+    parameters were read where they are), None for what there is not."""
     lib = _lib.load()
     geo, index = _norm_args(x, h, gate)
     B, C, HW, kind = geo
@@ -701,7 +702,7 @@ def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
                                        B, C, HW, s, _ptr(gate), kind, pw, pb, peps, nw, nb, neps, _ptr(r), _ptr(y),
                                        _ptr(stats), _stream(dev))
     _lib.check(rc, "residual_norm")
-    return r, y, stats, geo
+    return r, y, stats, geo, not keep
 
 
 def _contiguous(t):
@@ -722,15 +723,21 @@ def residual_norm(x, h, norm=None, res_scale=None, gate=None, post=None):
     return _residual_norm(_contiguous(x), _contiguous(h), norm, res_scale, _contiguous(gate), post, False)[:2]
 
 
-def _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, post_w, post_b, geo, shape, x_dtype, h_dtype,
-                            need):
-    """The launches behind residual_norm_backward, on arguments that a forward has checked."""
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(geo):
+    """Bytes of scratch of a backward of this geometry (the library's answer depends on nothing else)."""
+    return _lib.load().cvn_residual_norm_bwd_workspace(*geo)
+
+
+def _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, gate, post_w, post_b, geo, shape, x_dtype,
+                            h_dtype, need, direct=False):
+    """The launches behind residual_norm_backward, on arguments that a forward has checked; direct: it read the
+    parameters where they are."""
     lib = _lib.load()
     B, C, HW, kind = geo
     nx, nh, ns, ng, npw, npb, nnw, nnb = need
     gr, gy = _contiguous(gr), _contiguous(gy) if norm_w is not None else None
     dev = (gr if gr is not None else gy).device
-    index = dev.index
     keep = []
     f32 = torch.float32
     plain = res_scale is None and gate is None and post_w is None  # then the branch's gradient is x's
@@ -743,7 +750,7 @@ def _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, pos
         if nh and not same:
             gh = out_h = torch.empty(shape, dtype=h_dtype, device=dev)
         gnw = torch.empty(norm_w.shape, dtype=f32, device=dev) if nnw else None
-        gnb = torch.empty(norm_w.shape, dtype=f32, device=dev) if nnb else None
+        gnb = torch.empty(norm_b.shape, dtype=f32, device=dev) if nnb else None
     else:  # x's gradient is r's
         gx = gr
         if nh and plain and not same:
@@ -751,7 +758,8 @@ def _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, pos
         elif nh and not plain:
             gh = out_h = torch.empty(shape, dtype=h_dtype, device=dev)
         if norm_w is not None:  # y was not used
-            gnw, gnb = (torch.zeros(norm_w.shape, dtype=f32, device=dev) if w else None for w in (nnw, nnb))
+            gnw, gnb = (torch.zeros(t.shape, dtype=f32, device=dev) if w else None
+                        for t, w in ((norm_w, nnw), (norm_b, nnb)))
     if same:
         gh = gx
     if ns and res_scale is not None:
@@ -762,15 +770,18 @@ def _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, pos
         gpw = torch.empty(post_w.shape, dtype=f32, device=dev) if npw else None
         gpb = torch.empty(post_b.shape, dtype=f32, device=dev) if npb else None
     if gy is not None or out_h is not None or gs is not None or gg is not None or gpw is not None or gpb is not None:
-        nbytes = lib.cvn_residual_norm_bwd_workspace(B, C, HW, kind)
+        params = (res_scale, post_w, post_b, None if gy is None else norm_w)
+        if direct:
+            s, pw, pb, nw = map(_ptr, params)
+        else:
+            s, pw, pb, nw = (_param32(keep, t, C, dev.index, "a parameter") for t in params)
+        nbytes = _norm_workspace(geo)
         st = _stream(dev)
         ws = _scratch(dev, st)
         with _on(dev), ws.lock:
             rc = lib.cvn_residual_norm_bwd(
                 _ptr(gr), _ptr(gy), None if gy is None else base.data_ptr(), _lib.TYPES[x_dtype], _ptr(h),
-                _lib.TYPES[h_dtype or x_dtype], B, C, HW, _param32(keep, res_scale, C, index, "res_scale"), _ptr(gate), kind,
-                _param32(keep, post_w, C, index, "branch norm"), _param32(keep, post_b, C, index, "branch norm"),
-                None if gy is None else _param32(keep, norm_w, C, index, "norm weight"), _ptr(stats), _ptr(out_x),
+                _lib.TYPES[h_dtype or x_dtype], B, C, HW, s, _ptr(gate), kind, pw, pb, nw, _ptr(stats), _ptr(out_x),
                 _ptr(out_h), _ptr(gg), _ptr(gs), *((None, None) if gy is None else (_ptr(gnw), _ptr(gnb))), _ptr(gpw),
                 _ptr(gpb), ws.ptr(nbytes), nbytes, st)
         _lib.check(rc, "residual_norm_backward")
@@ -805,8 +816,8 @@ def residual_norm_backward(grad_r, grad_y, base, h, stats, norm_weight=None, res
     if grad_r is None and grad_y is None:
         raise RuntimeError("residual_norm_backward needs a gradient")
     pw, pb = (None, None) if post is None else post[:2]
-    return _residual_norm_backward(grad_r, grad_y, _contiguous(base), h, stats, norm_weight, res_scale, gate, pw, pb, geo,
-                                   ref.shape, ref.dtype, h_dtype, need)
+    return _residual_norm_backward(grad_r, grad_y, _contiguous(base), h, stats, norm_weight, norm_weight, res_scale, gate, pw,
+                                   pb, geo, ref.shape, ref.dtype, h_dtype, need)
 
 
 def residual_norm_stats(x, h, norm=None, res_scale=None, gate=None, post=None):
@@ -834,18 +845,18 @@ class ResidualNormFunction(torch.autograd.Function):
         x, h, gate = _contiguous(x), _contiguous(h), _contiguous(gate)
         post = None if post_w is None else (post_w, post_b, post_eps)
         norm = None if norm_w is None else (norm_w, norm_b, norm_eps)
-        r, y, stats, geo = _residual_norm(x, h, norm, res_scale, gate, post, True)
+        r, y, stats, geo, direct = _residual_norm(x, h, norm, res_scale, gate, post, True)
         f32 = x.dtype is torch.float32
         keep_h = h is not None and not (f32 and res_scale is None and gate is None and post is None)
         base = None if norm is None else (r if h is not None and f32 else x)
         ctx.save_for_backward(base, h if keep_h else None, res_scale, gate, post_w, post_b, norm_w, norm_b, stats)
-        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape)
+        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape, direct)
         return r if y is None else y if r is None else (r, y)
 
     @staticmethod
     def backward(ctx, *gos):
         base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = ctx.saved_tensors
-        post_eps, norm_eps, h_dtype, x_dtype, geo, shape = ctx.cfg
+        post_eps, norm_eps, h_dtype, x_dtype, geo, shape, direct = ctx.cfg
         gr = gos[0] if h_dtype is not None else None
         gy = gos[-1] if norm_w is not None else None
         need = ctx.needs_input_grad[:8]
@@ -855,8 +866,11 @@ class ResidualNormFunction(torch.autograd.Function):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
                                                      h_dtype, x_dtype, need) + (None, None)
-        gx, gh, gs, gg, *gp = _residual_norm_backward(gr, gy, base, h, stats, norm_w, res_scale, gate, post_w, post_b, geo,
-                                                      shape, x_dtype, h_dtype, need)
+        got = _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, gate, post_w, post_b, geo, shape,
+                                      x_dtype, h_dtype, need, direct)
+        if direct:  # float32 parameters, as their gradients
+            return got + (None, None)
+        gx, gh, gs, gg, *gp = got
         like = lambda g, t: g if g is None or t.dtype is torch.float32 else g.to(t.dtype)  # noqa: E731
         return (gx, gh, like(gs, res_scale), gg, *map(like, gp, (post_w, post_b, norm_w, norm_b)), None, None)
 

@@ -249,6 +249,25 @@ def test_parameters_of_16_bits():
     assert g["dw"].dtype == BF16 and g["ds"].shape == (1, 64, 1, 1)
 
 
+def test_parameters_of_other_shapes():
+    a = make((2, 24, 9, 7), gate="sample", post=True, seed=21)
+    shapes = {"w": (24, 1, 1), "b": (1, 24, 1, 1), "pw": (24,), "pb": (24, 1), "s": (24,)}
+    val, tol = oracle(a)
+    wide = torch.zeros(48, device="cuda")
+    d = {k: v.cuda().reshape(shapes.get(k, v.shape)).clone() for k, v in a.items()}
+    wide[::2] = d["pw"]
+    d["pw"] = wide[::2]  # strided
+    for k in ("x", "h", "gate", "s", "pw", "pb", "w", "b"):
+        d[k].requires_grad_(True)
+    out = call(d)
+    compare(out, val, tol, "shapes")
+    g = grads(d, out)
+    compare(g, val, tol, "shapes")
+    assert all(g["d" + k].shape == d[k].shape for k in shapes)
+    g = grads(d, call(d), use_y=False)  # y unused: zeros of each parameter's shape, or none
+    assert all(g["d" + k] is None or g["d" + k].shape == d[k].shape for k in shapes)
+
+
 @pytest.mark.parametrize("tx,th", TYPES)
 def test_forward_alone_is_the_same(tx, th):
     a = make((2, 64, 20, 22), tx, th, gate="full", post=True, seed=4)
