@@ -1018,9 +1018,8 @@ def grad_norm(grads, norm_type=2.0):
 
 
 def _written(ts):
-    """The library wrote these tensors: autograd sees it as it sees torch's in-place operations."""
-    if any(map(torch.Tensor.is_inference, ts)):
-        ts = [t for t in ts if not t.is_inference()]
+    """The library wrote these tensors: autograd sees it as it sees torch's in-place operations.  (Inference tensors have
+    no version, and are passed over.)"""
     torch.autograd.graph.increment_version(ts)
 
 
