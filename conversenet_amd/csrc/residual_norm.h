@@ -62,8 +62,8 @@ inline RnShape rn_shape(bool bwd, int64_t B, int64_t C, int64_t HW, bool gate_sa
   // where a sample's last tile is a small part of it, and only then may a lane take several pixels.
   const bool per_sample = (bwd && gate_sample) || HW >= 1024, pairs = HW >= 1024;
   // Few channels to a wave keep the backward's values in registers, more spare the forward waves to join.  Measured at
-  // 4 x 128 x 128 x 128 (float32 and bfloat16, gate and both norms): forward 25 us with 16 channels, 38 us with 8;
-  // backward 61 with 8, 147 with 16.
+  // 4 x 128 x 128 x 128 (float32 and bfloat16, gate and both norms): forward 25-28 us with 16 channels, 35-38 us with 8;
+  // backward 54-61 with 8, 147 with 16, which spill.
   if (C > 256) s.px = 0, s.ch = 16;
   else if (pairs && C <= (bwd ? 128 : 64) && C % 8 == 0) s.px = 2, s.ch = 8;
   else if (pairs && !bwd && C % 16 == 0) s.px = 2, s.ch = 16;

@@ -138,7 +138,8 @@ __device__ __forceinline__ void rn_store_own(T* p, const float (&o)[V], const Rn
 
 // A wave's channels of a tensor, from channel c0 on; those behind the n of this wave repeat its last.
 template <class T, int V, int NC>
-__device__ __forceinline__ void rn_load_all(float (&o)[NC][V], const void* p, const RnLane<V>& px, int64_t HW, int c0, int n) {
+__device__ __forceinline__ void rn_load_all(float (&o)[NC][V], const void* p, const RnLane<V>& px, int64_t HW, int c0,
+                                            int n) {
   const T* t = (const T*)p + px.base + c0 * HW;
 #pragma unroll
   for (int i = 0; i < NC; ++i) rn_load<T, V>(o[i], t + min(i, n - 1) * HW, px.off);
@@ -146,8 +147,8 @@ __device__ __forceinline__ void rn_load_all(float (&o)[NC][V], const void* p, co
 
 // The same as it was stored.
 template <class T, int V, int NC>
-__device__ __forceinline__ void rn_load_raw(typename RnVec<T, V>::v (&o)[NC], const void* p, const RnLane<V>& px, int64_t HW,
-                                            int c0, int n) {
+__device__ __forceinline__ void rn_load_raw(typename RnVec<T, V>::v (&o)[NC], const void* p, const RnLane<V>& px,
+                                            int64_t HW, int c0, int n) {
   const T* t = (const T*)p + px.base + c0 * HW;
 #pragma unroll
   for (int i = 0; i < NC; ++i) o[i] = *(const typename RnVec<T, V>::v*)(t + min(i, n - 1) * HW + px.off);
@@ -175,10 +176,11 @@ __device__ __forceinline__ void rn_get(float (&v)[V], const float* p) {
 }
 
 // Two values per pixel over the waves of a block, which each wave joins in the order of the waves.  red: two buffers of
-// nw 2 V 64 floats, taken in turn, so that one barrier a time is enough: a buffer is written again only after the barrier of the
-// other, which a wave reaches after its reads.
+// nw 2 V 64 floats, taken in turn, so that one barrier a time is enough: a buffer is written again only after the
+// barrier of the other, which a wave reaches after its reads.
 template <int V>
-__device__ __forceinline__ const float* rn_exchange(float* red, int& turn, int nw, int wave, int lane, const float (&v)[2][V]) {
+__device__ __forceinline__ const float* rn_exchange(float* red, int& turn, int nw, int wave, int lane,
+                                                    const float (&v)[2][V]) {
   float* buf = red + turn * nw * (2 * V * 64) + lane * V;
   turn ^= 1;
 #pragma unroll
@@ -296,21 +298,16 @@ __device__ __forceinline__ float rn_swap_add(float a, float b, bool upper) {
 
 template <int NC>
 __device__ __forceinline__ float rn_lane_sums(float (&v)[NC], int lane) {
-  static_assert(NC == 8 || NC == 16 || NC == 32, "");
+  static_assert(NC == 8 || NC == 16, "");
 #pragma unroll
   for (int i = 0; i < NC / 2; ++i) v[i] = rn_swap_add32(v[i], v[i + NC / 2]);
 #pragma unroll
   for (int i = 0; i < NC / 4; ++i) v[i] = rn_swap_add16(v[i], v[i + NC / 4]);
 #pragma unroll
   for (int i = 0; i < NC / 8; ++i) v[i] = rn_swap_add<kXor8>(v[i], v[i + NC / 8], lane & 8);
-  if constexpr (NC >= 16) {
-#pragma unroll
-    for (int i = 0; i < NC / 16; ++i) v[i] = rn_swap_add<kXor7>(v[i], v[i + NC / 16], lane & 4);
-  } else {
-    v[0] += rn_dpp<kXor7>(v[0]);
-  }
-  if constexpr (NC >= 32) v[0] = rn_swap_add<kXor2>(v[0], v[1], lane & 2);
-  else v[0] += rn_dpp<kXor2>(v[0]);
+  if constexpr (NC == 16) v[0] = rn_swap_add<kXor7>(v[0], v[1], lane & 4);
+  else v[0] += rn_dpp<kXor7>(v[0]);
+  v[0] += rn_dpp<kXor2>(v[0]);
   return v[0] + rn_dpp<kXor1>(v[0]);
 }
 
@@ -567,7 +564,10 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
         if (i >= n) break;
         float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = k[i] * d[i][j] * (POST ? fmaf(h[i][j], rn_const(a.pw, c0 + i), rn_const(a.pb, c0 + i)) : h[i][j]);
+        for (int j = 0; j < V; ++j) {
+          const float nv = POST ? fmaf(h[i][j], rn_const(a.pw, c0 + i), rn_const(a.pb, c0 + i)) : h[i][j];
+          o[j] = k[i] * d[i][j] * nv;
+        }
         rn_store_own<TH, V>((TH*)a.dg + at + i * HW, o, px);
       }
     }

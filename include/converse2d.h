@@ -277,7 +277,8 @@ enum { CVN_NORM_2 = 0, CVN_NORM_INF = 1 };
  * y = N(x) alone, r is not written.  x, r, y: (B,C,HW) of x_type; h, gate: of h_type, which is x_type or, on a float32
  * x, a 16-bit type; the parameters fp32.  Computed in fp32 and rounded once, r before its norm not at all.
  * stats: NULL, or fp32 (4,B HW), which the backward reads: mean and 1/deviation of r, then of h (rows of norms that
- * are not there are not written).  Up to 65536 channels and 2^31 - 256 pixels (B HW). */
+ * are not there are not written).  No output may share memory with an input or another output.  Up to 65536 channels
+ * and 2^31 - 256 pixels (B HW). */
 int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, int h_type, int64_t B, int64_t C, int64_t HW,
                           const float* res_scale, const void* gate, int gate_kind, const float* post_w,
                           const float* post_b, float post_eps, const float* norm_w, const float* norm_b,

@@ -58,7 +58,8 @@ def _run(m, x, go):
 def _close(got, ref, tol, what=""):
     for i, (g, r) in enumerate(zip(got, ref)):
         g, r = g.detach(), r.detach().double().cpu()
-        assert float((g.double().cpu() - r).norm()) <= tol * float(r.norm()) + 1e-12, (what, i, float((g.double().cpu() - r).norm()), float(r.norm()))
+        err = float((g.double().cpu() - r).norm())
+        assert err <= tol * float(r.norm()) + 1e-12, (what, i, err, float(r.norm()))
 
 
 def _inputs(shape, seed=1):
