@@ -206,6 +206,13 @@ def test_many_channels(shape, tx, th, scale, gate, post):
     check(make(shape, tx, th, scale, gate, post, seed=sum(shape)), what=str((shape, tx, th)))
 
 
+@pytest.mark.parametrize("shape,gate", [((5, 128, 96, 96), "sample"), ((2, 200, 100, 100), None), ((2, 192, 101, 99), "full"),
+                                        ((2, 100, 100, 100), "sample"), ((1, 300, 130, 130), "full")])
+def test_several_tiles_a_block(shape, gate):
+    """More tiles than blocks of the backward, of each kernel: the sums go on from tile to tile."""
+    check(make(shape, gate=gate, post=True, seed=sum(shape)), what=str(shape))
+
+
 @pytest.mark.parametrize("shape", [(1, 64, 1, 1), (2, 64, 33, 31), (2, 128, 16, 24), (1, 300, 7, 10), (3, 20, 64, 64)])
 @pytest.mark.parametrize("tx,th", TYPES[1:])
 @pytest.mark.parametrize("scale,gate,post", [(True, None, False), (False, None, False), (True, "full", True),
@@ -467,6 +474,32 @@ def test_one_tensor_as_stream_and_branch(scale):
     compare(out, val, tol, "shared")
     g, = torch.autograd.grad((out["r"], out["y"]), (d["x"],), (d["gr"], d["gy"]))
     compare({"dx": g}, {"dx": val["dx"] + val["dh"]}, {"dx": tol["dx"] + tol["dh"] + 2 * U * val["dx"].abs()}, "shared")
+
+
+def test_threads_on_one_stream():
+    """Passes of four threads at once, on the stream they share: each as alone."""
+    import threading
+
+    from conversenet_amd import functional as Fh
+
+    sets = [_dev(make((2, 64, 40, 41 + i), gate="sample", post=True, seed=60 + i)) for i in range(4)]
+    want = [grads(d, call(d)) for d in sets]
+    norms = [float(Fh.grad_norm(list(w.values()))) for w in want]
+    bad = []
+
+    def work(i):
+        for _ in range(8):
+            g = grads(sets[i], call(sets[i]))
+            n = float(Fh.grad_norm(list(g.values())))
+            if n != norms[i] or not all(torch.equal(g[k], want[i][k]) for k in g):
+                bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
 
 
 def test_other_stream():
