@@ -737,38 +737,37 @@ def _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, g
     B, C, HW, kind = geo
     nx, nh, ns, ng, npw, npb, nnw, nnb = need
     gr, gy = _contiguous(gr), _contiguous(gy) if norm_w is not None else None
-    dev = (gr if gr is not None else gy).device
+    some = gr if gr is not None else gy
+    dev = some.device
     keep = []
     f32 = torch.float32
+
+    def like(t, wanted):  # (empty_like takes half the time of empty)
+        if not wanted or t is None:
+            return None
+        return torch.empty_like(t) if direct else torch.empty(t.shape, dtype=f32, device=dev)
+
     plain = res_scale is None and gate is None and post_w is None  # then the branch's gradient is x's
-    gx = gh = gs = gg = gpw = gpb = gnw = gnb = out_x = out_h = None
+    gx = gh = gnw = gnb = out_x = out_h = None
     nh = nh and h_dtype is not None
     same = nh and plain and h_dtype is x_dtype
     if gy is not None:
         if nx or same:
-            gx = out_x = torch.empty(shape, dtype=x_dtype, device=dev)
-        if nh and not same:
-            gh = out_h = torch.empty(shape, dtype=h_dtype, device=dev)
-        gnw = torch.empty(norm_w.shape, dtype=f32, device=dev) if nnw else None
-        gnb = torch.empty(norm_b.shape, dtype=f32, device=dev) if nnb else None
+            gx = out_x = torch.empty_like(some)
+        gnw, gnb = like(norm_w, nnw), like(norm_b, nnb)
     else:  # x's gradient is r's
         gx = gr
-        if nh and plain and not same:
-            gh = gr.to(h_dtype)
-        elif nh and not plain:
-            gh = out_h = torch.empty(shape, dtype=h_dtype, device=dev)
         if norm_w is not None:  # y was not used
             gnw, gnb = (torch.zeros(t.shape, dtype=f32, device=dev) if w else None
                         for t, w in ((norm_w, nnw), (norm_b, nnb)))
     if same:
         gh = gx
-    if ns and res_scale is not None:
-        gs = torch.empty(res_scale.shape, dtype=f32, device=dev)
-    if ng and gate is not None:
-        gg = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-    if post_w is not None:
-        gpw = torch.empty(post_w.shape, dtype=f32, device=dev) if npw else None
-        gpb = torch.empty(post_b.shape, dtype=f32, device=dev) if npb else None
+    elif nh and plain and gy is None:
+        gh = gr.to(h_dtype)
+    elif nh:
+        gh = out_h = torch.empty_like(h) if h is not None else torch.empty(shape, dtype=h_dtype, device=dev)
+    gs, gpw, gpb = like(res_scale, ns), like(post_w, npw), like(post_b, npb)
+    gg = torch.empty_like(gate) if ng and gate is not None else None
     if gy is not None or out_h is not None or gs is not None or gg is not None or gpw is not None or gpb is not None:
         params = (res_scale, post_w, post_b, None if gy is None else norm_w)
         if direct:
@@ -841,8 +840,8 @@ class ResidualNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps):
+        # x, h and gate are contiguous: a copy made here would not be the caller's in a differentiated backward
         ctx.set_materialize_grads(False)
-        x, h, gate = _contiguous(x), _contiguous(h), _contiguous(gate)
         post = None if post_w is None else (post_w, post_b, post_eps)
         norm = None if norm_w is None else (norm_w, norm_b, norm_eps)
         r, y, stats, geo, direct = _residual_norm(x, h, norm, res_scale, gate, post, True)
@@ -936,13 +935,13 @@ def residual_norm_train(x, h, norm=None, res_scale=None, gate=None, post=None):
         raise RuntimeError("residual_norm needs a branch")
     pw, pb, pe = post or (None, None, 0.0)
     nw, nb, ne = norm or (None, None, 0.0)
-    out = ResidualNormFunction.apply(x, h, res_scale, gate, pw, pb, nw, nb, pe, ne)
+    out = ResidualNormFunction.apply(_contiguous(x), _contiguous(h), res_scale, _contiguous(gate), pw, pb, nw, nb, pe, ne)
     return (out, None) if norm is None else out
 
 
 def layernorm_cf_train(x, weight, bias, eps):
     """Differentiable layernorm_cf on the HIP kernels (forward and backward)."""
-    return ResidualNormFunction.apply(x, None, None, None, None, None, weight, bias, 0.0, eps)
+    return ResidualNormFunction.apply(_contiguous(x), None, None, None, None, None, weight, bias, 0.0, eps)
 
 
 def _grad_list(ts):

@@ -407,33 +407,35 @@ def test_gradients_against_differences():
         assert abs(float(got - diff)) <= 1e-5 * float((g["d" + k].double().cpu() * e).abs().sum()) + 1e-6, k
 
 
-def test_backward_is_differentiable():
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("tx,th,plain", [(F32, F32, False), (F32, F32, True), (F32, BF16, False), (BF16, BF16, False)])
+def test_backward_is_differentiable(tx, th, plain, strided):
     """A gradient penalty: gradients of gradients, against the same composition in 64 bits."""
     from conversenet_amd import composite
 
-    for tx, th, plain in ((F32, F32, False), (F32, F32, True), (F32, BF16, False), (BF16, BF16, False)):
-        a = make((2, 12, 5, 6), tx, th, scale=not plain, gate=None if plain else "full", post=not plain, seed=15)
-        keys = [k for k in ("x", "h", "gate", "s", "pw", "pb", "w", "b") if k in a]
+    a = make((2, 12, 5, 6), tx, th, scale=not plain, gate=None if plain else "full", post=not plain, seed=15)
+    keys = [k for k in ("x", "h", "gate", "s", "pw", "pb", "w", "b") if k in a]
 
-        def penalty(d, r, y):
-            g = torch.autograd.grad((r, y), [d[k] for k in ("x", "h", "w")], (d["gr"], d["gy"]), create_graph=True)
-            return sum((t.double() ** 2).sum() for t in g)
+    def penalty(d, r, y):
+        g = torch.autograd.grad((r, y), [d[k] for k in ("x", "h", "w")], (d["gr"], d["gy"]), create_graph=True)
+        return sum((t.double() ** 2).sum() for t in g)
 
-        d = _dev(a)
-        out = call(d)
-        got = torch.autograd.grad(penalty(d, out["r"], out["y"]), [d[k] for k in keys], allow_unused=True)
-        c = {k: v.double().requires_grad_(k in keys) for k, v in a.items()}
-        post = None if plain else (c["pw"], c["pb"], EPS)
-        r = c["x"] + composite.residual_branch(c["h"], c.get("s"), c.get("gate"), post)
-        y = composite.standardised(r, EPS)[0] * _cf(c["w"], 4) + _cf(c["b"], 4)
-        ref = torch.autograd.grad(penalty(c, r, y), [c[k] for k in keys], allow_unused=True)
-        # first gradients rounded to 16 bits enter the penalty's own gradient: a relative 2^-8 of its terms
-        rel = 1e-4 if tx == th == F32 else 2.0 ** -5
-        for k, g, w in zip(keys, got, ref):
-            if w is None or not w.abs().any():
-                assert g is None or float(g.abs().max()) <= rel
-                continue
-            assert float((g.double().cpu() - w).norm()) <= rel * float(w.norm()), (k, tx, th)
+    d = {k: (_expand(v.cuda()) if strided and v.dim() == 4 and k != "s" else v.cuda()).requires_grad_(k in keys)
+         for k, v in a.items()}
+    out = call(d)
+    got = torch.autograd.grad(penalty(d, out["r"], out["y"]), [d[k] for k in keys], allow_unused=True)
+    c = {k: v.double().requires_grad_(k in keys) for k, v in a.items()}
+    post = None if plain else (c["pw"], c["pb"], EPS)
+    r = c["x"] + composite.residual_branch(c["h"], c.get("s"), c.get("gate"), post)
+    y = composite.standardised(r, EPS)[0] * _cf(c["w"], 4) + _cf(c["b"], 4)
+    ref = torch.autograd.grad(penalty(c, r, y), [c[k] for k in keys], allow_unused=True)
+    # first gradients rounded to 16 bits enter the penalty's own gradient: a relative 2^-8 of its terms
+    rel = 1e-4 if tx == th == F32 else 2.0 ** -5
+    for k, g, w in zip(keys, got, ref):
+        if w is None or not w.abs().any():
+            assert g is None or float(g.abs().max()) <= rel
+            continue
+        assert float((g.double().cpu() - w).norm()) <= rel * float(w.norm()), (k, tx, th)
 
 
 @pytest.mark.parametrize("tx,th,gate,plain", [(F32, F32, "full", False), (BF16, BF16, "sample", False), (F32, F32, None, True),
