@@ -327,6 +327,21 @@ def test_strides_and_alignment():
         compare(grads(d, out), val, tol, "alignment")
 
 
+@pytest.mark.parametrize("shape", [(3, 37, 40, 40), (3, 65, 7, 9), (5, 8, 33, 33), (2, 257, 6, 5), (3, 131, 33, 32)])
+@pytest.mark.parametrize("tx,th", [(BF16, BF16), (F32, F16)])
+def test_sample_gates_at_any_address(shape, tx, th):
+    """16-bit gates of samples that start at multiples of 2 bytes only."""
+    a = make(shape, tx, th, gate="sample", post=True, seed=sum(shape))
+    val, tol = oracle(a)
+    d = _dev(a)
+    big = torch.zeros(a["gate"].numel() + 1, dtype=th, device="cuda")
+    big[1:].copy_(a["gate"].flatten())
+    d["gate"] = big[1:].view(a["gate"].shape).requires_grad_(True)
+    out = call(d)
+    compare(out, val, tol, "gates")
+    compare(grads(d, out), val, tol, "gates")
+
+
 def test_expanded_gradient_and_input():
     a = make((2, 32, 12, 12), seed=10)
     a["h"] = a["h"][:, :, :1, :1].expand(2, 32, 12, 12)
