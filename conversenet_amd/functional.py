@@ -865,6 +865,9 @@ class ResidualNormFunction(torch.autograd.Function):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
                                                      h_dtype, x_dtype, need) + (None, None)
+        # a saved-tensor hook may have given any of them other strides
+        base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = map(
+            _contiguous, (base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats))
         got = _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, gate, post_w, post_b, geo, shape,
                                       x_dtype, h_dtype, need, direct)
         if direct:  # float32 parameters, as their gradients

@@ -1,0 +1,107 @@
+"""What the host side of the training operators hands to the library, on CPU tensors and with a library that records its
+arguments in place of the kernels."""
+import ctypes
+
+import pytest
+import torch
+
+from conversenet_amd import functional
+
+EPS = 1e-5
+
+
+def _read(address, n):
+    return torch.tensor((ctypes.c_float * n).from_address(address)[:])
+
+
+class Library:
+    """cvn_residual_norm_fwd leaves 1, 2, 3 .. in each output; cvn_residual_norm_bwd keeps what it was given to read."""
+
+    def __init__(self):
+        self.forwards = 0
+        self.read = None
+
+    def cvn_residual_norm_fwd(self, x, xt, h, ht, B, C, HW, s, gate, kind, pw, pb, peps, nw, nb, neps, r, y, stats, stream):
+        self.forwards += 1
+        for p, n in ((r, B * C * HW), (y, B * C * HW), (stats, (4 if pw else 2) * B * HW)):
+            if p:
+                (ctypes.c_float * n).from_address(p)[:] = [float(i + 1) for i in range(n)]
+        return 0
+
+    def cvn_residual_norm_bwd_workspace(self, B, C, HW, kind):
+        return 64
+
+    def cvn_residual_norm_bwd(self, gr, gy, base, xt, h, ht, B, C, HW, s, gate, kind, pw, pb, nw, stats, *rest):
+        n = B * C * HW
+        sizes = dict(gr=n, gy=n, base=n, h=n, s=C, gate=n if kind == 2 else B * C, pw=C, pb=C, nw=C,
+                     stats=(4 if pw else 2) * B * HW)
+        at = dict(gr=gr, gy=gy, base=base, h=h, s=s, gate=gate, pw=pw, pb=pb, nw=nw, stats=stats)
+        self.read = {k: _read(at[k], sizes[k]) for k in at if at[k]}
+        return 0
+
+
+@pytest.fixture
+def library(monkeypatch):
+    lib = Library()
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(functional._lib, "load", lambda: lib)
+    monkeypatch.setattr(functional, "_stream", lambda dev: 0)
+    monkeypatch.setattr(functional, "_on", lambda dev: functional._NO_SWITCH)
+    functional._norm_workspace.cache_clear()
+    yield lib
+    functional._norm_workspace.cache_clear()
+    functional.release_workspace()
+
+
+def _args(shape=(2, 3, 4, 5), seed=0):
+    g = torch.Generator().manual_seed(seed)
+    C = shape[1]
+    d = {k: torch.randn(shape, generator=g) for k in ("x", "h", "gate")}
+    d.update({k: torch.randn(C, generator=g) for k in ("s", "w", "b", "pw", "pb")})
+    return {k: v.requires_grad_(True) for k, v in d.items()}
+
+
+def _call(d):
+    return functional.residual_norm_train(d["x"], d["h"], (d["w"], d["b"], EPS), d["s"], d["gate"], (d["pw"], d["pb"], EPS))
+
+
+def _spread(t):
+    """The same values, two addresses apart."""
+    big = torch.full((*t.shape, 2), float("nan"))
+    big[..., 0] = t
+    return big[..., 0]
+
+
+def _expanded(t):
+    """A tensor of one value as a view of a single element; what lies behind it is something else."""
+    big = torch.full((t.numel() + 1,), float("nan"))
+    big[0] = t.flatten()[0]
+    return big[:1].view((1,) * t.dim()).expand(t.shape)
+
+
+@pytest.mark.parametrize("layout", ["channels last", "spread", "expanded"])
+def test_saved_tensors_of_any_layout(library, layout):
+    """A saved-tensor hook may give a tensor back with other strides: its values, size and type are what counts."""
+    d = _args()
+    if layout == "expanded":
+        with torch.no_grad():
+            for i, v in enumerate(d.values()):
+                v.fill_(i + 0.5)
+
+    def unpack(t):
+        t = t.clone()
+        if layout == "channels last":
+            return t.to(memory_format=torch.channels_last) if t.dim() == 4 else t
+        if layout == "expanded":
+            return _expanded(t) if t.unique().numel() == 1 else t
+        return _spread(t)
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+        r, y = _call(d)
+    gr, gy = torch.randn(r.shape), torch.randn(y.shape)
+    torch.autograd.grad((r, y), list(d.values()), (gr, gy))
+    want = dict(gr=gr, gy=gy, base=r, h=d["h"], s=d["s"], gate=d["gate"], pw=d["pw"], pb=d["pb"], nw=d["w"],
+                stats=torch.arange(1.0, 4 * 2 * 20 + 1))
+    assert set(library.read) == set(want)
+    for k, v in want.items():
+        assert torch.equal(library.read[k], v.detach().flatten()), k
