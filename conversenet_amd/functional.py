@@ -19,6 +19,8 @@ from array import array
 
 import torch
 from torch.multiprocessing.reductions import StorageWeakRef
+from torch.overrides import _get_current_function_mode_stack
+from torch.utils._device import DeviceContext
 
 from . import _lib, composite
 
@@ -656,8 +658,31 @@ def _gate_kind(h, gate):
     raise RuntimeError("gate must have the branch's shape, or (B,C) or (B,C,1,..) for a factor per sample and channel")
 
 
+def _pre_dispatch() -> int:
+    return torch._ops._len_torch_dispatch_stack_pre_dispatch() if torch._C._len_torch_function_stack() else 0
+
+
+def observed() -> bool:
+    """Whether a mode of the caller's sees torch's operations: it would miss those that the library stands for.  (A
+    default device is such a mode, and changes nothing here.)"""
+    if torch._C._len_torch_dispatch_stack():
+        return True
+    return torch._C._len_torch_function_stack() > 0 and any(
+        type(m) is not DeviceContext for m in _get_current_function_mode_stack())
+
+
+def _untraced(what):
+    """Refuses a call that is being recorded as torch operations: the library's kernels are none, and the recorded graph
+    would return its outputs as they were allocated."""
+    if torch._C._get_tracing_state() is not None or _pre_dispatch() or (
+            torch._C._len_torch_dispatch_stack()
+            and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        raise RuntimeError(f"{what} cannot be traced as torch operations")
+
+
 def _norm_args(x, h, gate):
     """Checks the large arguments of a residual_norm call: ((B, C, HW, kind of gate), device index)."""
+    _untraced("residual_norm")
     index = x.get_device()
     for t in (x, h, gate):
         if t is not None and (t.get_device() != index or index < 0 or t.dtype not in _lib.TYPES):
@@ -836,7 +861,8 @@ def _in_memory(t):
 
 class ResidualNormFunction(torch.autograd.Function):
     """residual_norm (h None: LayerNorm alone) with the library's forward and backward kernels.  A backward that is
-    itself to be differentiated, or mapped over many gradients at once, runs as a composition of torch operations."""
+    itself to be differentiated, mapped over many gradients at once or seen by a dispatch mode (a tracer among them) runs as a
+    composition of torch operations."""
 
     @staticmethod
     def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps):
@@ -861,7 +887,8 @@ class ResidualNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad[:8]
         if gr is None and gy is None:
             return (None,) * 10
-        if torch.is_grad_enabled() or not (_in_memory(gr) and _in_memory(gy)):
+        if torch.is_grad_enabled() or torch._C._len_torch_dispatch_stack() or _pre_dispatch() or not (
+                _in_memory(gr) and _in_memory(gy)):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
                                                      h_dtype, x_dtype, need) + (None, None)
@@ -976,6 +1003,7 @@ def _all_contiguous(ts):
 
 def _clip(grads, out, max_norm, norm_type):
     """The norm of contiguous grads, and (out not None) their clipped values into contiguous out."""
+    _untraced("grad_norm" if out is None else "clip_grads")
     kind = _norm_kind(norm_type)
     max_norm = 0.0 if out is None else float(max_norm)
     if not max_norm >= 0.0:

@@ -86,7 +86,7 @@ def _plain(*ms) -> bool:
 def _norm_grad_eligible(x, *params) -> bool:
     """True when a norm (and residual) that autograd must differentiate runs on the library's kernels: contiguous fp32
     (B,C,H,W) HIP tensors within cvn_residual_norm_fwd's limits, a weight per channel, and plain backward: function
-    transforms, forward-mode gradients and tracing see the composition."""
+    transforms, forward-mode gradients, tracing and modes that observe torch's operations see the composition."""
     ts = (x, *params)
     if not all(t.is_cuda and t.dtype is torch.float32 for t in ts):
         return False
@@ -95,7 +95,7 @@ def _norm_grad_eligible(x, *params) -> bool:
     if type(x) not in _TENSORS or not all(type(p) in _TENSORS for p in params):
         return False
     if torch._C._are_functorch_transforms_active() or fwAD._current_level >= 0 or torch.compiler.is_compiling() \
-            or torch.jit.is_tracing():
+            or torch.jit.is_tracing() or functional.observed():
         return False
     if x.dim() != 4 or not x.is_contiguous() or not 0 < x.shape[1] <= 65536 or x.numel() // x.shape[1] > (1 << 31) - 256:
         return False

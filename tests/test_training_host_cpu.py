@@ -105,3 +105,120 @@ def test_saved_tensors_of_any_layout(library, layout):
     assert set(library.read) == set(want)
     for k, v in want.items():
         assert torch.equal(library.read[k], v.detach().flatten()), k
+
+
+@pytest.fixture
+def on_device(library, monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    return library
+
+
+def _norm_module(C=3):
+    from conversenet_amd import util_converse as U
+
+    m = U.LayerNorm(C, eps=EPS, data_format="channels_first")
+    with torch.no_grad():
+        m.weight.copy_(torch.arange(1.0, C + 1))
+        m.bias.copy_(torch.arange(C) - 0.5)
+    return m
+
+
+def _definition(m, x):
+    d = x - x.mean(1, keepdim=True)
+    hat = d / torch.sqrt(d.pow(2).mean(1, keepdim=True) + EPS)
+    return m.weight.view(-1, 1, 1) * hat + m.bias.view(-1, 1, 1)
+
+
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+def test_a_traced_norm_is_its_operations(on_device, pre_dispatch):
+    """A graph of torch operations cannot hold the library's calls: what traces a module's operations sees all of them."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    m = _norm_module()
+
+    def step(x, go):
+        y = m(x)
+        # (torch traces sqrt's gradient before dispatch with the result of the tracing call as a constant)
+        return (y,) if pre_dispatch else (y, *torch.autograd.grad(y, (x, m.weight), go))
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return torch.randn(2, 3, 4, 5, generator=g).requires_grad_(True), torch.randn(2, 3, 4, 5, generator=g)
+
+    graph = make_fx(step, pre_dispatch=pre_dispatch)(*inputs(0))
+    assert on_device.forwards == 0
+    x, go = inputs(1)
+    y = _definition(m, x)
+    want = (y, *torch.autograd.grad(y, (x, m.weight), go))
+    for a, b in zip(graph(x, go), want):
+        assert torch.allclose(a, b, rtol=0, atol=1e-5)
+    m(x)
+    assert on_device.forwards == 1
+
+
+def test_modes_see_a_norms_operations(on_device):
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(getattr(func, "__name__", ""))
+            return func(*args, **(kwargs or {}))
+
+    m = _norm_module()
+    x = torch.randn(1, 3, 2, 2, requires_grad=True)
+    for mode in (Dispatch, Function):
+        seen.clear()
+        with mode():
+            y = m(x)
+        assert torch.allclose(y, _definition(m, x), rtol=0, atol=1e-5) and any("mean" in s for s in seen)
+    assert on_device.forwards == 0
+    with torch.device("cpu"):  # a default device is a mode too, and observes nothing
+        m(x)
+    assert on_device.forwards == 1
+
+
+def test_a_traced_backward_is_its_operations(library):
+    """A forward on the library, and its backward traced."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    d = _args()
+    r, y = _call(d)
+    keys = ("x", "h", "gate", "s", "w", "b", "pw", "pb")
+
+    def back(gr, gy):
+        return torch.autograd.grad((r, y), [d[k] for k in keys], (gr, gy), retain_graph=True)
+
+    gr, gy = torch.randn(r.shape), torch.randn(y.shape)
+    graph = make_fx(back)(torch.randn(r.shape), torch.randn(y.shape))
+    assert library.read is None
+    want = torch.autograd.grad((r, y), [d[k] for k in keys], (gr, gy), create_graph=True)
+    for a, b in zip(graph(gr, gy), want):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)
+
+
+def test_traced_calls_are_refused(library):
+    """The library's calls leave nothing in a graph: tracing one raises, and does not give a graph of empty outputs."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    F = functional
+    x, w = torch.randn(1, 3, 2, 2), torch.ones(3)
+    norm = (w, w, EPS)
+    stats = torch.ones(2, 4)
+    calls = [lambda x: F.residual_norm(x, x, norm)[0], lambda x: F.residual_norm_stats(x, x, norm)[0],
+             lambda x: F.residual_norm_train(x, x, norm)[0], lambda x: F.layernorm_cf_train(x, w, w, EPS),
+             lambda x: F.residual_norm_backward(x, x, x, x, stats, w)[0], lambda x: F.grad_norm([x]),
+             lambda x: F.clip_grads([x], 1.0)[1]]
+    for f in calls:
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f)(x)
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+    assert library.forwards == 0 and library.read is None
