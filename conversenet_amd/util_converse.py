@@ -78,9 +78,11 @@ def _hip_grad_eligible(x, weight, bias, scale, padding, padding_mode) -> bool:
 
 
 def _plain(*ms) -> bool:
-    """True when calling these modules runs their forward alone: no hook observes or changes it."""
+    """True when calling these modules runs their class's forward alone: no hook observes or changes it, and none has a
+    forward of its own (set on the instance, or compiled)."""
     return not _has_any_global_hook() and not any(
-        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in ms)
+        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+        or m._compiled_call_impl is not None or "forward" in m.__dict__ for m in ms)
 
 
 def _norm_grad_eligible(x, *params) -> bool:

@@ -259,3 +259,18 @@ def test_checkpoint_and_inplace_after():
 
     got = _run(Inplace(), x, go)
     _close(got[1:], [2 * w for w in want[1:]], 1e-6)
+
+
+def test_a_norms_own_forward_is_called():
+    m = _fill(U.ConverseBlockAlphaVariant(32, 32, kernel_size=3, padding=1, padding_mode="circular")).cuda()
+    x, go = (t.cuda() for t in _inputs((1, 32, 12, 12)))
+    want = _run(m, x, go)
+    inner = m.conv2[0].forward
+    m.conv2[0].forward = lambda v: inner(v)
+    _close(_run(m, x, go), want, 1e-4)
+    m.conv2[0].forward = lambda v: 2 * inner(v)
+    twice = _run(m, x, go)
+    del m.conv2[0].forward
+    m.conv2[0].register_forward_hook(lambda mod, i, o: 2 * o)
+    _close(twice, _run(m, x, go), 1e-4)
+    assert float((twice[0] - want[0]).abs().max()) > 1e-3

@@ -222,3 +222,25 @@ def test_traced_calls_are_refused(library):
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(f, (x,), check_trace=False)
     assert library.forwards == 0 and library.read is None
+
+
+@pytest.mark.parametrize("change", ["forward", "compile"])
+@pytest.mark.parametrize("path", ["", "conv1", "conv2", "conv1.0", "conv2.0"])
+def test_modules_with_a_forward_of_their_own_are_called(on_device, monkeypatch, path, change):
+    from conversenet_amd import util_converse as U
+
+    blk = U.ConverseBlockAlphaVariant(4, 4, kernel_size=3, padding=1)
+    x = torch.randn(1, 4, 5, 5)
+    ran = []
+    monkeypatch.setattr(U, "_block_train", lambda b, x, n=None, ln=None: (ran.append("fused"), (x, n))[1])
+    assert U._trainable(blk, x) and U._plain(blk)
+    U.run_blocks([blk], x)
+    assert ran == ["fused"]
+    m = blk.get_submodule(path)
+    if change == "forward":
+        m.forward = lambda x: x
+    else:
+        m.compile(backend="eager")
+    assert not (U._trainable(blk, x) and U._plain(blk))
+    if path == "" and change == "forward":  # a chain calls it
+        assert U.run_blocks([blk], x) is x and ran == ["fused"]
