@@ -998,7 +998,10 @@ def _norm_kind(norm_type):
 
 
 def _all_contiguous(ts):
-    return ts if all(map(torch.Tensor.is_contiguous, ts)) else [t.contiguous() for t in ts]
+    if all(map(torch.Tensor.is_contiguous, ts)):
+        return ts
+    with torch.no_grad():
+        return [t.contiguous() for t in ts]
 
 
 def _clip(grads, out, max_norm, norm_type):
@@ -1085,9 +1088,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
                 raise RuntimeError("a gradient's elements share memory")
     norm = _clip(dense, dense, max_norm, norm_type)
     if dense is not grads:
-        for g, d in zip(grads, dense):
-            if d is not g:
-                g.copy_(d)
+        with torch.no_grad():
+            for g, d in zip(grads, dense):
+                if d is not g:
+                    g.copy_(d)
         dense = [d for g, d in zip(grads, dense) if d is g]
     _written(dense)
     return norm

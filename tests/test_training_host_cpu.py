@@ -15,7 +15,8 @@ def _read(address, n):
 
 
 class Library:
-    """cvn_residual_norm_fwd leaves 1, 2, 3 .. in each output; cvn_residual_norm_bwd keeps what it was given to read."""
+    """cvn_residual_norm_fwd leaves 1, 2, 3 .. in each output; cvn_residual_norm_bwd keeps what it was given to read;
+    cvn_clip_grads halves."""
 
     def __init__(self):
         self.forwards = 0
@@ -37,6 +38,16 @@ class Library:
                      stats=(4 if pw else 2) * B * HW)
         at = dict(gr=gr, gy=gy, base=base, h=h, s=s, gate=gate, pw=pw, pb=pb, nw=nw, stats=stats)
         self.read = {k: _read(at[k], sizes[k]) for k in at if at[k]}
+        return 0
+
+    def cvn_grad_norm_workspace(self, sizes, n):
+        return 64
+
+    def cvn_clip_grads(self, grads, out, sizes, types, n, *rest):
+        """Every output half its float32 gradient."""
+        table = lambda at, t: (t * n).from_address(at)[:]  # noqa: E731
+        for g, o, k in zip(table(grads, ctypes.c_uint64), table(out, ctypes.c_uint64), table(sizes, ctypes.c_int64)):
+            (ctypes.c_float * k).from_address(o)[:] = (_read(g, k) / 2).tolist()
         return 0
 
 
@@ -244,3 +255,22 @@ def test_modules_with_a_forward_of_their_own_are_called(on_device, monkeypatch, 
     assert not (U._trainable(blk, x) and U._plain(blk))
     if path == "" and change == "forward":  # a chain calls it
         assert U.run_blocks([blk], x) is x and ran == ["fused"]
+
+
+def test_clipping_records_nothing(library):
+    """Gradients that have a graph of their own (create_graph) are scaled outside of it, whatever their strides."""
+    ps = [torch.nn.Parameter(torch.zeros(3, 4)) for _ in range(5)]
+    leaf = torch.randn(3, 4, requires_grad=True)
+    strided = torch.randn(4, 3).t().requires_grad_(True)
+    base = torch.randn(4, 3, requires_grad=True)
+    for p, g in zip(ps, (leaf, leaf * 2, strided, strided * 2, base.t())):
+        p.grad = g
+    keep = [p.grad.detach().clone() for p in ps]
+    nodes = [p.grad.grad_fn for p in ps]
+    assert [p.grad.is_contiguous() for p in ps] == [True, True, False, False, False]
+    functional.clip_grad_norm_(ps, 1.0)
+    for i, (p, k, f) in enumerate(zip(ps, keep, nodes)):
+        assert torch.equal(p.grad.detach(), k / 2) and p.grad.requires_grad
+        assert i == 4 or p.grad.grad_fn is f  # (autograd writes a view's own node anew, with no_grad too)
+    out, _ = functional.clip_grads([p.grad for p in ps], 1.0)
+    assert not any(o.requires_grad for o in out) and torch.equal(out[2], keep[2] / 4)
