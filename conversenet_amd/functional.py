@@ -1004,6 +1004,19 @@ def _all_contiguous(ts):
         return [t.contiguous() for t in ts]
 
 
+def _as_stored(keep, grads, out, sizes, src):
+    """Puts into src the addresses of copies (held in `keep`) of gradients whose memory has the other sign than their
+    output's: views of an imaginary part, of which only those of one element are contiguous."""
+    i = -1
+    for _ in range(sizes.count(1)):
+        i = sizes.index(1, i + 1)
+        g, o = grads[i], out[i]
+        if g.is_neg() != o.is_neg():
+            with torch.no_grad():
+                keep.append(-g if o.is_neg() else g.resolve_neg())
+            src[i] = keep[-1].data_ptr()
+
+
 def _clip(grads, out, max_norm, norm_type):
     """The norm of contiguous grads, and (out not None) their clipped values into contiguous out."""
     _untraced("grad_norm" if out is None else "clip_grads")
@@ -1016,10 +1029,12 @@ def _clip(grads, out, max_norm, norm_type):
     lib = _lib.load()
     index, types, sizes, src = _grad_list(grads)
     dst = src
+    keep = []
     if out is not None and out is not grads:
         oi, ot, on, dst = _grad_list(out)
         if oi != index or ot != types or on != sizes:
             raise RuntimeError("out must have the gradients' sizes and types, on their device")
+        _as_stored(keep, grads, out, sizes, src)
     n = len(grads)
     dev = grads[0].device
     tables = (src, dst, sizes, types)  # held until the library has read them
@@ -1034,7 +1049,7 @@ def _clip(grads, out, max_norm, norm_type):
         else:
             rc = lib.cvn_clip_grads(src_at, dst_at, sizes_at, types_at, n, kind, max_norm, norm.data_ptr(),
                                     ws.ptr(nbytes), nbytes, st)
-    del tables
+    del tables, keep
     _lib.check(rc, "grad_norm" if out is None else "clip_grads")
     return norm
 

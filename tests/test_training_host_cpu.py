@@ -274,3 +274,21 @@ def test_clipping_records_nothing(library):
         assert i == 4 or p.grad.grad_fn is f  # (autograd writes a view's own node anew, with no_grad too)
     out, _ = functional.clip_grads([p.grad for p in ps], 1.0)
     assert not any(o.requires_grad for o in out) and torch.equal(out[2], keep[2] / 4)
+
+
+def test_a_gradient_that_is_a_negated_view(library):
+    """The gradient of a scalar that was an imaginary part may be a view whose memory holds its negative."""
+    ps = [torch.nn.Parameter(torch.tensor(v)) for v in (2.0, 3.0)]
+    (torch.complex(*ps).conj() * torch.tensor(1 + 2j)).abs().backward()
+    grads = [p.grad for p in ps] + [torch.ones(4), torch.ones(1)]
+    keep = [g.clone() for g in grads]
+    assert [g.is_neg() for g in grads] == [False, True, False, False]
+    for out in (None, [torch.zeros_like(g) for g in keep]):
+        got, _ = functional.clip_grads(grads, 1.0, out=out)
+        assert all(torch.equal(a, b / 2) for a, b in zip(got, keep))
+    turned = torch.tensor([3.0, 5.0], dtype=torch.complex64).conj().imag[:1]
+    functional.clip_grads([torch.ones(1)], 1.0, out=[turned])
+    assert turned.is_neg() and turned.item() == 0.5
+    functional.clip_grads(grads, 1.0, out=grads)
+    functional.clip_grad_norm_(ps, 1.0)
+    assert all(torch.equal(p.grad, k / 4) for p, k in zip(ps, keep))
