@@ -158,6 +158,8 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   if (!empty && ((!grad_r && !grad_y) || (grad_y && !norm_w) || (norm_w && !base) ||
                  (((norm_w && grad_y) || post_w) && !stats)))
     return fail(CVN_ERR_ARG, "null pointer");
+  if (!empty && x_type != CVN_F32 && grad_y && !h && (grad_r || grad_h))
+    return fail(CVN_ERR_ARG, "a 16-bit residual is summed up again from its branch");
   if (!empty && !grad_y && (grad_norm_w || grad_norm_b))
     return fail(CVN_ERR_ARG, "gradients of the norm's parameters without a gradient of y");
   const bool sample = gate_kind == CVN_GATE_SAMPLE;

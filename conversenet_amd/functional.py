@@ -826,7 +826,8 @@ def residual_norm_backward(grad_r, grad_y, base, h, stats, norm_weight=None, res
         raise RuntimeError("residual_norm_backward needs a gradient, and what its norm was of")
     if h is not None:
         h_dtype = h.dtype
-    elif res_scale is not None or gate is not None or post is not None or (ref.dtype != torch.float32 and h_dtype):
+    elif res_scale is not None or gate is not None or post is not None or (ref.dtype != torch.float32 and (
+            h_dtype or (grad_r is not None and grad_y is not None))):
         raise RuntimeError("residual_norm_backward needs the branch")
     h, gate = _contiguous(h), _contiguous(gate)
     geo, index = _norm_args(ref, h, gate)

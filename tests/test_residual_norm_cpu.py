@@ -47,6 +47,18 @@ def test_backward_argument_errors(kw, rc):
     assert bwd(**kw) == rc
 
 
+@pytest.mark.parametrize("t", [1, 2])
+def test_backward_of_a_16_bit_branch_needs_it(t):
+    """Of 16-bit maps the residual is summed up again, so a gradient of r or of h, which only a branch has, needs h."""
+    for kw in (dict(), dict(dh=None), dict(gr=None)):
+        assert bwd(xt=t, ht=t, h=None, **kw) == _lib.CVN_ERR_ARG
+    g = torch.zeros(2, 8, 4, dtype=(torch.bfloat16, torch.float16)[t - 1])
+    w, stats = torch.ones(8), torch.ones(2, 8)
+    for gr, gy, h_dtype in ((g, g, None), (g, g, g.dtype), (None, g, g.dtype)):
+        with pytest.raises(RuntimeError, match="needs the branch"):
+            functional.residual_norm_backward(gr, gy, g, None, stats, w, h_dtype=h_dtype)
+
+
 def test_backward_workspace():
     q = _lib.load().cvn_residual_norm_bwd_workspace
     assert q(1, 64, 1, 0) > 0 and q(2, 64, 100, 1) > q(2, 64, 100, 0) and q(1, 0, 1, 0) == 0 and q(1, 1 << 20, 1, 0) == 0
