@@ -647,3 +647,33 @@ def test_refusals_on_the_device():
         Fh.residual_norm(x, x, norm=(w.double(), w, EPS))
     with pytest.raises(RuntimeError):
         Fh.layernorm_cf_train(torch.zeros(8, device="cuda"), w, w, EPS)
+
+
+@pytest.mark.parametrize("shape", [(2, 64, 33, 32), (2, 64, 37, 53), (1, 128, 41, 43)])
+@pytest.mark.parametrize("tx,th", TYPES)
+@pytest.mark.parametrize("scale,gate,post", [(True, None, False), (True, "full", True), (False, "sample", True),
+                                             (False, "full", False)])
+def test_two_pixels_a_lane_with_a_rest(shape, tx, th, scale, gate, post):
+    """1024 pixels and more of 8 n channels, the last tile not a whole one."""
+    check(make(shape, tx, th, scale, gate, post, seed=sum(shape)), what=str((shape, tx, th)))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("tx,th", [(F32, F32), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("shape", [(2, 64, 33, 33), (2, 128, 45, 25), (2, 20, 33, 33), (2, 300, 33, 33)])
+def test_bad_pixels_at_a_samples_end(bad, tx, th, shape):
+    """The last pixels of a sample, which two lanes read where their number is odd."""
+    H, W = shape[2:]
+    for x_at, h_at in ((W - 1, W - 2), (W - 2, W - 1)):
+        a, clean = (make(shape, tx, th, gate="full", post=True, seed=12) for _ in range(2))
+        a["x"][0, 5, H - 1, x_at] = bad
+        a["h"][0, 7, H - 1, h_at] = bad
+        d, c = _dev(a), _dev(clean)
+        out, ref = call(d), call(c)
+        g, gref = grads(d, out), grads(c, ref)
+        ok = torch.ones(shape[0], 1, *shape[2:], dtype=torch.bool, device="cuda").expand(shape).clone()
+        ok[0, :, H - 1, W - 2:] = False
+        for t, u in ((out["r"], ref["r"]), (out["y"], ref["y"]), (g["dx"], gref["dx"]), (g["dh"], gref["dh"]),
+                     (g["dgate"], gref["dgate"])):
+            assert torch.equal(t[ok], u[ok])
+        assert not torch.isfinite(out["y"][0, :, H - 1, W - 2:]).any() and not torch.isfinite(g["dw"]).any()
