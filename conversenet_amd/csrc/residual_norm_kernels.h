@@ -740,9 +740,9 @@ struct RnWide {
         const float d = i < n ? x[i] - u : 0.f;
         q = fmaf(d, d, q);
       }
-      const float d = u - v[0][0], part = fn / (cnt + fn);
-      v[0][0] = fmaf(d, part, v[0][0]);
-      v[1][0] += fmaf(d * d, cnt * part, q);
+      const float d = u - v[0][0], step = d * (fn / (cnt + fn));
+      v[0][0] += step;
+      v[1][0] += fmaf(step, d * cnt, q);  // (d * d may overflow for the first group, where d is its mean and cnt 0)
       cnt += fn;
     });
     const float fC = (float)C;

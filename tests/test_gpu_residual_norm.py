@@ -677,3 +677,34 @@ def test_bad_pixels_at_a_samples_end(bad, tx, th, shape):
                      (g["dgate"], gref["dgate"])):
             assert torch.equal(t[ok], u[ok])
         assert not torch.isfinite(out["y"][0, :, H - 1, W - 2:]).any() and not torch.isfinite(g["dw"]).any()
+
+
+@pytest.mark.parametrize("C", [64, 256, 272, 512, 1040])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_means_beyond_the_root_of_float32(C, t):
+    """Values of 2^65, whose squares no float32 holds, without a spread and with one of 2^45 (2^58 in bfloat16: 1040
+    squares are below 2^127) about them.  Their means are exact in any order: sums of up to 2^11 equal values or pairs."""
+    from conversenet_amd import functional as Fh
+
+    big, step = 2.0 ** 65, 2.0 ** (45 if t == F32 else 58)
+    a = make((2, C, 5, 7), t, t, scale=False, seed=C)
+    w, b = a["w"].cuda(), a["b"].cuda()
+    cf = (1, -1, 1, 1)
+    x = torch.full((2, C, 5, 7), big, dtype=t, device="cuda").requires_grad_(True)
+    y = Fh.layernorm_cf_train(x, w, b, EPS)
+    assert torch.equal(y.detach(), b.view(cf).to(t).expand_as(y))
+    gx, = torch.autograd.grad(y, x, a["gy"].cuda())
+    gw = a["gy"].double() * a["w"].double().view(cf)
+    want = (gw - _mean(gw)) / EPS ** 0.5
+    # a product, a mean over C channels, a difference, and the deviation: 1 / sqrt(eps) of a rounded eps
+    lim = (gw.abs() + (C + 1) * _mean(gw.abs())) / EPS ** 0.5 * 8 * U + want.abs() * torch.finfo(t).eps / 2 * 1.001
+    assert ((gx.double().cpu() - want).abs() <= lim).all()
+    sign = (1 - 2 * (torch.arange(C) % 2)).double().view(cf)
+    x = (big + sign * step).to(t).expand(2, C, 5, 7).cuda()
+    assert torch.equal(x.double().cpu(), (big + sign * step).expand(2, C, 5, 7))
+    want = sign * a["w"].double().view(cf) + a["b"].double().view(cf)
+    y = Fh.residual_norm(torch.zeros_like(x), x, (w, b, EPS))[1]  # a branch on nothing
+    post = Fh.residual_norm(torch.zeros_like(x), x, None, post=(w, b, EPS))[0]  # and its own norm
+    lim = 4 * U * (a["w"].abs() + a["b"].abs()).double().view(cf) + want.abs() * torch.finfo(t).eps / 2 * 1.001
+    for got in (y, post):
+        assert ((got.double().cpu() - want).abs() <= lim).all()
