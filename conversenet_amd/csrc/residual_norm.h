@@ -32,6 +32,7 @@ struct RnArgs {
   float *part, *dgpart;  // [kRnSums][C][blocks]; [B C][tps]
   int64_t C, HW, total;  // total = B HW
   int64_t ntiles;
+  int64_t tile0;    // the first tile of a forward's launch
   int tps;          // tiles per sample, or 0: tiles of consecutive pixels of any samples
   bool gate_full;   // a gate per element; otherwise per sample and channel
 };
@@ -47,6 +48,9 @@ RnKernels rn_f32_bf16();
 RnKernels rn_f32_f16();
 RnKernels rn_bf16_bf16();
 RnKernels rn_f16_f16();
+
+// A launch holds fewer than 2^32 threads: its blocks at most, in whole runs of 64 (rn_order).
+inline int64_t rn_max_blocks(int threads) { return (((int64_t)1 << 32) - 1) / threads / 64 * 64; }
 
 // How a call runs: pixels of a lane (0: the kernels for many channels), channels of a wave, and its tiles of 64 px pixels
 // (64 there).

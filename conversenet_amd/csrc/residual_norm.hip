@@ -38,28 +38,28 @@ __device__ __forceinline__ double rn_row_sum(const float* p, int n, int lane) {
 
 __global__ void __launch_bounds__(256) k_rn_sums(RnSumArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
-  if (row >= a.C) {
-    const int64_t i = row - a.C;
-    const float s = (float)rn_row_sum(a.dgpart + i * a.tps, a.tps, lane);
-    if (lane) return;
-    if (a.dg_type == CVN_F32) ((float*)a.dg)[i] = s;
-    else if (a.dg_type == CVN_BF16) ((__bf16*)a.dg)[i] = (__bf16)s;
-    else ((_Float16*)a.dg)[i] = (_Float16)s;
-    return;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.rows; row += (int64_t)gridDim.x * 4) {
+    if (row >= a.C) {
+      const int64_t i = row - a.C;
+      const float s = (float)rn_row_sum(a.dgpart + i * a.tps, a.tps, lane);
+      if (lane) continue;
+      if (a.dg_type == CVN_F32) ((float*)a.dg)[i] = s;
+      else if (a.dg_type == CVN_BF16) ((__bf16*)a.dg)[i] = (__bf16)s;
+      else ((_Float16*)a.dg)[i] = (_Float16)s;
+      continue;
+    }
+    const int c = (int)row;
+    auto sum = [&](int k) { return rn_row_sum(a.part + ((int64_t)k * a.C + c) * a.G, a.G, lane); };
+    const double w = a.dw ? sum(0) : 0., b = a.db ? sum(1) : 0.;
+    const double sa = a.dpb || (a.ds && a.pw) ? sum(2) : 0., sh = a.ds || a.dpw ? sum(3) : 0.;
+    if (lane) continue;
+    const double s = a.s ? a.s[c] : 1.;
+    if (a.dw) a.dw[c] = (float)w;
+    if (a.db) a.db[c] = (float)b;
+    if (a.ds) a.ds[c] = (float)(a.pw ? a.pw[c] * sh + a.pb[c] * sa : sh);
+    if (a.dpw) a.dpw[c] = (float)(s * sh);
+    if (a.dpb) a.dpb[c] = (float)(s * sa);
   }
-  const int c = (int)row;
-  auto sum = [&](int k) { return rn_row_sum(a.part + ((int64_t)k * a.C + c) * a.G, a.G, lane); };
-  const double w = a.dw ? sum(0) : 0., b = a.db ? sum(1) : 0.;
-  const double sa = a.dpb || (a.ds && a.pw) ? sum(2) : 0., sh = a.ds || a.dpw ? sum(3) : 0.;
-  if (lane) return;
-  const double s = a.s ? a.s[c] : 1.;
-  if (a.dw) a.dw[c] = (float)w;
-  if (a.db) a.db[c] = (float)b;
-  if (a.ds) a.ds[c] = (float)(a.pw ? a.pw[c] * sh + a.pb[c] * sa : sh);
-  if (a.dpw) a.dpw[c] = (float)(s * sh);
-  if (a.dpb) a.dpb[c] = (float)(s * sa);
 }
 
 bool rn_kernels(int x_type, int h_type, RnKernels* k) {
@@ -214,6 +214,7 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   }
   s.rows = C + (s.dg ? B * C : 0);
   if (!s.dw && !s.db && !s.ds && !s.dpw && !s.dpb && !s.dg) return CVN_OK;
-  hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, s);
+  // a block for every 4 rows, as far as one launch goes: 2^26 gates of one tile each are more
+  hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)std::min((s.rows + 3) / 4, rn_max_blocks(256))), dim3(256), 0, st, s);
   return check_launch("residual_norm sums");
 }

@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
   extern __shared__ float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int C = (int)a.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
-  const RnLane<V> px(a, rn_order(blockIdx.x, gridDim.x), lane);
+  const RnLane<V> px(a, a.tile0 + rn_order(blockIdx.x, gridDim.x), lane);
   const int64_t HW = a.HW, at = px.base + c0 * HW;
   int turn = 0;
   // all loads first, as stored: a conversion would wait for its own
@@ -754,7 +754,7 @@ template <class T, class TH, bool POST>
 __global__ void __launch_bounds__(64 * kWideWaves) k_rn_fwd_wide(RnArgs a) {
   extern __shared__ float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  RnWide<T, TH, POST> e(a, blockIdx.x, wave, lane);
+  RnWide<T, TH, POST> e(a, a.tile0 + blockIdx.x, wave, lane);
   int turn = 0;
   if constexpr (POST) {
     float mh[1], rh[1];
@@ -943,13 +943,21 @@ __global__ void __launch_bounds__(64 * kWideWaves) k_rn_bwd_wide(RnArgs a) {
   }
 }
 
+// The blocks of a backward, or a forward's tiles in as many launches as they take.
+template <bool BWD>
+int rn_launch(void (*k)(RnArgs), RnArgs a, int64_t blocks, int threads, size_t lds, hipStream_t st) {
+  const int64_t most = rn_max_blocks(threads);
+  for (a.tile0 = 0; a.tile0 < blocks; a.tile0 += most)
+    hipLaunchKernelGGL(k, dim3((unsigned)std::min(most, blocks - a.tile0)), dim3(threads), lds, st, a);
+  return check_launch(BWD ? "residual_norm backward" : "residual_norm");
+}
+
 template <bool BWD, class T, class TH>
 int rn_launch_wide(const RnArgs& a, int64_t blocks, hipStream_t st) {
   void (*k)(RnArgs);
   if constexpr (BWD) k = a.pw ? k_rn_bwd_wide<T, TH, true> : k_rn_bwd_wide<T, TH, false>;
   else k = a.pw ? k_rn_fwd_wide<T, TH, true> : k_rn_fwd_wide<T, TH, false>;
-  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * kWideWaves), sizeof(float) * 2 * kWideWaves * 2 * 64, st, a);
-  return check_launch(BWD ? "residual_norm backward" : "residual_norm");
+  return rn_launch<BWD>(k, a, blocks, 64 * kWideWaves, sizeof(float) * 2 * kWideWaves * 2 * 64, st);
 }
 
 template <bool BWD, class T, class TH, int V, int NC, bool FULL>
@@ -964,8 +972,7 @@ int rn_launch_tile(const RnArgs& a, int64_t blocks, hipStream_t st) {
   else
     k = a.pw ? (fg ? k_rn_fwd<T, TH, V, NC, FULL, true, true> : k_rn_fwd<T, TH, V, NC, FULL, true, false>)
              : (fg ? k_rn_fwd<T, TH, V, NC, FULL, false, true> : k_rn_fwd<T, TH, V, NC, FULL, false, false>);
-  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * nw), lds, st, a);
-  return check_launch(BWD ? "residual_norm backward" : "residual_norm");
+  return rn_launch<BWD>(k, a, blocks, 64 * nw, lds, st);
 }
 
 template <class T, class TH>

@@ -285,8 +285,9 @@ int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, int h_type, 
                           float norm_eps, void* r, void* y, float* stats, cvn_stream_t stream);
 /* Its gradients from those of r and y (either may be NULL: zero).  base: the forward's r where x is float32; x itself
  * where x is a 16-bit type (the rounded r would not give r's norm), and then h is read too wherever the forward had
- * one (CVN_ERR_ARG for NULL with grad_r or grad_h beside grad_y).  Otherwise h may be NULL without scale, gate and post_w.  Outputs may each be NULL; grad_h without scale, gate
- * and post_w is grad_x rounded to h_type.  The sums over pixels are added up in the same order on every call. */
+ * one (CVN_ERR_ARG for NULL with grad_r or grad_h beside grad_y).  Otherwise h may be NULL without scale, gate and
+ * post_w.  Outputs may each be NULL; grad_h without scale, gate and post_w is grad_x rounded to h_type.  The sums over
+ * pixels are added up in the same order on every call. */
 size_t cvn_residual_norm_bwd_workspace(int64_t B, int64_t C, int64_t HW, int gate_kind);
 int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, const void* base, int x_type, const void* h,
                           int h_type, int64_t B, int64_t C, int64_t HW, const float* res_scale, const void* gate,

@@ -708,3 +708,63 @@ def test_means_beyond_the_root_of_float32(C, t):
     lim = 4 * U * (a["w"].abs() + a["b"].abs()).double().view(cf) + want.abs() * torch.finfo(t).eps / 2 * 1.001
     for got in (y, post):
         assert ((got.double().cpu() - want).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("shape", [(1024, 65536, 1), (1 << 20, 64, 2)])
+def test_many_gates_of_samples(shape):
+    """2^26 gates and more: a wave for each is more threads than one launch holds."""
+    from conversenet_amd import functional as Fh
+
+    B, C, n = shape
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, h, gr = (torch.randn(shape, device="cuda", generator=g).requires_grad_(i < 2) for i in range(3))
+    gate = torch.rand(B, C, device="cuda", generator=g).requires_grad_(True)
+    s = torch.randn(C, device="cuda", generator=g).requires_grad_(True)
+    r, _ = Fh.residual_norm_train(x, h, None, s, gate)
+    gx, gh, gg, gs = torch.autograd.grad(r, (x, h, gate, s), gr)
+    assert torch.equal(gx, gr)
+    for part in (slice(0, 64), slice(B // 2, B // 2 + 64), slice(B - 64, B)):
+        hp, dp, gp, sp = h[part].double(), gr[part].double(), gate[part].double()[..., None], s.double()[:, None]
+        want = x[part].double() + sp * gp * hp
+        assert ((r[part].double() - want).abs() <= 3 * U * ((sp * gp * hp).abs() + want.abs())).all()
+        want = sp * gp * dp
+        assert ((gh[part].double() - want).abs() <= 3 * U * want.abs()).all()
+        terms = dp * hp * sp
+        assert ((gg[part].double() - terms.sum(2)).abs() <= 4 * U * terms.abs().sum(2)).all()
+    want, size = torch.zeros(2, C, dtype=torch.float64, device="cuda")
+    for part in range(0, B, B // 8):
+        terms = (gr[part:part + B // 8] * h[part:part + B // 8].double() * gate[part:part + B // 8, :, None]).detach()
+        want += terms.sum((0, 2))
+        size += terms.abs().sum((0, 2))
+    P = B * n
+    assert ((gs.double() - want).abs() <= (256 + P / 64) * U * size).all()
+
+
+def test_more_tiles_than_one_launch_holds():
+    """1.45e9 pixels of 33 channels, 3 waves a tile: as many launches as they take, on either side of whose border (and at
+    both ends) pixels are what a call on them alone gives."""
+    from conversenet_amd import _lib, functional as Fh
+
+    C, n = 33, 1_450_000_000
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 2 * 2 * C * n + (8 << 30):
+        pytest.skip("needs 200 GB of device memory")
+    w, b = torch.randn(2, C, device="cuda")
+    border = ((1 << 32) - 1) // 192 // 64 * 64 * 64
+    assert 4096 < border < n - 4096
+    try:
+        x, y = (torch.empty(1, C, n, dtype=BF16, device="cuda") for _ in range(2))
+        parts = [slice(0, 2048), slice(border - 2048, border + 2048), slice(n - 2048, n)]
+        for p in parts:
+            x[:, :, p] = torch.randn(1, C, p.stop - p.start, device="cuda")
+            y[:, :, p] = 7.0
+        rc = _lib.load().cvn_residual_norm_fwd(
+            x.data_ptr(), _lib.TYPES[BF16], None, _lib.TYPES[BF16], 1, C, n, None, None, 0, None, None, 0.0, w.data_ptr(),
+            b.data_ptr(), EPS, None, y.data_ptr(), None, torch.cuda.current_stream().cuda_stream)
+        _lib.check(rc, "residual_norm")
+        for p in parts:
+            part = x[:, :, p].contiguous().requires_grad_(True)
+            assert torch.equal(y[:, :, p], Fh.layernorm_cf_train(part, w, b, EPS))
+    finally:
+        x = y = part = None
+        torch.cuda.empty_cache()
