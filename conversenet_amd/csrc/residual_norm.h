@@ -29,7 +29,8 @@ struct RnArgs {
   // backward
   const void *gr, *gy;
   void *dx, *dh, *dg;
-  float *part, *dgpart;  // [kRnSums][C][blocks]; [B C][tps]
+  void* part;     // [kRnSums][C][blocks], double for many channels, float otherwise
+  float* dgpart;  // [B C][tps]
   int64_t C, HW, total;  // total = B HW
   int64_t ntiles;
   int64_t tile0;    // the first tile of a forward's launch

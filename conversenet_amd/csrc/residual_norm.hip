@@ -10,7 +10,8 @@ namespace {
 // The parameters' gradients from the blocks' sums, and the per-sample gates' from their tiles': a wave per channel or
 // gate, in 64 bits, in the same order on every call.
 struct RnSumArgs {
-  const float *part, *dgpart;
+  const void* part;
+  const float* dgpart;
   const float *s, *pw, *pb;
   float *dw, *db, *ds, *dpw, *dpb;
   void* dg;  // (B C) of type dg_type, or null
@@ -19,11 +20,12 @@ struct RnSumArgs {
   int64_t rows;  // C, and B C for the gates
 };
 
-__device__ __forceinline__ double rn_row_sum(const float* p, int n, int lane) {
+template <class T>
+__device__ __forceinline__ double rn_row_sum(const T* p, int n, int lane) {
   double s[4] = {0., 0., 0., 0.};
   int i = lane;
   for (; i + 192 < n; i += 256) {
-    float v[4];
+    T v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = p[i + 64 * j];
 #pragma unroll
@@ -36,6 +38,7 @@ __device__ __forceinline__ double rn_row_sum(const float* p, int n, int lane) {
   return t;
 }
 
+template <class T>
 __global__ void __launch_bounds__(256) k_rn_sums(RnSumArgs a) {
   const int lane = threadIdx.x & 63;
   for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.rows; row += (int64_t)gridDim.x * 4) {
@@ -49,7 +52,7 @@ __global__ void __launch_bounds__(256) k_rn_sums(RnSumArgs a) {
       continue;
     }
     const int c = (int)row;
-    auto sum = [&](int k) { return rn_row_sum(a.part + ((int64_t)k * a.C + c) * a.G, a.G, lane); };
+    auto sum = [&](int k) { return rn_row_sum((const T*)a.part + ((int64_t)k * a.C + c) * a.G, a.G, lane); };
     const double w = a.dw ? sum(0) : 0., b = a.db ? sum(1) : 0.;
     const double sa = a.dpb || (a.ds && a.pw) ? sum(2) : 0., sh = a.ds || a.dpw ? sum(3) : 0.;
     if (lane) continue;
@@ -60,6 +63,10 @@ __global__ void __launch_bounds__(256) k_rn_sums(RnSumArgs a) {
     if (a.dpw) a.dpw[c] = (float)(s * sh);
     if (a.dpb) a.dpb[c] = (float)(s * sa);
   }
+}
+
+size_t rn_part_bytes(int64_t C, const RnShape& t) {
+  return align_up((t.px ? sizeof(float) : sizeof(double)) * kRnSums * (size_t)C * (size_t)rn_bwd_blocks(t));
 }
 
 bool rn_kernels(int x_type, int h_type, RnKernels* k) {
@@ -137,7 +144,7 @@ extern "C" size_t cvn_residual_norm_bwd_workspace(int64_t B, int64_t C, int64_t 
   if (rn_shape_ok(B, C, HW, CVN_F32, CVN_F32, &k) != CVN_OK) return 0;
   const bool sample = gate_kind == CVN_GATE_SAMPLE;
   const RnShape t = rn_shape(true, B, C, HW, sample);
-  const size_t part = align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)rn_bwd_blocks(t));
+  const size_t part = rn_part_bytes(C, t);
   return part + (sample ? sizeof(float) * (size_t)(B * C) * (size_t)t.tps : 0) + 256;
 }
 
@@ -169,8 +176,8 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   const int64_t G = rn_bwd_blocks(t);
   hipStream_t st = (hipStream_t)stream;
   RnArgs a = {};
-  a.part = (float*)align_up((size_t)workspace);
-  a.dgpart = (float*)((char*)a.part + align_up(sizeof(float) * kRnSums * (size_t)C * (size_t)G));
+  a.part = (void*)align_up((size_t)workspace);
+  a.dgpart = (float*)((char*)a.part + rn_part_bytes(C, t));
   a.x = base;
   a.h = h;
   a.gate = gate;
@@ -215,6 +222,6 @@ extern "C" int cvn_residual_norm_bwd(const void* grad_r, const void* grad_y, con
   s.rows = C + (s.dg ? B * C : 0);
   if (!s.dw && !s.db && !s.ds && !s.dpw && !s.dpb && !s.dg) return CVN_OK;
   // a block for every 4 rows, as far as one launch goes: 2^26 gates of one tile each are more
-  hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)std::min((s.rows + 3) / 4, rn_max_blocks(256))), dim3(256), 0, st, s);
+  hipLaunchKernelGGL(t.px ? k_rn_sums<float> : k_rn_sums<double>, dim3((unsigned)std::min((s.rows + 3) / 4, rn_max_blocks(256))), dim3(256), 0, st, s);
   return check_launch("residual_norm sums");
 }

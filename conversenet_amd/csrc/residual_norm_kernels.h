@@ -175,13 +175,15 @@ __device__ __forceinline__ void rn_get(float (&v)[V], const float* p) {
   }
 }
 
+constexpr int kRnRed = 2 * 2 * 64;  // floats of red for each wave and pixel of a lane
+
 // Two values per pixel over the waves of a block, which each wave joins in the order of the waves.  red: two buffers of
 // nw 2 V 64 floats, taken in turn, so that one barrier a time is enough: a buffer is written again only after the
 // barrier of the other, which a wave reaches after its reads.
 template <int V>
 __device__ __forceinline__ const float* rn_exchange(float* red, int& turn, int nw, int wave, int lane,
                                                     const float (&v)[2][V]) {
-  float* buf = red + turn * nw * (2 * V * 64) + lane * V;
+  float* buf = red + turn * nw * (kRnRed / 2 * V) + lane * V;
   turn ^= 1;
 #pragma unroll
   for (int k = 0; k < 2; ++k) rn_put<V>(buf + (2 * wave + k) * (V * 64), v[k]);
@@ -445,7 +447,16 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
   const bool norm = a0.nw && a0.gy, branch = a0.dh || a0.dg || a0.s || POST, sample = !FG && a0.gate;
   const int mine = lane / (64 / NC);  // the channel whose sums this lane ends with
   int turn = 0;
-  float acc[kRnSums] = {};  // the sums so far of channel c0 + mine
+  // The sums so far of channel c0 + mine, in 64 bits: float32 ones lose half a step a tile, and a block takes hundreds of a
+  // large map.  In shared memory, where one lane alone adds to each, in the order of its tiles; in registers they spill
+  // (8 x 64 x 256 x 256 bf16, gate per element: 137 us, against 121).
+  const bool owns = lane % (64 / NC) == 0 && mine < n;
+  double* const sums = (double*)(red + (nw == 1 ? 0 : kRnRed * V * nw)) + c0 + mine;
+  auto add = [&](int q, float v) {
+    if (owns) __hip_atomic_fetch_add(sums + q * C, (double)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  if (owns)
+    for (int q = 0; q < kRnSums; ++q) sums[q * C] = 0.;
   for (int64_t next = blockIdx.x; next < a0.ntiles; next += gridDim.x) {
     const int64_t tile = rn_order((uint32_t)next, (uint32_t)a0.ntiles);
     RnArgs a = a0;
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
           t[i] = fmaf(d[i][j], r[i][j], t[i]);
         }
       }
-      acc[0] += rn_lane_sums<NC>(t, lane);
+      add(0, rn_lane_sums<NC>(t, lane));
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const float w = i < n ? rn_const(a.nw, c0 + min(i, n - 1)) : 0.f;
@@ -528,7 +539,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
           s[1][j] = fmaf(d[i][j], r[i][j], s[1][j]);
         }
       }
-      acc[1] += rn_lane_sums<NC>(t, lane);
+      add(1, rn_lane_sums<NC>(t, lane));
       load_gate();
       rn_block_sums<V>(red, turn, nw, wave, lane, s);
 #pragma unroll
@@ -589,7 +600,7 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
           for (int j = 0; j < V; ++j) t[i] += d[i][j];
         }
         va = rn_lane_sums<NC>(t, lane);
-        acc[2] = fmaf(gt, va, acc[2]);
+        add(2, gt * va);
       }
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
@@ -598,8 +609,8 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
         for (int j = 0; j < V; ++j) t[i] = fmaf(d[i][j], h[i][j], t[i]);
       }
       const float vh = rn_lane_sums<NC>(t, lane);
-      acc[3] = fmaf(gt, vh, acc[3]);
-      if (sample && a.dg && lane % (64 / NC) == 0 && mine < n) {
+      add(3, gt * vh);
+      if (sample && a.dg && owns) {
         const float v = POST ? fmaf(a.pw[c], vh, a.pb[c] * va) : vh;
         a.dgpart[(px.b * C + c) * a.tps + tile % a.tps] = a.s ? a.s[c] * v : v;
       }
@@ -634,15 +645,15 @@ __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
       for (int i = 0; i < NC; ++i)
         if (i < n) rn_store_own<TH, V>((TH*)a.dh + at + i * HW, d[i], px);
   }
-  if (lane % (64 / NC) == 0 && mine < n)
-#pragma unroll
-    for (int q = 0; q < kRnSums; ++q) a0.part[((int64_t)q * C + c0 + mine) * gridDim.x + blockIdx.x] = acc[q];
+  if (owns)
+    for (int q = 0; q < kRnSums; ++q)
+      ((float*)a0.part)[((int64_t)q * C + c0 + mine) * gridDim.x + blockIdx.x] = (float)sums[q * C];
 }
 
 // ------------------------------------------------------------------------------------------------
 // More channels: a block of 16 waves per tile of 64 pixels, a pixel to a lane, each wave taking 16 channels of every 256
 // in turn.  The channels are read again for each step of the formulas, from the caches (a tile of 512 float32 channels is
-// 128 KB), and the sums over pixels are added to the block's row in memory.
+// 128 KB), and the sums over pixels are added to the block's row in memory, in 64 bits.
 // ------------------------------------------------------------------------------------------------
 constexpr int kWideWaves = 16, kWideCh = 16;
 
@@ -809,9 +820,9 @@ __global__ void __launch_bounds__(64 * kWideWaves) k_rn_bwd_wide(RnArgs a) {
       e.rh[0] = a.stats[3 * a.total + e.px.q];
     }
     // Adds a channel's sum over the tile, which the wave's lane `mine` of it holds, to the block's row.
-    auto add = [&](int k, int c0, int n, float v) {
+    auto add = [&](int k, int c0, int n, double v) {
       if (lane % (64 / kWideCh) || mine >= n) return;
-      float* o = a.part + ((int64_t)k * C + c0 + mine) * gridDim.x + blockIdx.x;
+      double* o = (double*)a.part + ((int64_t)k * C + c0 + mine) * gridDim.x + blockIdx.x;
       *o = tile == blockIdx.x ? v : *o + v;
     };
     // rhat and gy; a lane without a pixel of its own: zeros
@@ -900,12 +911,12 @@ __global__ void __launch_bounds__(64 * kWideWaves) k_rn_bwd_wide(RnArgs a) {
 #pragma unroll
         for (int i = 0; i < kWideCh; ++i) t[i] = d[i];
         va = rn_lane_sums<kWideCh>(t, lane);
-        add(2, c0, n, gt * va);
+        add(2, c0, n, (double)gt * va);
       }
 #pragma unroll
       for (int i = 0; i < kWideCh; ++i) t[i] = d[i] * h[i];
       const float vh = rn_lane_sums<kWideCh>(t, lane);
-      add(3, c0, n, gt * vh);
+      add(3, c0, n, (double)gt * vh);
       if (a.dg && sample && lane % (64 / kWideCh) == 0 && mine < n) {
         const float v = POST ? fmaf(a.pw[c], vh, a.pb[c] * va) : vh;
         a.dgpart[(e.px.b * C + c) * a.tps + tile % a.tps] = a.s ? a.s[c] * v : v;
@@ -957,13 +968,13 @@ int rn_launch_wide(const RnArgs& a, int64_t blocks, hipStream_t st) {
   void (*k)(RnArgs);
   if constexpr (BWD) k = a.pw ? k_rn_bwd_wide<T, TH, true> : k_rn_bwd_wide<T, TH, false>;
   else k = a.pw ? k_rn_fwd_wide<T, TH, true> : k_rn_fwd_wide<T, TH, false>;
-  return rn_launch<BWD>(k, a, blocks, 64 * kWideWaves, sizeof(float) * 2 * kWideWaves * 2 * 64, st);
+  return rn_launch<BWD>(k, a, blocks, 64 * kWideWaves, sizeof(float) * kRnRed * kWideWaves, st);
 }
 
 template <bool BWD, class T, class TH, int V, int NC, bool FULL>
 int rn_launch_tile(const RnArgs& a, int64_t blocks, hipStream_t st) {
   const int nw = (int)((a.C + NC - 1) / NC);
-  const size_t lds = nw == 1 ? 0 : sizeof(float) * 2 * nw * 2 * V * 64;
+  const size_t lds = (nw == 1 ? 0 : sizeof(float) * kRnRed * V * nw) + (BWD ? sizeof(double) * kRnSums * a.C : 0);
   const bool fg = a.gate && a.gate_full;
   void (*k)(RnArgs);
   if constexpr (BWD)
@@ -972,6 +983,8 @@ int rn_launch_tile(const RnArgs& a, int64_t blocks, hipStream_t st) {
   else
     k = a.pw ? (fg ? k_rn_fwd<T, TH, V, NC, FULL, true, true> : k_rn_fwd<T, TH, V, NC, FULL, true, false>)
              : (fg ? k_rn_fwd<T, TH, V, NC, FULL, false, true> : k_rn_fwd<T, TH, V, NC, FULL, false, false>);
+  if (BWD && lds > 64 * 1024)  // 121 to 128 channels
+    (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   return rn_launch<BWD>(k, a, blocks, 64 * nw, lds, st);
 }
 

@@ -768,3 +768,28 @@ def test_more_tiles_than_one_launch_holds():
     finally:
         x = y = part = None
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("C,H,W", [(64, 4096, 4096), (128, 2048, 4096), (200, 2048, 2048), (272, 2048, 2048)])
+def test_sums_over_many_pixels(C, H, W):
+    """The parameters' gradients of a map of equal pixels are those of 1024 of its pixels times a whole number: tiles of
+    equal sums, which 64 bits add up exactly, so that either is off by at most two roundings, of a block's sum and of the
+    gradient.  (In 32 bits a block's sum loses up to half a step a tile, always to one side.)"""
+    from conversenet_amd import functional as Fh
+
+    g = torch.Generator().manual_seed(C)
+    row = {k: torch.randn(1, C, 1, 1, generator=g).cuda() for k in ("x", "h", "gate", "gr", "gy")}
+    p = {k: torch.randn(C, generator=g).cuda().requires_grad_(True) for k in ("s", "w", "b", "pw", "pb")}
+
+    def sums(H, W):
+        d = {k: v.expand(1, C, H, W).contiguous() for k, v in row.items()}
+        out = Fh.residual_norm_train(d["x"], d["h"], (p["w"], p["b"], EPS), p["s"], d["gate"], (p["pw"], p["pb"], EPS))
+        return dict(zip(p, torch.autograd.grad(out, list(p.values()), (d["gr"], d["gy"]))))
+
+    n = H * W // 1024
+    big, small = sums(H, W), sums(32, 32)
+    size = {k: v.double().abs() for k, v in small.items()}
+    # the scale's gradient is a sum of two: the branch norm's, over the scale, times its parameters
+    size["s"] = (size["pw"] * p["pw"].abs() + size["pb"] * p["pb"].abs()) / p["s"].abs()
+    for k in p:
+        assert ((big[k].double() - n * small[k].double()).abs() <= 4 * U * 1.001 * n * size[k]).all(), k
