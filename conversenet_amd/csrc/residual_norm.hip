@@ -127,7 +127,7 @@ extern "C" int cvn_residual_norm_fwd(const void* x, int x_type, const void* h, i
   a.pb = post_b;
   a.neps = norm_eps;
   a.peps = post_eps;
-  a.r = h ? r : nullptr;
+  a.r = r;
   a.y = y;
   a.stats = stats;
   a.C = C;

@@ -390,16 +390,16 @@ __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         x[i][j] = fmaf(k[i], FG ? h[i][j] * rn_at<TH, V>(g[FG ? i : 0], j) : h[i][j], rn_at<T, V>(xr[i], j));
-    if (px.any())
-#pragma unroll
-      for (int i = 0; i < NC; ++i)
-        if (i < n) rn_store<T, V>((T*)a.r + at + i * HW, px.off, x[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) x[i][j] = rn_at<T, V>(xr[i], j);
   }
+  if (a.r && px.any())
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (i < n) rn_store<T, V>((T*)a.r + at + i * HW, px.off, x[i]);
   if (!a.nw) return;
   float mu[V], rho[V];
   rn_block_moments<V, NC, FULL>(red, turn, nw, wave, lane, C, n, a.neps, x, mu, rho);

@@ -700,9 +700,9 @@ def _norm_args(x, h, gate):
     return (shape[0], shape[1], math.prod(shape[2:]), _gate_kind(h, gate)), index
 
 
-def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
+def _residual_norm(x, h, norm, res_scale, gate, post, need_stats, copy=False):
     """The launch behind residual_norm, on contiguous x, h and gate: (r, y, stats, what _norm_args gave, whether the
-    parameters were read where they are), None for what there is not."""
+    parameters were read where they are), None for what there is not.  copy: r is a copy of x where there is no h."""
     lib = _lib.load()
     geo, index = _norm_args(x, h, gate)
     B, C, HW, kind = geo
@@ -717,7 +717,7 @@ def _residual_norm(x, h, norm, res_scale, gate, post, need_stats):
     if post is not None:
         pw, pb = _param32(keep, post[0], C, index, "branch norm"), _param32(keep, post[1], C, index, "branch norm")
         peps = float(post[2])
-    if h is not None:
+    if h is not None or copy:
         r = torch.empty_like(x)
     dev = x.device
     if need_stats and (norm is not None or post is not None):
@@ -866,43 +866,43 @@ class ResidualNormFunction(torch.autograd.Function):
     composition of torch operations."""
 
     @staticmethod
-    def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps):
+    def forward(ctx, x, h, res_scale, gate, post_w, post_b, norm_w, norm_b, post_eps, norm_eps, copy=False):
         # x, h and gate are contiguous: a copy made here would not be the caller's in a differentiated backward
         ctx.set_materialize_grads(False)
         post = None if post_w is None else (post_w, post_b, post_eps)
         norm = None if norm_w is None else (norm_w, norm_b, norm_eps)
-        r, y, stats, geo, direct = _residual_norm(x, h, norm, res_scale, gate, post, True)
+        r, y, stats, geo, direct = _residual_norm(x, h, norm, res_scale, gate, post, True, copy)
         f32 = x.dtype is torch.float32
         keep_h = h is not None and not (f32 and res_scale is None and gate is None and post is None)
-        base = None if norm is None else (r if h is not None and f32 else x)
+        base = None if norm is None else (r if copy or (h is not None and f32) else x)
         ctx.save_for_backward(base, h if keep_h else None, res_scale, gate, post_w, post_b, norm_w, norm_b, stats)
-        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape, direct)
+        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape, direct, r is not None)
         return r if y is None else y if r is None else (r, y)
 
     @staticmethod
     def backward(ctx, *gos):
         base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = ctx.saved_tensors
-        post_eps, norm_eps, h_dtype, x_dtype, geo, shape, direct = ctx.cfg
-        gr = gos[0] if h_dtype is not None else None
+        post_eps, norm_eps, h_dtype, x_dtype, geo, shape, direct, has_r = ctx.cfg
+        gr = gos[0] if has_r else None
         gy = gos[-1] if norm_w is not None else None
         need = ctx.needs_input_grad[:8]
         if gr is None and gy is None:
-            return (None,) * 10
+            return (None,) * 11
         if torch.is_grad_enabled() or torch._C._len_torch_dispatch_stack() or _pre_dispatch() or not (
                 _in_memory(gr) and _in_memory(gy)):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
-                                                     h_dtype, x_dtype, need) + (None, None)
+                                                     h_dtype, x_dtype, need) + (None, None, None)
         # a saved-tensor hook may have given any of them other strides
         base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = map(
             _contiguous, (base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats))
         got = _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, gate, post_w, post_b, geo, shape,
                                       x_dtype, h_dtype, need, direct)
         if direct:  # float32 parameters, as their gradients
-            return got + (None, None)
+            return got + (None, None, None)
         gx, gh, gs, gg, *gp = got
         like = lambda g, t: g if g is None or t.dtype is torch.float32 else g.to(t.dtype)  # noqa: E731
-        return (gx, gh, like(gs, res_scale), gg, *map(like, gp, (post_w, post_b, norm_w, norm_b)), None, None)
+        return (gx, gh, like(gs, res_scale), gg, *map(like, gp, (post_w, post_b, norm_w, norm_b)), None, None, None)
 
 
 def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy, h_dtype, x_dtype,
@@ -970,9 +970,13 @@ def residual_norm_train(x, h, norm=None, res_scale=None, gate=None, post=None):
     return (out, None) if norm is None else out
 
 
-def layernorm_cf_train(x, weight, bias, eps):
-    """Differentiable layernorm_cf on the HIP kernels (forward and backward)."""
-    return ResidualNormFunction.apply(_contiguous(x), None, None, None, None, None, weight, bias, 0.0, eps)
+def layernorm_cf_train(x, weight, bias, eps, copy=False):
+    """Differentiable layernorm_cf on the HIP kernels (forward and backward).  copy: the backward reads a copy of x that the
+    forward makes, so that x may be changed in place after it."""
+    if not copy:
+        return ResidualNormFunction.apply(_contiguous(x), None, None, None, None, None, weight, bias, 0.0, eps)
+    # the copy is an output, which a differentiated backward reaches x through
+    return ResidualNormFunction.apply(_contiguous(x), None, None, None, None, None, weight, bias, 0.0, eps, True)[1]
 
 
 def _grad_list(ts):

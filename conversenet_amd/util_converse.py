@@ -136,7 +136,7 @@ class LayerNorm(nn.Module):
         if _hip_eligible(x, self.weight, self.bias) and x.dim() >= 2:
             return functional.layernorm_cf(x, self.weight, self.bias, self.eps)
         if _norm_grad_eligible(x, self.weight, self.bias):
-            return functional.layernorm_cf_train(x, self.weight, self.bias, self.eps)
+            return functional.layernorm_cf_train(x, self.weight, self.bias, self.eps, copy=True)
         u = x.mean(1, keepdim=True)
         s = (x - u).pow(2).mean(1, keepdim=True)
         x = (x - u) / torch.sqrt(s + self.eps)
@@ -364,7 +364,7 @@ def _block_train(blk, x, n=None, next_ln=None):
     """A block under autograd, each residual fused with the norm behind it: (output, next_ln of it).  n: the block's first
     norm of x, where the previous block has it."""
     if n is None:
-        n = functional.layernorm_cf_train(x, blk.conv1[0].weight, blk.conv1[0].bias, blk.conv1[0].eps)
+        n = functional.layernorm_cf_train(x, blk.conv1[0].weight, blk.conv1[0].bias, blk.conv1[0].eps, copy=True)
     a1, a2 = (blk.alpha1, blk.alpha2) if hasattr(blk, "alpha1") else (None, None)
     for m in list(blk.conv1)[1:]:
         n = m(n)

@@ -274,7 +274,7 @@ enum { CVN_NORM_2 = 0, CVN_NORM_INF = 1 };
  *   r = x + res_scale[c] * gate * P(h),  y = N(r)
  * P: LayerNorm over the channels of h with (post_w, post_b, post_eps), or h itself where post_w is NULL; N: the same
  * of r with (norm_w, norm_b, norm_eps), or no y where norm_w is NULL; res_scale (C) and gate may be NULL.  h NULL:
- * y = N(x) alone, r is not written.  x, r, y: (B,C,HW) of x_type; h, gate: of h_type, which is x_type or, on a float32
+ * y = N(x) alone, and r, which may be NULL then, a copy of x.  x, r, y: (B,C,HW) of x_type; h, gate: of h_type, which is x_type or, on a float32
  * x, a 16-bit type; the parameters fp32.  Computed in fp32 and rounded once, r before its norm not at all.
  * stats: NULL, or fp32 (4,B HW), which the backward reads: mean and 1/deviation of r, then of h (rows of norms that
  * are not there are not written).  No output may share memory with an input or another output.  Up to 65536 channels

@@ -274,3 +274,59 @@ def test_a_norms_own_forward_is_called():
     m.conv2[0].register_forward_hook(lambda mod, i, o: 2 * o)
     _close(twice, _run(m, x, go), 1e-4)
     assert float((twice[0] - want[0]).abs().max()) > 1e-3
+
+
+@pytest.mark.parametrize("second", [False, True])
+def test_input_changed_in_place_behind_a_module(second):
+    """x += block(x), and the like: the backward has the values that the module had, as the composition's."""
+    for m in (_fill(U.LayerNorm(24, eps=1e-6, data_format="channels_first")),
+              _fill(U.ConverseBlockAlphaVariant(24, 24, kernel_size=3, padding=1, padding_mode="circular"))):
+        x, go = _inputs((2, 24, 9, 11))
+
+        def run(m, x, go, change):
+            x = x.clone().requires_grad_(True)
+            z = x * 1.5
+            y = m(z)
+            if change:
+                z.add_(y)
+            else:
+                z = z + y
+            if not second:
+                return torch.autograd.grad(z, [x, *m.parameters()], go)
+            gx, = torch.autograd.grad(z, x, go, create_graph=True)
+            return torch.autograd.grad((gx ** 2).sum(), x)
+
+        ref = run(copy.deepcopy(m).double(), x.double(), go.double(), False)
+        if type(m) is U.LayerNorm or not second:  # (Converse2D's backward is not differentiable)
+            _close(run(m.cuda(), x.cuda(), go.cuda(), True), ref, 1.6e-4, type(m).__name__)
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.to(memory_format=torch.channels_last) if t.dim() == 4 else t,
+                                    lambda t: torch.stack([t, t * 0], -1)[..., 0]])
+def test_saved_tensors_with_other_strides(unpack):
+    """Saved-tensor hooks that keep values, sizes and types, but not strides."""
+    for m, tol in ((_fill(U.LayerNorm(24, eps=1e-6, data_format="channels_first")), 1e-5),
+                   (_fill(U.ConverseBlockAlphaVariant(24, 24, kernel_size=3, padding=1, padding_mode="circular")), 1.6e-4)):
+        x, go = _inputs((2, 24, 9, 11))
+        ref = _run(copy.deepcopy(m).double(), x.double(), go.double())
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+            got = _run(m.cuda(), x.cuda(), go.cuda())
+        _close(got, ref, tol, type(m).__name__)
+    with torch.autograd.graph.save_on_cpu():
+        _close(_run(m, x.cuda(), go.cuda()), ref, tol)
+
+
+def test_traced_on_the_device():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    m = _fill(U.LayerNorm(16, eps=1e-6, data_format="channels_first")).cuda()
+
+    def step(x, go):
+        y = m(x)
+        return (y, *torch.autograd.grad(y, (x, m.weight), go))
+
+    x, go = (t.cuda() for t in _inputs((1, 16, 5, 6)))
+    graph = make_fx(step)(x.clone().requires_grad_(True), go)
+    x, go = (t.cuda() for t in _inputs((1, 16, 5, 6), seed=9))
+    x.requires_grad_(True)
+    _close(graph(x, go), [t.detach() for t in step(x, go)], 1e-5)

@@ -134,6 +134,17 @@ def _norm_module(C=3):
     return m
 
 
+def _block():
+    """A block of three channels whose convolutions are torch's."""
+    from conversenet_amd import util_converse as U
+
+    blk = U.ConverseBlockAlphaVariant(3, 3, kernel_size=3, padding=1)
+    for m in blk.modules():
+        if isinstance(m, U.Converse2D):
+            m.backend = "pytorch"
+    return blk
+
+
 def _definition(m, x):
     d = x - x.mean(1, keepdim=True)
     hat = d / torch.sqrt(d.pow(2).mean(1, keepdim=True) + EPS)
@@ -292,3 +303,20 @@ def test_a_gradient_that_is_a_negated_view(library):
     functional.clip_grads(grads, 1.0, out=grads)
     functional.clip_grad_norm_(ps, 1.0)
     assert all(torch.equal(p.grad, k / 4) for p, k in zip(ps, keep))
+
+
+def test_a_map_changed_after_its_norm(on_device):
+    """A module's input may be changed in place behind it, as the composition allows: its backward has the values that the
+    norm had."""
+    m = _norm_module()
+    x = torch.randn(2, 3, 4, 5, requires_grad=True)
+    z = x * 1.0
+    y = m(z)
+    z.add_(1.0)
+    torch.autograd.grad(y, x, torch.randn(2, 3, 4, 5))
+    assert torch.equal(on_device.read["base"], torch.arange(1.0, 121))  # the copy that the forward made
+    blk = _block()
+    z = x * 1.0
+    out = blk(z)
+    z.mul_(2.0)
+    torch.autograd.grad(out, x, torch.ones_like(x))
