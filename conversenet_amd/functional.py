@@ -754,7 +754,7 @@ def _norm_workspace(geo):
     return _lib.load().cvn_residual_norm_bwd_workspace(*geo)
 
 
-def _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, gate, post_w, post_b, geo, shape, x_dtype,
+def _residual_norm_backward(gr, gy, base, h, stats, norm_w, nb_shape, res_scale, gate, post_w, post_b, geo, shape, x_dtype,
                             h_dtype, need, direct=False):
     """The launches behind residual_norm_backward, on arguments that a forward has checked; direct: it read the
     parameters where they are."""
@@ -779,12 +779,14 @@ def _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, g
     if gy is not None:
         if nx or same:
             gx = out_x = torch.empty_like(some)
-        gnw, gnb = like(norm_w, nnw), like(norm_b, nnb)
+        gnw = like(norm_w, nnw)
+        if nnb:  # (empty_like where it can be)
+            gnb = like(norm_w, True) if norm_w.shape == nb_shape else torch.empty(nb_shape, dtype=f32, device=dev)
     else:  # x's gradient is r's
         gx = gr
         if norm_w is not None:  # y was not used
-            gnw, gnb = (torch.zeros(t.shape, dtype=f32, device=dev) if w else None
-                        for t, w in ((norm_w, nnw), (norm_b, nnb)))
+            gnw, gnb = (torch.zeros(t, dtype=f32, device=dev) if w else None
+                        for t, w in ((norm_w.shape, nnw), (nb_shape, nnb)))
     if same:
         gh = gx
     elif nh and plain and gy is None:
@@ -841,8 +843,9 @@ def residual_norm_backward(grad_r, grad_y, base, h, stats, norm_weight=None, res
     if grad_r is None and grad_y is None:
         raise RuntimeError("residual_norm_backward needs a gradient")
     pw, pb = (None, None) if post is None else post[:2]
-    return _residual_norm_backward(grad_r, grad_y, _contiguous(base), h, stats, norm_weight, norm_weight, res_scale, gate, pw,
-                                   pb, geo, ref.shape, ref.dtype, h_dtype, need)
+    return _residual_norm_backward(grad_r, grad_y, _contiguous(base), h, stats, norm_weight,
+                                   None if norm_weight is None else norm_weight.shape, res_scale, gate, pw, pb, geo, ref.shape,
+                                   ref.dtype, h_dtype, need)
 
 
 def residual_norm_stats(x, h, norm=None, res_scale=None, gate=None, post=None):
@@ -875,14 +878,16 @@ class ResidualNormFunction(torch.autograd.Function):
         f32 = x.dtype is torch.float32
         keep_h = h is not None and not (f32 and res_scale is None and gate is None and post is None)
         base = None if norm is None else (r if copy or (h is not None and f32) else x)
-        ctx.save_for_backward(base, h if keep_h else None, res_scale, gate, post_w, post_b, norm_w, norm_b, stats)
-        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape, direct, r is not None)
+        # (of the norm's bias no value is needed: it may change before the backward)
+        ctx.save_for_backward(base, h if keep_h else None, res_scale, gate, post_w, post_b, norm_w, stats)
+        ctx.cfg = (post_eps, norm_eps, None if h is None else h.dtype, x.dtype, geo, x.shape, direct, r is not None,
+                   None if norm is None else norm_b.shape, None if norm is None else norm_b.dtype)
         return r if y is None else y if r is None else (r, y)
 
     @staticmethod
     def backward(ctx, *gos):
-        base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = ctx.saved_tensors
-        post_eps, norm_eps, h_dtype, x_dtype, geo, shape, direct, has_r = ctx.cfg
+        base, h, res_scale, gate, post_w, post_b, norm_w, stats = ctx.saved_tensors
+        post_eps, norm_eps, h_dtype, x_dtype, geo, shape, direct, has_r, nb_shape, nb_dtype = ctx.cfg
         gr = gos[0] if has_r else None
         gy = gos[-1] if norm_w is not None else None
         need = ctx.needs_input_grad[:8]
@@ -891,22 +896,23 @@ class ResidualNormFunction(torch.autograd.Function):
         if torch.is_grad_enabled() or torch._C._len_torch_dispatch_stack() or _pre_dispatch() or not (
                 _in_memory(gr) and _in_memory(gy)):
             post = None if post_w is None else (post_w, post_b, post_eps)
-            return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy,
-                                                     h_dtype, x_dtype, need) + (None, None, None)
+            return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, nb_shape, nb_dtype, norm_eps, gr,
+                                                     gy, h_dtype, x_dtype, need) + (None, None, None)
         # a saved-tensor hook may have given any of them other strides
-        base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats = map(
-            _contiguous, (base, h, res_scale, gate, post_w, post_b, norm_w, norm_b, stats))
-        got = _residual_norm_backward(gr, gy, base, h, stats, norm_w, norm_b, res_scale, gate, post_w, post_b, geo, shape,
+        base, h, res_scale, gate, post_w, post_b, norm_w, stats = map(
+            _contiguous, (base, h, res_scale, gate, post_w, post_b, norm_w, stats))
+        got = _residual_norm_backward(gr, gy, base, h, stats, norm_w, nb_shape, res_scale, gate, post_w, post_b, geo, shape,
                                       x_dtype, h_dtype, need, direct)
         if direct:  # float32 parameters, as their gradients
             return got + (None, None, None)
-        gx, gh, gs, gg, *gp = got
+        gx, gh, gs, gg, *gp, gb = got
         like = lambda g, t: g if g is None or t.dtype is torch.float32 else g.to(t.dtype)  # noqa: E731
-        return (gx, gh, like(gs, res_scale), gg, *map(like, gp, (post_w, post_b, norm_w, norm_b)), None, None, None)
+        return (gx, gh, like(gs, res_scale), gg, *map(like, gp, (post_w, post_b, norm_w)), None if gb is None else
+                gb.to(nb_dtype), None, None, None)
 
 
-def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, norm_b, norm_eps, gr, gy, h_dtype, x_dtype,
-                                      need):
+def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, nb_shape, nb_dtype, norm_eps, gr, gy, h_dtype,
+                                      x_dtype, need):
     """The same gradients from their formulas in differentiable torch operations."""
     ref = next(t for t in (base, h, gr, gy) if t is not None)
     cf = (1, -1) + (1,) * (ref.dim() - 2)
@@ -926,7 +932,7 @@ def _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, no
         d = composite.standardised_grad(gy * norm_w.float().view(cf), hat, rho)
         dr = d if dr is None else dr + d
         gnw = like((gy * hat).sum(pixels), norm_w) if need[6] else None
-        gnb = like(gy.sum(pixels), norm_b) if need[7] else None
+        gnb = gy.sum(pixels).reshape(nb_shape).to(nb_dtype) if need[7] else None
     gx = dr.to(x_dtype) if need[0] else None
     gh = gs = gg = gpw = gpb = None
     if h is None:

@@ -320,3 +320,13 @@ def test_a_map_changed_after_its_norm(on_device):
     out = blk(z)
     z.mul_(2.0)
     torch.autograd.grad(out, x, torch.ones_like(x))
+
+
+def test_a_bias_changed_before_the_backward(library):
+    """The gradients do not depend on the norm's bias, and do not keep it."""
+    d = _args()
+    r, y = _call(d)
+    with torch.no_grad():
+        d["b"].add_(1.0)
+    g = torch.autograd.grad((r, y), list(d.values()), (torch.ones_like(r), torch.ones_like(y)))
+    assert g[5].shape == d["b"].shape and library.read is not None
