@@ -1100,8 +1100,11 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """Scales the parameters' .grad in place so that their norm is at most max_norm; returns the norm they had.  As
-    torch.nn.utils.clip_grad_norm_; error_if_nonfinite waits for the norm and raises before any gradient changes."""
+    """Scales the parameters' .grad in place so that their norm is at most max_norm; returns the norm they had, in float32.
+    As torch.nn.utils.clip_grad_norm_, for gradients that are float32, bfloat16 or float16 on one HIP device, each in memory
+    of its own (a parameter that is passed twice is refused), max_norm >= 0 and norm_type 2 or math.inf; RuntimeError
+    otherwise.  error_if_nonfinite waits for the norm and raises before any gradient changes.  Strided gradients are copied
+    there and back."""
     grads = [g for g in [p.grad for p in _tensors(parameters)] if g is not None]
     if error_if_nonfinite and grads:
         norm = grad_norm(grads, norm_type)
@@ -1112,6 +1115,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         for g in grads:
             if 0 in g.stride() and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
                 raise RuntimeError("a gradient's elements share memory")
+        strided = [g for g, d in zip(grads, dense) if d is not g and g.numel()]
+        if len({(g.data_ptr(), g.shape, g.stride()) for g in strided}) != len(strided):
+            raise RuntimeError("two gradients share memory")
     norm = _clip(dense, dense, max_norm, norm_type)
     if dense is not grads:
         with torch.no_grad():

@@ -330,3 +330,25 @@ def test_a_bias_changed_before_the_backward(library):
         d["b"].add_(1.0)
     g = torch.autograd.grad((r, y), list(d.values()), (torch.ones_like(r), torch.ones_like(y)))
     assert g[5].shape == d["b"].shape and library.read is not None
+
+
+def test_strided_gradients_in_one_place_are_refused(library):
+    """As contiguous ones are: each would be counted twice and scaled once."""
+    p, q, r = (torch.nn.Parameter(torch.zeros(3, 4)) for _ in range(3))
+    p.grad = torch.randn(4, 3).t()
+    q.grad = p.grad.view_as(p.grad)
+    r.grad = torch.randn(3, 4)
+    for ps in ((p, p), (p, q), (r, p, q)):
+        keep = [t.grad.clone() for t in ps]
+        with pytest.raises(RuntimeError, match="share memory"):
+            functional.clip_grad_norm_(ps, 1.0)
+        assert all(torch.equal(t.grad, k) for t, k in zip(ps, keep))
+    both = torch.randn(3, 8)  # columns of one matrix share none
+    p.grad, q.grad = both[:, :4], both[:, 4:]
+    keep = both.clone()
+    functional.clip_grad_norm_((p, q, r), 1.0)
+    assert torch.equal(both, keep / 2)
+    empty = [torch.nn.Parameter(torch.zeros(0, 2)) for _ in range(2)]
+    for e in empty:
+        e.grad = torch.zeros(2, 0).t()
+    functional.clip_grad_norm_((p, *empty), 1.0)
