@@ -658,31 +658,34 @@ def _gate_kind(h, gate):
     raise RuntimeError("gate must have the branch's shape, or (B,C) or (B,C,1,..) for a factor per sample and channel")
 
 
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_tracing_state = torch._C._get_tracing_state
+
+
 def _pre_dispatch() -> int:
-    return torch._ops._len_torch_dispatch_stack_pre_dispatch() if torch._C._len_torch_function_stack() else 0
+    return torch._ops._len_torch_dispatch_stack_pre_dispatch() if _function_modes() else 0
 
 
 def observed() -> bool:
     """Whether a mode of the caller's sees torch's operations: it would miss those that the library stands for.  (A
     default device is such a mode, and changes nothing here.)"""
-    if torch._C._len_torch_dispatch_stack():
+    if _dispatch_modes():
         return True
-    return torch._C._len_torch_function_stack() > 0 and any(
-        type(m) is not DeviceContext for m in _get_current_function_mode_stack())
+    return _function_modes() > 0 and any(type(m) is not DeviceContext for m in _get_current_function_mode_stack())
 
 
 def _untraced(what):
     """Refuses a call that is being recorded as torch operations: the library's kernels are none, and the recorded graph
     would return its outputs as they were allocated."""
-    if torch._C._get_tracing_state() is not None or _pre_dispatch() or (
-            torch._C._len_torch_dispatch_stack()
-            and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+    if _tracing_state() is not None or _pre_dispatch() or (
+            _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
         raise RuntimeError(f"{what} cannot be traced as torch operations")
 
 
 def _norm_args(x, h, gate):
     """Checks the large arguments of a residual_norm call: ((B, C, HW, kind of gate), device index)."""
-    _untraced("residual_norm")
+    if _dispatch_modes() or _function_modes() or _tracing_state() is not None:
+        _untraced("residual_norm")
     index = x.get_device()
     for t in (x, h, gate):
         if t is not None and (t.get_device() != index or index < 0 or t.dtype not in _lib.TYPES):
@@ -893,7 +896,7 @@ class ResidualNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad[:8]
         if gr is None and gy is None:
             return (None,) * 11
-        if torch.is_grad_enabled() or torch._C._len_torch_dispatch_stack() or _pre_dispatch() or not (
+        if torch.is_grad_enabled() or _dispatch_modes() or _pre_dispatch() or not (
                 _in_memory(gr) and _in_memory(gy)):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, nb_shape, nb_dtype, norm_eps, gr,
