@@ -820,3 +820,21 @@ def test_recorded_training_pass_of_128_channels():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+@pytest.mark.parametrize("shape", [(2, 64, 33, 33), (2, 24, 5, 7), (1, 20, 40, 30), (1, 128, 36, 36), (1, 300, 6, 5), (3, 16), (0, 8, 4, 4)])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_layernorm_that_keeps_a_copy(shape, t):
+    """The gradients of the values that the forward had, bit for bit, whatever becomes of x."""
+    from conversenet_amd import functional as Fh
+
+    a = make(shape, t, t, branch=False, seed=sum(shape))
+    got = []
+    for copy in (False, True):
+        d = _dev(a)
+        x = d["x"] * 1.0
+        y = Fh.layernorm_cf_train(x, d["w"], d["b"], EPS, copy=copy)
+        if copy:
+            x.fill_(float("nan"))
+        got.append([y, *torch.autograd.grad(y, (d["x"], d["w"], d["b"]), d["gy"])])
+    assert all(torch.equal(u, v) for u, v in zip(*got))
