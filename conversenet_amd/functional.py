@@ -896,7 +896,8 @@ class ResidualNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad[:8]
         if gr is None and gy is None:
             return (None,) * 11
-        if torch.is_grad_enabled() or _dispatch_modes() or _pre_dispatch() or not (
+        of_copy = gr is not None and h_dtype is None  # from a differentiated backward alone
+        if of_copy or torch.is_grad_enabled() or _dispatch_modes() or _pre_dispatch() or not (
                 _in_memory(gr) and _in_memory(gy)):
             post = None if post_w is None else (post_w, post_b, post_eps)
             return _residual_norm_backward_composite(base, h, res_scale, gate, post, norm_w, nb_shape, nb_dtype, norm_eps, gr,

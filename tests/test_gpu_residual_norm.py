@@ -838,3 +838,20 @@ def test_layernorm_that_keeps_a_copy(shape, t):
             x.fill_(float("nan"))
         got.append([y, *torch.autograd.grad(y, (d["x"], d["w"], d["b"]), d["gy"])])
     assert all(torch.equal(u, v) for u, v in zip(*got))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_gradient_penalty_through_a_copy(t):
+    """The gradient of the copy, which only a differentiated backward gives, beside that of the norm."""
+    from conversenet_amd import functional as Fh
+
+    a = make((2, 24, 7, 5), t, t, branch=False, seed=70)
+    got = []
+    for copy in (False, True):
+        d = _dev(a)
+        y = Fh.layernorm_cf_train(d["x"], d["w"], d["b"], EPS, copy=copy)
+        gx, = torch.autograd.grad(y, d["x"], d["gy"], create_graph=True)
+        loss = (gx.double() ** 2).sum() + (y.double() ** 3).sum()
+        got.append(torch.autograd.grad(loss, (d["x"], d["w"], d["b"])))
+    for u, v in zip(*got):  # the two gradients of x are added in one rounding there, in two here
+        assert float((u.double() - v.double()).norm()) <= 4 * torch.finfo(t).eps * float(u.double().norm())
