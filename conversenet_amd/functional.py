@@ -16,6 +16,7 @@ import operator
 import os
 import threading
 from array import array
+from typing import NamedTuple
 
 import torch
 from torch.multiprocessing.reductions import StorageWeakRef
@@ -1131,6 +1132,219 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         dense = [d for g, d in zip(grads, dense) if d is g]
     _written(dense)
     return norm
+
+
+class MXFP4(NamedTuple):
+    """A map (B,C,*) or matrix (N,C) in microscaled 4-bit floating point: its channels in blocks of 32, each a scale
+    2^(s - 127) and 32 codes of a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6, stored by pixels.  codes (B,*,16 blocks) and
+    scales (B,*,blocks) are uint8, a byte of codes holds the even channel in its lower half; channels is C."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    channels: int
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.channels, *self.codes.shape[1:-1])
+
+
+def _mx_parts(q, what):
+    """((B, C, pixels), codes, scales) of an MXFP4 argument, contiguous and aligned."""
+    codes, scales, C = q
+    blocks = (int(C) + 31) // 32
+    if not (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor)) or codes.dtype is not torch.uint8 \
+            or scales.dtype is not torch.uint8 or C < 1 or codes.dim() < 2 or codes.shape[:-1] != scales.shape[:-1] \
+            or codes.shape[-1] != 16 * blocks or scales.shape[-1] != blocks:
+        raise RuntimeError(f"{what}: codes (B,*,16 blocks) and scales (B,*,blocks) must be uint8 of {blocks} blocks")
+    if codes.get_device() < 0 or scales.get_device() != codes.get_device():
+        raise RuntimeError(f"{what} must be on one HIP device")
+    codes, scales = _contiguous(codes), _contiguous(scales)
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    return (codes.shape[0], int(C), math.prod(codes.shape[1:-1])), codes, scales
+
+
+def _mx_map(x, what):
+    """(B, C, pixels) of a map to be quantised."""
+    if x.get_device() < 0 or x.dtype not in _lib.TYPES:
+        raise RuntimeError(f"{what} needs a float32, bfloat16 or float16 tensor on a HIP device")
+    if x.dim() < 2 or x.shape[1] < 1:
+        raise RuntimeError(f"{what} needs (B,C,*) with channels")
+    return x.shape[0], x.shape[1], math.prod(x.shape[2:])
+
+
+def _mx_empty(x, C):
+    """The memory of x's MXFP4 form."""
+    lead = (x.shape[0], *x.shape[2:])
+    blocks = (C + 31) // 32
+    return (torch.empty((*lead, 16 * blocks), dtype=torch.uint8, device=x.device),
+            torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device))
+
+
+def quantize_mxfp4(x):
+    """A map (B,C,*) or matrix (N,C) in MXFP4: blocks of 32 channels with the scale 2^(floor(log2 max|x|) - 2) and each
+    value the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times it, ties to the even code, at most 6 (2^-127 is the smallest
+    scale).  A block with an infinity or a NaN becomes NaN.  x: float32, bfloat16 or float16."""
+    _untraced("quantize_mxfp4")
+    B, C, HW = _mx_map(x, "quantize_mxfp4")
+    lib = _lib.load()
+    x = _contiguous(x)
+    codes, scales = _mx_empty(x, C)
+    with _on(x.device):
+        rc = lib.cvn_mxfp4_quantize(x.data_ptr(), _lib.TYPES[x.dtype], B, C, HW, codes.data_ptr(), scales.data_ptr(),
+                                    _stream(x.device))
+    _lib.check(rc, "quantize_mxfp4")
+    return MXFP4(codes, scales, C)
+
+
+def dequantize_mxfp4(q, dtype=torch.float32):
+    """The values of an MXFP4 map or matrix as a tensor (B,C,*)."""
+    _untraced("dequantize_mxfp4")
+    (B, C, HW), codes, scales = _mx_parts(q, "dequantize_mxfp4")
+    if dtype not in _lib.TYPES:
+        raise RuntimeError("dequantize_mxfp4 gives float32, bfloat16 or float16")
+    lib = _lib.load()
+    dev = codes.device
+    y = torch.empty((B, C, *codes.shape[1:-1]), dtype=dtype, device=dev)
+    with _on(dev):
+        rc = lib.cvn_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), B, C, HW, y.data_ptr(), _lib.TYPES[dtype],
+                                      _stream(dev))
+    _lib.check(rc, "dequantize_mxfp4")
+    return y
+
+
+def _conv1x1_mxfp4(x, weight, bias, act, residual, res_scale, out, dtype, keep_x):
+    """The launches behind conv1x1_mxfp4: (y, x's MXFP4 form where keep_x)."""
+    _untraced("conv1x1_mxfp4")
+    lib = _lib.load()
+    if act not in (None, "gelu"):
+        raise RuntimeError(f"unknown activation {act!r}")
+    xc = xs = None
+    given = isinstance(x, MXFP4)
+    if given:
+        (B, C, HW), xc, xs = _mx_parts(x, "x")
+        dev, space = xc.device, tuple(xc.shape[1:-1])
+        dtype = dtype or (torch.float32 if residual is None else residual.dtype)
+        if dtype not in _lib.TYPES:
+            raise RuntimeError("conv1x1_mxfp4 gives float32, bfloat16 or float16")
+    else:
+        B, C, HW = _mx_map(x, "conv1x1_mxfp4")
+        if dtype not in (None, x.dtype):
+            raise RuntimeError("the result has the type of x")
+        x = _contiguous(x)
+        dev, space, dtype = x.device, tuple(x.shape[2:]), x.dtype
+    index = dev.index
+    if not isinstance(weight, MXFP4):
+        if weight.get_device() != index or weight.dim() < 2 or math.prod(weight.shape[2:]) != 1:
+            raise RuntimeError("weight must be a matrix (N,C) or (N,C,1,1) on the device of x")
+        weight = quantize_mxfp4(weight)
+    (N, wC, one), wc, ws = _mx_parts(weight, "weight")
+    if wC != C or one != 1 or N < 1 or wc.get_device() != index:
+        raise RuntimeError("weight does not match input channels")
+    shape = (B, N, *space)
+    for t, what in ((residual, "residual"), (out, "out")):
+        if t is not None and (tuple(t.shape) != shape or t.dtype is not dtype or t.get_device() != index):
+            raise RuntimeError(f"{what} must have the result's shape and type")
+    if out is not None and not out.is_contiguous():
+        raise RuntimeError("out must be contiguous")
+    keep = []
+    b, s = _param32(keep, bias, N, index, "bias"), _param32(keep, res_scale, N, index, "res_scale")
+    residual = _contiguous(residual)
+    y = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
+    if keep_x:
+        xc, xs = _mx_empty(x, C)
+    nbytes = lib.cvn_conv1x1_mxfp4_workspace(int(xc is not None), B, C, HW, N)
+    st = _stream(dev)
+    wsp = _scratch(dev, st)
+    with _on(dev), wsp.lock:
+        rc = lib.cvn_conv1x1_mxfp4(None if given else x.data_ptr(), _ptr(xc), _ptr(xs), B, C, HW, wc.data_ptr(),
+                                   ws.data_ptr(), N, b, _lib.ACT_GELU if act else _lib.ACT_NONE, _ptr(residual), s,
+                                   y.data_ptr(), _lib.TYPES[dtype], wsp.ptr(nbytes), nbytes, st)
+    _lib.check(rc, "conv1x1_mxfp4")
+    if out is not None:
+        _written([out])
+    return y, xc, xs, wc, ws
+
+
+def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None, out=None, dtype=None):
+    """conv1x1 of MXFP4 operands: act(W x + b) [then res_scale * . + residual], the products of 4-bit values summed in
+    float32 and the result rounded once.
+
+    x: a map (B,C,*) of float32, bfloat16 or float16, quantised in the call, or an MXFP4 one; weight: an MXFP4 matrix, or a
+    float (N,C) or (N,C,1,1), quantised in the call.  The result has x's type (of an MXFP4 x the residual's, or dtype).
+    residual and out have the result's shape and type, and may be one tensor.  Forward only; for gradients see
+    conv1x1_mxfp4_train."""
+    return _conv1x1_mxfp4(x, weight, bias, act, residual, res_scale, out, dtype, False)[0]
+
+
+def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
+    """Gradients of conv1x1_mxfp4's product and bias, straight through the quantisation: (x, weight, bias), None where
+    not asked for by `need`.  grad_y (B,N,*): float32, bfloat16 or float16, the type of x's gradient; the others are float32,
+    weight's (N,C).  x, weight: the MXFP4 operands of the forward (x None without weight's gradient, weight None without x's, where
+    the other gives the channels)."""
+    _untraced("conv1x1_mxfp4_backward")
+    lib = _lib.load()
+    B, N, HW = _mx_map(grad_y, "conv1x1_mxfp4_backward")
+    nx, nw, nb = need
+    if (nx and weight is None) or (nw and x is None):
+        raise RuntimeError("conv1x1_mxfp4_backward needs the operand")
+    index = grad_y.get_device()
+    C, xc, xs, wc, ws = 1, None, None, None, None
+    if x is not None and nw:
+        (xB, C, xHW), xc, xs = _mx_parts(x, "x")
+        if xB != B or xc.shape[1:-1] != grad_y.shape[2:] or xc.get_device() != index:
+            raise RuntimeError("x does not match the gradient")
+    if weight is not None and nx:
+        (wN, wC, one), wc, ws = _mx_parts(weight, "weight")
+        if wN != N or one != 1 or (xc is not None and wC != C) or wc.get_device() != index:
+            raise RuntimeError("weight does not match the gradient")
+        C = wC
+    gy = _contiguous(grad_y)
+    dev = gy.device
+    gx = torch.empty((B, C, *gy.shape[2:]), dtype=gy.dtype, device=dev) if nx else None
+    gw = torch.empty((N, C), dtype=torch.float32, device=dev) if nw else None
+    gb = torch.empty((N,), dtype=torch.float32, device=dev) if nb else None
+    nbytes = lib.cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N)
+    st = _stream(dev)
+    wsp = _scratch(dev, st)
+    with _on(dev), wsp.lock:
+        rc = lib.cvn_conv1x1_mxfp4_bwd(gy.data_ptr(), _lib.TYPES[gy.dtype], _ptr(xc), _ptr(xs), _ptr(wc), _ptr(ws), B, C, HW,
+                                       N, _ptr(gx), _ptr(gw), _ptr(gb), wsp.ptr(nbytes), nbytes, st)
+    _lib.check(rc, "conv1x1_mxfp4_backward")
+    return gx, gw, gb
+
+
+class Conv1x1MXFP4Function(torch.autograd.Function):
+    """conv1x1_mxfp4 of a float map and matrix, with gradients straight through both quantisations.  Keeps the operands in
+    MXFP4, 17/128 of a float32 map's bytes."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        nx, nw = ctx.needs_input_grad[:2]
+        y, xc, xs, wc, ws = _conv1x1_mxfp4(x, weight, bias, None, None, None, None, None, nw)
+        ctx.save_for_backward(*((xc, xs) if nw else (None, None)), *((wc, ws) if nx else (None, None)))
+        ctx.cfg = (x.shape[1], weight.shape, weight.dtype, None if bias is None else (bias.shape, bias.dtype))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        xc, xs, wc, ws = ctx.saved_tensors
+        C, w_shape, w_dtype, b = ctx.cfg
+        if not _in_memory(gy):
+            raise RuntimeError("conv1x1_mxfp4's gradients are of plain tensors")
+        gx, gw, gb = conv1x1_mxfp4_backward(gy, None if xc is None else MXFP4(xc, xs, C),
+                                            None if wc is None else MXFP4(wc, ws, C), ctx.needs_input_grad[:3])
+        return (gx, None if gw is None else gw.view(w_shape).to(w_dtype),
+                None if gb is None else gb.view(b[0]).to(b[1]))
+
+
+def conv1x1_mxfp4_train(x, weight, bias=None):
+    """Differentiable conv1x1_mxfp4 of a float map (B,C,*) and matrix (N,C) or (N,C,1,1), both quantised in the call: the
+    gradients pass the quantisation unchanged, those of x and weight are products with the other's 4-bit values.  (Not
+    differentiable twice.)"""
+    if isinstance(x, MXFP4) or isinstance(weight, MXFP4):
+        raise RuntimeError("conv1x1_mxfp4_train quantises x and weight itself")
+    return Conv1x1MXFP4Function.apply(x, weight, bias)
 
 
 def copy_(dst, src):

@@ -307,6 +307,36 @@ int cvn_clip_grads(const void* const* grads, void* const* out, const int64_t* nu
                    int norm_kind, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
                    cvn_stream_t stream);
 
+/* MXFP4: a pixel's channels (or a matrix row) in blocks of 32, each a scale 2^(s - 127), s a byte, and 32 codes of 4 bits:
+ * a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6.  s = max(0, e - 2), e the biased exponent of the block's largest magnitude; a
+ * code is the nearest to x / 2^(s - 127), ties to the even code, at most 6.  A block with an infinity or a NaN has
+ * s = 255: each of its values is NaN.  x: (B,C,HW) of x_type, or a matrix (B,C) with HW 1.  codes: (B HW, KB, 16) bytes
+ * aligned to 16, KB = ceil(C / 32), the even channel of a byte in its lower half; scales: (B HW, KB) bytes.  Channels
+ * past C are zeros.  Here and below up to 65536 channels and 2^31 - 256 pixels. */
+int cvn_mxfp4_quantize(const void* x, int x_type, int64_t B, int64_t C, int64_t HW, void* codes, void* scales,
+                       cvn_stream_t stream);
+/* The values, rounded to y_type: y (B,C,HW). */
+int cvn_mxfp4_dequantize(const void* codes, const void* scales, int64_t B, int64_t C, int64_t HW, void* y, int y_type,
+                         cvn_stream_t stream);
+/* y[b,n,p] = act(sum_c w[n][c] x[b,p][c] + bias[n]);  then, with res_scale or residual, y = res_scale[n] * y +
+ * residual[b,n,p]: cvn_conv1x1_f32 of MXFP4 operands, summed in fp32 and rounded once.  w: (N,C) in MXFP4.  x: (B,C,HW) of
+ * type, quantised in the call, its MXFP4 form written to x_codes and x_scales unless they are NULL; or x NULL and its MXFP4
+ * form given there.  y, residual: (B,N,HW) of type; bias, res_scale: fp32 (N).  bias, residual and res_scale may be NULL.
+ * y may be the residual itself, and shares no other memory with an input (CVN_ERR_ARG).
+ * _workspace: quantized: x_codes will be given (read or written). */
+size_t cvn_conv1x1_mxfp4_workspace(int quantized, int64_t B, int64_t C, int64_t HW, int64_t N);
+int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, int64_t C, int64_t HW, const void* w_codes,
+                      const void* w_scales, int64_t N, const float* bias, int act, const void* residual,
+                      const float* res_scale, void* y, int type, void* workspace, size_t workspace_bytes,
+                      cvn_stream_t stream);
+/* Gradients of the product and bias, straight through the quantisation: grad_x[b,c,p] = sum_n w[n][c] grad_y[b,n,p] of type,
+ * grad_w[n][c] = sum_bp grad_y[b,n,p] x[b,p][c] and grad_bias[n] = sum_bp grad_y[b,n,p] in fp32; each may be NULL, and
+ * then what only it needs.  No operand is rounded; sums are added up in the same order on every call. */
+size_t cvn_conv1x1_mxfp4_bwd_workspace(int64_t B, int64_t C, int64_t HW, int64_t N);
+int cvn_conv1x1_mxfp4_bwd(const void* grad_y, int type, const void* x_codes, const void* x_scales, const void* w_codes,
+                          const void* w_scales, int64_t B, int64_t C, int64_t HW, int64_t N, void* grad_x, float* grad_w,
+                          float* grad_bias, void* workspace, size_t workspace_bytes, cvn_stream_t stream);
+
 /* Plain device copy of n floats (bandwidth calibration). */
 int cvn_copy_f32(const float* src, float* dst, int64_t n, cvn_stream_t stream);
 

@@ -1,0 +1,424 @@
+"""MXFP4 maps, their 1x1 convolution and its gradients (functional.quantize_mxfp4, dequantize_mxfp4, conv1x1_mxfp4,
+conv1x1_mxfp4_train) against the same in 64 bits.
+
+Quantisation is exact: codes and scales are equal.  A product of 4-bit values is exact in float32, and so is a block's sum
+of 32 of them but for the scales; a sum over K blocks rounds once a block at most in whatever order, each time by 2^-24 of no
+more than the sum M of the terms' magnitudes (the matrix units align 128 terms to the largest one and may drop bits below
+2^-24 of it: twice that).  With the bias, |error| <= (K + 2) 2^-23 M.  GELU's slope is below 1.13 and its own error below 4e-7
+max(1, |v|).  A gradient's sum of T terms rounds T times in the worst order, and where its float32 operand is taken in parts,
+the smallest of them may lose 2^-24 of it: (T + 2) 2^-24 M.  Each result is rounded once more: eps / 2 of its type."""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import mxfp4_oracle as O
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+def fh():
+    from conversenet_amd import functional
+
+    return functional
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def make(shape, dtype=F32, seed=0):
+    """A feature map: channels of different size, some values far from the others."""
+    g = gen(seed)
+    x = torch.randn(shape, generator=g) * torch.exp(0.7 * torch.randn((1, shape[1]) + (1,) * (len(shape) - 2), generator=g))
+    x = torch.where(torch.rand(shape, generator=g) < 0.01, 20 * x, x)
+    return x.to(dtype)
+
+
+def np64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def flat(t):
+    a = np64(t)
+    return a.reshape(a.shape[0], a.shape[1], -1)
+
+
+def half_step(dtype, v):
+    """What a rounding to dtype may change v by."""
+    f = torch.finfo(dtype)
+    return np.abs(v) * f.eps / 2 + f.smallest_normal * f.eps
+
+
+def check(got, want, lim):
+    got, want = np64(got).reshape(want.shape), np.asarray(want)
+    bad = ~(np.abs(got - want) <= lim)
+    assert not bad.any(), (int(bad.sum()), bad.size, np.abs(got - want).max(), np.max(np.abs(got - want) / (lim + 1e-300)))
+
+
+def check_quantized(q, x):
+    codes, scales = O.quantize(flat(x))
+    assert q.channels == x.shape[1] and q.shape == tuple(x.shape)
+    assert np.array_equal(q.scales.cpu().numpy().reshape(scales.shape), scales)
+    assert np.array_equal(q.codes.cpu().numpy().reshape(codes.shape), codes)
+
+
+SHAPES = [(1, 1, 1, 1), (1, 64, 1, 1), (2, 31, 3, 5), (1, 32, 1, 7), (3, 33, 4, 4), (2, 64, 16, 16), (1, 100, 67, 45),
+          (5, 7, 2, 1), (2, 128, 9, 9), (300, 65), (1, 4096), (3, 257, 5), (2, 48, 3, 4, 5), (1, 320, 32, 33), (4, 96, 8, 63)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_round_trip(shape, dtype):
+    x = make(shape, dtype, sum(shape)).cuda()
+    q = fh().quantize_mxfp4(x)
+    check_quantized(q, x)
+    want = O.rounded(flat(x))
+    for t in TYPES:
+        v = fh().dequantize_mxfp4(q, t)
+        assert v.dtype is t and v.shape == x.shape
+        assert np.array_equal(flat(v), torch.from_numpy(want).to(t).double().numpy())
+
+
+def test_round_trip_of_every_tie_and_scale():
+    """Every border between two codes and its float32 neighbours, at every scale a number can have."""
+    rows = []
+    for e in range(-149, 128):
+        top = np.float32(2.0) ** np.float32(e) if e >= -126 else np.float32(np.ldexp(1.0, e))
+        unit = 2.0 ** max(e - 2, -127)
+        m = np.float32(np.concatenate(([0.0], O.MIDS, O.GRID)) * unit)
+        with np.errstate(over="ignore"):
+            v = np.concatenate((m, np.nextafter(m, np.float32(np.inf)), np.nextafter(m, np.float32(0))))
+        v = v[np.abs(v) < 2 * np.float64(top)][:31]
+        v = v * np.where(np.arange(v.size) % 2, -1, 1).astype(np.float32)
+        rows.append(np.concatenate(([top], v, np.zeros(31 - v.size, np.float32))))
+    x = torch.from_numpy(np.stack(rows).astype(np.float32)).cuda()
+    check_quantized(fh().quantize_mxfp4(x), x)
+    planes = x.t().reshape(1, 32, -1).contiguous()  # the same as the pixels of a map
+    check_quantized(fh().quantize_mxfp4(planes), planes)
+    assert np.array_equal(flat(fh().dequantize_mxfp4(fh().quantize_mxfp4(planes))), O.rounded(flat(planes)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_blocks_that_hold_no_number(dtype):
+    x = make((2, 70, 3, 5), dtype, 1)
+    x[0, 3, 1, 1], x[0, 40, 1, 2], x[1, 69, 0, 0], x[1, 0, 2, 4] = float("nan"), float("inf"), -float("inf"), float("nan")
+    x[0, :, 2, 2] = 0
+    x[0, :, 2, 3] = -0.0
+    x = x.cuda()
+    q = fh().quantize_mxfp4(x)
+    check_quantized(q, x)
+    v, want = flat(fh().dequantize_mxfp4(q)), O.rounded(flat(x))
+    assert np.array_equal(np.isnan(v), np.isnan(want)) and np.array_equal(np.nan_to_num(v), np.nan_to_num(want))
+    w = make((40, 70), F32, 2).cuda()
+    y = flat(fh().conv1x1_mxfp4(x, w))
+    bad = np.isnan(want).any(1)
+    assert bad.sum() == 4 and np.array_equal(np.isnan(y), np.broadcast_to(bad[:, None], y.shape))
+
+
+def limits(K, mag, y, act, res_scale, residual, dtype):
+    lim = (K + 2) * 2.0 ** -23 * mag
+    if act == "gelu":
+        lim = 1.13 * lim + 4e-7 * np.maximum(1, mag)
+    if res_scale is not None:
+        s = np.abs(np64(res_scale).reshape(1, -1, 1))
+        lim = lim * s + 2.0 ** -24 * np.abs(s) * (mag + 1)
+    if residual is not None:
+        lim = lim + 2.0 ** -23 * (np.abs(y) + np.abs(flat(residual)))
+    return lim + half_step(dtype, np.abs(y) + lim)
+
+
+CONVS = [  # B, N, C, pixels
+    (1, 1, 1, (1, 1)), (1, 16, 64, (1, 1)), (3, 50, 100, (1, 1)), (16, 96, 320, (1, 1)), (17, 33, 65, (1, 1)), (70, 40, 129, ()),
+    (1, 128, 64, (16, 16)), (2, 64, 128, (8, 33)), (1, 3, 7, (67, 45)), (2, 80, 48, (5, 7)), (1, 100, 31, (13,)),
+    (2, 260, 257, (9, 9)), (1, 65, 1000, (12, 20)), (3, 17, 33, (2, 1)), (1, 300, 512, (32, 20)), (4, 130, 96, (20, 12)),
+    (1, 40, 4100, (3, 3)), (2, 1, 300, (4, 65)), (1, 2048, 32, (4, 4)), (1, 70, 300, (2, 3, 7)),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", CONVS, ids=str)
+def test_conv1x1(case, dtype):
+    B, N, C, space = case
+    x, w = make((B, C, *space), dtype, 3).cuda(), (make((N, C), F32, 4) / C ** 0.5).cuda()
+    g = gen(5)
+    bias, s = torch.randn(N, generator=g).cuda(), torch.randn(N, generator=g).cuda()
+    residual = torch.randn((B, N, *space), generator=g).to(dtype).cuda()
+    xq, wq = O.rounded(flat(x)), O.rounded(np64(w)[:, :, None])[:, :, 0]
+    K = (C + 31) // 32
+    for b, act, r, rs in ((None, None, None, None), (bias, "gelu", None, None), (bias, None, residual, s), (bias, "gelu", residual, None)):
+        want, mag = O.conv1x1(xq, wq, None if b is None else np64(b), act, None if r is None else flat(r),
+                              None if rs is None else np64(rs))
+        lim = limits(K, mag, want, act, rs, r, dtype)
+        y = fh().conv1x1_mxfp4(x, w, b, act, r, rs)
+        assert y.dtype is dtype and y.shape == (B, N, *space)
+        check(y, want, lim)
+    # the same operands quantised before
+    q = fh().quantize_mxfp4(x)
+    wm = fh().quantize_mxfp4(w.view(N, C, 1, 1))
+    assert torch.equal(fh().conv1x1_mxfp4(x, wm, bias, "gelu", residual), y)
+    check(fh().conv1x1_mxfp4(q, wm, bias, "gelu", residual), want, lim)
+    want, mag = O.conv1x1(xq, wq)
+    check(fh().conv1x1_mxfp4(q, wm, dtype=BF16), want, limits(K, mag, want, None, None, None, BF16))
+
+
+def test_conv1x1_layouts_and_outputs():
+    F = fh()
+    x = make((2, 70, 12, 10), F32, 6).cuda()
+    w = make((50, 70), F32, 7).cuda()
+    ref = F.conv1x1_mxfp4(x, w)
+    base = torch.zeros(2 * 70 * 120 + 1, device="cuda")
+    odd = base[1:].view(2, 70, 12, 10)  # not aligned to 16 bytes
+    odd.copy_(x)
+    strided = torch.zeros(2, 70, 12, 20, device="cuda")[..., ::2]
+    strided.copy_(x)
+    for t in (odd, strided, x.to(memory_format=torch.channels_last), x.transpose(2, 3).contiguous().transpose(2, 3)):
+        assert torch.equal(F.conv1x1_mxfp4(t, w), ref)
+        check_quantized(F.quantize_mxfp4(t), x)
+    q = F.quantize_mxfp4(w)
+    moved = torch.zeros(q.codes.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view(q.codes.shape)
+    moved.copy_(q.codes)
+    assert torch.equal(F.conv1x1_mxfp4(x, F.MXFP4(moved, q.scales, 70)), ref)
+    out = torch.full((2, 50, 12, 10), 7.0, device="cuda")
+    assert F.conv1x1_mxfp4(x, w, out=out) is out and torch.equal(out, ref)
+    res = torch.randn(2, 50, 12, 10, device="cuda")
+    want = F.conv1x1_mxfp4(x, w, residual=res)
+    version = res._version
+    assert F.conv1x1_mxfp4(x, w, residual=res, out=res) is res and torch.equal(res, want) and res._version > version
+    guard = torch.full((2 * 50 * 120 + 64,), 3.0, device="cuda")
+    inner = guard[32:-32].view(2, 50, 12, 10)
+    F.conv1x1_mxfp4(x, w, out=inner)
+    assert torch.equal(inner, ref) and (guard[:32] == 3).all() and (guard[-32:] == 3).all()
+    for t in (F16, BF16):  # parameters of other types
+        assert torch.equal(F.conv1x1_mxfp4(x, w, torch.ones(50, dtype=t, device="cuda")), F.conv1x1_mxfp4(x, w, torch.ones(50, device="cuda")))
+
+
+def test_nothing_to_do():
+    F = fh()
+    w = make((5, 40), F32, 8).cuda()
+    for shape in ((0, 40, 3, 3), (2, 40, 0, 3), (0, 40)):
+        x = torch.empty(shape, device="cuda")
+        q = F.quantize_mxfp4(x)
+        assert F.dequantize_mxfp4(q).shape == x.shape and q.shape == x.shape
+        assert F.conv1x1_mxfp4(x, w).shape == F.conv1x1_mxfp4(q, w).shape == (shape[0], 5) + shape[2:]
+        x.requires_grad_(True)
+        wl, b = w.clone().requires_grad_(True), torch.zeros(5, device="cuda", requires_grad=True)
+        y = F.conv1x1_mxfp4_train(x, wl, b)
+        gx, gw, gb = torch.autograd.grad(y, (x, wl, b), torch.empty_like(y))
+        assert gx.shape == x.shape and (gw == 0).all() and (gb == 0).all()
+
+
+TRAINS = [(1, 1, 1, (1, 1)), (1, 16, 64, (1, 1)), (3, 50, 100, (1, 1)), (37, 33, 65, ()), (2, 128, 64, (16, 16)), (2, 64, 128, (8, 33)),
+          (1, 3, 7, (67, 45)), (3, 80, 48, (13, 7)), (1, 100, 31, (13,)), (2, 260, 257, (9, 9)), (3, 17, 33, (2, 1)),
+          (1, 300, 512, (32, 20)), (4, 130, 96, (20, 12)), (1, 64, 64, (129, 131)), (300, 5, 40, (1, 1)), (2, 257, 40, (3, 5, 2))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", TRAINS, ids=str)
+def test_gradients(case, dtype):
+    B, N, C, space = case
+    F = fh()
+    x, w = make((B, C, *space), dtype, 9).cuda(), (make((N, C, 1, 1), F32, 10) / C ** 0.5).cuda()
+    bias = torch.randn(N, generator=gen(11)).cuda()
+    gy = torch.randn((B, N, *space), generator=gen(12)).to(dtype).cuda()
+    for t in (x, w, bias):
+        t.requires_grad_(True)
+    y = F.conv1x1_mxfp4_train(x, w, bias)
+    assert y.dtype is dtype
+    grads = torch.autograd.grad(y, (x, w, bias), gy, retain_graph=True)
+    again = torch.autograd.grad(y, (x, w, bias), gy)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    xq, wq = O.rounded(flat(x)), O.rounded(np64(w)[:, :, 0])[:, :, 0]
+    want, mag = O.conv1x1(xq, wq, np64(bias))
+    check(y, want, limits((C + 31) // 32, mag, want, None, None, None, dtype))
+    P = flat(x).shape[0] * flat(x).shape[2]
+    for g, leaf, (want, mag), terms in zip(grads, (x, w, bias), O.gradients(flat(gy), xq, wq), (N, P, P)):
+        assert g.dtype is leaf.dtype and g.shape == leaf.shape
+        check(g, want, (terms + 2) * 2.0 ** -24 * mag + half_step(g.dtype, want))
+
+
+def test_gradients_against_differences():
+    """Straight through the quantisation the loss is that of the rounded operands: its differences about them."""
+    F = fh()
+    x, w = make((2, 40, 3, 4), F32, 13).cuda(), make((9, 40), F32, 14).cuda()
+    x.requires_grad_(True), w.requires_grad_(True)
+    b = torch.zeros(9, device="cuda", requires_grad=True)
+    gy = torch.randn(2, 9, 3, 4, generator=gen(15)).cuda()
+    gx, gw, gb = torch.autograd.grad(F.conv1x1_mxfp4_train(x, w, b), (x, w, b), gy)
+    xq, wq, g = O.rounded(flat(x)), O.rounded(np64(w)[:, :, None])[:, :, 0], flat(gy)
+    loss = lambda xv, wv, bv: (O.conv1x1(xv, wv, bv)[0] * g).sum()  # noqa: E731
+    rng = np.random.default_rng(16)
+    for leaf, grad in enumerate((gx, gw, gb)):
+        ops = [xq, wq, np.zeros(9)]
+        d = rng.standard_normal(ops[leaf].shape)
+        ends = []
+        for h in (0.5, -0.5):  # linear in each operand: any step will do
+            moved = list(ops)
+            moved[leaf] = ops[leaf] + h * d
+            ends.append(loss(*moved))
+        terms = np64(grad).reshape(d.shape) * d
+        assert abs((ends[0] - ends[1]) - terms.sum()) <= 60 * 2.0 ** -23 * np.abs(terms).sum() + 1e-12 * abs(ends[0])
+
+
+def test_gradient_arguments():
+    F = fh()
+    x, w = make((2, 70, 5, 6), F32, 17).cuda().requires_grad_(True), make((30, 70), F16, 18).cuda().requires_grad_(True)
+    b = torch.randn(30, device="cuda", dtype=BF16, requires_grad=True)
+    y = F.conv1x1_mxfp4_train(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y.sum(), (x, w, b), retain_graph=True)  # an expanded gradient
+    g1 = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert all(torch.equal(p, q) and p.dtype is q.dtype for p, q in zip((gx, gw, gb), g1))
+    assert gw.dtype is F16 and gb.dtype is BF16
+    # each gradient by itself, and the function behind them
+    for i, leaf in enumerate((x, w, b)):
+        ls = [t.detach().clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        yi = F.conv1x1_mxfp4_train(*ls)
+        assert torch.equal(torch.autograd.grad(yi, ls[i], torch.ones_like(yi))[0], g1[i])
+    gy = torch.randn(2, 30, 5, 6, device="cuda")
+    xq, wq = F.quantize_mxfp4(x.detach()), F.quantize_mxfp4(w.detach())
+    full = F.conv1x1_mxfp4_backward(gy, xq, wq)
+    strided = gy.to(memory_format=torch.channels_last)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (True, True, False)):
+        got = F.conv1x1_mxfp4_backward(strided, xq if need[1] else None, wq if need[0] else None, need)
+        assert all(g is None if not n else torch.equal(g, f) for g, f, n in zip(got, full, need))
+    # no bias, no gradients wanted, and twice
+    assert F.conv1x1_mxfp4_train(x.detach(), w.detach()).requires_grad is False
+    yb = F.conv1x1_mxfp4_train(x, w)
+    g2 = torch.autograd.grad(yb, (x, w), torch.ones_like(yb), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g2[0].sum(), w)
+    with pytest.raises(RuntimeError, match="plain tensors|vmap"):
+        torch.autograd.grad(F.conv1x1_mxfp4_train(x, w), x, torch.ones((2,) + tuple(y.shape), device="cuda"), is_grads_batched=True)
+
+
+def test_saved_operands_are_the_forward_s():
+    """x and weight may change in place between forward and backward: the operands are kept in 4 bits."""
+    F = fh()
+    x, w = make((2, 64, 8, 8), F32, 19).cuda(), make((32, 64), F32, 20).cuda()
+    gy = torch.randn(2, 32, 8, 8, device="cuda")
+    lx, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    want = torch.autograd.grad(F.conv1x1_mxfp4_train(lx, lw), (lx, lw), gy)
+    lx, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = F.conv1x1_mxfp4_train(lx, lw)
+    with torch.no_grad():
+        lx.zero_(), lw.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (lx, lw), gy), want))
+
+
+@pytest.mark.parametrize("shape", [(4, 320, 1, 1), (1, 64, 16, 16), (1, 320, 16, 16)])
+def test_graph_stream_and_threads(shape):
+    F = fh()
+    x, w = make(shape, F32, 21).cuda(), F.quantize_mxfp4(make((96, shape[1]), F32, 22).cuda())
+    ref = F.conv1x1_mxfp4(x, w, act="gelu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(F.conv1x1_mxfp4(x, w, act="gelu"), ref)
+        g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        xs = [x.clone(), x.clone()]
+        with torch.cuda.graph(g1, stream=side):
+            y1 = F.conv1x1_mxfp4(xs[0], w, act="gelu")
+        with torch.cuda.graph(g2, stream=side):
+            y2 = F.conv1x1_mxfp4(xs[1], w, act="gelu")
+    torch.cuda.synchronize()
+    for i in range(4):
+        xs[0].copy_(make(shape, F32, 30 + i)), xs[1].copy_(make(shape, F32, 40 + i))
+        g1.replay(), g2.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y1, F.conv1x1_mxfp4(xs[0], w, act="gelu")) and torch.equal(y2, F.conv1x1_mxfp4(xs[1], w, act="gelu"))
+    bad = []
+
+    def work(i):
+        xi = make(shape, F32, 50 + i).cuda()
+        want = F.conv1x1_mxfp4(xi, w)
+        for _ in range(20):
+            if not torch.equal(F.conv1x1_mxfp4(xi, w), want):
+                bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in ts], [t.join() for t in ts]
+    assert not bad
+
+
+def test_recorded_training_pass():
+    F = fh()
+    x, w = make((2, 64, 12, 12), F32, 23).cuda().requires_grad_(True), make((128, 64), F32, 24).cuda().requires_grad_(True)
+    b, gy = torch.zeros(128, device="cuda", requires_grad=True), torch.randn(2, 128, 12, 12, device="cuda")
+
+    def step():
+        y = F.conv1x1_mxfp4_train(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), gy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(make((2, 64, 12, 12), F32, 60 + i)), w.copy_(make((128, 64), F32, 70 + i))
+            gy.copy_(torch.randn(2, 128, 12, 12, generator=gen(80 + i)))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, step()))
+
+
+def test_offsets_past_32_bits():
+    """A map of more than 2^32 bytes whose last pixels count."""
+    F = fh()
+    x = torch.zeros((1, 64, 4100, 4200), device="cuda")  # 4.4 GB
+    x[..., -3:, -70:] = make((1, 64, 3, 70), F32, 25).cuda()
+    w = make((16, 64), F32, 26).cuda()
+    tail = x[..., -3:, -70:].contiguous()
+    assert torch.equal(F.conv1x1_mxfp4(x, w)[..., -3:, -70:], F.conv1x1_mxfp4(tail, w))
+    q = F.quantize_mxfp4(x)
+    assert torch.equal(q.codes[:, -3:, -70:], F.quantize_mxfp4(tail).codes)
+    assert torch.equal(F.dequantize_mxfp4(q)[..., -3:, -70:], F.dequantize_mxfp4(F.quantize_mxfp4(tail)))
+
+
+def test_refusals():
+    F = fh()
+    x, w = make((2, 40, 3, 3), F32, 27).cuda(), make((6, 40), F32, 28).cuda()
+    q, wm = F.quantize_mxfp4(x), F.quantize_mxfp4(w)
+    y = torch.empty(2, 6, 3, 3, device="cuda")
+    for call, what in (
+            (lambda: F.quantize_mxfp4(x.double()), "float32, bfloat16 or float16"),
+            (lambda: F.quantize_mxfp4(x.cpu()), "HIP device"),
+            (lambda: F.quantize_mxfp4(x[0, 0, 0]), "channels"),
+            (lambda: F.quantize_mxfp4(x[:, :0]), "channels"),
+            (lambda: F.dequantize_mxfp4(q, torch.float64), "float32, bfloat16 or float16"),
+            (lambda: F.dequantize_mxfp4(F.MXFP4(q.codes, q.scales, 65)), "blocks"),
+            (lambda: F.dequantize_mxfp4(F.MXFP4(q.codes.float(), q.scales, 40)), "uint8"),
+            (lambda: F.dequantize_mxfp4(F.MXFP4(q.codes.cpu(), q.scales.cpu(), 40)), "HIP device"),
+            (lambda: F.conv1x1_mxfp4(x, w[:, :39]), "input channels"),
+            (lambda: F.conv1x1_mxfp4(x, x), "matrix"),
+            (lambda: F.conv1x1_mxfp4(x, q), "input channels"),
+            (lambda: F.conv1x1_mxfp4(x, w.cpu()), "device"),
+            (lambda: F.conv1x1_mxfp4(x, w, torch.zeros(5, device="cuda")), "bias"),
+            (lambda: F.conv1x1_mxfp4(x, w, act="relu"), "activation"),
+            (lambda: F.conv1x1_mxfp4(x, w, residual=y[:1]), "residual"),
+            (lambda: F.conv1x1_mxfp4(x, w, residual=y.half()), "residual"),
+            (lambda: F.conv1x1_mxfp4(x, w, out=y.permute(0, 1, 3, 2)), "contiguous"),
+            (lambda: F.conv1x1_mxfp4(x, w, dtype=F16), "type of x"),
+            (lambda: F.conv1x1_mxfp4(q, wm, dtype=torch.float64), "float32, bfloat16 or float16"),
+            (lambda: F.conv1x1_mxfp4_train(q, w), "quantises"),
+            (lambda: F.conv1x1_mxfp4_backward(y, None, wm), "operand"),
+            (lambda: F.conv1x1_mxfp4_backward(y, q, F.quantize_mxfp4(w[:5])), "match"),
+            (lambda: F.conv1x1_mxfp4_backward(y[:1], q, wm), "match")):
+        with pytest.raises(RuntimeError, match=what):
+            call()
+    buf = torch.zeros(4 * 2 * 40 * 9, device="cuda")
+    xb = buf[:720].view(2, 40, 3, 3)
+    for lo in (0, 700):  # an output on top of x
+        with pytest.raises(RuntimeError, match="shares memory"):
+            F.conv1x1_mxfp4(xb, w, out=buf[lo:lo + 108].view(2, 6, 3, 3))
+    with pytest.raises(RuntimeError, match="shares memory"):
+        F.conv1x1_mxfp4(x, w, residual=buf[:108].view(2, 6, 3, 3), out=buf[8:116].view(2, 6, 3, 3))
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: F.conv1x1_mxfp4(t, wm), x)
