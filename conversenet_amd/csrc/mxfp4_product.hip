@@ -1,53 +1,545 @@
 // 1x1 convolution of MXFP4 maps with MXFP4 matrices (the format: mxfp4.h):
 //   y[b,n,p] = act(sum_c w[n][c] x[b,p][c] + bias[n]) [* res_scale[n] + residual[b,n,p]]
 // on the matrix units' scaled 4-bit products, which multiply 32 codes of two rows with both blocks' scales and add in float32.
+#include <algorithm>
+
 #include "mxfp4.h"
 
 namespace cvn {
 namespace {
 
-constexpr int kThreads = 256;
+// Operands of a product as the kernels read them; `x` is null where the map is given in MXFP4.
+struct MxIn {
+  const void* x;
+  mx_i32x4* xc;  // read, or written where x is given and they are kept
+  uint8_t* xs;
+  const mx_i32x4* wc;
+  const uint8_t* ws;
+  int64_t C;
+  int KB;
+};
 
+template <class T, int V>
+struct MxVec {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
 template <class T>
-__device__ __forceinline__ void mx_store(const MxOut& o, int64_t r, int64_t n, float v) {
-  if (r >= o.rows || n >= o.N) return;
-  const int64_t b = r / o.HW, i = (b * o.N + n) * o.HW + (r - b * o.HW);
-  if (o.bias) v += o.bias[n];
+struct MxVec<T, 1> {
+  typedef T type;
+};
+
+// What happens to a sum on its way out.
+template <class T>
+__device__ __forceinline__ float mx_finish(const MxOut& o, float v, float bias, float scale) {
+  v += bias;
   if (o.act == CVN_ACT_GELU) v = gelu_fast(v);
-  if (o.res_scale) v *= o.res_scale[n];
-  if (o.residual) v += (float)((const T*)o.residual)[i];
-  ((T*)o.y)[i] = (T)v;
+  return v * scale;
 }
 
-// A wave makes a tile of 16 channels and 16 pixels.  Of a step of 128 channels, lane l holds the block l / 16 of its
-// operands' rows l % 16, and of the result channels 4 (l / 16) .. + 3 of pixel l % 16.
+// Where a lane's V neighbouring pixels from row r0 on lie.
+struct MxGroup {
+  int64_t r0, b, p;
+  bool whole;  // all in one sample
+};
+template <int V>
+__device__ __forceinline__ MxGroup mx_group(int64_t r0, int64_t HW, int64_t rows) {
+  MxGroup g;
+  g.r0 = r0;
+  g.b = (uint32_t)r0 / (uint32_t)HW;  // (rows are below 2^31)
+  g.p = r0 - g.b * HW;
+  g.whole = r0 + V <= rows && g.p + V <= HW;
+  return g;
+}
+
+// R sums (rows of channels i, i + step, ..) of V elements side by side, from element `at` of the first on.
+template <class T, int V, int R>
+__device__ __forceinline__ void mx_store_rows(const MxOut& o, int64_t at, int64_t step, const float (*v)[V], const float (*bias)[V],
+                                              const float (*scale)[V]) {
+  typedef typename MxVec<T, V>::type W;
+  float t[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[r][e] = mx_finish<T>(o, v[r][e], bias[r][e], scale[r][e]);
+  if (o.residual) {
+    W res[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) res[r] = *(const W*)((const T*)o.residual + at + r * step);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[r][e] += (float)((const T*)&res[r])[e];
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    W out;
+#pragma unroll
+    for (int e = 0; e < V; ++e) ((T*)&out)[e] = (T)t[r][e];
+    __builtin_nontemporal_store(out, (W*)((T*)o.y + at + r * step));
+  }
+}
+
+// The elements of channel n of a group's V pixels, and which of them there are.
+template <int V>
+struct MxPixels {
+  int64_t at[V];
+  int live;
+};
+template <int V>
+__device__ __forceinline__ MxPixels<V> mx_pixels(const MxOut& o, const MxGroup& g, int64_t n) {
+  MxPixels<V> x;
+  x.live = 0;
+  int64_t b = g.b, p = g.p;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    x.at[e] = (b * o.N + n) * o.HW + p;
+    x.live |= (g.r0 + e < o.rows) << e;
+    if (++p == o.HW) p = 0, ++b;
+  }
+  return x;
+}
+// One channel of them, `step` elements further on, one by one.
+template <class T, int V>
+__device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V>& x, int64_t step, const float* v, float bias,
+                                                float scale) {
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (x.live >> e & 1) {
+      const int64_t i = x.at[e] + step;
+      float t = mx_finish<T>(o, v[e], bias, scale);
+      if (o.residual) t += (float)((const T*)o.residual)[i];
+      ((T*)o.y)[i] = (T)t;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many pixels of many channels: both operands in MXFP4, tiles staged through LDS.
+// ------------------------------------------------------------------------------------------------
+// A step takes 256 channels: 128 bytes of codes a row, which a wave fetches 8 rows at a time straight into LDS.  A row's
+// 16-byte pieces are stored in an order that depends on the row (piece ^ (row / D & 7)), so that lanes which read the same
+// piece of D-spaced rows hit different banks.  Lane l of a 32 x 32 x 64 product takes the blocks 4 (l / 32) + s of rows
+// l % 32 in steps s < 4: its four scales are one word.  Past the last block the codes of that block stand in, and both
+// scales are 2^-127: the products are lost below float32's range.
+constexpr int kStep = 8;  // blocks of a step
+
+// The word of four scales at place `at` of `total`, as loaded from the last place where a word fits ..
+__device__ __forceinline__ unsigned mx_scales_load(const uint8_t* s, int64_t at, int64_t total) {
+  typedef unsigned U __attribute__((aligned(1)));
+  if (total >= 4) return *(const U*)(s + min(at, total - 4));
+  unsigned v = 0;
+  for (int i = 0; i < 3; ++i)
+    if (at + i < total) v |= (unsigned)s[at + i] << (8 * i);
+  return v;
+}
+// .. and put right, for blocks kb .. of KB: 0 past the last.
+__device__ __forceinline__ unsigned mx_scales_tail(unsigned v, int64_t at, int64_t total, int kb, int KB) {
+  if (kb >= KB) return 0;
+  if (total >= 4) v >>= 8 * (int)(at - min(at, total - 4));
+  return KB - kb < 4 ? v & ((1u << (8 * (KB - kb))) - 1) : v;
+}
+
+typedef __attribute__((address_space(3))) void* mx_lds;
+typedef const __attribute__((address_space(1))) void* mx_glob;
+
+// Tiles of BA x BB rows of the two operands, WA x WB of them to a wave.  MAP: A is the matrix, B the pixels, and a lane
+// stores four pixels of a channel; otherwise (one pixel a sample) A is the pixels, and it stores four channels of a pixel.
+// In either case lane j of the four 32-row tiles of a group holds the rows 4 j + 0 .. 3 of B.
+template <class T, bool MAP, int BA, int BB, int WA, int WB>
+__global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
+    k_mx_gemm(const mx_i32x4* __restrict__ ac, const uint8_t* __restrict__ as, int64_t na, const mx_i32x4* __restrict__ bc,
+              const uint8_t* __restrict__ bs, int64_t nb, int KB, int ta, int tb, MxOut o) {
+  constexpr int NW = (BA / WA) * (BB / WB), TA = WA / 32, TB = WB / 32;
+  constexpr int D = TB;  // rows of B between neighbouring lanes
+  constexpr int kBytes = (BA + BB) * 128;
+  extern __shared__ char smem[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
+  // Blocks of one XCD take a run of tiles, in patches of eight A tiles: its L2 holds what they share.
+  const int nt = ta * tb;
+  int t = blockIdx.x;
+  {
+    const int q = nt / 8, rem = nt % 8, x = t & 7, i = t >> 3;
+    t = x < rem ? x * (q + 1) + i : rem * (q + 1) + (x - rem) * q + i;
+  }
+  const int patch = t / (8 * tb), a0 = patch * 8, aw = min(8, ta - a0), in = t - patch * 8 * tb;
+  const int64_t ra = (int64_t)(a0 + in % aw) * BA, rb = (int64_t)(in / aw) * BB;
+
+  // what this wave fetches: rows 8 (wave + NW i) + lane / 8 of the A then the B tile
+  constexpr int LA = BA / 8 / NW, LB = BB / 8 / NW;
+  const mx_i32x4* src[LA + LB];
+  int piece[LA + LB];
+#pragma unroll
+  for (int i = 0; i < LA + LB; ++i) {
+    const bool isa = i < LA;
+    const int row = 8 * (wave + NW * (isa ? i : i - LA)) + (lane >> 3);
+    src[i] = isa ? ac + min(ra + row, na - 1) * KB : bc + min(rb + row, nb - 1) * KB;
+    piece[i] = (lane & 7) ^ ((isa ? row : row / D) & 7);
+  }
+  auto fetch = [&](int kb0, char* buf) {
+#pragma unroll
+    for (int i = 0; i < LA + LB; ++i) {
+      const int row8 = (wave + NW * (i < LA ? i : i - LA)) * 8 + (i < LA ? 0 : BA);
+      __builtin_amdgcn_global_load_lds((mx_glob)(src[i] + min(kb0 + piece[i], KB - 1)), (mx_lds)(buf + row8 * 128), 16, 0, 0);
+    }
+  };
+  const int wa = wave % (BA / WA) * WA, wb = wave / (BA / WA) * WB;
+  int64_t sa_at[TA], sb_at[TB];
+#pragma unroll
+  for (int i = 0; i < TA; ++i) sa_at[i] = min(ra + wa + 32 * i + j, na - 1) * KB + 4 * h;
+#pragma unroll
+  for (int i = 0; i < TB; ++i) sb_at[i] = min(rb + wb + D * j + i, nb - 1) * KB + 4 * h;
+  unsigned sa[TA], sb[TB];
+  auto load_scales = [&](int kb0) {
+#pragma unroll
+    for (int i = 0; i < TA; ++i) sa[i] = mx_scales_load(as, sa_at[i] + kb0, na * KB);
+#pragma unroll
+    for (int i = 0; i < TB; ++i) sb[i] = mx_scales_load(bs, sb_at[i] + kb0, nb * KB);
+  };
+
+  // bias and residual scale of the tile's channels, behind the operands
+  float* bias = (float*)(smem + 2 * kBytes);
+  constexpr int NC = MAP ? BA : BB;
+  float* rscale = bias + NC;
+  for (int i = threadIdx.x; i < NC; i += NW * 64) {
+    const int64_t n = (MAP ? ra : rb) + i;
+    bias[i] = o.bias && n < o.N ? o.bias[n] : 0.f;
+    rscale[i] = o.res_scale && n < o.N ? o.res_scale[n] : 1.f;
+  }
+
+  mx_f32x16 acc[TA][TB];
+#pragma unroll
+  for (int i = 0; i < TA; ++i)
+#pragma unroll
+    for (int k = 0; k < TB; ++k) acc[i][k] = mx_f32x16{};
+  fetch(0, smem);
+  load_scales(0);
+  int cur = 0;
+  for (int kb0 = 0; kb0 < KB; kb0 += kStep) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    unsigned ua[TA], ub[TB];
+#pragma unroll
+    for (int i = 0; i < TA; ++i) ua[i] = sa[i];
+#pragma unroll
+    for (int i = 0; i < TB; ++i) ub[i] = sb[i];
+    if (kb0 + kStep < KB) {
+      fetch(kb0 + kStep, smem + (cur ^ 1) * kBytes);
+      load_scales(kb0 + kStep);
+    } else {
+#pragma unroll
+      for (int i = 0; i < TA; ++i) ua[i] = mx_scales_tail(ua[i], sa_at[i] + kb0, na * KB, kb0 + 4 * h, KB);
+#pragma unroll
+      for (int i = 0; i < TB; ++i) ub[i] = mx_scales_tail(ub[i], sb_at[i] + kb0, nb * KB, kb0 + 4 * h, KB);
+    }
+    const char* buf = smem + cur * kBytes;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      mx_i32x4 a[TA], b[TB];
+#pragma unroll
+      for (int i = 0; i < TA; ++i) {
+        const int row = wa + 32 * i + j;
+        a[i] = *(const mx_i32x4*)(buf + row * 128 + (((4 * h + s) ^ (row & 7)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < TB; ++i) {
+        const int row = wb + D * j + i;
+        b[i] = *(const mx_i32x4*)(buf + (BA + row) * 128 + (((4 * h + s) ^ ((row / D) & 7)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+#pragma unroll
+        for (int k = 0; k < TB; ++k) {
+          // (the byte of a scale word is part of the instruction)
+          if (s == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 0, ua[i], 0, ub[k]);
+          if (s == 1) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 1, ua[i], 1, ub[k]);
+          if (s == 2) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 2, ua[i], 2, ub[k]);
+          if (s == 3) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 3, ua[i], 3, ub[k]);
+        }
+    }
+    cur ^= 1;
+  }
+
+  // Element e of a 32 x 32 result is its row 8 (e / 4) + 4 h + e % 4, column j.
+  const int64_t c0 = rb + wb + D * j;  // this lane's first pixel (MAP) or channel
+  if (c0 >= nb) return;
+  MxGroup grp;
+  MxPixels<TB> pix;
+  bool whole = c0 + TB <= nb;
+  if (MAP) {
+    grp = mx_group<TB>(c0, o.HW, o.rows);
+    pix = mx_pixels<TB>(o, grp, 0);
+    whole = grp.whole;
+  }
+#pragma unroll
+  for (int i = 0; i < TA; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = wa + 32 * i + 8 * q + 4 * h;
+      float v[4][TB], bb[4][TB], ss[4][TB];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < TB; ++k) {
+          v[r][k] = acc[i][k][4 * q + r];
+          bb[r][k] = MAP ? bias[at + r] : bias[wb + D * j + k];
+          ss[r][k] = MAP ? rscale[at + r] : rscale[wb + D * j + k];
+        }
+      const int64_t a = ra + at;
+      if (whole && a + 4 <= na) {
+        mx_store_rows<T, TB, 4>(o, MAP ? pix.at[0] + a * o.HW : a * o.N + c0, MAP ? o.HW : o.N, v, bb, ss);
+        continue;
+      }
+      if (MAP) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (a + r < na) mx_store_pixels<T, TB>(o, pix, (a + r) * o.HW, v[r], bb[r][0], ss[r][0]);
+        continue;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < TB; ++k)
+          if (a + r < na && c0 + k < nb)
+            mx_store_rows<T, 1, 1>(o, (a + r) * o.N + c0 + k, 0, (const float(*)[1]) & v[r][k], (const float(*)[1]) & bb[r][k],
+                                   (const float(*)[1]) & ss[r][k]);
+    }
+}
+
+template <class T, bool MAP, int BA, int BB, int WA, int WB>
+int gemm_tile(const MxIn& in, const MxOut& o, hipStream_t st) {
+  constexpr int kThreads = (BA / WA) * (BB / WB) * 64, kLds = 2 * (BA + BB) * 128 + 8 * (MAP ? BA : BB);
+  const int64_t na = MAP ? o.N : o.rows, nb = MAP ? o.rows : o.N;
+  const int64_t ta = (na + BA - 1) / BA, tb = (nb + BB - 1) / BB;
+  if (ta * tb * kThreads >= (int64_t)1 << 32) return fail(CVN_ERR_UNSUPPORTED, "too many pixels and channels");
+  auto k = k_mx_gemm<T, MAP, BA, BB, WA, WB>;
+  static std::atomic<uint64_t> done;
+  once_per_device(done, [&] { (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds); });
+  hipLaunchKernelGGL(k, dim3((unsigned)(ta * tb)), dim3(kThreads), kLds, st, MAP ? in.wc : in.xc, MAP ? in.ws : in.xs, na,
+                     MAP ? in.xc : in.wc, MAP ? in.xs : in.ws, nb, in.KB, (int)ta, (int)tb, o);
+  return check_launch("conv1x1_mxfp4");
+}
+
+template <class T, bool MAP>
+int gemm(const MxIn& in, const MxOut& o, hipStream_t st) {
+  const int64_t na = MAP ? o.N : o.rows, nb = MAP ? o.rows : o.N;
+  auto tiles = [&](int64_t a, int64_t b) { return (na + a - 1) / a * ((nb + b - 1) / b); };
+  if (tiles(256, 256) >= 256) return gemm_tile<T, MAP, 256, 256, 64, 128>(in, o, st);
+  if (tiles(64, 128) >= 256 || nb > 64) return gemm_tile<T, MAP, 64, 128, 32, 64>(in, o, st);
+  return gemm_tile<T, MAP, 64, 64, 32, 32>(in, o, st);
+}
+
+// ------------------------------------------------------------------------------------------------
+// A few pixels: a block makes 16 channels of up to 16 of them, its waves take the channels in turn.
+// ------------------------------------------------------------------------------------------------
+// The matrix is read once and bounds this; the pixels' codes are made on the way by every block.
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_mx_product(const mx_i32x4* __restrict__ xc, const uint8_t* __restrict__ xs,
-                                                         const mx_i32x4* __restrict__ wc, const uint8_t* __restrict__ ws,
-                                                         int KB, MxOut o) {
-  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-  const int64_t tn = (o.N + 15) / 16, tr = (o.rows + 15) / 16, stride = (int64_t)gridDim.x * (kThreads / 64);
-  for (int64_t t = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); t < tn * tr; t += stride) {
-    const int64_t n0 = t / tr * 16, r0 = (t % tr) * 16;
-    const int64_t wrow = min(n0 + j, o.N - 1) * KB, xrow = min(r0 + j, o.rows - 1) * KB;
-    mx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < KB; k += 4) {
-      // past the last block both scales are 2^-127: what is read there instead is lost below float32's range
-      const int kb = min(k + g, KB - 1);
-      const int sw = k + g < KB ? ws[wrow + kb] : 0, sx = k + g < KB ? xs[xrow + kb] : 0;
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(wc[wrow + kb]), mx_operand(xc[xrow + kb]), acc,
-                                                             kMxFp4, kMxFp4, 0, sw, 0, sx);
+__device__ __forceinline__ unsigned mx_quantize_row(const T* x, int64_t step, int n, mx_i32x4* q) {
+  float v[kMxBlock];
+  unsigned mag = 0;
+  if (step == 1 && n == kMxBlock) {
+    typedef typename MxVec<T, 16 / sizeof(T)>::type V;
+#pragma unroll
+    for (int i = 0; i < kMxBlock / (16 / (int)sizeof(T)); ++i) {
+      const V t = ((const V*)x)[i];
+#pragma unroll
+      for (int e = 0; e < 16 / (int)sizeof(T); ++e) v[i * (16 / sizeof(T)) + e] = (float)t[e];
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < kMxBlock; ++c) v[c] = c < n ? (float)x[c * step] : 0.f;
+  }
+#pragma unroll
+  for (int c = 0; c < kMxBlock; ++c) mag = max(mag, mx_mag(v[c]));
+  const unsigned s = mx_scale_code(mag);
+  const float scale = mx_scale(s);
+  *q = mx_i32x4{(int)mx_pack8(v, scale), (int)mx_pack8(v + 8, scale), (int)mx_pack8(v + 16, scale), (int)mx_pack8(v + 24, scale)};
+  if (s == 255u) *q = mx_i32x4{0, 0, 0, 0};
+  return s;
+}
+
+constexpr int kFewWaves = 8, kFewRows = 16;
+template <class T>
+__global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
+  __shared__ float part[kFewWaves][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, wrow = min(n0 + j, o.N - 1) * in.KB;
+  const bool live = j < o.rows;
+  const int64_t b = live ? (uint32_t)j / (uint32_t)o.HW : 0, p = j - b * o.HW;
+  const T* x = (const T*)in.x + b * in.C * o.HW + p;
+  mx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 4 * wave; k < in.KB; k += 4 * kFewWaves) {
+    // lane l holds block k + l / 16 of its operands' rows l % 16; past the last both scales are 2^-127
+    const bool in_row = k + g < in.KB;
+    const int kb = min(k + g, in.KB - 1);
+    const mx_i32x4 w = in.wc[wrow + kb];
+    unsigned sw = in.ws[wrow + kb], sx = 0;
+    mx_i32x4 q = {0, 0, 0, 0};
+    if (live && in_row) {
+      if (in.x) {
+        sx = mx_quantize_row(x + (int64_t)kb * kMxBlock * o.HW, o.HW, (int)min((int64_t)kMxBlock, in.C - kb * kMxBlock), &q);
+        if (in.xc && blockIdx.x == 0) {
+          in.xc[(int64_t)j * in.KB + kb] = q;
+          in.xs[(int64_t)j * in.KB + kb] = (uint8_t)sx;
+        }
+      } else {
+        q = in.xc[(int64_t)j * in.KB + kb];
+        sx = in.xs[(int64_t)j * in.KB + kb];
+      }
+    }
+    if (!in_row) sw = 0;
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w), mx_operand(q), acc, kMxFp4, kMxFp4, 0, (int)sw, 0, (int)sx);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) part[wave][4 * g + e][j] = acc[e];
+  __syncthreads();
+  if (threadIdx.x < 256) {
+    // neighbouring threads store neighbours: channels of one pixel a sample, pixels otherwise
+    const int a = threadIdx.x & 15, c = threadIdx.x >> 4, n = o.HW == 1 ? a : c, r = o.HW == 1 ? c : a;
+    if (r >= o.rows || n0 + n >= o.N) return;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFewWaves; ++i) v += part[i][n][r];
+    const int64_t rb = (uint32_t)r / (uint32_t)o.HW;
+    const float bias = o.bias ? o.bias[n0 + n] : 0.f, scale = o.res_scale ? o.res_scale[n0 + n] : 1.f;
+    mx_store_rows<T, 1, 1>(o, (rb * o.N + n0 + n) * o.HW + (r - rb * o.HW), 0, (const float(*)[1])&v, (const float(*)[1])&bias,
+                           (const float(*)[1])&scale);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Maps of up to 256 channels: quantised in registers, every product and the store in one pass.
+// ------------------------------------------------------------------------------------------------
+// Bound by memory.  Lane l of a wave loads the blocks 2 s + l / 32 of four neighbouring pixels (16 bytes of a float32
+// channel, 512 in a row over 32 lanes), makes their codes, and keeps them as operands for every 32 channels of the result:
+// four products of pixels 4 j + v give it four neighbouring pixels of a channel again.  blockIdx.y takes a share of the
+// channels where there are too few pixels for the CUs.
+template <class T, int S>
+__global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share) {
+  constexpr int V = 4;
+  typedef typename MxVec<T, V>::type W;
+  const int lane = threadIdx.x & 63, j = lane & 31, h = lane >> 5;
+  const int64_t w0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (32 * V), r0 = w0 + V * j;
+  if (w0 >= o.rows) return;  // (no wave waits for another)
+  const MxGroup grp = mx_group<V>(min(r0, o.rows - 1), o.HW, o.rows);
+  // Channels are read from the wave's first pixel on, by 32-bit offsets (64-bit ones of 32 channels would fill the
+  // registers); lanes whose sample is too far off read one by one, as those whose pixels lie in two samples.
+  const int64_t b0 = (uint32_t)w0 / (uint32_t)o.HW, p0 = w0 - b0 * o.HW;
+  const int64_t off = ((grp.b - b0) * in.C + (int64_t)h * kMxBlock) * o.HW + grp.p - p0;
+  const bool near = grp.whole && off * (int64_t)sizeof(T) < (int64_t)1 << 31;
+  const uint32_t lane_off = (uint32_t)(near ? off : 0) * (uint32_t)sizeof(T);
+  mx_i32x4 q[S][V];
+  unsigned sx[S];  // the scales of the V pixels, a byte each
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int kb = 2 * s + h;
+    sx[s] = 0;
+    if (kb >= in.KB) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) q[s][e] = mx_i32x4{0, 0, 0, 0};
+      continue;
+    }
+    const int n = (int)min((int64_t)kMxBlock, in.C - kb * kMxBlock);
+    W t[kMxBlock];
+    if (near && n == kMxBlock) {
+      const char* x = (const char*)((const T*)in.x + (b0 * in.C + 2 * s * kMxBlock) * o.HW + p0);
+#pragma unroll
+      for (int c = 0; c < kMxBlock; ++c) {
+        t[c] = *(const W*)(x + lane_off);
+        x += o.HW * (int64_t)sizeof(T);
+      }
+    } else {
+      int64_t b = grp.b, p = grp.p;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const T* x = (const T*)in.x + (b * in.C + kb * kMxBlock) * o.HW + p;
+        const int ne = grp.r0 + e < o.rows ? n : 0;
+#pragma unroll
+        for (int c = 0; c < kMxBlock; ++c) {
+          t[c][e] = c < ne ? *x : (T)0.f;
+          x += o.HW;
+          asm volatile("" : "+v"(x));  // (one address at a time)
+        }
+        if (++p == o.HW) p = 0, ++b;
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) mx_store<T>(o, r0 + j, n0 + 4 * g + e, acc[e]);
+    for (int e = 0; e < V; ++e) {
+      float v[kMxBlock];
+      unsigned mag = 0;
+#pragma unroll
+      for (int c = 0; c < kMxBlock; ++c) {
+        v[c] = (float)t[c][e];
+        mag = max(mag, mx_mag(v[c]));
+      }
+      const unsigned code = mx_scale_code(mag);
+      const float scale = mx_scale(code);
+      q[s][e] = mx_i32x4{(int)mx_pack8(v, scale), (int)mx_pack8(v + 8, scale), (int)mx_pack8(v + 16, scale), (int)mx_pack8(v + 24, scale)};
+      if (code == 255u) q[s][e] = mx_i32x4{0, 0, 0, 0};
+      sx[s] |= code << (8 * e);
+      if (in.xc && blockIdx.y == 0 && r0 + e < o.rows) {
+        in.xc[(r0 + e) * in.KB + kb] = q[s][e];
+        in.xs[(r0 + e) * in.KB + kb] = (uint8_t)code;
+      }
+    }
+  }
+  const MxPixels<V> pix = mx_pixels<V>(o, grp, 4 * h);
+  const int64_t n1 = min(o.N, (int64_t)(blockIdx.y + 1) * share);
+  for (int64_t n0 = (int64_t)blockIdx.y * share; n0 < n1; n0 += 32) {
+    const int64_t wrow = min(n0 + j, o.N - 1) * in.KB;
+    mx_f32x16 acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = mx_f32x16{};
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int kb = 2 * s + h, at = min(kb, in.KB - 1);
+      const mx_i32x8 w = mx_operand(in.wc[wrow + at]);
+      const int sw = kb < in.KB ? in.ws[wrow + at] : 0;
+      acc[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][0]), acc[0], kMxFp4, kMxFp4, 0, sw, 0, (int)sx[s]);
+      acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][1]), acc[1], kMxFp4, kMxFp4, 0, sw, 1, (int)sx[s]);
+      acc[2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][2]), acc[2], kMxFp4, kMxFp4, 0, sw, 2, (int)sx[s]);
+      acc[3] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][3]), acc[3], kMxFp4, kMxFp4, 0, sw, 3, (int)sx[s]);
+    }
+    if (r0 >= o.rows) continue;
+    MxPixels<V> px = pix;
+#pragma unroll
+    for (int e = 0; e < V; ++e) asm volatile("" : "+v"(px.at[e]));  // (each row's address is made where it is used: kept
+                                                                    // over the loop, 64 of them would fill the registers)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t n = n0 + 8 * i + 4 * h;
+      float v[4][V], bb[4][V], ss[4][V];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t nr = min(n + r, o.N - 1);
+        const float bias = o.bias ? o.bias[nr] : 0.f, scale = o.res_scale ? o.res_scale[nr] : 1.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[r][e] = acc[e][4 * i + r], bb[r][e] = bias, ss[r][e] = scale;
+      }
+      const int64_t step = (n0 + 8 * i) * o.HW;
+      if (grp.whole && n + 4 <= o.N) {
+        mx_store_rows<T, V, 4>(o, px.at[0] + step, o.HW, v, bb, ss);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < o.N) mx_store_pixels<T, V>(o, px, step + r * o.HW, v[r], bb[r][0], ss[r][0]);
+      }
+    }
   }
 }
 
 template <class T>
-int product(const void* xc, const void* xs, const void* wc, const void* ws, int64_t KB, const MxOut& o, hipStream_t st) {
-  const int64_t tiles = (o.N + 15) / 16 * ((o.rows + 15) / 16);
-  hipLaunchKernelGGL(k_mx_product<T>, dim3(mx_grid((tiles + 3) / 4, kThreads)), dim3(kThreads), 0, st, (const mx_i32x4*)xc,
-                     (const uint8_t*)xs, (const mx_i32x4*)wc, (const uint8_t*)ws, (int)KB, o);
+int conv(const MxIn& in, const MxOut& o, bool keep, hipStream_t st) {
+  const int64_t tiles = (o.rows + 511) / 512, n32 = (o.N + 31) / 32;
+  // as many shares of the channels as give every CU two blocks
+  const int64_t shares = std::min(n32, std::max<int64_t>(1, 512 / tiles)), share = (n32 + shares - 1) / shares * 32;
+  const dim3 grid((unsigned)tiles, (unsigned)((o.N + share - 1) / share));
+  MxIn a = in;
+  if (!keep) a.xc = nullptr;
+  switch ((in.KB + 1) / 2) {
+    case 1: hipLaunchKernelGGL((k_mx_conv<T, 1>), grid, dim3(256), 0, st, a, o, (int)share); break;
+    case 2: hipLaunchKernelGGL((k_mx_conv<T, 2>), grid, dim3(256), 0, st, a, o, (int)share); break;
+    case 3: hipLaunchKernelGGL((k_mx_conv<T, 3>), grid, dim3(256), 0, st, a, o, (int)share); break;
+    default: hipLaunchKernelGGL((k_mx_conv<T, 4>), grid, dim3(256), 0, st, a, o, (int)share); break;
+  }
   return check_launch("conv1x1_mxfp4");
 }
 
@@ -61,6 +553,20 @@ int mx_check_product(int64_t B, int64_t C, int64_t HW, int64_t N, int type) {
 bool mx_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return a && b && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+template <class T>
+int product(const MxIn& in, const MxOut& o, int type, bool keep, hipStream_t st) {
+  if (o.rows <= kFewRows) {
+    hipLaunchKernelGGL(k_mx_few<T>, dim3((unsigned)((o.N + 15) / 16)), dim3(kFewWaves * 64), 0, st, in, o);
+    return check_launch("conv1x1_mxfp4");
+  }
+  if (in.x && in.KB <= 8 && o.HW > 1) return conv<T>(in, o, keep, st);
+  if (in.x) {
+    const int q = mx_quantize(in.x, type, o.rows / o.HW, in.C, o.HW, in.xc, in.xs, st);
+    if (q != CVN_OK) return q;
+  }
+  return o.HW == 1 ? gemm<T, false>(in, o, st) : gemm<T, true>(in, o, st);
 }
 
 }  // namespace
@@ -89,19 +595,17 @@ extern "C" int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, i
       mx_overlap(y, ny, x_codes, rows * KB * 16) || mx_overlap(y, ny, x_scales, rows * KB) ||
       (y != residual && mx_overlap(y, ny, residual, ny)))
     return fail(CVN_ERR_ARG, "the output shares memory with an input");
-  if (x && !x_codes) {
+  const bool keep = x_codes != nullptr;
+  if (x && !keep) {
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < cvn_conv1x1_mxfp4_workspace(0, B, C, HW, N))
       return fail(CVN_ERR_WORKSPACE, "workspace missing, too small or not aligned to 16 bytes");
     x_codes = workspace;
     x_scales = (char*)workspace + rows * KB * 16;
   }
   const hipStream_t st = (hipStream_t)stream;
-  if (x) {
-    const int q = mx_quantize(x, type, B, C, HW, x_codes, x_scales, st);
-    if (q != CVN_OK) return q;
-  }
+  const MxIn in = {x, (mx_i32x4*)x_codes, (uint8_t*)x_scales, (const mx_i32x4*)w_codes, (const uint8_t*)w_scales, C, (int)KB};
   const MxOut o = {bias, res_scale, residual, y, HW, N, rows, act};
-  if (type == CVN_F32) return product<float>(x_codes, x_scales, w_codes, w_scales, KB, o, st);
-  if (type == CVN_BF16) return product<__bf16>(x_codes, x_scales, w_codes, w_scales, KB, o, st);
-  return product<_Float16>(x_codes, x_scales, w_codes, w_scales, KB, o, st);
+  if (type == CVN_F32) return product<float>(in, o, type, keep, st);
+  if (type == CVN_BF16) return product<__bf16>(in, o, type, keep, st);
+  return product<_Float16>(in, o, type, keep, st);
 }
