@@ -1,86 +1,392 @@
 // Gradients of a 1x1 convolution of MXFP4 operands, straight through their quantisation (the format: mxfp4.h):
 //   gx[b,c,p] = sum_n w[n][c] gy[b,n,p]     gw[n][c] = sum_{b,p} gy[b,n,p] x[b,p][c]     gb[n] = sum_{b,p} gy[b,n,p]
-// with the 4-bit values as they are: no operand is rounded.
+// The 4-bit values times their scales are bfloat16 numbers, and gy is a sum of them: one (bfloat16), two (float16: 11 bits in
+// 8 + 3) or three (float32: 24 bits in 8 + 8 + 8).  So the products run on the bfloat16 matrix units, one a part, with no operand
+// rounded (parts of float32 below 2^-133 are lost), and are summed in float32.
+#include <algorithm>
+
 #include "mxfp4.h"
 
 namespace cvn {
 namespace {
 
-constexpr int kThreads = 256;
+typedef __bf16 mx_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
+typedef short mx_i16x4 __attribute__((ext_vector_type(4)));
+typedef short mx_i16x8 __attribute__((ext_vector_type(8)));
 
-// A thread makes eight channels of a pixel.
+constexpr int kThreads = 256;
+enum { kGradX, kGradW };
+
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_mx_grad_x(const T* __restrict__ gy, const unsigned* __restrict__ wc,
-                                                        const uint8_t* __restrict__ ws, int64_t C, int64_t N, int64_t HW,
-                                                        int64_t rows, int KB, T* __restrict__ gx) {
-  const int64_t stride = (int64_t)gridDim.x * kThreads, total = rows * ((C + 7) / 8);
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += stride) {
-    const int64_t c8 = i / rows, r = i - c8 * rows, b = r / HW, p = r - b * HW;
-    float acc[8] = {};
-    for (int64_t n = 0; n < N; ++n) {
-      float w[8];
-      mx_unpack8(wc[n * KB * 4 + c8], mx_scale(ws[n * KB + c8 / 4]), w);
-      const float g = (float)gy[(b * N + n) * HW + p];
+struct MxGrad;  // values of a 16-byte vector, parts of a value, terms of a step
+template <>
+struct MxGrad<float> {
+  static constexpr int V = 4, P = 3, K = 32;
+};
+template <>
+struct MxGrad<__bf16> {
+  static constexpr int V = 8, P = 1, K = 64;
+};
+template <>
+struct MxGrad<_Float16> {
+  static constexpr int V = 8, P = 2, K = 64;
+};
+
+// A value's parts, largest first.
+__device__ __forceinline__ void mx_split(__bf16 v, __bf16* p) { p[0] = v; }
+__device__ __forceinline__ void mx_split(_Float16 v, __bf16* p) {
+  const float f = (float)v;
+  p[0] = (__bf16)f;
+  const float r = f - (float)p[0];
+  p[1] = (__bf16)(r == r ? r : 0.f);  // (infinities and NaNs are whole in the first part)
+}
+__device__ __forceinline__ __bf16 mx_top(float v) { return __builtin_bit_cast(__bf16, (short)(__float_as_uint(v) >> 16)); }
+__device__ __forceinline__ void mx_split(float v, __bf16* p) {
+  p[0] = mx_top(v == v ? v : __uint_as_float(0x7fc00000u));  // (a NaN cut short may look like an infinity)
+  const float r = v - (float)p[0], s = r == r ? r : 0.f;
+  p[1] = mx_top(s);
+  p[2] = mx_top(s - (float)p[1]);
+}
+
+struct MxGradArgs {
+  const void* gy;
+  const mx_i32x4* codes;  // of the matrix (gx) or the map (gw)
+  const uint8_t* scales;
+  int64_t C, N, HW, rows;
+  int KB;
+  void* out;       // gx, or gw and its parts [splits][N][C]
+  double* gb;      // gw: parts [splits][N], or null
+  int64_t terms;   // of a split
+  int ta, tb;
+};
+
+// D[i][k] = sum over terms of A's row i and B's row k, on a tile of BA x BB, half of each to a wave.  gx: A the matrix' columns (c), B the pixels, terms n.  gw: A the
+// channels of gy (n), B those of x (c), terms the pixels.  The codes come by terms, 32 neighbours of a tile's row to a block, and
+// lie in LDS as they come: a transposing read gives a lane the terms of its column.  gy comes either way: with its
+// terms side by side (ONE false, gw, or ONE, gx), or by terms.
+template <class T, int KIND, bool ONE, int BA, int BB>
+__global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
+  typedef MxGrad<T> G;
+  constexpr int V = G::V, P = G::P, K = G::K;
+  constexpr int BC = KIND == kGradX ? BA : BB, BG = KIND == kGradX ? BB : BA;  // rows of the codes' and gy's tile
+  constexpr bool kByTerms = (KIND == kGradX) != ONE;                           // gy's tile [terms][rows]
+  constexpr int GR = kByTerms ? K : BG, GC = kByTerms ? BG : K;                // its rows and columns as stored
+  // Rows are padded so that what 16 lanes read at once lies in different banks: 32 bytes of four rows for the
+  // transposing reads, 16 of neighbouring rows otherwise.
+  constexpr int CS = BC * 2 + 32, GS = GC * 2 + (kByTerms ? 32 : 16);
+  constexpr int NG = GR * GC / V / kThreads, NC = (K * BC / 32 + kThreads - 1) / kThreads;
+  __shared__ __attribute__((aligned(16))) char lds[K * CS + P * GR * GS];
+  char* const lc = lds;
+  char* const lg = lds + K * CS;
+  typedef T W __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j = lane & 31, h = lane >> 5;
+
+  const int t = blockIdx.x;
+  const int64_t a0 = (int64_t)(t % a.ta) * BA, b0 = (int64_t)(t / a.ta) * BB;
+  const int64_t c0 = KIND == kGradX ? a0 : b0, g0 = KIND == kGradX ? b0 : a0;
+  const int64_t terms = KIND == kGradX ? a.N : a.rows;
+  const int64_t k_first = (int64_t)blockIdx.y * a.terms, k_end = min(terms, k_first + a.terms);
+  const T* const gy = (const T*)a.gy;
+
+  W g[NG];
+  mx_i32x4 q[NC];
+  unsigned qs[NC];
+  // Row n or pixel r of gy's vector i, its first element along the vector.
+  auto load = [&](int64_t k0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(g, w[e], acc[e]);
+    for (int i = 0; i < NG; ++i) {
+      const int at = tid + i * kThreads, row = at / (GC / V), col = at % (GC / V) * V;
+      g[i] = W{};
+      const int64_t k = k0 + (kByTerms ? row : col), m = g0 + (kByTerms ? col : row);
+      const int64_t n = KIND == kGradX ? k : m, r = KIND == kGradX ? m : k;
+      const int64_t n_end = KIND == kGradX ? k_end : a.N, r_end = KIND == kGradX ? a.rows : k_end;
+      if (n >= n_end || r >= r_end) continue;
+      if (ONE) {  // (rows, N): vectors along n
+        const T* src = gy + r * a.N + n;
+        if (n + V <= n_end) {
+          g[i] = *(const W*)src;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (n + e < n_end) g[i][e] = src[e];
+        }
+      } else {  // (B, N, HW): vectors along the pixels
+        int64_t b = (uint32_t)r / (uint32_t)a.HW, p = r - b * a.HW;
+        const T* src = gy + (b * a.N + n) * a.HW + p;
+        if (p + V <= a.HW && r + V <= r_end) {
+          g[i] = *(const W*)src;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            if (r + e < r_end) g[i][e] = *src;
+            ++src;
+            if (++p == a.HW) p = 0, src += (a.N - 1) * a.HW;
+          }
+        }
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c8 * 8 + e < C) gx[(b * C + c8 * 8 + e) * HW + p] = (T)acc[e];
+    for (int i = 0; i < NC; ++i) {
+      const int at = tid + i * kThreads, row = at / (BC / 32), piece = at % (BC / 32);
+      const int64_t k = k0 + row, kb = c0 / 32 + piece;
+      q[i] = mx_i32x4{0, 0, 0, 0};
+      qs[i] = 127;
+      if (row < K && k < k_end && kb < a.KB) {
+        q[i] = a.codes[k * a.KB + kb];
+        qs[i] = a.scales[k * a.KB + kb];
+      }
+    }
+  };
+  // Sums of gy over the pixels, of the rows or columns that this thread loads.
+  constexpr int NB = KIND != kGradW ? 1 : kByTerms ? V : NG;
+  double sum[NB] = {};
+  auto store = [&] {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int at = tid + i * kThreads, row = at / (GC / V), col = at % (GC / V) * V;
+      __bf16 part[P][V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        __bf16 x[P];
+        mx_split(g[i][e], x);
+#pragma unroll
+        for (int p = 0; p < P; ++p) part[p][e] = x[p];
+      }
+      typedef __bf16 S __attribute__((ext_vector_type(V)));
+#pragma unroll
+      for (int p = 0; p < P; ++p) *(S*)(lg + (p * GR + row) * GS + col * 2) = *(const S*)part[p];
+      if (KIND == kGradW && a.gb && b0 == 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[(kByTerms ? e : i) % NB] += (double)(float)g[i][e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int at = tid + i * kThreads, row = at / (BC / 32), piece = at % (BC / 32);
+      if (row >= K) continue;
+      const float scale = mx_scale(qs[i]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const mx_bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 0),
+                        v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 1),
+                        v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 2),
+                        v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 3);
+        *(mx_bf16x8*)(lc + row * CS + piece * 64 + w * 16) = mx_bf16x8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
+      }
+    }
+  };
+  // Eight terms, 16 step + 8 (l / 32) on, of row `row` + l % 32 of a tile.
+  typedef __attribute__((address_space(3))) mx_i16x4* lds_i16x4;
+  auto by_terms = [&](const char* base, int stride, int row, int step) {
+    const char* p = base + (16 * step + 8 * h + (lane & 15) / 4) * stride + (row + (lane & 16) + (lane & 3) * 4) * 2;
+    const mx_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)p),
+                   hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(p + 4 * stride));
+    return __builtin_bit_cast(mx_bf16x8, mx_i16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
+  };
+  auto side_by_side = [&](const char* base, int row, int step) {
+    return *(const mx_bf16x8*)(base + (row + j) * GS + (16 * step + 8 * h) * 2);
+  };
+
+  constexpr int TA = BA / 64, TB = BB / 64, TC = KIND == kGradX ? TA : TB, TG = KIND == kGradX ? TB : TA;
+  const int wa = (wave & 1) * (BA / 2), wb = (wave >> 1) * (BB / 2);
+  const int wc = KIND == kGradX ? wa : wb, wg = KIND == kGradX ? wb : wa;
+  mx_f32x16 acc[TA][TB];
+#pragma unroll
+  for (int i = 0; i < TA; ++i)
+#pragma unroll
+    for (int k = 0; k < TB; ++k) acc[i][k] = mx_f32x16{};
+  load(k_first);
+  for (int64_t k0 = k_first; k0 < k_end; k0 += K) {
+    __syncthreads();
+    store();
+    __syncthreads();
+    if (k0 + K < k_end) load(k0 + K);
+#pragma unroll
+    for (int s = 0; s < K / 16; ++s) {
+      mx_bf16x8 c[TC];
+#pragma unroll
+      for (int i = 0; i < TC; ++i) c[i] = by_terms(lc, CS, wc + 32 * i, s);
+#pragma unroll
+      for (int p = P - 1; p >= 0; --p) {
+        const char* base = lg + p * GR * GS;
+        mx_bf16x8 y[TG];
+#pragma unroll
+        for (int i = 0; i < TG; ++i) y[i] = kByTerms ? by_terms(base, GS, wg + 32 * i, s) : side_by_side(base, wg + 32 * i, s);
+#pragma unroll
+        for (int i = 0; i < TA; ++i)
+#pragma unroll
+          for (int k = 0; k < TB; ++k)
+            acc[i][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(KIND == kGradX ? c[i] : y[i], KIND == kGradX ? y[k] : c[k],
+                                                                acc[i][k], 0, 0, 0);
+      }
+    }
+  }
+
+  // Element e of a 32 x 32 result is its row 8 (e / 4) + 4 h + e % 4, column j.
+#pragma unroll
+  for (int k = 0; k < TB; ++k) {
+    const int64_t col = b0 + wb + 32 * k + j;
+    if (KIND == kGradX) {
+      if (col >= a.rows) continue;
+      const int64_t b = (uint32_t)col / (uint32_t)a.HW;
+      T* out = (T*)a.out + b * a.C * a.HW + (col - b * a.HW);
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int64_t c = a0 + wa + 32 * i + 8 * (e / 4) + 4 * h + e % 4;
+          if (c < a.C) out[c * a.HW] = (T)acc[i][k][e];
+        }
+    } else {
+      if (col >= a.C) continue;
+      float* out = (float*)a.out + (int64_t)blockIdx.y * a.N * a.C + col;
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int64_t n = a0 + wa + 32 * i + 8 * (e / 4) + 4 * h + e % 4;
+          if (n < a.N) out[n * a.C] = acc[i][k][e];
+        }
+    }
+  }
+  if (KIND == kGradW && a.gb && b0 == 0) {
+    double* const out = a.gb + (int64_t)blockIdx.y * a.N;
+    if (!kByTerms) {  // the threads of a row are neighbours
+      constexpr int TR = GC / V;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        double s = sum[i % NB];
+#pragma unroll
+        for (int d = TR / 2; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+        const int64_t n = a0 + (tid + i * kThreads) / TR;
+        if (tid % TR == 0 && n < a.N) out[n] = s;
+      }
+    } else {  // those of a column are GC / V apart
+      constexpr int TR = GC / V;
+      double(*red)[GC] = (double(*)[GC])lds;
+      static_assert(sizeof(double) * GC * (kThreads / TR) <= sizeof(lds), "sums fit the operands' memory");
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[tid / TR][tid % TR * V + e] = sum[e % NB];
+      __syncthreads();
+      for (int c = tid; c < GC; c += kThreads) {
+        double s = 0.;
+        for (int i = 0; i < kThreads / TR; ++i) s += red[i][c];
+        if (a0 + c < a.N) out[a0 + c] = s;
+      }
+    }
   }
 }
 
-// A block makes eight entries of a row of the matrix' gradient, its threads take the pixels in turn.
-template <class T>
-__global__ void __launch_bounds__(kThreads) k_mx_grad_w(const T* __restrict__ gy, const unsigned* __restrict__ xc,
-                                                        const uint8_t* __restrict__ xs, int64_t C, int64_t N, int64_t HW,
-                                                        int64_t rows, int KB, float* __restrict__ gw, float* __restrict__ gb) {
-  __shared__ double red[kThreads / 64][9];
-  const int64_t c8s = (C + 7) / 8;
-  for (int64_t t = blockIdx.x; t < N * c8s; t += gridDim.x) {
-    const int64_t n = t / c8s, c8 = t - n * c8s;
-    double acc[9] = {};
-    for (int64_t r = threadIdx.x; r < rows; r += kThreads) {
-      const int64_t b = r / HW, p = r - b * HW;
-      float v[8] = {};
-      if (gw) mx_unpack8(xc[r * KB * 4 + c8], mx_scale(xs[r * KB + c8 / 4]), v);
-      const double g = (double)(float)gy[(b * N + n) * HW + p];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fma(g, (double)v[e], acc[e]);
-      acc[8] += g;
-    }
-#pragma unroll
-    for (int e = 0; e < 9; ++e) {
-#pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) acc[e] += __shfl_xor(acc[e], d);
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][e] = acc[e];
-    }
-    __syncthreads();
-    if (threadIdx.x < 9) {
-      double s = 0.;
-      for (int i = 0; i < kThreads / 64; ++i) s += red[i][threadIdx.x];
-      const int64_t c = c8 * 8 + threadIdx.x;
-      if (threadIdx.x < 8) {
-        if (gw && c < C) gw[n * C + c] = (float)s;
-      } else if (gb && c8 == 0) {
-        gb[n] = (float)s;
-      }
-    }
-    __syncthreads();
+// The sum over the splits, in their order.
+__global__ void __launch_bounds__(kThreads) k_mx_grad_join(const float* __restrict__ part, int64_t n, const double* __restrict__ gbp,
+                                                           int64_t nb, int splits, float* __restrict__ gw, float* __restrict__ gb) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (part && i < n) {
+    double s = 0.;
+    for (int k = 0; k < splits; ++k) s += (double)part[k * n + i];
+    gw[i] = (float)s;
   }
+  if (gb && i < nb) {
+    double s = 0.;
+    for (int k = 0; k < splits; ++k) s += gbp[k * nb + i];
+    gb[i] = (float)s;
+  }
+}
+
+// The bias' gradient alone: a block for a channel.
+template <class T>
+__global__ void __launch_bounds__(kThreads) k_mx_grad_bias(const T* __restrict__ gy, int64_t N, int64_t HW, int64_t rows,
+                                                           float* __restrict__ gb) {
+  __shared__ double red[kThreads / 64];
+  const int64_t n = blockIdx.x;
+  double s = 0.;
+  for (int64_t r = threadIdx.x; r < rows; r += kThreads) {
+    const int64_t b = (uint32_t)r / (uint32_t)HW;
+    s += (double)(float)gy[(b * N + n) * HW + (r - b * HW)];
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) gb[n] = (float)(red[0] + red[1] + red[2] + red[3]);
+}
+
+__global__ void __launch_bounds__(kThreads) k_mx_zero(float* p, int64_t n, float* q, int64_t m) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n || i < m; i += (int64_t)gridDim.x * kThreads) {
+    if (i < n) p[i] = 0.f;
+    if (i < m) q[i] = 0.f;
+  }
+}
+
+// How gw's terms (the pixels) are shared out: enough splits for two blocks a CU, of at least 256 pixels, in whole steps.
+struct MxSplit {
+  int64_t terms, splits;
+};
+MxSplit mx_split_terms(int64_t rows, int64_t C, int64_t N) {
+  const int64_t tiles = (N + 127) / 128 * ((C + 127) / 128);
+  const int64_t want = std::max<int64_t>(1, std::min((rows + 255) / 256, 512 / tiles));
+  MxSplit s;
+  s.terms = std::max<int64_t>(256, ((rows + want - 1) / want + 63) / 64 * 64);
+  s.splits = (rows + s.terms - 1) / s.terms;
+  return s;
+}
+size_t mx_part_bytes(const MxSplit& s, int64_t C, int64_t N) {
+  return (s.splits > 1 ? align_up((size_t)(s.splits * N * C) * sizeof(float)) : 0) + (size_t)(s.splits * N) * sizeof(double);
+}
+
+template <class T, int KIND, bool ONE, int BA, int BB>
+int grad_tile(MxGradArgs a, int64_t na, int64_t nb, int64_t splits, hipStream_t st) {
+  const int64_t ta = (na + BA - 1) / BA, tb = (nb + BB - 1) / BB;
+  if (ta * tb * splits * kThreads >= (int64_t)1 << 32) return fail(CVN_ERR_UNSUPPORTED, "too many pixels and channels");
+  a.ta = (int)ta, a.tb = (int)tb;
+  hipLaunchKernelGGL((k_mx_grad<T, KIND, ONE, BA, BB>), dim3((unsigned)(ta * tb), (unsigned)splits), dim3(kThreads), 0, st, a);
+  return check_launch("conv1x1_mxfp4_backward");
+}
+
+template <class T, bool ONE>
+int grads(const void* gy, const void* xc, const void* xs, const void* wc, const void* ws, int64_t C, int64_t HW, int64_t rows,
+          int64_t N, void* gx, float* gw, float* gb, void* work, hipStream_t st) {
+  const int KB = (int)mx_blocks(C);
+  if (gx) {
+    const MxGradArgs a = {gy, (const mx_i32x4*)wc, (const uint8_t*)ws, C, N, HW, rows, KB, gx, nullptr, N, 0, 0};
+    const int rc = C <= 64 ? grad_tile<T, kGradX, ONE, 64, 128>(a, C, rows, 1, st)
+                           : grad_tile<T, kGradX, ONE, 128, 128>(a, C, rows, 1, st);
+    if (rc != CVN_OK) return rc;
+  }
+  if (gw) {
+    const MxSplit s = mx_split_terms(rows, C, N);
+    float* const part = s.splits > 1 ? (float*)work : gw;
+    double* const gbp = (double*)((char*)work + (s.splits > 1 ? align_up((size_t)(s.splits * N * C) * sizeof(float)) : 0));
+    const MxGradArgs a = {gy, (const mx_i32x4*)xc, (const uint8_t*)xs, C, N, HW, rows, KB, part, gb ? gbp : nullptr, s.terms, 0, 0};
+    int rc;
+    if (C <= 64) rc = N <= 64 ? grad_tile<T, kGradW, ONE, 64, 64>(a, N, C, s.splits, st) : grad_tile<T, kGradW, ONE, 128, 64>(a, N, C, s.splits, st);
+    else rc = N <= 64 ? grad_tile<T, kGradW, ONE, 64, 128>(a, N, C, s.splits, st) : grad_tile<T, kGradW, ONE, 128, 128>(a, N, C, s.splits, st);
+    if (rc != CVN_OK) return rc;
+    if (s.splits > 1 || gb) {
+      const int64_t n = s.splits > 1 ? N * C : 0;
+      hipLaunchKernelGGL(k_mx_grad_join, dim3((unsigned)((std::max(n, N) + kThreads - 1) / kThreads)), dim3(kThreads), 0, st,
+                         s.splits > 1 ? part : nullptr, n, gbp, N, (int)s.splits, gw, gb);
+    }
+  } else if (gb) {
+    hipLaunchKernelGGL(k_mx_grad_bias<T>, dim3((unsigned)N), dim3(kThreads), 0, st, (const T*)gy, N, HW, rows, gb);
+  }
+  return check_launch("conv1x1_mxfp4_backward");
 }
 
 template <class T>
 int grads(const void* gy, const void* xc, const void* xs, const void* wc, const void* ws, int64_t C, int64_t HW, int64_t rows,
-          int64_t N, void* gx, float* gw, float* gb, hipStream_t st) {
-  const int KB = (int)mx_blocks(C);
-  if (gx && rows)
-    hipLaunchKernelGGL(k_mx_grad_x<T>, dim3(mx_grid((rows * ((C + 7) / 8) + kThreads - 1) / kThreads, kThreads)),
-                       dim3(kThreads), 0, st, (const T*)gy, (const unsigned*)wc, (const uint8_t*)ws, C, N, HW, rows, KB, (T*)gx);
-  if (gw || gb)
-    hipLaunchKernelGGL(k_mx_grad_w<T>, dim3(mx_grid(N * (gw ? (C + 7) / 8 : 1), kThreads)), dim3(kThreads), 0, st,
-                       (const T*)gy, (const unsigned*)xc, (const uint8_t*)xs, gw ? C : 1, N, HW, rows, KB, gw, gb);
-  return check_launch("conv1x1_mxfp4_backward");
+          int64_t N, void* gx, float* gw, float* gb, void* work, hipStream_t st) {
+  return HW == 1 ? grads<T, true>(gy, xc, xs, wc, ws, C, HW, rows, N, gx, gw, gb, work, st)
+                 : grads<T, false>(gy, xc, xs, wc, ws, C, HW, rows, N, gx, gw, gb, work, st);
+}
+
+int mx_check_grad(int64_t B, int64_t C, int64_t HW, int64_t N) {
+  if (B < 0 || HW < 0 || C < 1 || N < 1) return fail(CVN_ERR_ARG, "bad shape");
+  if (C > kMxMaxChannels || N > kMxMaxChannels || (HW && B > kMxMaxRows / HW))
+    return fail(CVN_ERR_UNSUPPORTED, "too many channels or pixels");
+  return CVN_OK;
 }
 
 }  // namespace
@@ -89,26 +395,33 @@ int grads(const void* gy, const void* xc, const void* xs, const void* wc, const 
 using namespace cvn;
 
 extern "C" size_t cvn_conv1x1_mxfp4_bwd_workspace(int64_t B, int64_t C, int64_t HW, int64_t N) {
-  (void)B, (void)C, (void)HW, (void)N;
-  return 0;
+  if (mx_check_grad(B, C, HW, N) != CVN_OK || B * HW == 0) return 0;
+  return mx_part_bytes(mx_split_terms(B * HW, C, N), C, N);
 }
 
 extern "C" int cvn_conv1x1_mxfp4_bwd(const void* grad_y, int type, const void* x_codes, const void* x_scales,
                                      const void* w_codes, const void* w_scales, int64_t B, int64_t C, int64_t HW, int64_t N,
                                      void* grad_x, float* grad_w, float* grad_bias, void* workspace, size_t workspace_bytes,
                                      cvn_stream_t stream) {
-  (void)workspace, (void)workspace_bytes;
-  if (B < 0 || HW < 0 || C < 1 || N < 1 || !mx_type_size(type)) return fail(CVN_ERR_ARG, "bad shape or type");
-  if (C > kMxMaxChannels || N > kMxMaxChannels || (HW && B > kMxMaxRows / HW))
-    return fail(CVN_ERR_UNSUPPORTED, "too many channels or pixels");
+  const int rc = mx_check_grad(B, C, HW, N);
+  if (rc != CVN_OK) return rc;
+  if (!mx_type_size(type)) return fail(CVN_ERR_ARG, "bad type");
   if (!grad_x && !grad_w && !grad_bias) return CVN_OK;
   const int64_t rows = B * HW;
-  if ((rows && !grad_y) || (grad_x && rows && (!w_codes || !w_scales)) || (grad_w && rows && (!x_codes || !x_scales)))
+  const hipStream_t st = (hipStream_t)stream;
+  if (rows == 0) {
+    if (grad_w || grad_bias)
+      hipLaunchKernelGGL(k_mx_zero, dim3(256), dim3(kThreads), 0, st, grad_w, grad_w ? N * C : 0, grad_bias, grad_bias ? N : 0);
+    return check_launch("conv1x1_mxfp4_backward");
+  }
+  if (!grad_y || (grad_x && (!w_codes || !w_scales)) || (grad_w && (!x_codes || !x_scales)))
     return fail(CVN_ERR_ARG, "null pointer");
   if (((uintptr_t)w_codes | (uintptr_t)x_codes) & 15) return fail(CVN_ERR_ARG, "codes must be aligned to 16 bytes");
-  const hipStream_t st = (hipStream_t)stream;
-  if (type == CVN_F32) return grads<float>(grad_y, x_codes, x_scales, w_codes, w_scales, C, HW, rows, N, grad_x, grad_w, grad_bias, st);
+  if (grad_w && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N)))
+    return fail(CVN_ERR_WORKSPACE, "workspace missing, too small or not aligned to 16 bytes");
+  if (type == CVN_F32)
+    return grads<float>(grad_y, x_codes, x_scales, w_codes, w_scales, C, HW, rows, N, grad_x, grad_w, grad_bias, workspace, st);
   if (type == CVN_BF16)
-    return grads<__bf16>(grad_y, x_codes, x_scales, w_codes, w_scales, C, HW, rows, N, grad_x, grad_w, grad_bias, st);
-  return grads<_Float16>(grad_y, x_codes, x_scales, w_codes, w_scales, C, HW, rows, N, grad_x, grad_w, grad_bias, st);
+    return grads<__bf16>(grad_y, x_codes, x_scales, w_codes, w_scales, C, HW, rows, N, grad_x, grad_w, grad_bias, workspace, st);
+  return grads<_Float16>(grad_y, x_codes, x_scales, w_codes, w_scales, C, HW, rows, N, grad_x, grad_w, grad_bias, workspace, st);
 }
