@@ -72,6 +72,7 @@ struct MxOut {
   void* y;
   int64_t HW, N, rows;  // rows = B HW
   int act;
+  bool lines;  // rows of y start on cache lines
 };
 
 int mx_quantize(const void* x, int type, int64_t B, int64_t C, int64_t HW, void* codes, void* scales, hipStream_t st);

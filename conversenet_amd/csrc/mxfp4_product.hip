@@ -28,14 +28,6 @@ struct MxVec<T, 1> {
   typedef T type;
 };
 
-// What happens to a sum on its way out.
-template <class T>
-__device__ __forceinline__ float mx_finish(const MxOut& o, float v, float bias, float scale) {
-  v += bias;
-  if (o.act == CVN_ACT_GELU) v = gelu_fast(v);
-  return v * scale;
-}
-
 // Where a lane's V neighbouring pixels from row r0 on lie.
 struct MxGroup {
   int64_t r0, b, p;
@@ -51,16 +43,29 @@ __device__ __forceinline__ MxGroup mx_group(int64_t r0, int64_t HW, int64_t rows
   return g;
 }
 
-// R sums (rows of channels i, i + step, ..) of V elements side by side, from element `at` of the first on.
-template <class T, int V, int R>
-__device__ __forceinline__ void mx_store_rows(const MxOut& o, int64_t at, int64_t step, const float (*v)[V], const float (*bias)[V],
-                                              const float (*scale)[V]) {
+// What happens to R rows of V sums with their bias on the way out: act, residual scale.
+template <int V, int R>
+__device__ __forceinline__ void mx_finish(const MxOut& o, float (*v)[V], const float (*scale)[V]) {
+  if (o.act == CVN_ACT_GELU) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[r][e] = gelu_fast(v[r][e]);
+  }
+  if (o.res_scale) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[r][e] *= scale[r][e];
+  }
+}
+
+// Stores R rows, `step` elements apart, of V finished values side by side, from element `at` of the first on.  NT: past the
+// caches, for rows that start on cache lines (8 x 64 x 256 x 256 float32 to 128 channels: 74 us, through the caches 98); a
+// line that two waves store parts of is better put together in the cache (64 x 321 x 481 to 128: 30 us, past it 42).
+template <class T, bool NT, int V, int R>
+__device__ __forceinline__ void mx_store_rows(const MxOut& o, int64_t at, int64_t step, float (*v)[V]) {
   typedef typename MxVec<T, V>::type W;
-  float t[R][V];
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int e = 0; e < V; ++e) t[r][e] = mx_finish<T>(o, v[r][e], bias[r][e], scale[r][e]);
   if (o.residual) {
     W res[R];
 #pragma unroll
@@ -68,18 +73,20 @@ __device__ __forceinline__ void mx_store_rows(const MxOut& o, int64_t at, int64_
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int e = 0; e < V; ++e) t[r][e] += (float)((const T*)&res[r])[e];
+      for (int e = 0; e < V; ++e) v[r][e] += (float)((const T*)&res[r])[e];
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     W out;
 #pragma unroll
-    for (int e = 0; e < V; ++e) ((T*)&out)[e] = (T)t[r][e];
-    __builtin_nontemporal_store(out, (W*)((T*)o.y + at + r * step));
+    for (int e = 0; e < V; ++e) ((T*)&out)[e] = (T)v[r][e];
+    W* const to = (W*)((T*)o.y + at + r * step);
+    if (NT) __builtin_nontemporal_store(out, to);
+    else *to = out;
   }
 }
 
-// The elements of channel n of a group's V pixels, and which of them there are.
+// V elements of a row (channel n of a group's pixels), and which of them there are.
 template <int V>
 struct MxPixels {
   int64_t at[V];
@@ -98,17 +105,14 @@ __device__ __forceinline__ MxPixels<V> mx_pixels(const MxOut& o, const MxGroup& 
   }
   return x;
 }
-// One channel of them, `step` elements further on, one by one.
+// A row of them, `step` elements further on, one by one.
 template <class T, int V>
-__device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V>& x, int64_t step, const float* v, float bias,
-                                                float scale) {
+__device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V>& x, int64_t step, const float* v) {
 #pragma unroll
   for (int e = 0; e < V; ++e)
     if (x.live >> e & 1) {
       const int64_t i = x.at[e] + step;
-      float t = mx_finish<T>(o, v[e], bias, scale);
-      if (o.residual) t += (float)((const T*)o.residual)[i];
-      ((T*)o.y)[i] = (T)t;
+      ((T*)o.y)[i] = (T)(o.residual ? v[e] + (float)((const T*)o.residual)[i] : v[e]);
     }
 }
 
@@ -122,19 +126,20 @@ __device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V
 // scales are 2^-127: the products are lost below float32's range.
 constexpr int kStep = 8;  // blocks of a step
 
-// The word of four scales at place `at` of `total`, as loaded from the last place where a word fits ..
-__device__ __forceinline__ unsigned mx_scales_load(const uint8_t* s, int64_t at, int64_t total) {
+// The word of four scales at byte `at` of an operand's scales, as loaded from `last` at most, where the last whole word is
+// (below 0 where there are fewer than four bytes) ..
+__device__ __forceinline__ unsigned mx_scales_load(const uint8_t* s, int at, int last) {
   typedef unsigned U __attribute__((aligned(1)));
-  if (total >= 4) return *(const U*)(s + min(at, total - 4));
+  if (last >= 0) return *(const U*)(s + (unsigned)min(at, last));
   unsigned v = 0;
   for (int i = 0; i < 3; ++i)
-    if (at + i < total) v |= (unsigned)s[at + i] << (8 * i);
+    if (at + i < last + 4) v |= (unsigned)s[at + i] << (8 * i);
   return v;
 }
 // .. and put right, for blocks kb .. of KB: 0 past the last.
-__device__ __forceinline__ unsigned mx_scales_tail(unsigned v, int64_t at, int64_t total, int kb, int KB) {
+__device__ __forceinline__ unsigned mx_scales_tail(unsigned v, int at, int last, int kb, int KB) {
   if (kb >= KB) return 0;
-  if (total >= 4) v >>= 8 * (int)(at - min(at, total - 4));
+  if (last >= 0) v >>= 8 * (at - min(at, last));
   return KB - kb < 4 ? v & ((1u << (8 * (KB - kb))) - 1) : v;
 }
 
@@ -142,65 +147,78 @@ typedef __attribute__((address_space(3))) void* mx_lds;
 typedef const __attribute__((address_space(1))) void* mx_glob;
 
 // Tiles of BA x BB rows of the two operands, WA x WB of them to a wave.  MAP: A is the matrix, B the pixels, and a lane
-// stores four pixels of a channel; otherwise (one pixel a sample) A is the pixels, and it stores four channels of a pixel.
-// In either case lane j of the four 32-row tiles of a group holds the rows 4 j + 0 .. 3 of B.
-template <class T, bool MAP, int BA, int BB, int WA, int WB>
+// stores TB pixels of a channel; otherwise (one pixel a sample) A is the pixels, and it stores TB channels of a pixel.
+// In either case lane j of the TB 32-row tiles of a wave holds the rows TB j + 0 .. TB - 1 of B.
+// A block makes tile after tile, and fetches the first step of the next before it stores.
+template <class T, bool MAP, bool NT, int BA, int BB, int WA, int WB>
 __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
     k_mx_gemm(const mx_i32x4* __restrict__ ac, const uint8_t* __restrict__ as, int64_t na, const mx_i32x4* __restrict__ bc,
               const uint8_t* __restrict__ bs, int64_t nb, int KB, int ta, int tb, MxOut o) {
   constexpr int NW = (BA / WA) * (BB / WB), TA = WA / 32, TB = WB / 32;
   constexpr int D = TB;  // rows of B between neighbouring lanes
   constexpr int kBytes = (BA + BB) * 128;
-  extern __shared__ char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
-  // Blocks of one XCD take a run of tiles, in patches of eight A tiles: its L2 holds what they share.
-  const int nt = ta * tb;
-  int t = blockIdx.x;
-  {
-    const int q = nt / 8, rem = nt % 8, x = t & 7, i = t >> 3;
-    t = x < rem ? x * (q + 1) + i : rem * (q + 1) + (x - rem) * q + i;
-  }
-  const int patch = t / (8 * tb), a0 = patch * 8, aw = min(8, ta - a0), in = t - patch * 8 * tb;
-  const int64_t ra = (int64_t)(a0 + in % aw) * BA, rb = (int64_t)(in / aw) * BB;
-
-  // what this wave fetches: rows 8 (wave + NW i) + lane / 8 of the A then the B tile
   constexpr int LA = BA / 8 / NW, LB = BB / 8 / NW;
-  const mx_i32x4* src[LA + LB];
-  int piece[LA + LB];
-#pragma unroll
-  for (int i = 0; i < LA + LB; ++i) {
-    const bool isa = i < LA;
-    const int row = 8 * (wave + NW * (isa ? i : i - LA)) + (lane >> 3);
-    src[i] = isa ? ac + min(ra + row, na - 1) * KB : bc + min(rb + row, nb - 1) * KB;
-    piece[i] = (lane & 7) ^ ((isa ? row : row / D) & 7);
-  }
-  auto fetch = [&](int kb0, char* buf) {
-#pragma unroll
-    for (int i = 0; i < LA + LB; ++i) {
-      const int row8 = (wave + NW * (i < LA ? i : i - LA)) * 8 + (i < LA ? 0 : BA);
-      __builtin_amdgcn_global_load_lds((mx_glob)(src[i] + min(kb0 + piece[i], KB - 1)), (mx_lds)(buf + row8 * 128), 16, 0, 0);
-    }
-  };
+  static_assert(8 / D * NW % 8 == 0, "a wave's fetches of a tile put a row's pieces in one order");
+  extern __shared__ char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
   const int wa = wave % (BA / WA) * WA, wb = wave / (BA / WA) * WB;
-  int64_t sa_at[TA], sb_at[TB];
+  const int nt = ta * tb;
+
+  // A tile's place, and what a wave reads of it: rows 8 (wave + NW i) + lane / 8 of its codes, its rows' scales.  (32-bit offsets
+  // from the tile's first row: 128 rows of 65536 channels are 4 MB.)
+  int64_t ra, rb;
+  const char *acodes, *bcodes;
+  const uint8_t *ascales, *bscales;
+  int alast, blast;
+  uint32_t aoff[LA], boff[LB];
+  int as_at[TA], bs_at[TB];
+  const int apiece = (lane & 7) ^ (lane >> 3), bpiece = (lane & 7) ^ (((8 * wave + (lane >> 3)) / D) & 7);
+  auto place = [&](int t) {
+    // Blocks of one XCD take a run of tiles, in patches of eight A tiles: its L2 holds what they share.
+    const int per = nt / 8, rem = nt % 8, x = t & 7, i8 = t >> 3;
+    const int tile = x < rem ? x * (per + 1) + i8 : rem * (per + 1) + (x - rem) * per + i8;
+    const int patch = tile / (8 * tb), a0 = patch * 8, aw = min(8, ta - a0), in = tile - patch * 8 * tb;
+    ra = (int64_t)(a0 + in % aw) * BA, rb = (int64_t)(in / aw) * BB;
+    acodes = (const char*)(ac + ra * KB), bcodes = (const char*)(bc + rb * KB);
+    ascales = as + ra * KB, bscales = bs + rb * KB;
+    const int amost = (int)min((int64_t)BA, na - ra) - 1, bmost = (int)min((int64_t)BB, nb - rb) - 1;
+    alast = (int)min((na - ra) * KB, (int64_t)1 << 30) - 4, blast = (int)min((nb - rb) * KB, (int64_t)1 << 30) - 4;
 #pragma unroll
-  for (int i = 0; i < TA; ++i) sa_at[i] = min(ra + wa + 32 * i + j, na - 1) * KB + 4 * h;
+    for (int i = 0; i < LA; ++i) aoff[i] = (uint32_t)(min(8 * (wave + NW * i) + (lane >> 3), amost) * KB) * 16;
 #pragma unroll
-  for (int i = 0; i < TB; ++i) sb_at[i] = min(rb + wb + D * j + i, nb - 1) * KB + 4 * h;
+    for (int i = 0; i < LB; ++i) boff[i] = (uint32_t)(min(8 * (wave + NW * i) + (lane >> 3), bmost) * KB) * 16;
+#pragma unroll
+    for (int i = 0; i < TA; ++i) as_at[i] = min(wa + 32 * i + j, amost) * KB + 4 * h;
+#pragma unroll
+    for (int i = 0; i < TB; ++i) bs_at[i] = min(wb + D * j + i, bmost) * KB + 4 * h;
+  };
   unsigned sa[TA], sb[TB];
-  auto load_scales = [&](int kb0) {
+  auto fetch = [&](int kb0, char* buf) {
+    const uint32_t ap = (uint32_t)min(kb0 + apiece, KB - 1) * 16, bp = (uint32_t)min(kb0 + bpiece, KB - 1) * 16;
 #pragma unroll
-    for (int i = 0; i < TA; ++i) sa[i] = mx_scales_load(as, sa_at[i] + kb0, na * KB);
+    for (int i = 0; i < LA; ++i)
+      __builtin_amdgcn_global_load_lds((mx_glob)(acodes + (aoff[i] + ap)), (mx_lds)(buf + (wave + NW * i) * 1024), 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < TB; ++i) sb[i] = mx_scales_load(bs, sb_at[i] + kb0, nb * KB);
+    for (int i = 0; i < LB; ++i)
+      __builtin_amdgcn_global_load_lds((mx_glob)(bcodes + (boff[i] + bp)), (mx_lds)(buf + BA * 128 + (wave + NW * i) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TA; ++i) sa[i] = mx_scales_load(ascales, as_at[i] + kb0, alast);
+#pragma unroll
+    for (int i = 0; i < TB; ++i) sb[i] = mx_scales_load(bscales, bs_at[i] + kb0, blast);
   };
 
-  // bias and residual scale of the tile's channels, behind the operands
-  float* bias = (float*)(smem + 2 * kBytes);
+  place(blockIdx.x);
+  fetch(0, smem);
+  int cur = 0;
+  // bias and residual scale of a tile's channels, behind the operands, for this tile and the next
   constexpr int NC = MAP ? BA : BB;
-  float* rscale = bias + NC;
+  float* bias = (float*)(smem + 2 * kBytes);
+  for (int t = blockIdx.x;;) {
+  const int64_t ra0 = ra, rb0 = rb;
+  const int next = t + (int)gridDim.x;
+  float* const rscale = bias + NC;
   for (int i = threadIdx.x; i < NC; i += NW * 64) {
-    const int64_t n = (MAP ? ra : rb) + i;
+    const int64_t n = (MAP ? ra0 : rb0) + i;
     bias[i] = o.bias && n < o.N ? o.bias[n] : 0.f;
     rscale[i] = o.res_scale && n < o.N ? o.res_scale[n] : 1.f;
   }
@@ -210,9 +228,6 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
   for (int i = 0; i < TA; ++i)
 #pragma unroll
     for (int k = 0; k < TB; ++k) acc[i][k] = mx_f32x16{};
-  fetch(0, smem);
-  load_scales(0);
-  int cur = 0;
   for (int kb0 = 0; kb0 < KB; kb0 += kStep) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -223,12 +238,15 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
     for (int i = 0; i < TB; ++i) ub[i] = sb[i];
     if (kb0 + kStep < KB) {
       fetch(kb0 + kStep, smem + (cur ^ 1) * kBytes);
-      load_scales(kb0 + kStep);
     } else {
 #pragma unroll
-      for (int i = 0; i < TA; ++i) ua[i] = mx_scales_tail(ua[i], sa_at[i] + kb0, na * KB, kb0 + 4 * h, KB);
+      for (int i = 0; i < TA; ++i) ua[i] = mx_scales_tail(ua[i], as_at[i] + kb0, alast, kb0 + 4 * h, KB);
 #pragma unroll
-      for (int i = 0; i < TB; ++i) ub[i] = mx_scales_tail(ub[i], sb_at[i] + kb0, nb * KB, kb0 + 4 * h, KB);
+      for (int i = 0; i < TB; ++i) ub[i] = mx_scales_tail(ub[i], bs_at[i] + kb0, blast, kb0 + 4 * h, KB);
+      if (next < nt) {
+        place(next);
+        fetch(0, smem + (cur ^ 1) * kBytes);
+      }
     }
     const char* buf = smem + cur * kBytes;
 #pragma unroll
@@ -259,72 +277,80 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
   }
 
   // Element e of a 32 x 32 result is its row 8 (e / 4) + 4 h + e % 4, column j.
-  const int64_t c0 = rb + wb + D * j;  // this lane's first pixel (MAP) or channel
-  if (c0 >= nb) return;
-  MxGroup grp;
-  MxPixels<TB> pix;
+  const int64_t c0 = rb0 + wb + D * j, a0 = ra0 + wa + 4 * h, step = MAP ? o.HW : o.N;  // this lane's first column and row
+  MxPixels<TB> at;
   bool whole = c0 + TB <= nb;
   if (MAP) {
-    grp = mx_group<TB>(c0, o.HW, o.rows);
-    pix = mx_pixels<TB>(o, grp, 0);
+    const MxGroup grp = mx_group<TB>(min(c0, nb - 1), o.HW, o.rows);
+    at = mx_pixels<TB>(o, grp, a0);
     whole = grp.whole;
+  } else {
+    at.live = 0;
+#pragma unroll
+    for (int k = 0; k < TB; ++k) at.at[k] = a0 * o.N + c0 + k, at.live |= (c0 + k < nb) << k;
   }
+  if (c0 < nb) {
 #pragma unroll
-  for (int i = 0; i < TA; ++i)
+    for (int i = 0; i < TA; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = wa + 32 * i + 8 * q + 4 * h;
-      float v[4][TB], bb[4][TB], ss[4][TB];
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int k = 0; k < TB; ++k) {
-          v[r][k] = acc[i][k][4 * q + r];
-          bb[r][k] = MAP ? bias[at + r] : bias[wb + D * j + k];
-          ss[r][k] = MAP ? rscale[at + r] : rscale[wb + D * j + k];
-        }
-      const int64_t a = ra + at;
-      if (whole && a + 4 <= na) {
-        mx_store_rows<T, TB, 4>(o, MAP ? pix.at[0] + a * o.HW : a * o.N + c0, MAP ? o.HW : o.N, v, bb, ss);
-        continue;
-      }
-      if (MAP) {
+      for (int q = 0; q < 4; ++q) {
+        const int off = 32 * i + 8 * q;
+        float v[4][TB], ss[4][TB];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (a + r < na) mx_store_pixels<T, TB>(o, pix, (a + r) * o.HW, v[r], bb[r][0], ss[r][0]);
-        continue;
+#pragma unroll
+          for (int k = 0; k < TB; ++k) {
+            const int n = MAP ? wa + off + 4 * h + r : wb + D * j + k;
+            v[r][k] = acc[i][k][4 * q + r] + bias[n], ss[r][k] = rscale[n];
+          }
+        mx_finish<TB, 4>(o, v, ss);
+        const int64_t left = na - a0 - off;
+        if (whole && left >= 4) {
+          mx_store_rows<T, NT, TB, 4>(o, at.at[0] + off * step, step, v);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < left) mx_store_pixels<T, TB>(o, at, (off + r) * step, v[r]);
+        }
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int k = 0; k < TB; ++k)
-          if (a + r < na && c0 + k < nb)
-            mx_store_rows<T, 1, 1>(o, (a + r) * o.N + c0 + k, 0, (const float(*)[1]) & v[r][k], (const float(*)[1]) & bb[r][k],
-                                   (const float(*)[1]) & ss[r][k]);
-    }
+  }
+  if (next >= nt) return;
+  t = next;
+  bias = bias == (float*)(smem + 2 * kBytes) ? bias + 2 * NC : bias - 2 * NC;
+  }
 }
 
-template <class T, bool MAP, int BA, int BB, int WA, int WB>
+template <class T, bool MAP, bool NT, int BA, int BB, int WA, int WB>
 int gemm_tile(const MxIn& in, const MxOut& o, hipStream_t st) {
-  constexpr int kThreads = (BA / WA) * (BB / WB) * 64, kLds = 2 * (BA + BB) * 128 + 8 * (MAP ? BA : BB);
+  constexpr int kThreads = (BA / WA) * (BB / WB) * 64, kLds = 2 * (BA + BB) * 128 + 16 * (MAP ? BA : BB);
   const int64_t na = MAP ? o.N : o.rows, nb = MAP ? o.rows : o.N;
   const int64_t ta = (na + BA - 1) / BA, tb = (nb + BB - 1) / BB;
-  if (ta * tb * kThreads >= (int64_t)1 << 32) return fail(CVN_ERR_UNSUPPORTED, "too many pixels and channels");
-  auto k = k_mx_gemm<T, MAP, BA, BB, WA, WB>;
+  if (ta * tb >= (int64_t)1 << 30) return fail(CVN_ERR_UNSUPPORTED, "too many pixels and channels");
+  auto k = k_mx_gemm<T, MAP, NT, BA, BB, WA, WB>;
   static std::atomic<uint64_t> done;
   once_per_device(done, [&] { (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds); });
-  hipLaunchKernelGGL(k, dim3((unsigned)(ta * tb)), dim3(kThreads), kLds, st, MAP ? in.wc : in.xc, MAP ? in.ws : in.xs, na,
+  // as many blocks as the CUs hold at once; each takes tiles in turn
+  static std::atomic<int> most[64];
+  std::atomic<int>& m = most[current_device() & 63];
+  if (!m.load(std::memory_order_relaxed)) {
+    int per = 0, cus = 0;
+    (void)hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, (const void*)k, kThreads, kLds);
+    (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, current_device());
+    m.store(std::max(8, std::max(1, per) * cus / 8 * 8), std::memory_order_relaxed);
+  }
+  const int64_t blocks = std::min<int64_t>(ta * tb, m.load(std::memory_order_relaxed));
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kThreads), kLds, st, MAP ? in.wc : in.xc, MAP ? in.ws : in.xs, na,
                      MAP ? in.xc : in.wc, MAP ? in.xs : in.ws, nb, in.KB, (int)ta, (int)tb, o);
   return check_launch("conv1x1_mxfp4");
 }
 
 template <class T, bool MAP>
 int gemm(const MxIn& in, const MxOut& o, hipStream_t st) {
-  const int64_t na = MAP ? o.N : o.rows, nb = MAP ? o.rows : o.N;
-  auto tiles = [&](int64_t a, int64_t b) { return (na + a - 1) / a * ((nb + b - 1) / b); };
-  if (tiles(256, 256) >= 256) return gemm_tile<T, MAP, 256, 256, 64, 128>(in, o, st);
-  if (tiles(64, 128) >= 256 || nb > 64) return gemm_tile<T, MAP, 64, 128, 32, 64>(in, o, st);
-  return gemm_tile<T, MAP, 64, 64, 32, 32>(in, o, st);
+  // Tiles of 128 from one for every CU on, 64 below.  (16384 pixels, 2048 to 4096 channels: 131 us, 64: 208, 256 x 256 with
+  // eight waves 133; 8192 pixels, 1024 to 1024: 14.7, 64: 19, 256 x 256: 16.5; 256 pixels, 2048 to 2048: 14.7, 64: 12.5.)
+  if ((o.N + 127) / 128 * ((o.rows + 127) / 128) >= 256)
+    return o.lines ? gemm_tile<T, MAP, true, 128, 128, 64, 64>(in, o, st) : gemm_tile<T, MAP, false, 128, 128, 64, 64>(in, o, st);
+  return gemm_tile<T, MAP, false, 64, 64, 32, 32>(in, o, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -399,22 +425,24 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
 #pragma unroll
     for (int i = 0; i < kFewWaves; ++i) v += part[i][n][r];
     const int64_t rb = (uint32_t)r / (uint32_t)o.HW;
-    const float bias = o.bias ? o.bias[n0 + n] : 0.f, scale = o.res_scale ? o.res_scale[n0 + n] : 1.f;
-    mx_store_rows<T, 1, 1>(o, (rb * o.N + n0 + n) * o.HW + (r - rb * o.HW), 0, (const float(*)[1])&v, (const float(*)[1])&bias,
-                           (const float(*)[1])&scale);
+    float out[1][1] = {{o.bias ? v + o.bias[n0 + n] : v}};
+    const float scale[1][1] = {{o.res_scale ? o.res_scale[n0 + n] : 1.f}};
+    mx_finish<1, 1>(o, out, scale);
+    mx_store_rows<T, false, 1, 1>(o, (rb * o.N + n0 + n) * o.HW + (r - rb * o.HW), 0, out);
   }
 }
 
 // ------------------------------------------------------------------------------------------------
 // Maps of up to 256 channels: quantised in registers, every product and the store in one pass.
 // ------------------------------------------------------------------------------------------------
-// Bound by memory.  Lane l of a wave loads the blocks 2 s + l / 32 of four neighbouring pixels (16 bytes of a float32
-// channel, 512 in a row over 32 lanes), makes their codes, and keeps them as operands for every 32 channels of the result:
-// four products of pixels 4 j + v give it four neighbouring pixels of a channel again.  blockIdx.y takes a share of the
-// channels where there are too few pixels for the CUs.
-template <class T, int S>
+// Bound by memory.  Lane l of a wave loads the blocks 2 s + l / 32 of two neighbouring pixels (8 bytes of a float32 channel,
+// 256 in a row over 32 lanes), makes their codes, and keeps them as operands for every 32 channels of the result: the
+// products of pixels 2 j and 2 j + 1 give it two neighbouring pixels of a channel again.  (Four pixels a lane: 128 x 256 x 256
+// x 8 float32 to 64 90 us, two 77, half the registers.)  blockIdx.y takes a share of the channels where there are too few
+// pixels for the CUs.
+template <class T, bool NT, int S>
 __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share) {
-  constexpr int V = 4;
+  constexpr int V = 2;
   typedef typename MxVec<T, V>::type W;
   const int lane = threadIdx.x & 63, j = lane & 31, h = lane >> 5;
   const int64_t w0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (32 * V), r0 = w0 + V * j;
@@ -485,18 +513,24 @@ __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share)
   const int64_t n1 = min(o.N, (int64_t)(blockIdx.y + 1) * share);
   for (int64_t n0 = (int64_t)blockIdx.y * share; n0 < n1; n0 += 32) {
     const int64_t wrow = min(n0 + j, o.N - 1) * in.KB;
-    mx_f32x16 acc[V];
+    // the sums begin with the bias of their rows: element e of a result is its row 8 (e / 4) + 4 h + e % 4
+    mx_f32x16 acc[V], ss;
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = mx_f32x16{};
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t n = min((uint32_t)n0 + 8 * (e / 4) + 4 * h + e % 4, (uint32_t)o.N - 1);
+      acc[0][e] = o.bias ? o.bias[n] : 0.f;
+      ss[e] = o.res_scale ? o.res_scale[n] : 1.f;
+    }
+#pragma unroll
+    for (int e = 1; e < V; ++e) acc[e] = acc[0];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const int kb = 2 * s + h, at = min(kb, in.KB - 1);
       const mx_i32x8 w = mx_operand(in.wc[wrow + at]);
       const int sw = kb < in.KB ? in.ws[wrow + at] : 0;
+      // (the byte of the scales is part of the instruction)
       acc[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][0]), acc[0], kMxFp4, kMxFp4, 0, sw, 0, (int)sx[s]);
       acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][1]), acc[1], kMxFp4, kMxFp4, 0, sw, 1, (int)sx[s]);
-      acc[2] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][2]), acc[2], kMxFp4, kMxFp4, 0, sw, 2, (int)sx[s]);
-      acc[3] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][3]), acc[3], kMxFp4, kMxFp4, 0, sw, 3, (int)sx[s]);
     }
     if (r0 >= o.rows) continue;
     MxPixels<V> px = pix;
@@ -506,41 +540,44 @@ __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t n = n0 + 8 * i + 4 * h;
-      float v[4][V], bb[4][V], ss[4][V];
+      float v[4][V], sc[4][V];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t nr = min(n + r, o.N - 1);
-        const float bias = o.bias ? o.bias[nr] : 0.f, scale = o.res_scale ? o.res_scale[nr] : 1.f;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[r][e] = acc[e][4 * i + r], bb[r][e] = bias, ss[r][e] = scale;
-      }
+        for (int e = 0; e < V; ++e) v[r][e] = acc[e][4 * i + r], sc[r][e] = ss[4 * i + r];
+      mx_finish<V, 4>(o, v, sc);
       const int64_t step = (n0 + 8 * i) * o.HW;
       if (grp.whole && n + 4 <= o.N) {
-        mx_store_rows<T, V, 4>(o, px.at[0] + step, o.HW, v, bb, ss);
+        mx_store_rows<T, NT, V, 4>(o, px.at[0] + step, o.HW, v);
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (n + r < o.N) mx_store_pixels<T, V>(o, px, step + r * o.HW, v[r], bb[r][0], ss[r][0]);
+          if (n + r < o.N) mx_store_pixels<T, V>(o, px, step + r * o.HW, v[r]);
       }
     }
   }
 }
 
-template <class T>
-int conv(const MxIn& in, const MxOut& o, bool keep, hipStream_t st) {
-  const int64_t tiles = (o.rows + 511) / 512, n32 = (o.N + 31) / 32;
-  // as many shares of the channels as give every CU two blocks
-  const int64_t shares = std::min(n32, std::max<int64_t>(1, 512 / tiles)), share = (n32 + shares - 1) / shares * 32;
+template <class T, bool NT>
+int conv_to(const MxIn& a, const MxOut& o, hipStream_t st) {
+  const int64_t tiles = (o.rows + 255) / 256, n32 = (o.N + 31) / 32;
+  // as many shares of the channels as give every CU four blocks (160 x 177 x 131 x 4 float32 to 352: 55 us, eight 67)
+  const int64_t shares = std::min(n32, std::max<int64_t>(1, 1024 / tiles)), share = (n32 + shares - 1) / shares * 32;
   const dim3 grid((unsigned)tiles, (unsigned)((o.N + share - 1) / share));
-  MxIn a = in;
-  if (!keep) a.xc = nullptr;
-  switch ((in.KB + 1) / 2) {
-    case 1: hipLaunchKernelGGL((k_mx_conv<T, 1>), grid, dim3(256), 0, st, a, o, (int)share); break;
-    case 2: hipLaunchKernelGGL((k_mx_conv<T, 2>), grid, dim3(256), 0, st, a, o, (int)share); break;
-    case 3: hipLaunchKernelGGL((k_mx_conv<T, 3>), grid, dim3(256), 0, st, a, o, (int)share); break;
-    default: hipLaunchKernelGGL((k_mx_conv<T, 4>), grid, dim3(256), 0, st, a, o, (int)share); break;
+  switch ((a.KB + 1) / 2) {
+    case 1: hipLaunchKernelGGL((k_mx_conv<T, NT, 1>), grid, dim3(256), 0, st, a, o, (int)share); break;
+    case 2: hipLaunchKernelGGL((k_mx_conv<T, NT, 2>), grid, dim3(256), 0, st, a, o, (int)share); break;
+    case 3: hipLaunchKernelGGL((k_mx_conv<T, NT, 3>), grid, dim3(256), 0, st, a, o, (int)share); break;
+    default: hipLaunchKernelGGL((k_mx_conv<T, NT, 4>), grid, dim3(256), 0, st, a, o, (int)share); break;
   }
   return check_launch("conv1x1_mxfp4");
+}
+
+template <class T>
+int conv(const MxIn& in, const MxOut& o, bool keep, hipStream_t st) {
+  MxIn a = in;
+  if (!keep) a.xc = nullptr;
+  return o.lines ? conv_to<T, true>(a, o, st) : conv_to<T, false>(a, o, st);
 }
 
 int mx_check_product(int64_t B, int64_t C, int64_t HW, int64_t N, int type) {
@@ -604,7 +641,8 @@ extern "C" int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, i
   }
   const hipStream_t st = (hipStream_t)stream;
   const MxIn in = {x, (mx_i32x4*)x_codes, (uint8_t*)x_scales, (const mx_i32x4*)w_codes, (const uint8_t*)w_scales, C, (int)KB};
-  const MxOut o = {bias, res_scale, residual, y, HW, N, rows, act};
+  const bool lines = (((HW > 1 ? HW : N) * es) | (int64_t)(uintptr_t)y) % 128 == 0;
+  const MxOut o = {bias, res_scale, residual, y, HW, N, rows, act, lines};
   if (type == CVN_F32) return product<float>(in, o, type, keep, st);
   if (type == CVN_BF16) return product<__bf16>(in, o, type, keep, st);
   return product<_Float16>(in, o, type, keep, st);
