@@ -95,9 +95,9 @@ SIGNATURES = {
     "cvn_clip_grads": (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _int, _f64, _ptr, _ptr, _size, _ptr]),
     "cvn_mxfp4_quantize": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr]),
     "cvn_mxfp4_dequantize": (_int, [_ptr, _ptr, _i64, _i64, _i64, _ptr, _int, _ptr]),
-    "cvn_conv1x1_mxfp4_workspace": (_size, [_int, _i64, _i64, _i64, _i64]),
-    "cvn_conv1x1_mxfp4": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr, _int, _ptr, _ptr, _ptr, _int,
-                                 _ptr, _size, _ptr]),
+    "cvn_conv1x1_mxfp4_workspace": (_size, [_int, _int, _i64, _i64, _i64, _i64]),
+    "cvn_conv1x1_mxfp4": (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr, _int, _ptr, _ptr, _i64, _ptr, _int, _ptr, _ptr, _ptr,
+                                 _int, _ptr, _size, _ptr]),
     "cvn_conv1x1_mxfp4_bwd_workspace": (_size, [_i64, _i64, _i64, _i64]),
     "cvn_conv1x1_mxfp4_bwd": (_int, [_ptr, _int, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr,
                                      _size, _ptr]),

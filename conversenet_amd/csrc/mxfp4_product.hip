@@ -611,35 +611,63 @@ int product(const MxIn& in, const MxOut& o, int type, bool keep, hipStream_t st)
 
 using namespace cvn;
 
-extern "C" size_t cvn_conv1x1_mxfp4_workspace(int quantized, int64_t B, int64_t C, int64_t HW, int64_t N) {
-  if (mx_check_product(B, C, HW, N, CVN_F32) != CVN_OK || quantized) return 0;
-  return align_up((size_t)(B * HW * mx_blocks(C)) * 17, 16);
+extern "C" size_t cvn_conv1x1_mxfp4_workspace(int x_given, int w_given, int64_t B, int64_t C, int64_t HW, int64_t N) {
+  if (mx_check_product(B, C, HW, N, CVN_F32) != CVN_OK) return 0;
+  return (x_given ? 0 : align_up((size_t)(B * HW * mx_blocks(C)) * 17)) + (w_given ? 0 : align_up((size_t)(N * mx_blocks(C)) * 17));
 }
 
-extern "C" int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, int64_t C, int64_t HW,
-                                 const void* w_codes, const void* w_scales, int64_t N, const float* bias, int act,
+extern "C" int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, int64_t C, int64_t HW, const void* w,
+                                 int w_type, void* w_codes, void* w_scales, int64_t N, const float* bias, int act,
                                  const void* residual, const float* res_scale, void* y, int type, void* workspace,
                                  size_t workspace_bytes, cvn_stream_t stream) {
   const int rc = mx_check_product(B, C, HW, N, type);
   if (rc != CVN_OK) return rc;
   if (act != CVN_ACT_NONE && act != CVN_ACT_GELU) return fail(CVN_ERR_ARG, "unknown activation");
+  if (w && !mx_type_size(w_type)) return fail(CVN_ERR_ARG, "bad type of the matrix");
   const int64_t rows = B * HW, KB = mx_blocks(C), es = mx_type_size(type);
-  if (rows == 0) return CVN_OK;
-  if (!w_codes || !w_scales || !y || (!x && !x_codes) || !x_codes != !x_scales) return fail(CVN_ERR_ARG, "null pointer");
+  if (!x_codes != !x_scales || !w_codes != !w_scales || (!w && !w_codes) || (rows && (!y || (!x && !x_codes))))
+    return fail(CVN_ERR_ARG, "null pointer");
   if (((uintptr_t)w_codes | (uintptr_t)x_codes) & 15) return fail(CVN_ERR_ARG, "codes must be aligned to 16 bytes");
-  const int64_t ny = rows * N * es;
-  if (mx_overlap(y, ny, x, rows * C * es) || mx_overlap(y, ny, w_codes, N * KB * 16) || mx_overlap(y, ny, w_scales, N * KB) ||
-      mx_overlap(y, ny, x_codes, rows * KB * 16) || mx_overlap(y, ny, x_scales, rows * KB) ||
-      (y != residual && mx_overlap(y, ny, residual, ny)))
-    return fail(CVN_ERR_ARG, "the output shares memory with an input");
+  // What is written is apart from all else, but y may be the residual.
+  const struct {
+    const void* p;
+    int64_t n;
+  } mem[] = {{y, rows * N * es},
+             {x ? x_codes : nullptr, rows * KB * 16},
+             {x ? x_scales : nullptr, rows * KB},
+             {w ? w_codes : nullptr, N * KB * 16},
+             {w ? w_scales : nullptr, N * KB},  // written up to here
+             {x, rows * C * es},
+             {w, w ? N * C * mx_type_size(w_type) : 0},
+             {x ? nullptr : x_codes, rows * KB * 16},
+             {x ? nullptr : x_scales, rows * KB},
+             {w ? nullptr : w_codes, N * KB * 16},
+             {w ? nullptr : w_scales, N * KB},
+             {residual == y ? nullptr : residual, rows * N * es}};
+  for (int i = 0; i < 5; ++i)
+    for (int k = i + 1; k < 12; ++k)
+      if (mx_overlap(mem[i].p, mem[i].n, mem[k].p, mem[k].n))
+        return fail(CVN_ERR_ARG, "an output shares memory with an input or another output");
   const bool keep = x_codes != nullptr;
-  if (x && !keep) {
-    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < cvn_conv1x1_mxfp4_workspace(0, B, C, HW, N))
-      return fail(CVN_ERR_WORKSPACE, "workspace missing, too small or not aligned to 16 bytes");
-    x_codes = workspace;
-    x_scales = (char*)workspace + rows * KB * 16;
-  }
+  const size_t need = cvn_conv1x1_mxfp4_workspace(keep, w_codes != nullptr, B, C, HW, N);
+  if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+    return fail(CVN_ERR_WORKSPACE, "workspace missing, too small or not aligned to 16 bytes");
+  char* work = (char*)workspace;
   const hipStream_t st = (hipStream_t)stream;
+  if (!w_codes) {
+    w_codes = work;
+    w_scales = work + N * KB * 16;
+    work += align_up((size_t)(N * KB) * 17);
+  }
+  if (w) {
+    const int q = mx_quantize(w, w_type, N, C, 1, w_codes, w_scales, st);
+    if (q != CVN_OK) return q;
+  }
+  if (rows == 0) return CVN_OK;
+  if (!keep) {
+    x_codes = work;
+    x_scales = work + rows * KB * 16;
+  }
   const MxIn in = {x, (mx_i32x4*)x_codes, (uint8_t*)x_scales, (const mx_i32x4*)w_codes, (const uint8_t*)w_scales, C, (int)KB};
   const bool lines = (((HW > 1 ? HW : N) * es) | (int64_t)(uintptr_t)y) % 128 == 0;
   const MxOut o = {bias, res_scale, residual, y, HW, N, rows, act, lines};

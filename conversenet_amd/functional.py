@@ -1212,57 +1212,13 @@ def dequantize_mxfp4(q, dtype=torch.float32):
     return y
 
 
-def _conv1x1_mxfp4(x, weight, bias, act, residual, res_scale, out, dtype, keep_x):
-    """The launches behind conv1x1_mxfp4: (y, x's MXFP4 form where keep_x)."""
-    _untraced("conv1x1_mxfp4")
-    lib = _lib.load()
-    if act not in (None, "gelu"):
-        raise RuntimeError(f"unknown activation {act!r}")
-    xc = xs = None
-    given = isinstance(x, MXFP4)
-    if given:
-        (B, C, HW), xc, xs = _mx_parts(x, "x")
-        dev, space = xc.device, tuple(xc.shape[1:-1])
-        dtype = dtype or (torch.float32 if residual is None else residual.dtype)
-        if dtype not in _lib.TYPES:
-            raise RuntimeError("conv1x1_mxfp4 gives float32, bfloat16 or float16")
-    else:
-        B, C, HW = _mx_map(x, "conv1x1_mxfp4")
-        if dtype not in (None, x.dtype):
-            raise RuntimeError("the result has the type of x")
-        x = _contiguous(x)
-        dev, space, dtype = x.device, tuple(x.shape[2:]), x.dtype
-    index = dev.index
-    if not isinstance(weight, MXFP4):
-        if weight.get_device() != index or weight.dim() < 2 or math.prod(weight.shape[2:]) != 1:
-            raise RuntimeError("weight must be a matrix (N,C) or (N,C,1,1) on the device of x")
-        weight = quantize_mxfp4(weight)
-    (N, wC, one), wc, ws = _mx_parts(weight, "weight")
-    if wC != C or one != 1 or N < 1 or wc.get_device() != index:
+def _mx_weight(weight, C, index):
+    """(N, C) of a float matrix to be quantised."""
+    if weight.get_device() != index or weight.dim() < 2 or math.prod(weight.shape[2:]) != 1 or weight.dtype not in _lib.TYPES:
+        raise RuntimeError("weight must be a matrix (N,C) or (N,C,1,1) on the device of x: float32, bfloat16 or float16")
+    if weight.shape[1] != C or weight.shape[0] < 1:
         raise RuntimeError("weight does not match input channels")
-    shape = (B, N, *space)
-    for t, what in ((residual, "residual"), (out, "out")):
-        if t is not None and (tuple(t.shape) != shape or t.dtype is not dtype or t.get_device() != index):
-            raise RuntimeError(f"{what} must have the result's shape and type")
-    if out is not None and not out.is_contiguous():
-        raise RuntimeError("out must be contiguous")
-    keep = []
-    b, s = _param32(keep, bias, N, index, "bias"), _param32(keep, res_scale, N, index, "res_scale")
-    residual = _contiguous(residual)
-    y = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
-    if keep_x:
-        xc, xs = _mx_empty(x, C)
-    nbytes = lib.cvn_conv1x1_mxfp4_workspace(int(xc is not None), B, C, HW, N)
-    st = _stream(dev)
-    wsp = _scratch(dev, st)
-    with _on(dev), wsp.lock:
-        rc = lib.cvn_conv1x1_mxfp4(None if given else x.data_ptr(), _ptr(xc), _ptr(xs), B, C, HW, wc.data_ptr(),
-                                   ws.data_ptr(), N, b, _lib.ACT_GELU if act else _lib.ACT_NONE, _ptr(residual), s,
-                                   y.data_ptr(), _lib.TYPES[dtype], wsp.ptr(nbytes), nbytes, st)
-    _lib.check(rc, "conv1x1_mxfp4")
-    if out is not None:
-        _written([out])
-    return y, xc, xs, wc, ws
+    return weight.shape[0]
 
 
 def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None, out=None, dtype=None):
@@ -1273,7 +1229,54 @@ def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None,
     float (N,C) or (N,C,1,1), quantised in the call.  The result has x's type (of an MXFP4 x the residual's, or dtype).
     residual and out have the result's shape and type, and may be one tensor.  Forward only; for gradients see
     conv1x1_mxfp4_train."""
-    return _conv1x1_mxfp4(x, weight, bias, act, residual, res_scale, out, dtype, False)[0]
+    _untraced("conv1x1_mxfp4")
+    lib = _lib.load()
+    if act not in (None, "gelu"):
+        raise RuntimeError(f"unknown activation {act!r}")
+    xc = xs = wc = ws = None
+    if isinstance(x, MXFP4):
+        (B, C, HW), xc, xs = _mx_parts(x, "x")
+        x, dev, space = None, xc.device, xc.shape[1:-1]
+        dtype = dtype or (torch.float32 if residual is None else residual.dtype)
+        if dtype not in _lib.TYPES:
+            raise RuntimeError("conv1x1_mxfp4 gives float32, bfloat16 or float16")
+    else:
+        B, C, HW = _mx_map(x, "conv1x1_mxfp4")
+        if dtype not in (None, x.dtype):
+            raise RuntimeError("the result has the type of x")
+        x = _contiguous(x)
+        dev, space, dtype = x.device, x.shape[2:], x.dtype
+    index = dev.index
+    if isinstance(weight, MXFP4):
+        (N, wC, one), wc, ws = _mx_parts(weight, "weight")
+        weight = None
+        if wC != C or one != 1 or N < 1 or wc.get_device() != index:
+            raise RuntimeError("weight does not match input channels")
+    else:
+        N = _mx_weight(weight, C, index)
+        weight = _contiguous(weight)
+    shape = (B, N, *space)
+    for t, what in ((residual, "residual"), (out, "out")):
+        if t is not None and (tuple(t.shape) != shape or t.dtype is not dtype or t.get_device() != index):
+            raise RuntimeError(f"{what} must have the result's shape and type")
+    if out is not None and not out.is_contiguous():
+        raise RuntimeError("out must be contiguous")
+    keep = []
+    b, s = _param32(keep, bias, N, index, "bias"), _param32(keep, res_scale, N, index, "res_scale")
+    residual = _contiguous(residual)
+    y = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
+    nbytes = lib.cvn_conv1x1_mxfp4_workspace(x is None, weight is None, B, C, HW, N)
+    st = _stream(dev)
+    work = _scratch(dev, st)
+    with _on(dev), work.lock:
+        rc = lib.cvn_conv1x1_mxfp4(_ptr(x), _ptr(xc), _ptr(xs), B, C, HW, _ptr(weight),
+                                   0 if weight is None else _lib.TYPES[weight.dtype], _ptr(wc), _ptr(ws), N, b,
+                                   _lib.ACT_GELU if act else _lib.ACT_NONE, _ptr(residual), s, y.data_ptr(),
+                                   _lib.TYPES[dtype], work.ptr(nbytes), nbytes, st)
+    _lib.check(rc, "conv1x1_mxfp4")
+    if out is not None:
+        _written([out])
+    return y
 
 
 def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
@@ -1282,7 +1285,6 @@ def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
     weight's (N,C).  x, weight: the MXFP4 operands of the forward (x None without weight's gradient, weight None without x's, where
     the other gives the channels)."""
     _untraced("conv1x1_mxfp4_backward")
-    lib = _lib.load()
     B, N, HW = _mx_map(grad_y, "conv1x1_mxfp4_backward")
     nx, nw, nb = need
     if (nx and weight is None) or (nw and x is None):
@@ -1303,39 +1305,99 @@ def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
     gx = torch.empty((B, C, *gy.shape[2:]), dtype=gy.dtype, device=dev) if nx else None
     gw = torch.empty((N, C), dtype=torch.float32, device=dev) if nw else None
     gb = torch.empty((N,), dtype=torch.float32, device=dev) if nb else None
-    nbytes = lib.cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N)
-    st = _stream(dev)
-    wsp = _scratch(dev, st)
-    with _on(dev), wsp.lock:
-        rc = lib.cvn_conv1x1_mxfp4_bwd(gy.data_ptr(), _lib.TYPES[gy.dtype], _ptr(xc), _ptr(xs), _ptr(wc), _ptr(ws), B, C, HW,
-                                       N, _ptr(gx), _ptr(gw), _ptr(gb), wsp.ptr(nbytes), nbytes, st)
-    _lib.check(rc, "conv1x1_mxfp4_backward")
+    _mx_grads(gy, _ptr(xc), _ptr(xs), _ptr(wc), _ptr(ws), B, C, HW, N, gx, gw, gb)
     return gx, gw, gb
 
 
+def _mx_grads(gy, xc, xs, wc, ws, B, C, HW, N, gx, gw, gb):
+    """The launches behind conv1x1_mxfp4's gradients."""
+    lib = _lib.load()
+    dev = gy.device
+    nbytes = lib.cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N) if gw is not None else 0
+    st = _stream(dev)
+    work = _scratch(dev, st)
+    with _on(dev), work.lock:
+        rc = lib.cvn_conv1x1_mxfp4_bwd(gy.data_ptr(), _lib.TYPES[gy.dtype], xc, xs, wc, ws, B, C, HW, N, _ptr(gx), _ptr(gw),
+                                       _ptr(gb), work.ptr(nbytes), nbytes, st)
+    _lib.check(rc, "conv1x1_mxfp4_backward")
+
+
+def _mx_layout(rows, C, N, keep_x, keep_w):
+    """Where a forward keeps its operands in one buffer: (codes and scales of x, of the matrix, bytes), None for what is
+    not kept."""
+    blocks = (C + 31) // 32
+    at, out = 0, []
+    for n, wanted in ((16 * rows, keep_x), (16 * N, keep_w), (rows, keep_x), (N, keep_w)):
+        out.append(at if wanted else None)
+        at += (n * blocks + 255) // 256 * 256 if wanted else 0
+    return out[0], out[2], out[1], out[3], at
+
+
 class Conv1x1MXFP4Function(torch.autograd.Function):
-    """conv1x1_mxfp4 of a float map and matrix, with gradients straight through both quantisations.  Keeps the operands in
-    MXFP4, 17/128 of a float32 map's bytes."""
+    """conv1x1_mxfp4 of a float map and matrix, with gradients straight through both quantisations.  Keeps the operands that
+    the gradients need in MXFP4, 17/128 of float32's bytes, in one buffer."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
+        if _dispatch_modes() or _function_modes() or _tracing_state() is not None:
+            _untraced("conv1x1_mxfp4_train")
+        lib = _lib.load()
+        B, C, HW = _mx_map(x, "conv1x1_mxfp4_train")
+        dev, dtype = x.device, x.dtype
+        index = dev.index
+        N = _mx_weight(weight, C, index)
+        x, w = _contiguous(x), _contiguous(weight)
+        keep = []
+        b = _param32(keep, bias, N, index, "bias")
         nx, nw = ctx.needs_input_grad[:2]
-        y, xc, xs, wc, ws = _conv1x1_mxfp4(x, weight, bias, None, None, None, None, None, nw)
-        ctx.save_for_backward(*((xc, xs) if nw else (None, None)), *((wc, ws) if nx else (None, None)))
-        ctx.cfg = (x.shape[1], weight.shape, weight.dtype, None if bias is None else (bias.shape, bias.dtype))
+        where = _mx_layout(B * HW, C, N, nw, nx)
+        kept = torch.empty(where[4], dtype=torch.uint8, device=dev) if nx or nw else None
+        base = 0 if kept is None else kept.data_ptr()
+        xc, xs, wc, ws = (None if o is None or not base else base + o for o in where[:4])
+        y = torch.empty((B, N, *x.shape[2:]), dtype=dtype, device=dev)
+        nbytes = lib.cvn_conv1x1_mxfp4_workspace(xc is not None, wc is not None, B, C, HW, N)
+        st = _stream(dev)
+        work = _scratch(dev, st)
+        with _on(dev), work.lock:
+            rc = lib.cvn_conv1x1_mxfp4(x.data_ptr(), xc, xs, B, C, HW, w.data_ptr(), _lib.TYPES[w.dtype], wc, ws, N, b, 0, None,
+                                       None, y.data_ptr(), _lib.TYPES[dtype], work.ptr(nbytes), nbytes, st)
+        _lib.check(rc, "conv1x1_mxfp4_train")
+        ctx.save_for_backward(kept)
+        ctx.cfg = (where, x.shape, weight.shape, weight.dtype, None if bias is None else (bias.shape, bias.dtype))
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        xc, xs, wc, ws = ctx.saved_tensors
-        C, w_shape, w_dtype, b = ctx.cfg
-        if not _in_memory(gy):
-            raise RuntimeError("conv1x1_mxfp4's gradients are of plain tensors")
-        gx, gw, gb = conv1x1_mxfp4_backward(gy, None if xc is None else MXFP4(xc, xs, C),
-                                            None if wc is None else MXFP4(wc, ws, C), ctx.needs_input_grad[:3])
-        return (gx, None if gw is None else gw.view(w_shape).to(w_dtype),
-                None if gb is None else gb.view(b[0]).to(b[1]))
+        # (a backward that is itself to be differentiated gives gradients that refuse it)
+        return _mx_backward_once(ctx, gy) if torch.is_grad_enabled() else _mx_backward(ctx, gy)
+
+
+def _mx_backward(ctx, gy):
+    kept, = ctx.saved_tensors
+    where, x_shape, w_shape, w_dtype, bias = ctx.cfg
+    nx, nw, nb = ctx.needs_input_grad
+    if not _in_memory(gy) or not _in_memory(kept):
+        raise RuntimeError("conv1x1_mxfp4's gradients are of plain tensors")
+    gy, kept = _contiguous(gy), _contiguous(kept)
+    dev = gy.device
+    B, C, N, HW = x_shape[0], x_shape[1], w_shape[0], math.prod(x_shape[2:])
+    base = 0 if kept is None else kept.data_ptr()
+    if base % 16:  # (a saved-tensor hook may have moved it)
+        kept = kept.clone()
+        base = kept.data_ptr()
+    xc, xs, wc, ws = (None if o is None or not base else base + o for o in where[:4])
+    gx = torch.empty(x_shape, dtype=gy.dtype, device=dev) if nx else None
+    gw = torch.empty(w_shape, dtype=torch.float32, device=dev) if nw else None
+    gb = torch.empty(bias[0], dtype=torch.float32, device=dev) if nb else None
+    _mx_grads(gy, xc, xs, wc, ws, B, C, HW, N, gx, gw, gb)
+    if nw and w_dtype is not torch.float32:
+        gw = gw.to(w_dtype)
+    if nb and bias[1] is not torch.float32:
+        gb = gb.to(bias[1])
+    return gx, gw, gb
+
+
+_mx_backward_once = torch.autograd.function.once_differentiable(_mx_backward)
 
 
 def conv1x1_mxfp4_train(x, weight, bias=None):

@@ -319,14 +319,14 @@ int cvn_mxfp4_quantize(const void* x, int x_type, int64_t B, int64_t C, int64_t 
 int cvn_mxfp4_dequantize(const void* codes, const void* scales, int64_t B, int64_t C, int64_t HW, void* y, int y_type,
                          cvn_stream_t stream);
 /* y[b,n,p] = act(sum_c w[n][c] x[b,p][c] + bias[n]);  then, with res_scale or residual, y = res_scale[n] * y +
- * residual[b,n,p]: cvn_conv1x1_f32 of MXFP4 operands, summed in fp32 and rounded once.  w: (N,C) in MXFP4.  x: (B,C,HW) of
- * type, quantised in the call, its MXFP4 form written to x_codes and x_scales unless they are NULL; or x NULL and its MXFP4
- * form given there.  y, residual: (B,N,HW) of type; bias, res_scale: fp32 (N).  bias, residual and res_scale may be NULL.
- * y may be the residual itself, and shares no other memory with an input (CVN_ERR_ARG).
- * _workspace: quantized: x_codes will be given (read or written). */
-size_t cvn_conv1x1_mxfp4_workspace(int quantized, int64_t B, int64_t C, int64_t HW, int64_t N);
-int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, int64_t C, int64_t HW, const void* w_codes,
-                      const void* w_scales, int64_t N, const float* bias, int act, const void* residual,
+ * residual[b,n,p]: cvn_conv1x1_f32 of MXFP4 operands, summed in fp32 and rounded once.  x: (B,C,HW) of type, quantised in
+ * the call, its MXFP4 form written to x_codes and x_scales unless they are NULL; or x NULL and its MXFP4 form given there.
+ * w: (N,C) of w_type, likewise.  y, residual: (B,N,HW) of type; bias, res_scale: fp32 (N).  bias, residual and res_scale may be
+ * NULL.  y may be the residual itself; what is written shares no other memory with anything else (CVN_ERR_ARG).
+ * _workspace: x_given, w_given: x_codes, w_codes will be given (read or written). */
+size_t cvn_conv1x1_mxfp4_workspace(int x_given, int w_given, int64_t B, int64_t C, int64_t HW, int64_t N);
+int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, int64_t C, int64_t HW, const void* w,
+                      int w_type, void* w_codes, void* w_scales, int64_t N, const float* bias, int act, const void* residual,
                       const float* res_scale, void* y, int type, void* workspace, size_t workspace_bytes,
                       cvn_stream_t stream);
 /* Gradients of the product and bias, straight through the quantisation: grad_x[b,c,p] = sum_n w[n][c] grad_y[b,n,p] of type,

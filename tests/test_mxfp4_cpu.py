@@ -44,19 +44,22 @@ def test_arguments():
     assert q(None, 0, 0, 32, 4, None, None, None) == d(None, None, 3, 32, 0, None, 0, None) == _lib.CVN_OK
     assert d(None, None, 1, 32, 4, None, 0, None) == A and d(D, D, 1, 32, 4, D, 7, None) == A
 
-    def conv(x=D, xc=None, xs=None, B=1, C=64, HW=4, wc=D << 20, ws=D << 24, N=8, act=0, res=None, y=D << 30, type=0, wsp=D << 10,
-             wsb=1 << 20):
-        return f(x, xc, xs, B, C, HW, wc, ws, N, None, act, res, None, y, type, wsp, wsb, None)
+    def conv(x=D, xc=None, xs=None, B=1, C=64, HW=4, w=None, wt=0, wc=D << 20, ws=D << 24, N=8, act=0, res=None, y=D << 30, type=0,
+             wsp=D << 10, wsb=1 << 20):
+        return f(x, xc, xs, B, C, HW, w, wt, wc, ws, N, None, act, res, None, y, type, wsp, wsb, None)
 
     assert conv(B=0) == _lib.CVN_OK
     for bad in (dict(x=None), dict(wc=None), dict(ws=None), dict(y=None), dict(act=2), dict(type=3), dict(N=0), dict(C=0),
                 dict(xc=D << 12), dict(x=None, xc=D << 12), dict(wc=(D << 20) + 4), dict(y=D), dict(y=D + 1020), dict(y=(D << 20) + 16),
-                dict(res=(D << 30) + 4)):
+                dict(res=(D << 30) + 4), dict(wc=None, ws=None), dict(w=D << 28, wt=3), dict(w=D << 28, wc=D << 28),
+                dict(w=D << 28, wc=D, ws=D << 24), dict(xc=D << 12, xs=D << 12), dict(xc=D << 20, xs=D << 13)):
         assert conv(**bad) == A, bad
     assert conv(N=65537) == conv(C=65537) == conv(B=1 << 16, HW=1 << 16) == U
-    need = lib.cvn_conv1x1_mxfp4_workspace(0, 1, 64, 4, 8)
-    assert need >= 4 * 2 * 17 and lib.cvn_conv1x1_mxfp4_workspace(0, 1, 0, 4, 8) == 0
+    need = lib.cvn_conv1x1_mxfp4_workspace(0, 1, 1, 64, 4, 8)
+    assert need >= 4 * 2 * 17 and lib.cvn_conv1x1_mxfp4_workspace(0, 1, 1, 0, 4, 8) == 0
+    assert lib.cvn_conv1x1_mxfp4_workspace(0, 0, 1, 64, 4, 8) >= need + 8 * 2 * 17
     assert conv(wsb=need - 1) == conv(wsp=None) == conv(wsp=(D << 10) + 8) == W
+    assert conv(w=D << 28, wc=None, ws=None, wsb=need) == W
 
     def bwd(gy=D, xc=D << 20, xs=D << 21, wc=D << 22, ws=D << 23, B=1, C=64, HW=4, N=8, type=0, gx=D << 24, gw=D << 25, gb=None):
         return g(gy, type, xc, xs, wc, ws, B, C, HW, N, gx, gw, gb, D << 26, 1 << 24, None)
