@@ -116,3 +116,36 @@ def residual_branch(h, res_scale=None, gate=None, post=None):
     if gate is not None:
         u = u * (gate if gate.shape == h.shape else gate.reshape(gate.shape[:2] + (1,) * (h.dim() - 2)))
     return u if res_scale is None else res_scale.reshape(cf) * u
+
+
+def mxfp4_values(x):
+    """What the MXFP4 form of a map (B,C,*) or matrix stands for, rounded to x's type: blocks of 32 channels, each a scale
+    2^s, s = max(-127, floor(log2 max|x|) - 2), and the values +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} nearest to x / 2^s, ties to
+    the even one, 6 at most; NaN in a block that holds an infinity or a NaN."""
+    B, C = x.shape[:2]
+    blocks = (C + 31) // 32
+    v = x.double()
+    if 32 * blocks != C:
+        v = torch.cat((v, v.new_zeros((B, 32 * blocks - C) + v.shape[2:])), 1)
+    v = v.reshape((B, blocks, 32) + x.shape[2:])
+    top = v.abs().amax(2, keepdim=True)
+    whole = torch.isfinite(top)
+    m = torch.frexp(torch.where(whole, top, torch.zeros_like(top)))[0]
+    # top / m is the power of two above top; a block of zeros has the smallest scale
+    unit = torch.where(m > 0, torch.clamp(top / m / 8, min=2.0 ** -127), torch.full_like(top, 2.0 ** -127))
+    a = v.abs() / unit
+    step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
+    q = torch.clamp(torch.round(a / step) * step, max=6.0) * unit
+    q = torch.where(whole, torch.copysign(q, v), torch.full_like(v, float("nan")))
+    return q.flatten(1, 2)[:, :C].to(x.dtype)
+
+
+def _straight(x):
+    """mxfp4_values with the gradient of the identity (x - x is zero, or NaN where the values are)."""
+    return mxfp4_values(x.detach()) + (x - x.detach())
+
+
+def conv1x1_mxfp4(x, weight, bias=None):
+    """1x1 convolution of the values that MXFP4 gives x (B,C,H,W) and weight (N,C,1,1), differentiable straight through
+    both roundings."""
+    return F.conv2d(_straight(x), _straight(weight), bias)

@@ -51,6 +51,13 @@ __device__ __forceinline__ unsigned mx_pack8(const float* v, float scale) {
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
   return q;
 }
+// A block's values to its codes, of scale code s (of a block that holds no number they are zeros).
+__device__ __forceinline__ mx_i32x4 mx_pack32(const float* v, unsigned s) {
+  const float scale = mx_scale(s);
+  const mx_i32x4 q = {(int)mx_pack8(v, scale), (int)mx_pack8(v + 8, scale), (int)mx_pack8(v + 16, scale),
+                      (int)mx_pack8(v + 24, scale)};
+  return s == 255u ? mx_i32x4{0, 0, 0, 0} : q;
+}
 // Eight codes to their values.
 __device__ __forceinline__ void mx_unpack8(unsigned q, float scale, float* v) {
   mx_f32x2 t;

@@ -11,11 +11,12 @@ constexpr int kThreads = 256;
 // the whole map, 64 channel blocks of 16384 bfloat16 pixels took 38 us.)
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads) k_mx_quantize(const T* __restrict__ x, int64_t C, int64_t HW, int64_t rows, int KB,
-                                                          uint4* __restrict__ codes, uint8_t* __restrict__ scales) {
+                                                          mx_i32x4* __restrict__ codes, uint8_t* __restrict__ scales) {
   typedef T W __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   const int lane = threadIdx.x & 63;
   const int64_t units = (rows + 64 * V - 1) / (64 * V) * KB, stride = (int64_t)gridDim.x * (kThreads / 64);
-  for (int64_t u = (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += stride) {
+  int64_t u = (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (; u < units; u += stride) {
     const int64_t tile = u / KB, kb = u - tile * KB, r0 = (tile * 64 + lane) * V;
     if (r0 >= rows) continue;
     const int n = (int)min((int64_t)kMxBlock, C - kb * kMxBlock);
@@ -54,11 +55,8 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const T* __restrict__ 
         mag = max(mag, mx_mag(v[c]));
       }
       const unsigned s = mx_scale_code(mag);
-      const float scale = mx_scale(s);
-      uint4 q = {mx_pack8(v, scale), mx_pack8(v + 8, scale), mx_pack8(v + 16, scale), mx_pack8(v + 24, scale)};
-      if (s == 255u) q = uint4{0, 0, 0, 0};
       if (r0 + e < rows) {
-        codes[(r0 + e) * KB + kb] = q;
+        codes[(r0 + e) * KB + kb] = mx_pack32(v, s);
         scales[(r0 + e) * KB + kb] = (uint8_t)s;
       }
     }
@@ -118,8 +116,9 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const uint4* __restr
 
 // Rows: a thread makes eight neighbouring channels.  (Blocks to threads, 8192 x 2048 float32 take 89 us.)
 template <class T>
-__global__ void __launch_bounds__(kThreads) k_mx_dequantize_rows(const unsigned* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                                 int64_t C, int64_t rows, int KB, T* __restrict__ y) {
+__global__ void __launch_bounds__(kThreads) k_mx_dequantize_rows(const unsigned* __restrict__ codes,
+                                                                 const uint8_t* __restrict__ scales, int64_t C, int64_t rows,
+                                                                 int KB, T* __restrict__ y) {
   typedef T W __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   const int64_t total = rows * KB * 4, stride = (int64_t)gridDim.x * kThreads;
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += stride) {
@@ -151,7 +150,7 @@ template <class T, int V>
 void quantize_map(const T* x, int64_t C, int64_t HW, int64_t rows, int KB, void* codes, void* scales, hipStream_t st) {
   const int64_t units = (rows + 64 * V - 1) / (64 * V) * KB;
   hipLaunchKernelGGL((k_mx_quantize<T, V>), dim3(mx_grid((units + 3) / 4, kThreads)), dim3(kThreads), 0, st, x, C, HW, rows, KB,
-                     (uint4*)codes, (uint8_t*)scales);
+                     (mx_i32x4*)codes, (uint8_t*)scales);
 }
 
 template <class T>

@@ -61,10 +61,11 @@ struct MxGradArgs {
   int ta, tb;
 };
 
-// D[i][k] = sum over terms of A's row i and B's row k, on a tile of BA x BB, half of each to a wave.  gx: A the matrix' columns (c), B the pixels, terms n.  gw: A the
-// channels of gy (n), B those of x (c), terms the pixels.  The codes come by terms, 32 neighbours of a tile's row to a block, and
-// lie in LDS as they come: a transposing read gives a lane the terms of its column.  gy comes either way: with its
-// terms side by side (ONE false, gw, or ONE, gx), or by terms.
+// D[i][k] = sum over terms of A's row i and B's row k, in tiles of BA x BB, a quarter to a wave.  gx: A are the matrix' columns
+// (c), B the pixels, the terms n.  gw: A are the channels of gy (n), B those of x (c), the terms the pixels, shared out over
+// blockIdx.y.  The codes come by terms, 32 neighbours of a tile's rows to a block, and lie in LDS as they come, in bfloat16: a
+// transposing read gives a lane the terms of its column.  gy comes either way: its terms side by side (gw of maps, gx of one
+// pixel a sample: ONE), or by terms.
 template <class T, int KIND, bool ONE, int BA, int BB>
 __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
   typedef MxGrad<T> G;
@@ -73,8 +74,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
   constexpr bool kByTerms = (KIND == kGradX) != ONE;                           // gy's tile [terms][rows]
   constexpr int GR = kByTerms ? K : BG, GC = kByTerms ? BG : K;                // its rows and columns as stored
   // Rows are padded so that what 16 lanes read at once lies in different banks: 32 bytes of four rows for the
-  // transposing reads, 16 of neighbouring rows otherwise.
-  constexpr int CS = BC * 2 + 32, GS = GC * 2 + (kByTerms ? 32 : 16);
+  // transposing reads (64 of four for the two halves of a tile), 16 of neighbouring rows otherwise.
+  constexpr int CS = BC * 2 + 64, GS = GC * 2 + (kByTerms ? 64 : 16);
   constexpr int NG = GR * GC / V / kThreads, NC = (K * BC / 32 + kThreads - 1) / kThreads;
   __shared__ __attribute__((aligned(16))) char lds[K * CS + P * GR * GS];
   char* const lc = lds;
@@ -89,37 +90,69 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
   const int64_t k_first = (int64_t)blockIdx.y * a.terms, k_end = min(terms, k_first + a.terms);
   const T* const gy = (const T*)a.gy;
 
-  W g[NG];
-  mx_i32x4 q[NC];
-  unsigned qs[NC];
-  // Row n or pixel r of gy's vector i, its first element along the vector.
-  auto load = [&](int64_t k0) {
+  // What is under way from memory for the next step.  (Two steps under way change nothing: 33 us either way for gx of 8192
+  // bfloat16 pixels, 1024 to 1024 channels.)
+  struct Step {
+    W g[NG];
+    mx_i32x4 q[NC];
+    unsigned qs[NC];
+  };
+  // This thread's first vector of gy's tile and piece of the codes' (the others: a fixed number of rows on).
+  constexpr int RG = kThreads / (GC / V), RC = kThreads / (BC / 32);
+  const int grow = tid / (GC / V), gcol = tid % (GC / V) * V, crow = tid / (BC / 32), cpiece = tid % (BC / 32);
+  // A tile whose rows are all there, with every vector in one sample, is read without a look at each vector.
+  const bool inside = g0 + BG <= (KIND == kGradX ? a.rows : a.N) && c0 / 32 + BC / 32 <= a.KB && (ONE || a.HW % V == 0);
+  const int64_t ghop = ONE ? a.N : a.HW;  // elements from a row of gy's tile to the next
+  auto load = [&](int64_t k0, Step& s) {
+    const bool fast = inside && k0 + K <= k_end;
+    const mx_i32x4* codes = a.codes + (k0 + crow) * a.KB + c0 / 32 + cpiece;
+    const uint8_t* scales = a.scales + (k0 + crow) * a.KB + c0 / 32 + cpiece;
+    if (fast) {
+      const int64_t k = k0 + (kByTerms ? grow : gcol), m = g0 + (kByTerms ? gcol : grow);
+      const int64_t n = KIND == kGradX ? k : m, r = KIND == kGradX ? m : k;
+      const int64_t b = ONE ? r : (uint32_t)r / (uint32_t)a.HW;
+      const T* src = gy + (ONE ? r * a.N + n : (b * a.N + n) * a.HW + (r - b * a.HW));
+#pragma unroll
+      for (int i = 0; i < NG; ++i) s.g[i] = *(const W*)(src + i * RG * ghop);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        s.q[i] = mx_i32x4{0, 0, 0, 0};
+        s.qs[i] = 127;
+        if (kThreads * (i + 1) <= K * BC / 32 || crow + i * RC < K) {
+          s.q[i] = codes[(int64_t)i * RC * a.KB];
+          s.qs[i] = scales[(int64_t)i * RC * a.KB];
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      const int at = tid + i * kThreads, row = at / (GC / V), col = at % (GC / V) * V;
-      g[i] = W{};
-      const int64_t k = k0 + (kByTerms ? row : col), m = g0 + (kByTerms ? col : row);
+      const int row = grow + i * RG;
+      s.g[i] = W{};
+      const int64_t k = k0 + (kByTerms ? row : gcol), m = g0 + (kByTerms ? gcol : row);
       const int64_t n = KIND == kGradX ? k : m, r = KIND == kGradX ? m : k;
       const int64_t n_end = KIND == kGradX ? k_end : a.N, r_end = KIND == kGradX ? a.rows : k_end;
       if (n >= n_end || r >= r_end) continue;
       if (ONE) {  // (rows, N): vectors along n
         const T* src = gy + r * a.N + n;
+        asm volatile("" : "+v"(src));
         if (n + V <= n_end) {
-          g[i] = *(const W*)src;
+          s.g[i] = *(const W*)src;
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e)
-            if (n + e < n_end) g[i][e] = src[e];
+            if (n + e < n_end) s.g[i][e] = src[e];
         }
       } else {  // (B, N, HW): vectors along the pixels
         int64_t b = (uint32_t)r / (uint32_t)a.HW, p = r - b * a.HW;
         const T* src = gy + (b * a.N + n) * a.HW + p;
+        asm volatile("" : "+v"(src), "+v"(p));  // (addresses of single elements kept over the loop would fill the registers)
         if (p + V <= a.HW && r + V <= r_end) {
-          g[i] = *(const W*)src;
+          s.g[i] = *(const W*)src;
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            if (r + e < r_end) g[i][e] = *src;
+            if (r + e < r_end) s.g[i][e] = *src;
             ++src;
             if (++p == a.HW) p = 0, src += (a.N - 1) * a.HW;
           }
@@ -128,51 +161,49 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int at = tid + i * kThreads, row = at / (BC / 32), piece = at % (BC / 32);
-      const int64_t k = k0 + row, kb = c0 / 32 + piece;
-      q[i] = mx_i32x4{0, 0, 0, 0};
-      qs[i] = 127;
-      if (row < K && k < k_end && kb < a.KB) {
-        q[i] = a.codes[k * a.KB + kb];
-        qs[i] = a.scales[k * a.KB + kb];
+      s.q[i] = mx_i32x4{0, 0, 0, 0};
+      s.qs[i] = 127;
+      if (crow + i * RC < K && k0 + crow + i * RC < k_end && c0 / 32 + cpiece < a.KB) {
+        s.q[i] = codes[(int64_t)i * RC * a.KB];
+        s.qs[i] = scales[(int64_t)i * RC * a.KB];
       }
     }
   };
   // Sums of gy over the pixels, of the rows or columns that this thread loads.
   constexpr int NB = KIND != kGradW ? 1 : kByTerms ? V : NG;
   double sum[NB] = {};
-  auto store = [&] {
+  auto store = [&](const Step& s) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
-      const int at = tid + i * kThreads, row = at / (GC / V), col = at % (GC / V) * V;
+      const int row = grow + i * RG;
       __bf16 part[P][V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         __bf16 x[P];
-        mx_split(g[i][e], x);
+        mx_split(s.g[i][e], x);
 #pragma unroll
         for (int p = 0; p < P; ++p) part[p][e] = x[p];
       }
       typedef __bf16 S __attribute__((ext_vector_type(V)));
 #pragma unroll
-      for (int p = 0; p < P; ++p) *(S*)(lg + (p * GR + row) * GS + col * 2) = *(const S*)part[p];
+      for (int p = 0; p < P; ++p) *(S*)(lg + (p * GR + row) * GS + gcol * 2) = *(const S*)part[p];
       if (KIND == kGradW && a.gb && b0 == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[(kByTerms ? e : i) % NB] += (double)(float)g[i][e];
+        for (int e = 0; e < V; ++e) sum[(kByTerms ? e : i) % NB] += (double)(float)s.g[i][e];
       }
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int at = tid + i * kThreads, row = at / (BC / 32), piece = at % (BC / 32);
+      const int row = crow + i * RC;
       if (row >= K) continue;
-      const float scale = mx_scale(qs[i]);
+      const float scale = mx_scale(s.qs[i]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const mx_bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 0),
-                        v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 1),
-                        v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 2),
-                        v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)q[i][w], scale, 3);
-        *(mx_bf16x8*)(lc + row * CS + piece * 64 + w * 16) = mx_bf16x8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
+        const mx_bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)s.q[i][w], scale, 0),
+                        v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)s.q[i][w], scale, 1),
+                        v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)s.q[i][w], scale, 2),
+                        v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)s.q[i][w], scale, 3);
+        *(mx_bf16x8*)(lc + row * CS + cpiece * 64 + w * 16) = mx_bf16x8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
       }
     }
   };
@@ -196,32 +227,43 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
   for (int i = 0; i < TA; ++i)
 #pragma unroll
     for (int k = 0; k < TB; ++k) acc[i][k] = mx_f32x16{};
-  load(k_first);
-  for (int64_t k0 = k_first; k0 < k_end; k0 += K) {
+  auto step = [&](int64_t k0, Step& st) {
     __syncthreads();
-    store();
+    store(st);
     __syncthreads();
-    if (k0 + K < k_end) load(k0 + K);
+    if (k0 + K < k_end) load(k0 + K, st);
+    // Each sixteen terms' operands come from LDS while the ones before are multiplied.
+    mx_bf16x8 c[2][TC], y[2][P][TG];
+    auto operands = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < TC; ++i) c[s & 1][i] = by_terms(lc, CS, wc + 32 * i, s);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < TG; ++i) {
+          const char* base = lg + p * GR * GS;
+          y[s & 1][p][i] = kByTerms ? by_terms(base, GS, wg + 32 * i, s) : side_by_side(base, wg + 32 * i, s);
+        }
+    };
+    operands(0);
 #pragma unroll
     for (int s = 0; s < K / 16; ++s) {
-      mx_bf16x8 c[TC];
+      if (s + 1 < K / 16) operands(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < TC; ++i) c[i] = by_terms(lc, CS, wc + 32 * i, s);
-#pragma unroll
-      for (int p = P - 1; p >= 0; --p) {
-        const char* base = lg + p * GR * GS;
-        mx_bf16x8 y[TG];
-#pragma unroll
-        for (int i = 0; i < TG; ++i) y[i] = kByTerms ? by_terms(base, GS, wg + 32 * i, s) : side_by_side(base, wg + 32 * i, s);
+      for (int p = P - 1; p >= 0; --p)
 #pragma unroll
         for (int i = 0; i < TA; ++i)
 #pragma unroll
           for (int k = 0; k < TB; ++k)
-            acc[i][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(KIND == kGradX ? c[i] : y[i], KIND == kGradX ? y[k] : c[k],
-                                                                acc[i][k], 0, 0, 0);
-      }
+            acc[i][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(KIND == kGradX ? c[s & 1][i] : y[s & 1][p][i],
+                                                                KIND == kGradX ? y[s & 1][p][k] : c[s & 1][k], acc[i][k], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-  }
+  };
+  Step st;
+  load(k_first, st);
+  for (int64_t k0 = k_first; k0 < k_end; k0 += K) step(k0, st);
 
   // Element e of a 32 x 32 result is its row 8 (e / 4) + 4 h + e % 4, column j.
 #pragma unroll
@@ -279,27 +321,40 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
   }
 }
 
-// The sum over the splits, in the same order on every call: eight threads an element take every eighth of them.  (One
-// thread an element leaves few to wait for long chains of loads: 288 splits of 8192 elements take 134 us that way.)
-__global__ void __launch_bounds__(kThreads) k_mx_grad_join(const float* __restrict__ part, int64_t n, const double* __restrict__ gbp,
-                                                           int64_t nb, int splits, float* __restrict__ gw, float* __restrict__ gb) {
-  __shared__ double red[8][32];
-  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
-  const int64_t blocks = (n + 31) / 32;
+// The sum over the splits, in the same order on every call: R threads an element take every R-th of them.  (One thread an
+// element leaves few to wait for long chains of loads: 288 splits of 8192 elements take 134 us that way, 8 threads 4; 8
+// splits of a million elements take 9 and 16.)
+template <int R>
+__global__ void __launch_bounds__(kThreads) k_mx_grad_join(const float* __restrict__ part, int64_t n,
+                                                           const double* __restrict__ gbp, int64_t nb, int splits,
+                                                           float* __restrict__ gw, float* __restrict__ gb) {
+  constexpr int kCols = kThreads / R;
+  __shared__ double red[R][kCols];
+  const int col = threadIdx.x % kCols, row = threadIdx.x / kCols;
+  const int64_t blocks = (n + kCols - 1) / kCols;
   const bool bias = blockIdx.x >= blocks;
-  const int64_t i = ((int64_t)blockIdx.x - (bias ? blocks : 0)) * 32 + col, end = bias ? nb : n;
+  const int64_t i = ((int64_t)blockIdx.x - (bias ? blocks : 0)) * kCols + col, end = bias ? nb : n;
   double s = 0.;
   if (i < end) {
 #pragma unroll 4
-    for (int k = row; k < splits; k += 8) s += bias ? gbp[k * nb + i] : (double)part[k * n + i];
+    for (int k = row; k < splits; k += R) s += bias ? gbp[k * nb + i] : (double)part[k * n + i];
   }
-  red[row][col] = s;
-  __syncthreads();
+  if (R > 1) {
+    red[row][col] = s;
+    __syncthreads();
+  }
   if (row == 0 && i < end) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += red[k][col];
+    for (int k = 1; k < R; ++k) s += red[k][col];
     (bias ? gb : gw)[i] = (float)s;
   }
+}
+
+template <int R>
+void grad_join(const float* part, int64_t n, const double* gbp, int64_t nb, int64_t splits, float* gw, float* gb, hipStream_t st) {
+  constexpr int kCols = kThreads / R;
+  const int64_t blocks = (n + kCols - 1) / kCols + (gb ? (nb + kCols - 1) / kCols : 0);
+  hipLaunchKernelGGL(k_mx_grad_join<R>, dim3((unsigned)blocks), dim3(kThreads), 0, st, part, n, gbp, nb, (int)splits, gw, gb);
 }
 
 // The bias' gradient alone: a block for a channel.
@@ -358,7 +413,8 @@ int grads(const void* gy, const void* xc, const void* xs, const void* wc, const 
   const int KB = (int)mx_blocks(C);
   if (gx) {
     const MxGradArgs a = {gy, (const mx_i32x4*)wc, (const uint8_t*)ws, C, N, HW, rows, KB, gx, nullptr, N, 0, 0};
-    const int rc = C <= 64 ? grad_tile<T, kGradX, ONE, 64, 128>(a, C, rows, 1, st)
+    // (256 pixels, 2048 to 2048 channels: 36 us by 32 tiles of 128 channels, 25 by 64 of 64)
+    const int rc = C <= 64 || (C + 127) / 128 * ((rows + 127) / 128) < 256 ? grad_tile<T, kGradX, ONE, 64, 128>(a, C, rows, 1, st)
                            : grad_tile<T, kGradX, ONE, 128, 128>(a, C, rows, 1, st);
     if (rc != CVN_OK) return rc;
   }
@@ -367,14 +423,15 @@ int grads(const void* gy, const void* xc, const void* xs, const void* wc, const 
     float* const part = s.splits > 1 ? (float*)work : gw;
     double* const gbp = (double*)((char*)work + (s.splits > 1 ? align_up((size_t)(s.splits * N * C) * sizeof(float)) : 0));
     const MxGradArgs a = {gy, (const mx_i32x4*)xc, (const uint8_t*)xs, C, N, HW, rows, KB, part, gb ? gbp : nullptr, s.terms, 0, 0};
-    int rc;
-    if (C <= 64) rc = N <= 64 ? grad_tile<T, kGradW, ONE, 64, 64>(a, N, C, s.splits, st) : grad_tile<T, kGradW, ONE, 128, 64>(a, N, C, s.splits, st);
-    else rc = N <= 64 ? grad_tile<T, kGradW, ONE, 64, 128>(a, N, C, s.splits, st) : grad_tile<T, kGradW, ONE, 128, 128>(a, N, C, s.splits, st);
+    const int rc = C <= 64 ? (N <= 64 ? grad_tile<T, kGradW, ONE, 64, 64>(a, N, C, s.splits, st)
+                                      : grad_tile<T, kGradW, ONE, 128, 64>(a, N, C, s.splits, st))
+                           : (N <= 64 ? grad_tile<T, kGradW, ONE, 64, 128>(a, N, C, s.splits, st)
+                                      : grad_tile<T, kGradW, ONE, 128, 128>(a, N, C, s.splits, st));
     if (rc != CVN_OK) return rc;
     if (s.splits > 1 || gb) {
       const int64_t n = s.splits > 1 ? N * C : 0;
-      hipLaunchKernelGGL(k_mx_grad_join, dim3((unsigned)((n + 31) / 32 + (gb ? (N + 31) / 32 : 0))), dim3(kThreads), 0, st, part,
-                         n, gbp, N, (int)s.splits, gw, gb);
+      if (n >= 1 << 18) grad_join<1>(part, n, gbp, N, s.splits, gw, gb, st);
+      else grad_join<8>(part, n, gbp, N, s.splits, gw, gb, st);
     }
   } else if (gb) {
     hipLaunchKernelGGL(k_mx_grad_bias<T>, dim3((unsigned)N), dim3(kThreads), 0, st, (const T*)gy, N, HW, rows, gb);

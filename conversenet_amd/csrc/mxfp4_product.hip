@@ -120,26 +120,22 @@ __device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V
 // Many pixels of many channels: both operands in MXFP4, tiles staged through LDS.
 // ------------------------------------------------------------------------------------------------
 // A step takes 256 channels: 128 bytes of codes a row, which a wave fetches 8 rows at a time straight into LDS.  A row's
-// 16-byte pieces are stored in an order that depends on the row (piece ^ (row / D & 7)), so that lanes which read the same
-// piece of D-spaced rows hit different banks.  Lane l of a 32 x 32 x 64 product takes the blocks 4 (l / 32) + s of rows
+// 16-byte pieces are stored in an order that depends on the row (piece ^ (row / 2 & 7)), so that 16 lanes which read the
+// same piece of neighbouring rows hit all 64 banks.  Lane l of a 32 x 32 x 64 product takes the blocks 4 (l / 32) + s of rows
 // l % 32 in steps s < 4: its four scales are one word.  Past the last block the codes of that block stand in, and both
 // scales are 2^-127: the products are lost below float32's range.
 constexpr int kStep = 8;  // blocks of a step
 
 // The word of four scales at byte `at` of an operand's scales, as loaded from `last` at most, where the last whole word is
-// (below 0 where there are fewer than four bytes) ..
+// (from there the four are shifted: mx_scales_tail) ..
 __device__ __forceinline__ unsigned mx_scales_load(const uint8_t* s, int at, int last) {
   typedef unsigned U __attribute__((aligned(1)));
-  if (last >= 0) return *(const U*)(s + (unsigned)min(at, last));
-  unsigned v = 0;
-  for (int i = 0; i < 3; ++i)
-    if (at + i < last + 4) v |= (unsigned)s[at + i] << (8 * i);
-  return v;
+  return *(const U*)(s + (int64_t)min(at, last));
 }
 // .. and put right, for blocks kb .. of KB: 0 past the last.
 __device__ __forceinline__ unsigned mx_scales_tail(unsigned v, int at, int last, int kb, int KB) {
   if (kb >= KB) return 0;
-  if (last >= 0) v >>= 8 * (at - min(at, last));
+  v >>= 8 * (at - min(at, last));
   return KB - kb < 4 ? v & ((1u << (8 * (KB - kb))) - 1) : v;
 }
 
@@ -158,7 +154,7 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
   constexpr int D = TB;  // rows of B between neighbouring lanes
   constexpr int kBytes = (BA + BB) * 128;
   constexpr int LA = BA / 8 / NW, LB = BB / 8 / NW;
-  static_assert(8 / D * NW % 8 == 0, "a wave's fetches of a tile put a row's pieces in one order");
+  static_assert(NW % 2 == 0, "a wave's fetches of a tile put a row's pieces in one order");
   extern __shared__ char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
   const int wa = wave % (BA / WA) * WA, wb = wave / (BA / WA) * WB;
@@ -172,7 +168,7 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
   int alast, blast;
   uint32_t aoff[LA], boff[LB];
   int as_at[TA], bs_at[TB];
-  const int apiece = (lane & 7) ^ (lane >> 3), bpiece = (lane & 7) ^ (((8 * wave + (lane >> 3)) / D) & 7);
+  const int piece = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
   auto place = [&](int t) {
     // Blocks of one XCD take a run of tiles, in patches of eight A tiles: its L2 holds what they share.
     const int per = nt / 8, rem = nt % 8, x = t & 7, i8 = t >> 3;
@@ -186,7 +182,10 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
 #pragma unroll
     for (int i = 0; i < LA; ++i) aoff[i] = (uint32_t)(min(8 * (wave + NW * i) + (lane >> 3), amost) * KB) * 16;
 #pragma unroll
-    for (int i = 0; i < LB; ++i) boff[i] = (uint32_t)(min(8 * (wave + NW * i) + (lane >> 3), bmost) * KB) * 16;
+    for (int i = 0; i < LB; ++i) {  // row 32 v + j of a wave's part in LDS is its row D j + v
+      const int row = 8 * (wave + NW * i) + (lane >> 3), in = row % WB;
+      boff[i] = (uint32_t)(min(row - in + D * (in % 32) + in / 32, bmost) * KB) * 16;
+    }
 #pragma unroll
     for (int i = 0; i < TA; ++i) as_at[i] = min(wa + 32 * i + j, amost) * KB + 4 * h;
 #pragma unroll
@@ -194,13 +193,14 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
   };
   unsigned sa[TA], sb[TB];
   auto fetch = [&](int kb0, char* buf) {
-    const uint32_t ap = (uint32_t)min(kb0 + apiece, KB - 1) * 16, bp = (uint32_t)min(kb0 + bpiece, KB - 1) * 16;
+    const uint32_t at = (uint32_t)min(kb0 + piece, KB - 1) * 16;
 #pragma unroll
     for (int i = 0; i < LA; ++i)
-      __builtin_amdgcn_global_load_lds((mx_glob)(acodes + (aoff[i] + ap)), (mx_lds)(buf + (wave + NW * i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((mx_glob)(acodes + (aoff[i] + at)), (mx_lds)(buf + (wave + NW * i) * 1024), 16, 0, 0);
 #pragma unroll
     for (int i = 0; i < LB; ++i)
-      __builtin_amdgcn_global_load_lds((mx_glob)(bcodes + (boff[i] + bp)), (mx_lds)(buf + BA * 128 + (wave + NW * i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((mx_glob)(bcodes + (boff[i] + at)), (mx_lds)(buf + BA * 128 + (wave + NW * i) * 1024),
+                                       16, 0, 0);
 #pragma unroll
     for (int i = 0; i < TA; ++i) sa[i] = mx_scales_load(ascales, as_at[i] + kb0, alast);
 #pragma unroll
@@ -214,109 +214,109 @@ __global__ void __launch_bounds__((BA / WA) * (BB / WB) * 64, 1)
   constexpr int NC = MAP ? BA : BB;
   float* bias = (float*)(smem + 2 * kBytes);
   for (int t = blockIdx.x;;) {
-  const int64_t ra0 = ra, rb0 = rb;
-  const int next = t + (int)gridDim.x;
-  float* const rscale = bias + NC;
-  for (int i = threadIdx.x; i < NC; i += NW * 64) {
-    const int64_t n = (MAP ? ra0 : rb0) + i;
-    bias[i] = o.bias && n < o.N ? o.bias[n] : 0.f;
-    rscale[i] = o.res_scale && n < o.N ? o.res_scale[n] : 1.f;
-  }
-
-  mx_f32x16 acc[TA][TB];
-#pragma unroll
-  for (int i = 0; i < TA; ++i)
-#pragma unroll
-    for (int k = 0; k < TB; ++k) acc[i][k] = mx_f32x16{};
-  for (int kb0 = 0; kb0 < KB; kb0 += kStep) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    unsigned ua[TA], ub[TB];
-#pragma unroll
-    for (int i = 0; i < TA; ++i) ua[i] = sa[i];
-#pragma unroll
-    for (int i = 0; i < TB; ++i) ub[i] = sb[i];
-    if (kb0 + kStep < KB) {
-      fetch(kb0 + kStep, smem + (cur ^ 1) * kBytes);
-    } else {
-#pragma unroll
-      for (int i = 0; i < TA; ++i) ua[i] = mx_scales_tail(ua[i], as_at[i] + kb0, alast, kb0 + 4 * h, KB);
-#pragma unroll
-      for (int i = 0; i < TB; ++i) ub[i] = mx_scales_tail(ub[i], bs_at[i] + kb0, blast, kb0 + 4 * h, KB);
-      if (next < nt) {
-        place(next);
-        fetch(0, smem + (cur ^ 1) * kBytes);
-      }
+    const int64_t ra0 = ra, rb0 = rb;
+    const int next = t + (int)gridDim.x;
+    float* const rscale = bias + NC;
+    for (int i = threadIdx.x; i < NC; i += NW * 64) {
+      const int64_t n = (MAP ? ra0 : rb0) + i;
+      bias[i] = o.bias && n < o.N ? o.bias[n] : 0.f;
+      rscale[i] = o.res_scale && n < o.N ? o.res_scale[n] : 1.f;
     }
-    const char* buf = smem + cur * kBytes;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      mx_i32x4 a[TA], b[TB];
-#pragma unroll
-      for (int i = 0; i < TA; ++i) {
-        const int row = wa + 32 * i + j;
-        a[i] = *(const mx_i32x4*)(buf + row * 128 + (((4 * h + s) ^ (row & 7)) << 4));
-      }
-#pragma unroll
-      for (int i = 0; i < TB; ++i) {
-        const int row = wb + D * j + i;
-        b[i] = *(const mx_i32x4*)(buf + (BA + row) * 128 + (((4 * h + s) ^ ((row / D) & 7)) << 4));
-      }
-#pragma unroll
-      for (int i = 0; i < TA; ++i)
-#pragma unroll
-        for (int k = 0; k < TB; ++k) {
-          // (the byte of a scale word is part of the instruction)
-          if (s == 0) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 0, ua[i], 0, ub[k]);
-          if (s == 1) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 1, ua[i], 1, ub[k]);
-          if (s == 2) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 2, ua[i], 2, ub[k]);
-          if (s == 3) acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[i]), mx_operand(b[k]), acc[i][k], kMxFp4, kMxFp4, 3, ua[i], 3, ub[k]);
-        }
-    }
-    cur ^= 1;
-  }
 
-  // Element e of a 32 x 32 result is its row 8 (e / 4) + 4 h + e % 4, column j.
-  const int64_t c0 = rb0 + wb + D * j, a0 = ra0 + wa + 4 * h, step = MAP ? o.HW : o.N;  // this lane's first column and row
-  MxPixels<TB> at;
-  bool whole = c0 + TB <= nb;
-  if (MAP) {
-    const MxGroup grp = mx_group<TB>(min(c0, nb - 1), o.HW, o.rows);
-    at = mx_pixels<TB>(o, grp, a0);
-    whole = grp.whole;
-  } else {
-    at.live = 0;
-#pragma unroll
-    for (int k = 0; k < TB; ++k) at.at[k] = a0 * o.N + c0 + k, at.live |= (c0 + k < nb) << k;
-  }
-  if (c0 < nb) {
+    mx_f32x16 acc[TA][TB];
 #pragma unroll
     for (int i = 0; i < TA; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int off = 32 * i + 8 * q;
-        float v[4][TB], ss[4][TB];
+      for (int k = 0; k < TB; ++k) acc[i][k] = mx_f32x16{};
+    for (int kb0 = 0; kb0 < KB; kb0 += kStep) {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      unsigned ua[TA], ub[TB];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+      for (int i = 0; i < TA; ++i) ua[i] = sa[i];
 #pragma unroll
-          for (int k = 0; k < TB; ++k) {
-            const int n = MAP ? wa + off + 4 * h + r : wb + D * j + k;
-            v[r][k] = acc[i][k][4 * q + r] + bias[n], ss[r][k] = rscale[n];
-          }
-        mx_finish<TB, 4>(o, v, ss);
-        const int64_t left = na - a0 - off;
-        if (whole && left >= 4) {
-          mx_store_rows<T, NT, TB, 4>(o, at.at[0] + off * step, step, v);
-        } else {
+      for (int i = 0; i < TB; ++i) ub[i] = sb[i];
+      if (kb0 + kStep < KB) {
+        fetch(kb0 + kStep, smem + (cur ^ 1) * kBytes);
+      } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r < left) mx_store_pixels<T, TB>(o, at, (off + r) * step, v[r]);
+        for (int i = 0; i < TA; ++i) ua[i] = mx_scales_tail(ua[i], as_at[i] + kb0, alast, kb0 + 4 * h, KB);
+#pragma unroll
+        for (int i = 0; i < TB; ++i) ub[i] = mx_scales_tail(ub[i], bs_at[i] + kb0, blast, kb0 + 4 * h, KB);
+        if (next < nt) {
+          place(next);
+          fetch(0, smem + (cur ^ 1) * kBytes);
         }
       }
-  }
-  if (next >= nt) return;
-  t = next;
-  bias = bias == (float*)(smem + 2 * kBytes) ? bias + 2 * NC : bias - 2 * NC;
+      const char* buf = smem + cur * kBytes;
+      // Each quarter's operands come from LDS while the ones before are multiplied.
+      mx_i32x4 a[2][TA], b[2][TB];
+      auto operands = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < TA; ++i) {
+          const int row = wa + 32 * i + j;
+          a[s & 1][i] = *(const mx_i32x4*)(buf + row * 128 + (((4 * h + s) ^ (row >> 1 & 7)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+          const int row = wb + 32 * i + j;
+          b[s & 1][i] = *(const mx_i32x4*)(buf + (BA + row) * 128 + (((4 * h + s) ^ (row >> 1 & 7)) << 4));
+        }
+      };
+      operands(0);
+#define MX_STEP(s)                                                                                                 \
+  if (s < 3) operands(s + 1);                                                                                      \
+  __builtin_amdgcn_sched_barrier(0);                                                                               \
+  _Pragma("unroll") for (int i = 0; i < TA; ++i) _Pragma("unroll") for (int k = 0; k < TB; ++k) acc[i][k] =        \
+      __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a[s & 1][i]), mx_operand(b[s & 1][k]), acc[i][k], \
+                                                      kMxFp4, kMxFp4, s, ua[i], s, ub[k]);                         \
+  __builtin_amdgcn_sched_barrier(0);
+      MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)  // (the byte of a scale word is part of the instruction)
+#undef MX_STEP
+      cur ^= 1;
+    }
+
+    // Element e of a 32 x 32 result is its row 8 (e / 4) + 4 h + e % 4, column j.
+    const int64_t c0 = rb0 + wb + D * j, a0 = ra0 + wa + 4 * h, step = MAP ? o.HW : o.N;  // this lane's first column and row
+    MxPixels<TB> at;
+    bool whole = c0 + TB <= nb;
+    if (MAP) {
+      const MxGroup grp = mx_group<TB>(min(c0, nb - 1), o.HW, o.rows);
+      at = mx_pixels<TB>(o, grp, a0);
+      whole = grp.whole;
+    } else {
+      at.live = 0;
+#pragma unroll
+      for (int k = 0; k < TB; ++k) at.at[k] = a0 * o.N + c0 + k, at.live |= (c0 + k < nb) << k;
+    }
+    if (c0 < nb) {
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int off = 32 * i + 8 * q;
+          float v[4][TB], ss[4][TB];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int k = 0; k < TB; ++k) {
+              const int n = MAP ? wa + off + 4 * h + r : wb + D * j + k;
+              v[r][k] = acc[i][k][4 * q + r] + bias[n], ss[r][k] = rscale[n];
+            }
+          mx_finish<TB, 4>(o, v, ss);
+          const int64_t left = na - a0 - off;
+          if (whole && left >= 4) {
+            mx_store_rows<T, NT, TB, 4>(o, at.at[0] + off * step, step, v);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r < left) mx_store_pixels<T, TB>(o, at, (off + r) * step, v[r]);
+          }
+        }
+    }
+    if (next >= nt) return;
+    t = next;
+    bias = bias == (float*)(smem + 2 * kBytes) ? bias + 2 * NC : bias - 2 * NC;
   }
 }
 
@@ -354,7 +354,7 @@ int gemm(const MxIn& in, const MxOut& o, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// A few pixels: a block makes 16 channels of up to 16 of them, its waves take the channels in turn.
+// A few pixels: a block makes 16 channels of 16 of them at a time, its waves take the channels in turn.
 // ------------------------------------------------------------------------------------------------
 // The matrix is read once and bounds this; the pixels' codes are made on the way by every block.
 template <class T>
@@ -376,9 +376,7 @@ __device__ __forceinline__ unsigned mx_quantize_row(const T* x, int64_t step, in
 #pragma unroll
   for (int c = 0; c < kMxBlock; ++c) mag = max(mag, mx_mag(v[c]));
   const unsigned s = mx_scale_code(mag);
-  const float scale = mx_scale(s);
-  *q = mx_i32x4{(int)mx_pack8(v, scale), (int)mx_pack8(v + 8, scale), (int)mx_pack8(v + 16, scale), (int)mx_pack8(v + 24, scale)};
-  if (s == 255u) *q = mx_i32x4{0, 0, 0, 0};
+  *q = mx_pack32(v, s);
   return s;
 }
 
@@ -388,47 +386,54 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
   __shared__ float part[kFewWaves][16][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16, wrow = min(n0 + j, o.N - 1) * in.KB;
-  const bool live = j < o.rows;
-  const int64_t b = live ? (uint32_t)j / (uint32_t)o.HW : 0, p = j - b * o.HW;
-  const T* x = (const T*)in.x + b * in.C * o.HW + p;
-  mx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 4 * wave; k < in.KB; k += 4 * kFewWaves) {
-    // lane l holds block k + l / 16 of its operands' rows l % 16; past the last both scales are 2^-127
-    const bool in_row = k + g < in.KB;
-    const int kb = min(k + g, in.KB - 1);
-    const mx_i32x4 w = in.wc[wrow + kb];
-    unsigned sw = in.ws[wrow + kb], sx = 0;
-    mx_i32x4 q = {0, 0, 0, 0};
-    if (live && in_row) {
-      if (in.x) {
-        sx = mx_quantize_row(x + (int64_t)kb * kMxBlock * o.HW, o.HW, (int)min((int64_t)kMxBlock, in.C - kb * kMxBlock), &q);
-        if (in.xc && blockIdx.x == 0) {
-          in.xc[(int64_t)j * in.KB + kb] = q;
-          in.xs[(int64_t)j * in.KB + kb] = (uint8_t)sx;
+  for (int64_t r0 = (int64_t)blockIdx.y * 16; r0 < o.rows; r0 += (int64_t)gridDim.y * 16) {
+    const int64_t r = r0 + j;
+    const bool live = r < o.rows;
+    const int64_t b = live ? (uint32_t)r / (uint32_t)o.HW : 0, p = r - b * o.HW;
+    const T* x = (const T*)in.x + b * in.C * o.HW + p;
+    mx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 4 * wave; k < in.KB; k += 4 * kFewWaves) {
+      // lane l holds block k + l / 16 of its operands' rows l % 16; past the last both scales are 2^-127
+      const bool in_row = k + g < in.KB;
+      const int kb = min(k + g, in.KB - 1);
+      const mx_i32x4 w = in.wc[wrow + kb];
+      unsigned sw = in.ws[wrow + kb], sx = 0;
+      mx_i32x4 q = {0, 0, 0, 0};
+      if (live && in_row) {
+        if (in.x) {
+          sx = mx_quantize_row(x + (int64_t)kb * kMxBlock * o.HW, o.HW, (int)min((int64_t)kMxBlock, in.C - kb * kMxBlock), &q);
+          if (blockIdx.x == 0) {
+            in.xc[r * in.KB + kb] = q;
+            in.xs[r * in.KB + kb] = (uint8_t)sx;
+          }
+        } else {
+          q = in.xc[r * in.KB + kb];
+          sx = in.xs[r * in.KB + kb];
         }
-      } else {
-        q = in.xc[(int64_t)j * in.KB + kb];
-        sx = in.xs[(int64_t)j * in.KB + kb];
+      }
+      if (!in_row) sw = 0;
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w), mx_operand(q), acc, kMxFp4, kMxFp4, 0, (int)sw, 0,
+                                                             (int)sx);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][4 * g + e][j] = acc[e];
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      // neighbouring threads store neighbours: channels of one pixel a sample, pixels otherwise
+      const int a = threadIdx.x & 15, c = threadIdx.x >> 4, n = o.HW == 1 ? a : c, k = o.HW == 1 ? c : a;
+      const int64_t rk = r0 + k;
+      if (rk < o.rows && n0 + n < o.N) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < kFewWaves; ++i) v += part[i][n][k];
+        const int64_t rb = (uint32_t)rk / (uint32_t)o.HW;
+        float out[1][1] = {{o.bias ? v + o.bias[n0 + n] : v}};
+        const float scale[1][1] = {{o.res_scale ? o.res_scale[n0 + n] : 1.f}};
+        mx_finish<1, 1>(o, out, scale);
+        mx_store_rows<T, false, 1, 1>(o, (rb * o.N + n0 + n) * o.HW + (rk - rb * o.HW), 0, out);
       }
     }
-    if (!in_row) sw = 0;
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w), mx_operand(q), acc, kMxFp4, kMxFp4, 0, (int)sw, 0, (int)sx);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) part[wave][4 * g + e][j] = acc[e];
-  __syncthreads();
-  if (threadIdx.x < 256) {
-    // neighbouring threads store neighbours: channels of one pixel a sample, pixels otherwise
-    const int a = threadIdx.x & 15, c = threadIdx.x >> 4, n = o.HW == 1 ? a : c, r = o.HW == 1 ? c : a;
-    if (r >= o.rows || n0 + n >= o.N) return;
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kFewWaves; ++i) v += part[i][n][r];
-    const int64_t rb = (uint32_t)r / (uint32_t)o.HW;
-    float out[1][1] = {{o.bias ? v + o.bias[n0 + n] : v}};
-    const float scale[1][1] = {{o.res_scale ? o.res_scale[n0 + n] : 1.f}};
-    mx_finish<1, 1>(o, out, scale);
-    mx_store_rows<T, false, 1, 1>(o, (rb * o.N + n0 + n) * o.HW + (r - rb * o.HW), 0, out);
+    __syncthreads();
   }
 }
 
@@ -499,9 +504,7 @@ __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share)
         mag = max(mag, mx_mag(v[c]));
       }
       const unsigned code = mx_scale_code(mag);
-      const float scale = mx_scale(code);
-      q[s][e] = mx_i32x4{(int)mx_pack8(v, scale), (int)mx_pack8(v + 8, scale), (int)mx_pack8(v + 16, scale), (int)mx_pack8(v + 24, scale)};
-      if (code == 255u) q[s][e] = mx_i32x4{0, 0, 0, 0};
+      q[s][e] = mx_pack32(v, code);
       sx[s] |= code << (8 * e);
       if (in.xc && blockIdx.y == 0 && r0 + e < o.rows) {
         in.xc[(r0 + e) * in.KB + kb] = q[s][e];
@@ -529,8 +532,10 @@ __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share)
       const mx_i32x8 w = mx_operand(in.wc[wrow + at]);
       const int sw = kb < in.KB ? in.ws[wrow + at] : 0;
       // (the byte of the scales is part of the instruction)
-      acc[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][0]), acc[0], kMxFp4, kMxFp4, 0, sw, 0, (int)sx[s]);
-      acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][1]), acc[1], kMxFp4, kMxFp4, 0, sw, 1, (int)sx[s]);
+      acc[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][0]), acc[0], kMxFp4, kMxFp4, 0, sw, 0,
+                                                               (int)sx[s]);
+      acc[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, mx_operand(q[s][1]), acc[1], kMxFp4, kMxFp4, 0, sw, 1,
+                                                               (int)sx[s]);
     }
     if (r0 >= o.rows) continue;
     MxPixels<V> px = pix;
@@ -594,8 +599,10 @@ bool mx_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 
 template <class T>
 int product(const MxIn& in, const MxOut& o, int type, bool keep, hipStream_t st) {
-  if (o.rows <= kFewRows) {
-    hipLaunchKernelGGL(k_mx_few<T>, dim3((unsigned)((o.N + 15) / 16)), dim3(kFewWaves * 64), 0, st, in, o);
+  // (the tiled kernel reads scales by words of four)
+  if (o.rows <= kFewRows || o.N * in.KB < 4) {
+    hipLaunchKernelGGL(k_mx_few<T>, dim3((unsigned)((o.N + 15) / 16), (unsigned)std::min<int64_t>((o.rows + 15) / 16, 4096)),
+                       dim3(kFewWaves * 64), 0, st, in, o);
     return check_launch("conv1x1_mxfp4");
   }
   if (in.x && in.KB <= 8 && o.HW > 1) return conv<T>(in, o, keep, st);

@@ -244,12 +244,15 @@ def _model_device(model):
     return p.device if p is not None else _device()
 
 
-def _load(model, path):
+def _load(model, path, mxfp4=False):
     if path:
         model.load_state_dict(torch.load(path, map_location="cpu", weights_only=True), strict=True)
     model.eval()
     for p in model.parameters():
         p.requires_grad_(False)
+    if mxfp4:
+        from .util_converse import use_mxfp4
+        use_mxfp4(model)
     return model.to(_device())
 
 
@@ -317,6 +320,8 @@ def main(argv=None):
     ap.add_argument("--sf", type=int, default=None, help="scale factor (srresnet: 4, usrnet: 1)")
     ap.add_argument("--kernel", default=None, help="usrnet: blur kernel (.npy)")
     ap.add_argument("--results", default=None, help="folder for the estimated images")
+    ap.add_argument("--mxfp4", action="store_true",
+                    help="run the blocks' 1x1 convolutions in microscaled 4-bit floating point")
     args = ap.parse_args(argv)
     paths = get_image_paths(args.testset)
     if not paths:
@@ -326,7 +331,7 @@ def main(argv=None):
     if args.task == "dncnn":
         from .converse_dncnn import ConverseDnCNN
         model = _load(ConverseDnCNN(in_channels=1, kernel_size=7, num_features=64, padding=6,
-                                    padding_mode="circular"), args.model_path)
+                                    padding_mode="circular"), args.model_path, args.mxfp4)
         res = eval_dncnn(paths, model, 25 if args.noise_level is None else args.noise_level, args.results)
         for name, psnr, ssim in res:
             print(f"{name} - PSNR: {psnr:.2f} dB; SSIM: {ssim:.4f}.")
@@ -336,7 +341,7 @@ def main(argv=None):
         from .converse_srresnet import ConverseMSRResNet
         sf = args.sf or 4
         model = _load(ConverseMSRResNet(in_channels=3, out_channels=3, num_features=64, num_blocks=16, upscale=sf),
-                      args.model_path)
+                      args.model_path, args.mxfp4)
         res = eval_srresnet(paths, model, sf, args.results)
         for name, psnr, ssim, psnr_y, ssim_y in res:
             print(f"{name} - PSNR: {psnr:.2f} dB; SSIM: {ssim:.4f}; PSNR_Y: {psnr_y:.2f} dB; SSIM_Y: {ssim_y:.4f}.")
@@ -350,7 +355,7 @@ def main(argv=None):
             raise SystemExit("usrnet needs --kernel (a blur kernel .npy, e.g. blur_kernels/kernel_1.npy)")
         kernel = np.load(args.kernel, allow_pickle=False)
         sf = args.sf or 1
-        model = _load(ConverseNet(num_iterations=5, in_channels=64, num_blocks=7), args.model_path)
+        model = _load(ConverseNet(num_iterations=5, in_channels=64, num_blocks=7), args.model_path, args.mxfp4)
         res = eval_usrnet(paths, model, kernel, sf, 2.55 if args.noise_level is None else args.noise_level,
                           args.results)
         for name, psnr in res:

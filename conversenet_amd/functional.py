@@ -1400,12 +1400,40 @@ def _mx_backward(ctx, gy):
 _mx_backward_once = torch.autograd.function.once_differentiable(_mx_backward)
 
 
+_RECORDING = "conversenet_amd.recording"
+
+
+def _accumulator(leaf):
+    """The node that a leaf's gradients end in: the one that lives, or a new one."""
+    return leaf.view_as(leaf).grad_fn.next_functions[0][0]
+
+
+def _own_leaves(leaves, stream):
+    """Refuses a recording whose leaves are part of a graph from outside of it: such a leaf's node lives on the stream that it
+    was made on, the recorded backward would make that stream wait for the recording, and the recording's end would end the
+    process."""
+    for t in leaves:
+        if _accumulator(t).metadata.get(_RECORDING) == stream:
+            continue
+        _accumulator(t).metadata[_RECORDING] = None
+        if _RECORDING in _accumulator(t).metadata:  # (a node made here would be gone)
+            raise RuntimeError("a training pass cannot be recorded while a graph made before holds one of its leaves: let go of "
+                               "that graph's outputs first")
+
+
 def conv1x1_mxfp4_train(x, weight, bias=None):
     """Differentiable conv1x1_mxfp4 of a float map (B,C,*) and matrix (N,C) or (N,C,1,1), both quantised in the call: the
     gradients pass the quantisation unchanged, those of x and weight are products with the other's 4-bit values.  (Not
-    differentiable twice.)"""
+    differentiable twice.  Recorded into a graph, its leaves are in no graph that lives from before.)"""
     if isinstance(x, MXFP4) or isinstance(weight, MXFP4):
         raise RuntimeError("conv1x1_mxfp4_train quantises x and weight itself")
+    if x.is_cuda and torch.is_grad_enabled() and _capturing(stream := _stream(x.device)):
+        leaves = [t for t in (x, weight, bias) if t is not None and t.requires_grad and t.is_leaf]
+        _own_leaves(leaves, stream)
+        y = Conv1x1MXFP4Function.apply(x, weight, bias)
+        for t in leaves:
+            _accumulator(t).metadata[_RECORDING] = stream
+        return y
     return Conv1x1MXFP4Function.apply(x, weight, bias)
 
 

@@ -14,7 +14,8 @@ Dispatch (mirrors the reference's backend selection, util_converse.py:150-169):
 A forward that autograd must differentiate runs the library's forward and backward kernels
 (functional.Converse2DFunction) where the backward supports the configuration, and the composition
 otherwise.  So do channels-first LayerNorms and the blocks' scaled residuals (functional.residual_norm_train, each
-residual fused with the norm behind it); the 1x1 kernels are forward-only (torch's convolutions run under autograd).
+residual fused with the norm behind it); the 1x1 kernels are forward-only (torch's convolutions run under autograd), but for
+Conv1x1MXFP4's.
 """
 from __future__ import annotations
 
@@ -251,6 +252,64 @@ class Converse2D(nn.Module):
 
 """
 # --------------------------------------------
+# 1x1 convolutions in microscaled 4-bit floating point
+# --------------------------------------------
+"""
+
+
+def _mxfp4_eligible(x, *params) -> bool:
+    """True when an MXFP4 convolution runs on the library's kernels: HIP tensors of its types, and no transform, tracer or mode
+    that looks into torch's operations (those see the composition)."""
+    ts = [t for t in (x, *params) if t is not None]
+    if not all(t.is_cuda and t.dtype in _lib.TYPES for t in ts) or type(x) not in _TENSORS:
+        return False
+    if torch._C._are_functorch_transforms_active() or fwAD._current_level >= 0 or torch.compiler.is_compiling() \
+            or torch.jit.is_tracing() or functional.observed():
+        return False
+    _lib.load()
+    return True
+
+
+class Conv1x1MXFP4(nn.Conv2d):
+    """nn.Conv2d(in_channels, out_channels, 1) whose product runs on MXFP4 values of its input and weight, quantised in every
+    call; gradients pass the quantisation unchanged.  The parameters stay as they are, with nn.Conv2d's names."""
+
+    def __init__(self, in_channels, out_channels, bias=True, device=None, dtype=None):
+        super().__init__(in_channels, out_channels, 1, bias=bias, device=device, dtype=dtype)
+
+    @classmethod
+    def of(cls, conv):
+        """An MXFP4 convolution with a 1x1 nn.Conv2d's parameters (the same tensors)."""
+        if conv.kernel_size != (1, 1) or conv.stride != (1, 1) or conv.padding != (0, 0) or conv.groups != 1:
+            raise ValueError("not a 1x1 convolution")
+        new = cls(conv.in_channels, conv.out_channels, conv.bias is not None, device="meta")
+        new.weight, new.bias = conv.weight, conv.bias
+        new.train(conv.training)
+        return new
+
+    def forward(self, x):
+        if not _mxfp4_eligible(x, self.weight, self.bias) or x.dim() != 4:
+            return composite.conv1x1_mxfp4(x, self.weight, self.bias)
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad
+                                        or (self.bias is not None and self.bias.requires_grad)):
+            return functional.conv1x1_mxfp4_train(x, self.weight, self.bias)
+        return functional.conv1x1_mxfp4(x, self.weight, self.bias)
+
+
+def use_mxfp4(model):
+    """Runs the 1x1 convolutions of a model's ConverseBlocks in MXFP4, for evaluation and training: each becomes a
+    Conv1x1MXFP4 of the same parameters.  Returns the model, whose state dict stays as it was."""
+    for blk in model.modules():
+        if isinstance(blk, (ConverseBlock, ConverseBlockAlphaVariant)):
+            for seq in (blk.conv1, blk.conv2):
+                for name, m in seq.named_children():
+                    if type(m) is nn.Conv2d and m.kernel_size == (1, 1):
+                        setattr(seq, name, Conv1x1MXFP4.of(m))
+    return model
+
+
+"""
+# --------------------------------------------
 # Converse Blocks
 # --------------------------------------------
 """
@@ -261,6 +320,8 @@ def _block_parts(blk):
     outside the instantiated HIP tiles."""
     ln1, c11, _, cv, _, c15 = blk.conv1
     ln2, c21, _, c23 = blk.conv2
+    if any(isinstance(c, Conv1x1MXFP4) for c in (c11, c15, c21, c23)):
+        return None
     C = c11.in_channels
     mid = c11.out_channels
     if (C, mid) not in MFMA_SHAPES or (mid, C) not in MFMA_SHAPES or (C, c21.out_channels) not in MLP_SHAPES:
@@ -328,12 +389,34 @@ def _parts_supported(parts, x):
 def _fused_block_forward(blk, x, alpha1=None, alpha2=None):
     """LN+1x1+GELU -> Converse2D+GELU -> 1x1+residual and the LN-MLP branch + residual.
     Returns None when a shape is outside the instantiated HIP tiles or the library's limits."""
+    if _all_mxfp4(blk):
+        return _mxfp4_block_forward(blk, x, alpha1, alpha2)
     parts = _block_parts(blk)
     if parts is None or not _parts_supported(parts, x):
         return None
     t = _block_head(parts, x)
     gin = _gelu_in_tail(parts, t.shape, x)
     return _block_tail(parts, _block_converse(parts, t, None if gin else "gelu"), x, t_act="gelu" if gin else None)[0]
+
+
+def _all_mxfp4(blk) -> bool:
+    return len(blk.conv1) == 6 and len(blk.conv2) == 4 and all(
+        type(m) is Conv1x1MXFP4 for m in (blk.conv1[1], blk.conv1[5], blk.conv2[1], blk.conv2[3]))
+
+
+def _mxfp4_block_forward(blk, x, alpha1, alpha2):
+    """A block whose 1x1 convolutions run in MXFP4: their GELUs and residuals are part of the products."""
+    cv = blk.conv1[3]
+    if not isinstance(cv, Converse2D) or _backend(cv.backend) == "pytorch" or not _mxfp4_eligible(x) or not functional.supported(
+            None, cv.weight, cv.scale, cv.padding, shape=(x.shape[0], cv.in_channels, x.shape[2], x.shape[3])):
+        return None
+    f = functional.conv1x1_mxfp4
+    for seq, alpha in ((blk.conv1, alpha1), (blk.conv2, alpha2)):
+        t = f(seq[0](x), seq[1].weight, seq[1].bias, act="gelu")
+        if seq is blk.conv1:
+            t = cv(t, act="gelu")
+        x = f(t, seq[-1].weight, seq[-1].bias, residual=x, res_scale=alpha)
+    return x
 
 
 def _trainable(blk, x) -> bool:

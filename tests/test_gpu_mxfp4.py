@@ -7,6 +7,7 @@ more than the sum M of the terms' magnitudes (the matrix units align 128 terms t
 2^-24 of it: twice that).  With the bias, |error| <= (K + 2) 2^-23 M.  GELU's slope is below 1.13 and its own error below 4e-7
 max(1, |v|).  A gradient's sum of T terms rounds T times in the worst order, and where its float32 operand is taken in parts,
 the smallest of them may lose 2^-24 of it: (T + 2) 2^-24 M.  Each result is rounded once more: eps / 2 of its type."""
+import copy
 import threading
 
 import numpy as np
@@ -149,7 +150,8 @@ def test_conv1x1(case, dtype):
     residual = torch.randn((B, N, *space), generator=g).to(dtype).cuda()
     xq, wq = O.rounded(flat(x)), O.rounded(np64(w)[:, :, None])[:, :, 0]
     K = (C + 31) // 32
-    for b, act, r, rs in ((None, None, None, None), (bias, "gelu", None, None), (bias, None, residual, s), (bias, "gelu", residual, None)):
+    for b, act, r, rs in ((None, None, None, None), (bias, "gelu", None, None), (bias, None, residual, s),
+                          (bias, "gelu", residual, None)):
         want, mag = O.conv1x1(xq, wq, None if b is None else np64(b), act, None if r is None else flat(r),
                               None if rs is None else np64(rs))
         lim = limits(K, mag, want, act, rs, r, dtype)
@@ -193,7 +195,8 @@ def test_conv1x1_layouts_and_outputs():
     F.conv1x1_mxfp4(x, w, out=inner)
     assert torch.equal(inner, ref) and (guard[:32] == 3).all() and (guard[-32:] == 3).all()
     for t in (F16, BF16):  # parameters of other types
-        assert torch.equal(F.conv1x1_mxfp4(x, w, torch.ones(50, dtype=t, device="cuda")), F.conv1x1_mxfp4(x, w, torch.ones(50, device="cuda")))
+        assert torch.equal(F.conv1x1_mxfp4(x, w, torch.ones(50, dtype=t, device="cuda")),
+                           F.conv1x1_mxfp4(x, w, torch.ones(50, device="cuda")))
 
 
 def test_nothing_to_do():
@@ -211,8 +214,8 @@ def test_nothing_to_do():
         assert gx.shape == x.shape and (gw == 0).all() and (gb == 0).all()
 
 
-TRAINS = [(1, 1, 1, (1, 1)), (1, 16, 64, (1, 1)), (3, 50, 100, (1, 1)), (37, 33, 65, ()), (2, 128, 64, (16, 16)), (2, 64, 128, (8, 33)),
-          (1, 3, 7, (67, 45)), (3, 80, 48, (13, 7)), (1, 100, 31, (13,)), (2, 260, 257, (9, 9)), (3, 17, 33, (2, 1)),
+TRAINS = [(1, 1, 1, (1, 1)), (1, 16, 64, (1, 1)), (3, 50, 100, (1, 1)), (37, 33, 65, ()), (2, 128, 64, (16, 16)),
+          (2, 64, 128, (8, 33)), (1, 3, 7, (67, 45)), (3, 80, 48, (13, 7)), (1, 100, 31, (13,)), (2, 260, 257, (9, 9)), (3, 17, 33, (2, 1)),
           (1, 300, 512, (32, 20)), (4, 130, 96, (20, 12)), (1, 64, 64, (129, 131)), (300, 5, 40, (1, 1)), (2, 257, 40, (3, 5, 2))]
 
 
@@ -422,3 +425,110 @@ def test_refusals():
         F.conv1x1_mxfp4(x, w, residual=buf[:108].view(2, 6, 3, 3), out=buf[8:116].view(2, 6, 3, 3))
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda t: F.conv1x1_mxfp4(t, wm), x)
+
+
+def block(cls, C=64, k=5, seed=0):
+    from conversenet_amd import util_converse as U
+    torch.manual_seed(seed)
+    blk = getattr(U, cls)(C, C, kernel_size=k, padding=2, padding_mode="circular")
+    if cls != "ConverseBlock":
+        torch.nn.init.normal_(blk.alpha1), torch.nn.init.normal_(blk.alpha2)
+    return U.use_mxfp4(blk).cuda()
+
+
+@pytest.mark.parametrize("cls", ["ConverseBlock", "ConverseBlockAlphaVariant"])
+@pytest.mark.parametrize("C,shape", [(64, (2, 64, 24, 20)), (24, (1, 24, 13, 9))])
+def test_block_of_mxfp4_convolutions(cls, C, shape):
+    """Quantisation, products with GELU and residuals, norms and the Converse2D of a block, as its forward runs them."""
+    F = fh()
+    blk = block(cls, C)
+    x = make(shape, F32, 31).cuda()
+    with torch.no_grad():
+        y = blk(x)
+        t = x
+        for seq, alpha in ((blk.conv1, getattr(blk, "alpha1", None)), (blk.conv2, getattr(blk, "alpha2", None))):
+            v = F.conv1x1_mxfp4(seq[0](t), F.quantize_mxfp4(seq[1].weight), seq[1].bias, act="gelu")
+            if seq is blk.conv1:
+                v = seq[3](v, act="gelu")
+            t = F.conv1x1_mxfp4(v, F.quantize_mxfp4(seq[-1].weight), seq[-1].bias, residual=t, res_scale=alpha)
+    assert torch.equal(y, t)
+    from conversenet_amd.util_converse import run_blocks
+    with torch.no_grad():
+        assert torch.equal(run_blocks([blk, blk], x), blk(blk(x)))
+
+
+def test_training_step_of_mxfp4_blocks():
+    """Forward, gradients, clipping and an update of two blocks, each gradient against the chain of functions."""
+    F = fh()
+    blks = torch.nn.Sequential(block("ConverseBlockAlphaVariant", seed=1), block("ConverseBlockAlphaVariant", seed=2))
+    x = make((2, 64, 16, 18), F32, 32).cuda()
+    opt = torch.optim.SGD(blks.parameters(), lr=1e-3)
+
+    def convs(h, seq):
+        for m in list(seq)[1:]:
+            h = F.conv1x1_mxfp4_train(h, m.weight, m.bias) if isinstance(m, torch.nn.Conv2d) else m(h)
+        return h
+
+    def chain(v):
+        for b in blks:
+            n1, n2 = b.conv1[0], b.conv2[0]
+            h = convs(F.layernorm_cf_train(v, n1.weight, n1.bias, n1.eps, copy=True), b.conv1)
+            v, h = F.residual_norm_train(v, h, (n2.weight, n2.bias, n2.eps), b.alpha1)
+            v, _ = F.residual_norm_train(v, convs(h, b.conv2), None, b.alpha2)
+        return v
+
+    for _ in range(2):
+        want = torch.autograd.grad(chain(x).square().mean(), list(blks.parameters()))
+        opt.zero_grad()
+        blks(x).square().mean().backward()
+        assert all(torch.equal(p.grad, w) and torch.isfinite(w).all() for p, w in zip(blks.parameters(), want))
+        F.clip_grad_norm_(blks.parameters(), 1.0)
+        opt.step()
+    assert torch.isfinite(blks(x)).all()
+
+
+def test_recording_beside_an_eager_graph_is_refused():
+    """A training pass is not recorded while an eager graph of the same leaves lives, and is once that is gone."""
+    F = fh()
+    x, w = make((2, 64, 12, 12), F32, 33).cuda().requires_grad_(True), make((32, 64), F32, 34).cuda().requires_grad_(True)
+    gy = torch.randn(2, 32, 12, 12, device="cuda")
+    alive = F.conv1x1_mxfp4_train(x, w)
+    gx = torch.zeros_like(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        gx.add_(1)
+        for leaf in (x, w):
+            with pytest.raises(RuntimeError, match="holds one of its leaves"):
+                F.conv1x1_mxfp4_train(x if leaf is x else x.detach(), w if leaf is w else w.detach())
+        with torch.no_grad():
+            F.conv1x1_mxfp4_train(x, w)
+    want = torch.autograd.grad(alive, (x, w), gy)
+    del alive, g
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = F.conv1x1_mxfp4_train(x, w)
+        z = F.conv1x1_mxfp4_train(x, w)  # the same leaves twice in one recording
+        got = torch.autograd.grad(y, (x, w), gy), torch.autograd.grad(z, (x, w), gy)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for pair in got for a, c in zip(pair, want))
+
+
+def test_modules_under_modes_and_transforms():
+    """Tracers, transforms and observers see torch operations, hooks and other types what they asked for."""
+    from conversenet_amd.util_converse import Conv1x1MXFP4
+    conv = Conv1x1MXFP4(40, 8).cuda()
+    x = make((2, 40, 5, 6), F32, 35).cuda()
+    ref = conv(x)
+    mag = O.conv1x1(O.rounded(flat(x)), O.rounded(flat(conv.weight))[:, :, 0], np64(conv.bias))[1]
+    lim = 2 * 42 * 2.0 ** -23 * mag.max()  # both sides' sums of 41 terms
+    traced = torch.jit.trace(conv, x)
+    assert torch.allclose(traced(x), ref, rtol=0, atol=lim)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    assert torch.allclose(make_fx(lambda t: conv(t))(x)(x), ref, rtol=0, atol=lim)
+    assert torch.equal(conv(x.half()), fh().conv1x1_mxfp4(x.half(), conv.weight, conv.bias))
+    d = copy.deepcopy(conv).double()
+    assert d(x.double()).dtype is torch.float64 and torch.allclose(d(x.double()).float(), ref, rtol=0, atol=lim)
+    with torch.inference_mode():
+        assert torch.equal(conv(x), ref)

@@ -1,7 +1,13 @@
-"""The MXFP4 entry points' checks of arguments, without a device, and the oracle's own figures."""
-import numpy as np
+"""The MXFP4 entry points' checks of arguments, without a device, the modules on the CPU, and the oracle's own figures."""
+import copy
 
-from conversenet_amd import _lib
+import numpy as np
+import pytest
+import torch
+
+from conversenet_amd import _lib, composite
+from conversenet_amd import functional as F
+from conversenet_amd.util_converse import Conv1x1MXFP4, ConverseBlock, ConverseBlockAlphaVariant, use_mxfp4
 from oracle import mxfp4_oracle as O
 
 D = 256  # an address that is never used: the checks fail first
@@ -50,7 +56,8 @@ def test_arguments():
 
     assert conv(B=0) == _lib.CVN_OK
     for bad in (dict(x=None), dict(wc=None), dict(ws=None), dict(y=None), dict(act=2), dict(type=3), dict(N=0), dict(C=0),
-                dict(xc=D << 12), dict(x=None, xc=D << 12), dict(wc=(D << 20) + 4), dict(y=D), dict(y=D + 1020), dict(y=(D << 20) + 16),
+                dict(xc=D << 12), dict(x=None, xc=D << 12), dict(wc=(D << 20) + 4), dict(y=D), dict(y=D + 1020),
+                dict(y=(D << 20) + 16),
                 dict(res=(D << 30) + 4), dict(wc=None, ws=None), dict(w=D << 28, wt=3), dict(w=D << 28, wc=D << 28),
                 dict(w=D << 28, wc=D, ws=D << 24), dict(xc=D << 12, xs=D << 12), dict(xc=D << 20, xs=D << 13)):
         assert conv(**bad) == A, bad
@@ -69,3 +76,101 @@ def test_arguments():
                 dict(HW=-1), dict(wc=(D << 22) + 8), dict(xc=(D << 20) + 1)):
         assert bwd(**bad) == A, bad
     assert bwd(C=65537) == bwd(N=65537) == bwd(B=1 << 16, HW=1 << 16) == U
+
+
+def test_device_tensors_are_needed():
+    x, w = torch.zeros(1, 32, 2, 2), torch.zeros(4, 32)
+    q = F.MXFP4(torch.zeros(1, 2, 2, 16, dtype=torch.uint8), torch.zeros(1, 2, 2, 1, dtype=torch.uint8), 32)
+    assert q.shape == (1, 32, 2, 2)
+    for call in (lambda: F.quantize_mxfp4(x), lambda: F.dequantize_mxfp4(q), lambda: F.conv1x1_mxfp4(x, w),
+                 lambda: F.conv1x1_mxfp4(q, w), lambda: F.conv1x1_mxfp4_train(x.requires_grad_(), w),
+                 lambda: F.conv1x1_mxfp4_backward(x, q, None)):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(2, 70, 3, 5), (4, 32), (1, 1, 1), (3, 100, 2)])
+def test_composite_values(shape, dtype):
+    g = torch.Generator().manual_seed(len(shape))
+    x = (torch.randn(shape, generator=g) * 10 ** torch.randn(shape, generator=g)).to(dtype)
+    flat = x.double().numpy().reshape(shape[0], shape[1], -1)
+    got = composite.mxfp4_values(x)
+    assert got.dtype is dtype and got.shape == x.shape
+    # (rounded to x's type: fp16 keeps no value below half its smallest number)
+    assert np.array_equal(got.double().numpy().reshape(flat.shape), torch.from_numpy(O.rounded(flat)).to(dtype).double().numpy())
+    x[0, 0] = float("inf")
+    assert torch.isnan(composite.mxfp4_values(x)[0, :min(32, shape[1])]).all()
+
+
+def test_convolution_on_the_cpu():
+    """Float64 as the oracle, with its gradients; parameters shared with the convolution it was made of."""
+    conv = torch.nn.Conv2d(40, 9, 1).double()
+    mx = Conv1x1MXFP4.of(conv)
+    assert mx.weight is conv.weight and mx.bias is conv.bias and list(mx.state_dict()) == list(conv.state_dict())
+    x = torch.randn(2, 40, 3, 4, dtype=torch.float64, requires_grad=True)
+    gy = torch.randn(2, 9, 3, 4, dtype=torch.float64)
+    y = mx(x)
+    grads = torch.autograd.grad(y, (x, mx.weight, mx.bias), gy)
+    n = lambda t: t.detach().numpy().reshape(t.shape[0], t.shape[1], -1)  # noqa: E731
+    xq, wq = O.rounded(n(x)), O.rounded(n(conv.weight))[:, :, 0]
+    want, mag = O.conv1x1(xq, wq, conv.bias.detach().numpy())
+    assert (np.abs(n(y) - want) <= 42 * 2.0 ** -52 * mag).all()
+    for g, (want, mag), terms in zip(grads, O.gradients(n(gy), xq, wq), (9, 24, 24)):
+        assert (np.abs(g.numpy().reshape(want.shape) - want) <= (terms + 2) * 2.0 ** -52 * mag).all()
+    for bad in (torch.nn.Conv2d(4, 4, 3), torch.nn.Conv2d(4, 4, 1, stride=2), torch.nn.Conv2d(4, 4, 1, groups=2)):
+        with pytest.raises(ValueError):
+            Conv1x1MXFP4.of(bad)
+
+
+@pytest.mark.parametrize("cls", [ConverseBlock, ConverseBlockAlphaVariant])
+def test_block_on_the_cpu(cls):
+    torch.manual_seed(0)
+    blk = cls(8, 8, kernel_size=3, padding=2, padding_mode="circular")
+    if cls is ConverseBlockAlphaVariant:
+        torch.nn.init.normal_(blk.alpha1), torch.nn.init.normal_(blk.alpha2)
+    keys, plain = list(blk.state_dict()), copy.deepcopy(blk)
+    assert use_mxfp4(blk) is blk and list(blk.state_dict()) == keys
+    kinds = [type(m) for m in (blk.conv1[1], blk.conv1[5], blk.conv2[1], blk.conv2[3])]
+    assert kinds == [Conv1x1MXFP4] * 4
+    x = torch.randn(2, 8, 6, 7)
+    y = blk(x)
+    t = x
+    for seq, alpha in ((plain.conv1, getattr(plain, "alpha1", 1)), (plain.conv2, getattr(plain, "alpha2", 1))):
+        v = t
+        for m in seq:
+            v = composite.conv1x1_mxfp4(v, m.weight, m.bias) if type(m) is torch.nn.Conv2d else m(v)
+        t = alpha * v + t
+    assert torch.equal(y, t)
+    y.square().sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in blk.parameters())
+    blk.load_state_dict(plain.state_dict(), strict=True)
+
+
+def test_evaluation_flag(tmp_path, capsys):
+    from PIL import Image
+
+    from conversenet_amd import evaluate as E
+    rng = np.random.default_rng(0)
+    Image.fromarray(rng.integers(0, 255, (16, 20), dtype=np.uint8)).save(tmp_path / "a.png")
+    lines = []
+    for flags in ([], ["--mxfp4"]):
+        torch.manual_seed(0)
+        E.main(["dncnn", "--testset", str(tmp_path), *flags])
+        lines.append(capsys.readouterr().out)
+    assert all("Average PSNR" in t for t in lines) and lines[0] != lines[1]
+
+
+def test_leaves_of_other_graphs_are_found():
+    x, w = torch.randn(3, requires_grad=True), torch.randn(3, requires_grad=True)
+    F._own_leaves([x, w], 5)
+    y = x * 2
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="holds one of its leaves"):
+            F._own_leaves([w, x], 5)
+    F._accumulator(x).metadata[F._RECORDING] = 5  # made in the recording on stream 5
+    F._own_leaves([x, w], 5)
+    with pytest.raises(RuntimeError, match="holds one of its leaves"):
+        F._own_leaves([x], 6)
+    del y
+    F._own_leaves([x, w], 6)
