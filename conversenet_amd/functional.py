@@ -1265,7 +1265,7 @@ def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None,
     b, s = _param32(keep, bias, N, index, "bias"), _param32(keep, res_scale, N, index, "res_scale")
     residual = _contiguous(residual)
     y = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
-    nbytes = lib.cvn_conv1x1_mxfp4_workspace(x is None, weight is None, B, C, HW, N)
+    nbytes = 0 if x is None and weight is None else lib.cvn_conv1x1_mxfp4_workspace(x is None, weight is None, B, C, HW, N)
     st = _stream(dev)
     work = _scratch(dev, st)
     with _on(dev), work.lock:
@@ -1309,11 +1309,17 @@ def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
     return gx, gw, gb
 
 
+@functools.lru_cache(maxsize=1024)
+def _mx_grad_workspace(B, C, HW, N):
+    """Bytes of scratch of a gradient of the matrix (the library's answer depends on nothing else)."""
+    return _lib.load().cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N)
+
+
 def _mx_grads(gy, xc, xs, wc, ws, B, C, HW, N, gx, gw, gb):
     """The launches behind conv1x1_mxfp4's gradients."""
     lib = _lib.load()
     dev = gy.device
-    nbytes = lib.cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N) if gw is not None else 0
+    nbytes = _mx_grad_workspace(B, C, HW, N) if gw is not None else 0
     st = _stream(dev)
     work = _scratch(dev, st)
     with _on(dev), work.lock:
@@ -1322,6 +1328,7 @@ def _mx_grads(gy, xc, xs, wc, ws, B, C, HW, N, gx, gw, gb):
     _lib.check(rc, "conv1x1_mxfp4_backward")
 
 
+@functools.lru_cache(maxsize=1024)
 def _mx_layout(rows, C, N, keep_x, keep_w):
     """Where a forward keeps its operands in one buffer: (codes and scales of x, of the matrix, bytes), None for what is
     not kept."""
@@ -1355,7 +1362,7 @@ class Conv1x1MXFP4Function(torch.autograd.Function):
         base = 0 if kept is None else kept.data_ptr()
         xc, xs, wc, ws = (None if o is None or not base else base + o for o in where[:4])
         y = torch.empty((B, N, *x.shape[2:]), dtype=dtype, device=dev)
-        nbytes = lib.cvn_conv1x1_mxfp4_workspace(xc is not None, wc is not None, B, C, HW, N)
+        nbytes = 0 if nx and nw else lib.cvn_conv1x1_mxfp4_workspace(xc is not None, wc is not None, B, C, HW, N)
         st = _stream(dev)
         work = _scratch(dev, st)
         with _on(dev), work.lock:
