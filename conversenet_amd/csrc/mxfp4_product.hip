@@ -47,10 +47,23 @@ __device__ __forceinline__ MxGroup mx_group(int64_t r0, int64_t HW, int64_t rows
 template <int V, int R>
 __device__ __forceinline__ void mx_finish(const MxOut& o, float (*v)[V], const float (*scale)[V]) {
   if (o.act == CVN_ACT_GELU) {
+    float top = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[r][e] = gelu_fast(v[r][e]);
+      for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(v[r][e]));
+    if (top == __builtin_inff()) {  // (gelu_fast makes 0 times infinity of it)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          v[r][e] = fabsf(v[r][e]) == __builtin_inff() ? fmaxf(v[r][e], 0.f) : gelu_fast(v[r][e]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[r][e] = gelu_fast(v[r][e]);
+    }
   }
   if (o.res_scale) {
 #pragma unroll
@@ -445,6 +458,27 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
 // products of pixels 2 j and 2 j + 1 give it two neighbouring pixels of a channel again.  (Four pixels a lane: 128 x 256 x 256
 // x 8 float32 to 64 90 us, two 77, half the registers.)  blockIdx.y takes a share of the channels where there are too few
 // pixels for the CUs.
+// A parameter's values at the 16 rows of a lane's part of a result: element e of it is row 8 (e / 4) + 4 h + e % 4.
+__device__ __forceinline__ mx_f32x16 mx_channels(const float* p, int64_t n0, int h, int64_t N, float none) {
+  mx_f32x16 v;
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = none;
+  } else if (n0 + 32 <= N) {
+    typedef MxVec<float, 4>::type W;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const W w = *(const W*)(p + n0 + 8 * i + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = w[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = p[min((uint32_t)n0 + 8 * (e / 4) + 4 * h + e % 4, (uint32_t)N - 1)];
+  }
+  return v;
+}
+
 template <class T, bool NT, int S>
 __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share) {
   constexpr int V = 2;
@@ -516,14 +550,8 @@ __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share)
   const int64_t n1 = min(o.N, (int64_t)(blockIdx.y + 1) * share);
   for (int64_t n0 = (int64_t)blockIdx.y * share; n0 < n1; n0 += 32) {
     const int64_t wrow = min(n0 + j, o.N - 1) * in.KB;
-    // the sums begin with the bias of their rows: element e of a result is its row 8 (e / 4) + 4 h + e % 4
-    mx_f32x16 acc[V], ss;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint32_t n = min((uint32_t)n0 + 8 * (e / 4) + 4 * h + e % 4, (uint32_t)o.N - 1);
-      acc[0][e] = o.bias ? o.bias[n] : 0.f;
-      ss[e] = o.res_scale ? o.res_scale[n] : 1.f;
-    }
+    mx_f32x16 acc[V];
+    acc[0] = mx_channels(o.bias, n0, h, o.N, 0.f);  // the sums begin with the bias of their rows
 #pragma unroll
     for (int e = 1; e < V; ++e) acc[e] = acc[0];
 #pragma unroll
@@ -538,6 +566,7 @@ __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share)
                                                                (int)sx[s]);
     }
     if (r0 >= o.rows) continue;
+    const mx_f32x16 ss = mx_channels(o.res_scale, n0, h, o.N, 1.f);
     MxPixels<V> px = pix;
 #pragma unroll
     for (int e = 0; e < V; ++e) asm volatile("" : "+v"(px.at[e]));  // (each row's address is made where it is used: kept
@@ -650,9 +679,11 @@ extern "C" int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, i
              {x ? nullptr : x_scales, rows * KB},
              {w ? nullptr : w_codes, N * KB * 16},
              {w ? nullptr : w_scales, N * KB},
-             {residual == y ? nullptr : residual, rows * N * es}};
+             {residual == y ? nullptr : residual, rows * N * es},
+             {bias, N * 4},
+             {res_scale, N * 4}};
   for (int i = 0; i < 5; ++i)
-    for (int k = i + 1; k < 12; ++k)
+    for (int k = i + 1; k < 14; ++k)
       if (mx_overlap(mem[i].p, mem[i].n, mem[k].p, mem[k].n))
         return fail(CVN_ERR_ARG, "an output shares memory with an input or another output");
   const bool keep = x_codes != nullptr;

@@ -1147,6 +1147,14 @@ class MXFP4(NamedTuple):
         return (self.codes.shape[0], self.channels, *self.codes.shape[1:-1])
 
 
+def _values(t):
+    """A contiguous tensor of t's values as stored (None for None): a view of an imaginary part may hold their negatives."""
+    if t is None:
+        return None
+    t = t if t.is_contiguous() else t.contiguous()
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _mx_parts(q, what):
     """((B, C, pixels), codes, scales) of an MXFP4 argument, contiguous and aligned."""
     codes, scales, C = q
@@ -1187,7 +1195,7 @@ def quantize_mxfp4(x):
     _untraced("quantize_mxfp4")
     B, C, HW = _mx_map(x, "quantize_mxfp4")
     lib = _lib.load()
-    x = _contiguous(x)
+    x = _values(x)
     codes, scales = _mx_empty(x, C)
     with _on(x.device):
         rc = lib.cvn_mxfp4_quantize(x.data_ptr(), _lib.TYPES[x.dtype], B, C, HW, codes.data_ptr(), scales.data_ptr(),
@@ -1244,7 +1252,7 @@ def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None,
         B, C, HW = _mx_map(x, "conv1x1_mxfp4")
         if dtype not in (None, x.dtype):
             raise RuntimeError("the result has the type of x")
-        x = _contiguous(x)
+        x = _values(x)
         dev, space, dtype = x.device, x.shape[2:], x.dtype
     index = dev.index
     if isinstance(weight, MXFP4):
@@ -1254,16 +1262,16 @@ def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None,
             raise RuntimeError("weight does not match input channels")
     else:
         N = _mx_weight(weight, C, index)
-        weight = _contiguous(weight)
+        weight = _values(weight)
     shape = (B, N, *space)
     for t, what in ((residual, "residual"), (out, "out")):
         if t is not None and (tuple(t.shape) != shape or t.dtype is not dtype or t.get_device() != index):
             raise RuntimeError(f"{what} must have the result's shape and type")
-    if out is not None and not out.is_contiguous():
-        raise RuntimeError("out must be contiguous")
+    if out is not None and (not out.is_contiguous() or out.is_neg()):
+        raise RuntimeError("out must be contiguous, and no negated view")
     keep = []
     b, s = _param32(keep, bias, N, index, "bias"), _param32(keep, res_scale, N, index, "res_scale")
-    residual = _contiguous(residual)
+    residual = _values(residual)
     y = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
     nbytes = 0 if x is None and weight is None else lib.cvn_conv1x1_mxfp4_workspace(x is None, weight is None, B, C, HW, N)
     st = _stream(dev)
@@ -1300,7 +1308,7 @@ def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
         if wN != N or one != 1 or (xc is not None and wC != C) or wc.get_device() != index:
             raise RuntimeError("weight does not match the gradient")
         C = wC
-    gy = _contiguous(grad_y)
+    gy = _values(grad_y)
     dev = gy.device
     gx = torch.empty((B, C, *gy.shape[2:]), dtype=gy.dtype, device=dev) if nx else None
     gw = torch.empty((N, C), dtype=torch.float32, device=dev) if nw else None
@@ -1353,7 +1361,7 @@ class Conv1x1MXFP4Function(torch.autograd.Function):
         dev, dtype = x.device, x.dtype
         index = dev.index
         N = _mx_weight(weight, C, index)
-        x, w = _contiguous(x), _contiguous(weight)
+        x, w = _values(x), _values(weight)
         keep = []
         b = _param32(keep, bias, N, index, "bias")
         nx, nw = ctx.needs_input_grad[:2]
@@ -1385,7 +1393,7 @@ def _mx_backward(ctx, gy):
     nx, nw, nb = ctx.needs_input_grad
     if not _in_memory(gy) or not _in_memory(kept):
         raise RuntimeError("conv1x1_mxfp4's gradients are of plain tensors")
-    gy, kept = _contiguous(gy), _contiguous(kept)
+    gy, kept = _values(gy), _contiguous(kept)
     dev = gy.device
     B, C, N, HW = x_shape[0], x_shape[1], w_shape[0], math.prod(x_shape[2:])
     base = 0 if kept is None else kept.data_ptr()

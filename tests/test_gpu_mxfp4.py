@@ -199,6 +199,38 @@ def test_conv1x1_layouts_and_outputs():
                            F.conv1x1_mxfp4(x, w, torch.ones(50, device="cuda")))
 
 
+@pytest.mark.parametrize("shape", [(2, 70, 3, 5), (1, 70), (40, 300)])
+def test_infinite_sums(shape):
+    """GELU of an infinity is that infinity or zero, of a NaN a NaN, beside numbers that stay as they are."""
+    F = fh()
+    x, w = make(shape, F32, 36).cuda(), make((9, shape[1]), F32, 37).cuda()
+    bias = torch.zeros(9, device="cuda")
+    ref = F.conv1x1_mxfp4(x, w, bias, act="gelu")
+    bias[2], bias[5], bias[7] = float("inf"), -float("inf"), float("nan")
+    y = F.conv1x1_mxfp4(x, w, bias, act="gelu")
+    assert (y[:, 2] == float("inf")).all() and (y[:, 5] == 0).all() and torch.isnan(y[:, 7]).all()
+    keep = [0, 1, 3, 4, 6, 8]
+    assert torch.equal(y[:, keep], ref[:, keep])
+
+
+def test_negated_views():
+    F = fh()
+    for shape in ((2, 40, 3, 3), (1, 1, 1, 1)):
+        z = torch.randn(shape, dtype=torch.complex64, device="cuda")
+        x = z.conj().imag
+        assert x.is_neg()
+        plain = x.resolve_neg().clone()
+        w = torch.randn(6, shape[1], device="cuda")
+        assert torch.equal(F.dequantize_mxfp4(F.quantize_mxfp4(x)), F.dequantize_mxfp4(F.quantize_mxfp4(plain)))
+        res = torch.randn((shape[0], 6) + shape[2:], dtype=torch.complex64, device="cuda").conj().imag
+        assert torch.equal(F.conv1x1_mxfp4(x, w, residual=res), F.conv1x1_mxfp4(plain, w, residual=res.resolve_neg().clone()))
+        lx, lw = plain.requires_grad_(True), w.requires_grad_(True)
+        gy = torch.randn((shape[0], 6) + shape[2:], dtype=torch.complex64, device="cuda").conj().imag
+        y = F.conv1x1_mxfp4_train(lx, lw)
+        got = torch.autograd.grad(y, (lx, lw), gy, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(y, (lx, lw), gy.resolve_neg().clone())))
+
+
 def test_nothing_to_do():
     F = fh()
     w = make((5, 40), F32, 8).cuda()
@@ -423,6 +455,8 @@ def test_refusals():
             F.conv1x1_mxfp4(xb, w, out=buf[lo:lo + 108].view(2, 6, 3, 3))
     with pytest.raises(RuntimeError, match="shares memory"):
         F.conv1x1_mxfp4(x, w, residual=buf[:108].view(2, 6, 3, 3), out=buf[8:116].view(2, 6, 3, 3))
+    with pytest.raises(RuntimeError, match="shares memory"):
+        F.conv1x1_mxfp4(x, w, buf[100:106], out=buf[:108].view(2, 6, 3, 3))
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda t: F.conv1x1_mxfp4(t, wm), x)
 
@@ -527,6 +561,7 @@ def test_modules_under_modes_and_transforms():
     assert torch.allclose(traced(x), ref, rtol=0, atol=lim)
     from torch.fx.experimental.proxy_tensor import make_fx
     assert torch.allclose(make_fx(lambda t: conv(t))(x)(x), ref, rtol=0, atol=lim)
+    assert torch.equal(conv(x[0]), conv(x[:1])[0])
     assert torch.equal(conv(x.half()), fh().conv1x1_mxfp4(x.half(), conv.weight, conv.bias))
     d = copy.deepcopy(conv).double()
     assert d(x.double()).dtype is torch.float64 and torch.allclose(d(x.double()).float(), ref, rtol=0, atol=lim)

@@ -118,6 +118,7 @@ def test_convolution_on_the_cpu():
     assert (np.abs(n(y) - want) <= 42 * 2.0 ** -52 * mag).all()
     for g, (want, mag), terms in zip(grads, O.gradients(n(gy), xq, wq), (9, 24, 24)):
         assert (np.abs(g.numpy().reshape(want.shape) - want) <= (terms + 2) * 2.0 ** -52 * mag).all()
+    assert torch.equal(mx(x[0]), mx(x[:1])[0])
     for bad in (torch.nn.Conv2d(4, 4, 3), torch.nn.Conv2d(4, 4, 1, stride=2), torch.nn.Conv2d(4, 4, 1, groups=2)):
         with pytest.raises(ValueError):
             Conv1x1MXFP4.of(bad)
