@@ -323,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
 }
 
 // The sum over the splits, in the same order on every call: R threads an element take every R-th of them.  (One thread an
-// element leaves few to wait for long chains of loads: 288 splits of 8192 elements take 134 us that way, 8 threads 4; 8
-// splits of a million elements take 9 and 16.)
+// element leaves few to wait for long chains of loads: 288 splits of 8192 elements take 134 us that way, 8 threads an element
+// 11.6, 16 threads 7.4; 8 splits of a million elements take 9 with one thread, 16 with eight.)
 template <int R>
 __global__ void __launch_bounds__(kThreads) k_mx_grad_join(const float* __restrict__ part, int64_t n,
                                                            const double* __restrict__ gbp, int64_t nb, int splits,
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_grad_join(const float* __restri
   const int64_t i = ((int64_t)blockIdx.x - (bias ? blocks : 0)) * kCols + col, end = bias ? nb : n;
   double s = 0.;
   if (i < end) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = row; k < splits; k += R) s += bias ? gbp[k * nb + i] : (double)part[k * n + i];
   }
   if (R > 1) {
@@ -432,7 +432,7 @@ int grads(const void* gy, const void* xc, const void* xs, const void* wc, const 
     if (s.splits > 1 || gb) {
       const int64_t n = s.splits > 1 ? N * C : 0;
       if (n >= 1 << 18) grad_join<1>(part, n, gbp, N, s.splits, gw, gb, st);
-      else grad_join<8>(part, n, gbp, N, s.splits, gw, gb, st);
+      else grad_join<16>(part, n, gbp, N, s.splits, gw, gb, st);
     }
   } else if (gb) {
     hipLaunchKernelGGL(k_mx_grad_bias<T>, dim3((unsigned)N), dim3(kThreads), 0, st, (const T*)gy, N, HW, rows, gb);

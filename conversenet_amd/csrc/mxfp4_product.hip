@@ -367,7 +367,7 @@ int gemm(const MxIn& in, const MxOut& o, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// A few pixels: a block makes 16 channels of 16 of them at a time, its waves take the channels in turn.
+// A few pixels: a block makes 16 NT channels of 16 of them at a time, its waves take the channels of the sum in turn.
 // ------------------------------------------------------------------------------------------------
 // The matrix is read once and bounds this; the pixels' codes are made on the way by every block.
 template <class T>
@@ -394,23 +394,29 @@ __device__ __forceinline__ unsigned mx_quantize_row(const T* x, int64_t step, in
 }
 
 constexpr int kFewWaves = 8, kFewRows = 16;
-template <class T>
+template <class T, int NT>
 __global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
-  __shared__ float part[kFewWaves][16][17];
+  __shared__ float part[kFewWaves][16 * NT][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, wrow = min(n0 + j, o.N - 1) * in.KB;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
   for (int64_t r0 = (int64_t)blockIdx.y * 16; r0 < o.rows; r0 += (int64_t)gridDim.y * 16) {
     const int64_t r = r0 + j;
     const bool live = r < o.rows;
     const int64_t b = live ? (uint32_t)r / (uint32_t)o.HW : 0, p = r - b * o.HW;
     const T* x = (const T*)in.x + b * in.C * o.HW + p;
-    mx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    mx_f32x4 acc[NT] = {};
     for (int k = 4 * wave; k < in.KB; k += 4 * kFewWaves) {
       // lane l holds block k + l / 16 of its operands' rows l % 16; past the last both scales are 2^-127
       const bool in_row = k + g < in.KB;
       const int kb = min(k + g, in.KB - 1);
-      const mx_i32x4 w = in.wc[wrow + kb];
-      unsigned sw = in.ws[wrow + kb], sx = 0;
+      mx_i32x4 w[NT];
+      unsigned sw[NT], sx = 0;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int64_t at = min(n0 + 16 * i + j, o.N - 1) * in.KB + kb;
+        w[i] = in.wc[at];
+        sw[i] = in.ws[at];
+      }
       mx_i32x4 q = {0, 0, 0, 0};
       if (live && in_row) {
         if (in.x) {
@@ -424,21 +430,25 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
           sx = in.xs[r * in.KB + kb];
         }
       }
-      if (!in_row) sw = 0;
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w), mx_operand(q), acc, kMxFp4, kMxFp4, 0, (int)sw, 0,
-                                                             (int)sx);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w[i]), mx_operand(q), acc[i], kMxFp4, kMxFp4, 0,
+                                                                  in_row ? (int)sw[i] : 0, 0, (int)sx);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][4 * g + e][j] = acc[e];
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave][16 * i + 4 * g + e][j] = acc[i][e];
     __syncthreads();
-    if (threadIdx.x < 256) {
+    if (threadIdx.x < 256 * NT) {
       // neighbouring threads store neighbours: channels of one pixel a sample, pixels otherwise
-      const int a = threadIdx.x & 15, c = threadIdx.x >> 4, n = o.HW == 1 ? a : c, k = o.HW == 1 ? c : a;
+      const int a = threadIdx.x & 15, c = threadIdx.x >> 4 & 15, i = threadIdx.x >> 8;
+      const int n = 16 * i + (o.HW == 1 ? a : c), k = o.HW == 1 ? c : a;
       const int64_t rk = r0 + k;
       if (rk < o.rows && n0 + n < o.N) {
         float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < kFewWaves; ++i) v += part[i][n][k];
+        for (int w = 0; w < kFewWaves; ++w) v += part[w][n][k];
         const int64_t rb = (uint32_t)rk / (uint32_t)o.HW;
         float out[1][1] = {{o.bias ? v + o.bias[n0 + n] : v}};
         const float scale[1][1] = {{o.res_scale ? o.res_scale[n0 + n] : 1.f}};
@@ -630,8 +640,14 @@ template <class T>
 int product(const MxIn& in, const MxOut& o, int type, bool keep, hipStream_t st) {
   // (the tiled kernel reads scales by words of four)
   if (o.rows <= kFewRows || o.N * in.KB < 4) {
-    hipLaunchKernelGGL(k_mx_few<T>, dim3((unsigned)((o.N + 15) / 16), (unsigned)std::min<int64_t>((o.rows + 15) / 16, 4096)),
-                       dim3(kFewWaves * 64), 0, st, in, o);
+    // Every block reads all of x: two tiles to a block from two blocks a CU on (16 float16 pixels, 2048 to 8192 channels: 7.3 us,
+    // one tile 9.0).
+    const unsigned y = (unsigned)std::min<int64_t>((o.rows + 15) / 16, 4096);
+    if (o.N >= 16 * 512) {
+      hipLaunchKernelGGL((k_mx_few<T, 2>), dim3((unsigned)((o.N + 31) / 32), y), dim3(kFewWaves * 64), 0, st, in, o);
+    } else {
+      hipLaunchKernelGGL((k_mx_few<T, 1>), dim3((unsigned)((o.N + 15) / 16), y), dim3(kFewWaves * 64), 0, st, in, o);
+    }
     return check_launch("conv1x1_mxfp4");
   }
   if (in.x && in.KB <= 8 && o.HW > 1) return conv<T>(in, o, keep, st);

@@ -136,7 +136,8 @@ CONVS = [  # B, N, C, pixels
     (1, 1, 1, (1, 1)), (1, 16, 64, (1, 1)), (3, 50, 100, (1, 1)), (16, 96, 320, (1, 1)), (17, 33, 65, (1, 1)), (70, 40, 129, ()),
     (1, 128, 64, (16, 16)), (2, 64, 128, (8, 33)), (1, 3, 7, (67, 45)), (2, 80, 48, (5, 7)), (1, 100, 31, (13,)),
     (2, 260, 257, (9, 9)), (1, 65, 1000, (12, 20)), (3, 17, 33, (2, 1)), (1, 300, 512, (32, 20)), (4, 130, 96, (20, 12)),
-    (1, 40, 4100, (3, 3)), (2, 1, 300, (4, 65)), (1, 2048, 32, (4, 4)), (1, 70, 300, (2, 3, 7)),
+    (1, 40, 4100, (3, 3)), (2, 1, 300, (4, 65)), (1, 2048, 32, (4, 4)), (1, 70, 300, (2, 3, 7)), (5, 8210, 100, (1, 1)),
+    (2, 8192, 33, (2, 3)),
 ]
 
 
