@@ -132,6 +132,9 @@ __device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V
 // ------------------------------------------------------------------------------------------------
 // Many pixels of many channels: both operands in MXFP4, tiles staged through LDS.
 // ------------------------------------------------------------------------------------------------
+// 16384 pixels, 2048 to 4096 channels: 119 us behind the quantisation, 2.3 PFLOP/s (150 us call after call, where the card's
+// clock falls; a library's 8192^3 product: 3.1 PFLOP/s), bound by the wait for each step's fetch; the matrix units are busy a fifth
+// of the time, LDS an eighth.  Another order of the tiles, two patches of the longer side, changes nothing.
 // A step takes 256 channels: 128 bytes of codes a row, which a wave fetches 8 rows at a time straight into LDS.  A row's
 // 16-byte pieces are stored in an order that depends on the row (piece ^ (row / 2 & 7)), so that 16 lanes which read the
 // same piece of neighbouring rows hit all 64 banks.  Lane l of a 32 x 32 x 64 product takes the blocks 4 (l / 32) + s of rows
@@ -369,7 +372,9 @@ int gemm(const MxIn& in, const MxOut& o, hipStream_t st) {
 // ------------------------------------------------------------------------------------------------
 // A few pixels: a block makes 16 NT channels of 16 of them at a time, its waves take the channels of the sum in turn.
 // ------------------------------------------------------------------------------------------------
-// The matrix is read once and bounds this; the pixels' codes are made on the way by every block.
+// The matrix is read once; the pixels' codes are made on the way by every block.  4096 to 4096 channels: 7.3 us, four rounds
+// of loads, quantisation and products a wave, not the 9 MB (1.7 us); four rounds' loads at once took as long, and twice as long
+// for 16 pixels, whose loads past the end cost as much as the others.
 template <class T>
 __device__ __forceinline__ unsigned mx_quantize_row(const T* x, int64_t step, int n, mx_i32x4* q) {
   float v[kMxBlock];
@@ -460,14 +465,6 @@ __global__ void __launch_bounds__(kFewWaves * 64) k_mx_few(MxIn in, MxOut o) {
   }
 }
 
-// ------------------------------------------------------------------------------------------------
-// Maps of up to 256 channels: quantised in registers, every product and the store in one pass.
-// ------------------------------------------------------------------------------------------------
-// Bound by memory.  Lane l of a wave loads the blocks 2 s + l / 32 of two neighbouring pixels (8 bytes of a float32 channel,
-// 256 in a row over 32 lanes), makes their codes, and keeps them as operands for every 32 channels of the result: the
-// products of pixels 2 j and 2 j + 1 give it two neighbouring pixels of a channel again.  (Four pixels a lane: 128 x 256 x 256
-// x 8 float32 to 64 90 us, two 77, half the registers.)  blockIdx.y takes a share of the channels where there are too few
-// pixels for the CUs.
 // A parameter's values at the 16 rows of a lane's part of a result: element e of it is row 8 (e / 4) + 4 h + e % 4.
 __device__ __forceinline__ mx_f32x16 mx_channels(const float* p, int64_t n0, int h, int64_t N, float none) {
   mx_f32x16 v;
@@ -489,6 +486,14 @@ __device__ __forceinline__ mx_f32x16 mx_channels(const float* p, int64_t n0, int
   return v;
 }
 
+// ------------------------------------------------------------------------------------------------
+// Maps of up to 256 channels: quantised in registers, every product and the store in one pass.
+// ------------------------------------------------------------------------------------------------
+// Bound by memory.  Lane l of a wave loads the blocks 2 s + l / 32 of two neighbouring pixels (8 bytes of a float32 channel,
+// 256 in a row over 32 lanes), makes their codes, and keeps them as operands for every 32 channels of the result: the
+// products of pixels 2 j and 2 j + 1 give it two neighbouring pixels of a channel again.  (Four pixels a lane: 128 x 256 x 256
+// x 8 float32 to 64 90 us, two 77, half the registers.)  blockIdx.y takes a share of the channels where there are too few
+// pixels for the CUs.
 template <class T, bool NT, int S>
 __global__ void __launch_bounds__(256, 2) k_mx_conv(MxIn in, MxOut o, int share) {
   constexpr int V = 2;
