@@ -2,7 +2,8 @@
 //   gx[b,c,p] = sum_n w[n][c] gy[b,n,p]     gw[n][c] = sum_{b,p} gy[b,n,p] x[b,p][c]     gb[n] = sum_{b,p} gy[b,n,p]
 // The 4-bit values times their scales are bfloat16 numbers, and gy is a sum of them: one (bfloat16), two (float16: 11 bits in
 // 8 + 3) or three (float32: 24 bits in 8 + 8 + 8).  So the products run on the bfloat16 matrix units, one a part, with no operand
-// rounded (parts of float32 below 2^-133 are lost), and are summed in float32.
+// rounded, and are summed in float32.  (Those units take numbers below 2^-126 for zeros: parts of gy, and 4-bit values of the
+// smallest scales.)
 #include <algorithm>
 
 #include "mxfp4.h"

@@ -1290,7 +1290,7 @@ def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None,
 def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
     """Gradients of conv1x1_mxfp4's product and bias, straight through the quantisation: (x, weight, bias), None where
     not asked for by `need`.  grad_y (B,N,*): float32, bfloat16 or float16, the type of x's gradient; the others are float32,
-    weight's (N,C).  x, weight: the MXFP4 operands of the forward (x None without weight's gradient, weight None without x's, where
+    weight's (N,C).  (Parts of an operand below 2^-126 count as zeros.)  x, weight: the MXFP4 operands of the forward (x None without weight's gradient, weight None without x's, where
     the other gives the channels)."""
     _untraced("conv1x1_mxfp4_backward")
     B, N, HW = _mx_map(grad_y, "conv1x1_mxfp4_backward")
@@ -1395,6 +1395,8 @@ def _mx_backward(ctx, gy):
         raise RuntimeError("conv1x1_mxfp4's gradients are of plain tensors")
     gy, kept = _values(gy), _contiguous(kept)
     dev = gy.device
+    if kept is not None and (kept.device != dev or kept.dtype is not torch.uint8 or kept.numel() != where[4]):
+        raise RuntimeError("a hook has changed what conv1x1_mxfp4_train kept")
     B, C, N, HW = x_shape[0], x_shape[1], w_shape[0], math.prod(x_shape[2:])
     base = 0 if kept is None else kept.data_ptr()
     if base % 16:  # (a saved-tensor hook may have moved it)

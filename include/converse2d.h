@@ -331,7 +331,8 @@ int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, i
                       cvn_stream_t stream);
 /* Gradients of the product and bias, straight through the quantisation: grad_x[b,c,p] = sum_n w[n][c] grad_y[b,n,p] of type,
  * grad_w[n][c] = sum_bp grad_y[b,n,p] x[b,p][c] and grad_bias[n] = sum_bp grad_y[b,n,p] in fp32; each may be NULL, and
- * then what only it needs.  No operand is rounded; sums are added up in the same order on every call. */
+ * then what only it needs.  No operand is rounded, but parts of one below 2^-126 count as zeros; sums are added up in the
+ * same order on every call. */
 size_t cvn_conv1x1_mxfp4_bwd_workspace(int64_t B, int64_t C, int64_t HW, int64_t N);
 int cvn_conv1x1_mxfp4_bwd(const void* grad_y, int type, const void* x_codes, const void* x_scales, const void* w_codes,
                           const void* w_scales, int64_t B, int64_t C, int64_t HW, int64_t N, void* grad_x, float* grad_w,

@@ -276,6 +276,61 @@ def test_gradients(case, dtype):
         check(g, want, (terms + 2) * 2.0 ** -24 * mag + half_step(g.dtype, want))
 
 
+@pytest.mark.parametrize("shape", [(2, 70, 5, 6), (5, 70)])
+@pytest.mark.parametrize("mag", [1e-37, 1e-30, 1e30, 1e37])
+def test_gradients_of_far_sizes(shape, mag):
+    """The matrix units take bfloat16 numbers below 2^-126 for zeros: of each term, three parts of less than that are lost.
+    Where the terms' magnitudes add up to more than float32's largest number, so may a sum on its way."""
+    F = fh()
+    x, w = make(shape, F32, 38).cuda(), make((30, 70), F32, 39).cuda()
+    gy = (mag * torch.randn((shape[0], 30) + shape[2:], generator=gen(40))).cuda()
+    xq, wq = F.quantize_mxfp4(x), F.quantize_mxfp4(w)
+    got = F.conv1x1_mxfp4_backward(gy, xq, wq)
+    xv, wv = O.rounded(flat(x)), O.rounded(np64(w)[:, :, None])[:, :, 0]
+    P = xv.shape[0] * xv.shape[2]
+    lost = (3 * 2.0 ** -126 * np.abs(wv).sum(0).max(), 3 * 2.0 ** -126 * np.abs(xv).sum((0, 2)).max(), 0)
+    for g, (want, m), terms, tiny in zip(got, O.gradients(flat(gy), xv, wv), (30, P, P), lost):
+        keep = m <= torch.finfo(F32).max
+        g = np64(g).reshape(want.shape)[keep]
+        assert (np.abs(g - want[keep]) <= ((terms + 2) * 2.0 ** -24 * m + tiny + half_step(F32, want))[keep]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_that_are_no_numbers(dtype):
+    """An infinite or NaN gradient reaches what its terms reach, and nothing else."""
+    F = fh()
+    x, w = make((2, 70, 5, 6), dtype, 41).cuda(), make((30, 70), F32, 42).cuda()
+    w[:, 3] = 0  # a channel with zeros only: infinity times zero
+    gy = torch.randn((2, 30, 5, 6), generator=gen(43)).to(dtype).cuda()
+    gy[0, 4, 1, 2], gy[1, 7, 0, 0], gy[1, 20, 4, 5] = float("inf"), -float("inf"), float("nan")
+    xq, wq = F.quantize_mxfp4(x), F.quantize_mxfp4(w)
+    xv, wv = O.rounded(flat(x)), O.rounded(np64(w)[:, :, None])[:, :, 0]
+    with np.errstate(invalid="ignore"):
+        wants = O.gradients(flat(gy), xv, wv)
+    for g, (want, m), terms in zip(F.conv1x1_mxfp4_backward(gy, xq, wq), wants, (30, 60, 60)):
+        g = np64(g).reshape(want.shape)
+        fin = np.isfinite(want)
+        assert np.array_equal(np.isnan(g), np.isnan(want)) and np.array_equal(np.isinf(g), np.isinf(want))
+        assert np.array_equal(g[np.isinf(g)], want[np.isinf(want)])
+        lim = (terms + 2) * 2.0 ** -24 * m[fin] + half_step(dtype, want[fin])
+        assert (np.abs(g[fin] - want[fin]) <= lim).all()
+
+
+def test_hooks_that_change_what_is_kept():
+    F = fh()
+    x, w = make((2, 40, 3, 3), F32, 44).cuda().requires_grad_(True), make((8, 40), F32, 45).cuda().requires_grad_(True)
+    gy = torch.randn(2, 8, 3, 3, device="cuda")
+    want = torch.autograd.grad(F.conv1x1_mxfp4_train(x, w), (x, w), gy)
+    with torch.autograd.graph.save_on_cpu():
+        y = F.conv1x1_mxfp4_train(x, w)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), gy), want))
+    for unpack in (lambda t: t.cpu(), lambda t: t[1:], lambda t: t.float()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = F.conv1x1_mxfp4_train(x, w)
+        with pytest.raises(RuntimeError, match="hook"):
+            torch.autograd.grad(y, (x, w), gy)
+
+
 def test_gradients_against_differences():
     """Straight through the quantisation the loss is that of the rounded operands: its differences about them."""
     F = fh()
