@@ -52,17 +52,17 @@ __device__ __forceinline__ void mx_finish(const MxOut& o, float (*v)[V], const f
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(v[r][e]));
-    if (top == __builtin_inff()) {  // (gelu_fast makes 0 times infinity of it)
+    if (top == __builtin_inff()) {  // (mx_gelu makes 0 times infinity of it)
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          v[r][e] = fabsf(v[r][e]) == __builtin_inff() ? fmaxf(v[r][e], 0.f) : gelu_fast(v[r][e]);
+          v[r][e] = fabsf(v[r][e]) == __builtin_inff() ? fmaxf(v[r][e], 0.f) : mx_gelu(v[r][e]);
     } else {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[r][e] = gelu_fast(v[r][e]);
+        for (int e = 0; e < V; ++e) v[r][e] = mx_gelu(v[r][e]);
     }
   }
   if (o.res_scale) {
