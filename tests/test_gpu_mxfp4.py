@@ -168,6 +168,56 @@ def test_conv1x1(case, dtype):
     check(fh().conv1x1_mxfp4(q, wm, dtype=BF16), want, limits(K, mag, want, None, None, None, BF16))
 
 
+def by_channels(t):
+    """A map (B,C,*) as (C, pixels) in 64 bits, on the device."""
+    return t.detach().double().flatten(2).transpose(0, 1).flatten(1) if t.dim() > 2 else t.detach().double().t()
+
+
+def check64(got, want, lim):
+    bad = ~((got.double() - want).abs() <= lim)
+    assert not bad.any(), (int(bad.sum()), bad.numel(), float((got.double() - want).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("case", [((1, 290, 4100), 2100), ((3, 520, 37, 37), 2176), ((2, 300, 32, 64), 2210), ((4100, 290), 2100),
+                                  ((4096, 544), 2176)], ids=str)
+def test_conv1x1_of_many_tiles(case, dtype):
+    """More tiles than blocks, whole and partial ones, rows of the result on lines and off them."""
+    shape, N = case
+    F = fh()
+    x, w = make(shape, dtype, 46).cuda(), F.quantize_mxfp4((make((N, shape[1]), F32, 47) / shape[1] ** 0.5).cuda())
+    bias = torch.randn(N, generator=gen(48)).cuda()
+    res = torch.randn((shape[0], N) + shape[2:], generator=gen(49)).to(dtype).cuda()
+    q = F.quantize_mxfp4(x)
+    xv, wv = by_channels(F.dequantize_mxfp4(q)), F.dequantize_mxfp4(w).double()
+    want, mag = wv @ xv + bias.double()[:, None], wv.abs() @ xv.abs() + bias.double().abs()[:, None]
+    want = want * torch.special.erfc(-want / 2 ** 0.5) / 2 + by_channels(res)
+    K = (shape[1] + 31) // 32
+    lim = 1.13 * (K + 2) * 2.0 ** -23 * mag + 4e-7 * mag.clamp(min=1) + (2.0 ** -23 + torch.finfo(dtype).eps / 2) * (
+        want.abs() + by_channels(res).abs() + 1)
+    for v in (x, q):
+        y = F.conv1x1_mxfp4(v, w, bias, "gelu", res)
+        assert y.shape == res.shape and y.dtype is dtype
+        check64(by_channels(y), want, lim)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [((1, 200, 130, 131), 40), ((17000, 200), 33), ((3, 130, 80, 71), 130), ((2, 500, 32, 33), 600),
+                                  ((2000, 500), 600), ((2, 96, 160, 128), 64)], ids=str)
+def test_gradients_of_many_tiles(case, dtype):
+    shape, N = case
+    F = fh()
+    x, w = F.quantize_mxfp4(make(shape, dtype, 50).cuda()), F.quantize_mxfp4(make((N, shape[1]), F32, 51).cuda())
+    gy = torch.randn((shape[0], N) + shape[2:], generator=gen(52)).to(dtype).cuda()
+    gx, gw, gb = F.conv1x1_mxfp4_backward(gy, x, w)
+    xv, wv, g = by_channels(F.dequantize_mxfp4(x)), F.dequantize_mxfp4(w).double(), by_channels(gy)
+    P = g.shape[1]
+    for got, a, b, terms, t in ((by_channels(gx), wv.t().contiguous(), g, N, dtype), (gw, g, xv.t().contiguous(), P, F32),
+                                (gb, g, torch.ones_like(g[:1]).t().contiguous(), P, F32)):
+        want, mag = (a @ b).view(got.shape), (a.abs() @ b.abs()).view(got.shape)
+        check64(got, want, (terms + 2) * 2.0 ** -24 * mag + torch.finfo(t).eps / 2 * want.abs() + torch.finfo(t).smallest_normal)
+
+
 def test_conv1x1_layouts_and_outputs():
     F = fh()
     x = make((2, 70, 12, 10), F32, 6).cuda()
