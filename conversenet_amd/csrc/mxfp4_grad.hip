@@ -21,7 +21,8 @@ enum { kGradX, kGradW };
 
 template <class T>
 struct MxGrad;  // values of a 16-byte vector, parts of a value, terms of a step of gx and of gw
-// (gw of 8 x 64 x 256 x 256 float32 to 128: 104 us by steps of 128 bytes of a channel, 96 by 256; of bfloat16 49 either way)
+// (gw of 8 x 64 x 256 x 256 float32 to 128: 96 us by steps of 128 bytes of a channel, 76 by 256, with gx 150 and 145; of
+// bfloat16 40 and 36.5, but with gx 65 and 66.5)
 template <>
 struct MxGrad<float> {
   static constexpr int V = 4, P = 3, K = 32, KW = 64;
@@ -65,31 +66,38 @@ struct MxGradArgs {
 
 // D[i][k] = sum over terms of A's row i and B's row k, in tiles of BA x BB, a quarter to a wave.  gx: A are the matrix' columns
 // (c), B the pixels, the terms n.  gw: A are the channels of gy (n), B those of x (c), the terms the pixels, shared out over
-// blockIdx.y.  The codes come by terms, 32 neighbours of a tile's rows to a block, and lie in LDS as they come, in bfloat16: a
+// the splits.  The codes come by terms, 32 neighbours of a tile's rows to a block, and lie in LDS as they come, in bfloat16: a
 // transposing read gives a lane the terms of its column.  gy comes either way: its terms side by side (gw of maps, gx of one
 // pixel a sample: ONE), or by terms.
 template <class T, int KIND, bool ONE, int BA, int BB>
-__global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
+struct MxTile {
   typedef MxGrad<T> G;
-  constexpr int V = G::V, P = G::P, K = KIND == kGradX ? G::K : G::KW;
-  constexpr int BC = KIND == kGradX ? BA : BB, BG = KIND == kGradX ? BB : BA;  // rows of the codes' and gy's tile
-  constexpr bool kByTerms = (KIND == kGradX) != ONE;                           // gy's tile [terms][rows]
-  constexpr int GR = kByTerms ? K : BG, GC = kByTerms ? BG : K;                // its rows and columns as stored
+  static constexpr int V = G::V, P = G::P, K = KIND == kGradX ? G::K : G::KW;
+  static constexpr int BC = KIND == kGradX ? BA : BB, BG = KIND == kGradX ? BB : BA;  // rows of the codes' and gy's tile
+  static constexpr bool kByTerms = (KIND == kGradX) != ONE;                           // gy's tile [terms][rows]
+  static constexpr int GR = kByTerms ? K : BG, GC = kByTerms ? BG : K;                // its rows and columns as stored
   // Rows are padded so that what 16 lanes read at once lies in different banks: 32 bytes of four rows for the
   // transposing reads (64 of four for the two halves of a tile), 16 of neighbouring rows otherwise.
-  constexpr int CS = BC * 2 + 64, GS = GC * 2 + (kByTerms ? 64 : 16);
+  static constexpr int CS = BC * 2 + 64, GS = GC * 2 + (kByTerms ? 64 : 16);
+  static constexpr int kLds = K * CS + P * GR * GS;
+};
+
+template <class T, int KIND, bool ONE, int BA, int BB>
+__device__ __forceinline__ void mx_grad(const MxGradArgs& a, int t, int split, char* lds) {
+  typedef MxTile<T, KIND, ONE, BA, BB> M;
+  constexpr int V = M::V, P = M::P, K = M::K, BC = M::BC, GR = M::GR, GC = M::GC, CS = M::CS, GS = M::GS;
+  constexpr int BG = M::BG;
+  constexpr bool kByTerms = M::kByTerms;
   constexpr int NG = GR * GC / V / kThreads, NC = (K * BC / 32 + kThreads - 1) / kThreads;
-  __shared__ __attribute__((aligned(16))) char lds[K * CS + P * GR * GS];
   char* const lc = lds;
   char* const lg = lds + K * CS;
   typedef T W __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j = lane & 31, h = lane >> 5;
 
-  const int t = blockIdx.x;
   const int64_t a0 = (int64_t)(t % a.ta) * BA, b0 = (int64_t)(t / a.ta) * BB;
   const int64_t c0 = KIND == kGradX ? a0 : b0, g0 = KIND == kGradX ? b0 : a0;
   const int64_t terms = KIND == kGradX ? a.N : a.rows;
-  const int64_t k_first = (int64_t)blockIdx.y * a.terms, k_end = min(terms, k_first + a.terms);
+  const int64_t k_first = (int64_t)split * a.terms, k_end = min(terms, k_first + a.terms);
   const T* const gy = (const T*)a.gy;
 
   // What is under way from memory for the next step.  (Two steps under way change nothing: 33 us either way for gx of 8192
@@ -284,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
         }
     } else {
       if (col >= a.C) continue;
-      float* out = (float*)a.out + (int64_t)blockIdx.y * a.N * a.C + col;
+      float* out = (float*)a.out + (int64_t)split * a.N * a.C + col;
 #pragma unroll
       for (int i = 0; i < TA; ++i)
 #pragma unroll
@@ -295,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
     }
   }
   if (KIND == kGradW && a.gb && b0 == 0) {
-    double* const out = a.gb + (int64_t)blockIdx.y * a.N;
+    double* const out = a.gb + (int64_t)split * a.N;
     if (!kByTerms) {  // the threads of a row are neighbours
       constexpr int TR = GC / V;
 #pragma unroll
@@ -309,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
     } else {  // those of a column are GC / V apart
       constexpr int TR = GC / V;
       double(*red)[GC] = (double(*)[GC])lds;
-      static_assert(sizeof(double) * GC * (kThreads / TR) <= sizeof(lds), "sums fit the operands' memory");
+      static_assert(sizeof(double) * GC * (kThreads / TR) <= M::kLds, "sums fit the operands' memory");
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < V; ++e) red[tid / TR][tid % TR * V + e] = sum[e % NB];
@@ -320,6 +328,29 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
         if (a0 + c < a.N) out[a0 + c] = s;
       }
     }
+  }
+}
+
+template <class T, int KIND, bool ONE, int BA, int BB>
+__global__ void __launch_bounds__(kThreads, 2) k_mx_grad(MxGradArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[MxTile<T, KIND, ONE, BA, BB>::kLds];
+  const int tiles = a.ta * a.tb;
+  mx_grad<T, KIND, ONE, BA, BB>(a, blockIdx.x % tiles, blockIdx.x / tiles, lds);
+}
+// Both gradients, the blocks of gw first, whose sums a kernel behind waits for.  (Against a launch each, with the sums: float16
+// maps of 3x67x45, 48 to 80 channels, 27.7 us and here 14.5; float32 of 8x96x96, 64 to 128, 41.5 and 32.6; float32 of
+// 8x256x256, 64 to 128, 164 and 145; bfloat16 of 4x31x33, 2048 to 512, 103 and 88.  gw has tiles of 64 of gy's channels: tiles
+// of 128 leave a CU fewer blocks of either kind, and the four take 17.3, 35.5, 171 and 96 us; they are better by 3% where
+// bfloat16 of 8x32x32 goes from 1024 to 1024 channels, 76 us to 79.)
+template <class T, bool ONE, int XA, int WB>
+__global__ void __launch_bounds__(kThreads, 2) k_mx_grads(MxGradArgs x, MxGradArgs w, int wblocks) {
+  constexpr int kX = MxTile<T, kGradX, ONE, XA, 128>::kLds, kW = MxTile<T, kGradW, ONE, 64, WB>::kLds;
+  __shared__ __attribute__((aligned(16))) char lds[kX > kW ? kX : kW];
+  if ((int)blockIdx.x < wblocks) {
+    const int tiles = w.ta * w.tb;
+    mx_grad<T, kGradW, ONE, 64, WB>(w, blockIdx.x % tiles, blockIdx.x / tiles, lds);
+  } else {
+    mx_grad<T, kGradX, ONE, XA, 128>(x, blockIdx.x - wblocks, 0, lds);
   }
 }
 
@@ -389,7 +420,7 @@ struct MxSplit {
   int64_t terms, splits;
 };
 MxSplit mx_split_terms(int64_t rows, int64_t C, int64_t N) {
-  const int64_t tiles = (N + 127) / 128 * ((C + 127) / 128);
+  const int64_t tiles = (N + 63) / 64 * ((C + 127) / 128);
   const int64_t want = std::max<int64_t>(1, std::min((rows + 255) / 256, 512 / tiles));
   MxSplit s;
   s.terms = std::max<int64_t>(256, ((rows + want - 1) / want + 63) / 64 * 64);
@@ -400,12 +431,25 @@ size_t mx_part_bytes(const MxSplit& s, int64_t C, int64_t N) {
   return (s.splits > 1 ? align_up((size_t)(s.splits * N * C) * sizeof(float)) : 0) + (size_t)(s.splits * N) * sizeof(double);
 }
 
-template <class T, int KIND, bool ONE, int BA, int BB>
-int grad_tile(MxGradArgs a, int64_t na, int64_t nb, int64_t splits, hipStream_t st) {
-  const int64_t ta = (na + BA - 1) / BA, tb = (nb + BB - 1) / BB;
-  if (ta * tb * splits * kThreads >= (int64_t)1 << 32) return fail(CVN_ERR_UNSUPPORTED, "too many pixels and channels");
-  a.ta = (int)ta, a.tb = (int)tb;
-  hipLaunchKernelGGL((k_mx_grad<T, KIND, ONE, BA, BB>), dim3((unsigned)(ta * tb), (unsigned)splits), dim3(kThreads), 0, st, a);
+// The launches of one shape of tiles; x, w: null where that gradient is not wanted.
+template <class T, bool ONE, int XA, int WB>
+int grad_tiles(MxGradArgs* x, MxGradArgs* w, int64_t C, int64_t N, int64_t rows, int64_t splits, hipStream_t st) {
+  int64_t xblocks = 0, wblocks = 0;
+  if (x) {
+    const int64_t ta = (C + XA - 1) / XA, tb = (rows + 127) / 128;
+    xblocks = ta * tb;
+    x->ta = (int)ta, x->tb = (int)tb;
+  }
+  if (w) {
+    const int64_t ta = (N + 63) / 64, tb = (C + WB - 1) / WB;
+    wblocks = ta * tb * splits;
+    w->ta = (int)ta, w->tb = (int)tb;
+  }
+  if ((xblocks + wblocks) * kThreads >= (int64_t)1 << 32) return fail(CVN_ERR_UNSUPPORTED, "too many pixels and channels");
+  const dim3 grid((unsigned)(xblocks + wblocks));
+  if (x && w) hipLaunchKernelGGL((k_mx_grads<T, ONE, XA, WB>), grid, dim3(kThreads), 0, st, *x, *w, (int)wblocks);
+  else if (x) hipLaunchKernelGGL((k_mx_grad<T, kGradX, ONE, XA, 128>), grid, dim3(kThreads), 0, st, *x);
+  else hipLaunchKernelGGL((k_mx_grad<T, kGradW, ONE, 64, WB>), grid, dim3(kThreads), 0, st, *w);
   return check_launch("conv1x1_mxfp4_backward");
 }
 
@@ -413,29 +457,25 @@ template <class T, bool ONE>
 int grads(const void* gy, const void* xc, const void* xs, const void* wc, const void* ws, int64_t C, int64_t HW, int64_t rows,
           int64_t N, void* gx, float* gw, float* gb, void* work, hipStream_t st) {
   const int KB = (int)mx_blocks(C);
-  if (gx) {
-    const MxGradArgs a = {gy, (const mx_i32x4*)wc, (const uint8_t*)ws, C, N, HW, rows, KB, gx, nullptr, N, 0, 0};
-    // (256 pixels, 2048 to 2048 channels: 36 us by 32 tiles of 128 channels, 25 by 64 of 64)
-    const int rc = C <= 64 || (C + 127) / 128 * ((rows + 127) / 128) < 256 ? grad_tile<T, kGradX, ONE, 64, 128>(a, C, rows, 1, st)
-                           : grad_tile<T, kGradX, ONE, 128, 128>(a, C, rows, 1, st);
+  const MxSplit s = mx_split_terms(rows, C, N);
+  float* const part = s.splits > 1 ? (float*)work : gw;
+  double* const gbp = (double*)((char*)work + (s.splits > 1 ? align_up((size_t)(s.splits * N * C) * sizeof(float)) : 0));
+  MxGradArgs x = {gy, (const mx_i32x4*)wc, (const uint8_t*)ws, C, N, HW, rows, KB, gx, nullptr, N, 0, 0};
+  MxGradArgs w = {gy, (const mx_i32x4*)xc, (const uint8_t*)xs, C, N, HW, rows, KB, part, gb ? gbp : nullptr, s.terms, 0, 0};
+  if (gx || gw) {
+    MxGradArgs *px = gx ? &x : nullptr, *pw = gw ? &w : nullptr;
+    // (256 pixels, 2048 to 2048 channels: gx 36 us by 32 tiles of 128 channels, 25 by 64 of 64)
+    const bool few = (C + 127) / 128 * ((rows + 127) / 128) < 256;
+    const int rc = C <= 64 ? grad_tiles<T, ONE, 64, 64>(px, pw, C, N, rows, s.splits, st)
+                   : few   ? grad_tiles<T, ONE, 64, 128>(px, pw, C, N, rows, s.splits, st)
+                           : grad_tiles<T, ONE, 128, 128>(px, pw, C, N, rows, s.splits, st);
     if (rc != CVN_OK) return rc;
   }
-  if (gw) {
-    const MxSplit s = mx_split_terms(rows, C, N);
-    float* const part = s.splits > 1 ? (float*)work : gw;
-    double* const gbp = (double*)((char*)work + (s.splits > 1 ? align_up((size_t)(s.splits * N * C) * sizeof(float)) : 0));
-    const MxGradArgs a = {gy, (const mx_i32x4*)xc, (const uint8_t*)xs, C, N, HW, rows, KB, part, gb ? gbp : nullptr, s.terms, 0, 0};
-    const int rc = C <= 64 ? (N <= 64 ? grad_tile<T, kGradW, ONE, 64, 64>(a, N, C, s.splits, st)
-                                      : grad_tile<T, kGradW, ONE, 128, 64>(a, N, C, s.splits, st))
-                           : (N <= 64 ? grad_tile<T, kGradW, ONE, 64, 128>(a, N, C, s.splits, st)
-                                      : grad_tile<T, kGradW, ONE, 128, 128>(a, N, C, s.splits, st));
-    if (rc != CVN_OK) return rc;
-    if (s.splits > 1 || gb) {
-      const int64_t n = s.splits > 1 ? N * C : 0;
-      if (n >= 1 << 18) grad_join<1>(part, n, gbp, N, s.splits, gw, gb, st);
-      else grad_join<16>(part, n, gbp, N, s.splits, gw, gb, st);
-    }
-  } else if (gb) {
+  if (gw && (s.splits > 1 || gb)) {
+    const int64_t n = s.splits > 1 ? N * C : 0;
+    if (n >= 1 << 18) grad_join<1>(part, n, gbp, N, s.splits, gw, gb, st);
+    else grad_join<16>(part, n, gbp, N, s.splits, gw, gb, st);
+  } else if (gb && !gw) {
     hipLaunchKernelGGL(k_mx_grad_bias<T>, dim3((unsigned)N), dim3(kThreads), 0, st, (const T*)gy, N, HW, rows, gb);
   }
   return check_launch("conv1x1_mxfp4_backward");
