@@ -1290,8 +1290,8 @@ def conv1x1_mxfp4(x, weight, bias=None, act=None, residual=None, res_scale=None,
 def conv1x1_mxfp4_backward(grad_y, x, weight, need=(True, True, True)):
     """Gradients of conv1x1_mxfp4's product and bias, straight through the quantisation: (x, weight, bias), None where
     not asked for by `need`.  grad_y (B,N,*): float32, bfloat16 or float16, the type of x's gradient; the others are float32,
-    weight's (N,C).  (Parts of an operand below 2^-126 count as zeros.)  x, weight: the MXFP4 operands of the forward (x None without weight's gradient, weight None without x's, where
-    the other gives the channels)."""
+    weight's (N,C).  (Parts of an operand below 2^-126 count as zeros.)  x, weight: the MXFP4 operands of the forward (x
+    None without weight's gradient, weight None without x's, where the other gives the channels)."""
     _untraced("conv1x1_mxfp4_backward")
     B, N, HW = _mx_map(grad_y, "conv1x1_mxfp4_backward")
     nx, nw, nb = need
