@@ -13,6 +13,8 @@ import torch  # (loads the HIP runtime the library binds to)
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CVN_LIB", os.path.join(_HERE, "lib", "libcvn_hip.so"))
 
+AUTOGRAD_LIB_PATH = os.path.join(_HERE, "lib", "libcvn_autograd.so")
+
 CVN_OK = 0
 CVN_ERR_ARG = -1
 CVN_ERR_UNSUPPORTED = -2
@@ -123,6 +125,33 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_graph_streams = None
+
+
+def graph_streams(t):
+    """(device index, stream id) of the streams but the current ones that the nodes which a tensor's gradient reaches were made
+    on (csrc/autograd_stream.cpp); (-1, 0): a leaf's node on the CPU.  Raises ImportError if libcvn_autograd.so is not built, or
+    for another torch."""
+    global _graph_streams
+    if _graph_streams is None:
+        try:
+            fn = ctypes.PyDLL(AUTOGRAD_LIB_PATH).cvn_graph_streams  # (runs under the interpreter's lock)
+        except OSError as e:
+            raise ImportError(f"conversenet_amd: {AUTOGRAD_LIB_PATH} does not load ({e}); build it with "
+                              "`python -m conversenet_amd.build` (or __graft_entry__.build())") from e
+        fn.restype, fn.argtypes = _int, [ctypes.py_object, ctypes.POINTER(_i64), ctypes.POINTER(_int), _int]
+        _graph_streams = fn
+    most = 16
+    while True:
+        ids, devices = (_i64 * most)(), (_int * most)()
+        n = _graph_streams(t, ids, devices, most)
+        if n < 0:
+            raise RuntimeError("not a tensor whose graph can be read")
+        if n <= most:
+            return list(zip(devices[:n], ids[:n]))
+        most = n
 
 
 def available() -> bool:

@@ -1438,18 +1438,43 @@ def _own_leaves(leaves, stream):
                                "that graph's outputs first")
 
 
+def _recorded_too(device, stream_id):
+    """Whether a stream is part of a recording (one that forks onto it); the null stream cannot be."""
+    if stream_id == 0:
+        return False
+    with torch.cuda.stream(torch.cuda.Stream(stream_id=stream_id, device_index=device, device_type=_DEVICE_TYPE)):
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
+_DEVICE_TYPE = 1  # (torch's number for devices named cuda)
+
+
+def _elsewhere(t):
+    """Whether a node that a tensor's gradient reaches was made on a stream outside of the recording on the current one."""
+    return not all(_recorded_too(*s) for s in _lib.graph_streams(t))
+
+
+def _own_operands(operands, stream):
+    """Refuses a recording whose operands come from nodes outside of it, leaves or not (see _own_leaves)."""
+    _own_leaves([t for t in operands if t.is_leaf], stream)
+    if any(not t.is_leaf and _elsewhere(t) for t in operands):
+        raise RuntimeError("a training pass cannot be recorded with an operand whose graph, or a leaf of it, was made outside of the "
+                           "recording: let go of earlier graphs' outputs first, and make views in the recording")
+
+
 def conv1x1_mxfp4_train(x, weight, bias=None):
     """Differentiable conv1x1_mxfp4 of a float map (B,C,*) and matrix (N,C) or (N,C,1,1), both quantised in the call: the
     gradients pass the quantisation unchanged, those of x and weight are products with the other's 4-bit values.  (Not
-    differentiable twice.  Recorded into a graph, its leaves are in no graph that lives from before.)"""
+    differentiable twice.  Recorded into a graph, nothing that its gradients reach is in a graph that lives from before.)"""
     if isinstance(x, MXFP4) or isinstance(weight, MXFP4):
         raise RuntimeError("conv1x1_mxfp4_train quantises x and weight itself")
     if x.is_cuda and torch.is_grad_enabled() and _capturing(stream := _stream(x.device)):
-        leaves = [t for t in (x, weight, bias) if t is not None and t.requires_grad and t.is_leaf]
-        _own_leaves(leaves, stream)
+        operands = [t for t in (x, weight, bias) if t is not None and t.requires_grad]
+        _own_operands(operands, stream)
         y = Conv1x1MXFP4Function.apply(x, weight, bias)
-        for t in leaves:
-            _accumulator(t).metadata[_RECORDING] = stream
+        for t in operands:
+            if t.is_leaf:
+                _accumulator(t).metadata[_RECORDING] = stream
         return y
     return Conv1x1MXFP4Function.apply(x, weight, bias)
 

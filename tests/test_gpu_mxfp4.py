@@ -673,3 +673,33 @@ def test_modules_under_modes_and_transforms():
     assert d(x.double()).dtype is torch.float64 and torch.allclose(d(x.double()).float(), ref, rtol=0, atol=lim)
     with torch.inference_mode():
         assert torch.equal(conv(x), ref)
+
+
+def test_recording_with_views_of_held_leaves_is_refused():
+    """Operands that are views of a leaf, or come from it, are refused where the leaf itself would be; views made in the recording of
+    leaves that no other graph holds are recorded."""
+    from conversenet_amd.util_converse import Conv1x1MXFP4
+    F = fh()
+    x, w = make((64, 12, 12), F32, 33).cuda().requires_grad_(True), make((32, 64), F32, 34).cuda().requires_grad_(True)
+    gy = torch.randn(1, 32, 12, 12, device="cuda")
+    plain_x, plain_w, conv = x.detach()[None], w.detach(), Conv1x1MXFP4(64, 32, bias=False).cuda()
+    alive = [x * 2, w * 2]
+    early = w.view(32, 64, 1, 1)
+    fill = torch.zeros(4, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fill.add_(1)
+        for a, b in ((plain_x, w.view(32, 64, 1, 1)), (plain_x, w.flatten(1) * 1.0), (x.unsqueeze(0), plain_w), (plain_x, early)):
+            with pytest.raises(RuntimeError, match="outside of the recording"):
+                F.conv1x1_mxfp4_train(a, b)
+        with pytest.raises(RuntimeError, match="outside of the recording"):
+            conv(x)  # (a single sample)
+    want = torch.autograd.grad(F.conv1x1_mxfp4_train(x[None], w), (x, w), gy)
+    del alive, early, a, b, g
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(F.conv1x1_mxfp4_train(x.unsqueeze(0), w.view(32, 64, 1, 1)), (x, w), gy)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -175,3 +175,35 @@ def test_leaves_of_other_graphs_are_found():
         F._own_leaves([x], 6)
     del y
     F._own_leaves([x, w], 6)
+
+
+def test_views_of_leaves_of_other_graphs_are_found():
+    """An operand that is a view (or another result) of a leaf is refused as the leaf itself is."""
+    w, x = torch.randn(6, 4, requires_grad=True), torch.randn(3, 4)
+    F._own_operands([w], 5)
+    alive = w * 2
+    for v in (w.view(6, 4, 1, 1), w.flatten(), w.unsqueeze(0), w * 1.0, (w * 1.0).exp().view(4, 6)):
+        with pytest.raises(RuntimeError, match="outside of the recording"):
+            F._own_operands([v], 5)
+    with pytest.raises(RuntimeError, match="holds one of its leaves"):
+        F._own_operands([w], 5)
+    del alive, v
+    F._own_operands([w], 5)
+    F._own_operands([t for t in (x, w) if t.requires_grad], 5)
+
+
+def test_graphs_are_walked():
+    """Every node behind a tensor is looked at, each once; a tensor without a graph has none."""
+    from conversenet_amd import _lib
+    w, x = torch.randn(4, requires_grad=True), torch.randn(4)
+    assert _lib.graph_streams(w) == [] and _lib.graph_streams(x) == []
+    y = w
+    for _ in range(200):  # 2^200 paths, 200 nodes
+        y = y + y
+    assert _lib.graph_streams(y) == [(-1, 0)] == _lib.graph_streams(w)
+    with torch.no_grad():
+        assert _lib.graph_streams(y.detach()) == []
+    del y
+    assert _lib.graph_streams(w) == []
+    with pytest.raises(RuntimeError, match="not a tensor"):
+        _lib.graph_streams(None)
