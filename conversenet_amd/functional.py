@@ -1425,19 +1425,6 @@ def _accumulator(leaf):
     return leaf.view_as(leaf).grad_fn.next_functions[0][0]
 
 
-def _own_leaves(leaves, stream):
-    """Refuses a recording whose leaves are part of a graph from outside of it: such a leaf's node lives on the stream that it
-    was made on, the recorded backward would make that stream wait for the recording, and the recording's end would end the
-    process."""
-    for t in leaves:
-        if _accumulator(t).metadata.get(_RECORDING) == stream:
-            continue
-        _accumulator(t).metadata[_RECORDING] = None
-        if _RECORDING in _accumulator(t).metadata:  # (a node made here would be gone)
-            raise RuntimeError("a training pass cannot be recorded while a graph made before holds one of its leaves: let go of "
-                               "that graph's outputs first")
-
-
 def _recorded_too(device, stream_id):
     """Whether a stream is part of a recording (one that forks onto it); the null stream cannot be."""
     if stream_id == 0:
@@ -1452,6 +1439,15 @@ _DEVICE_TYPE = 1  # (torch's number for devices named cuda)
 def _elsewhere(t):
     """Whether a node that a tensor's gradient reaches was made on a stream outside of the recording on the current one."""
     return not all(_recorded_too(*s) for s in _lib.graph_streams(t))
+
+
+def _own_leaves(leaves, stream):
+    """Refuses a recording whose leaves are part of a graph from outside of it: such a leaf's node lives on the stream that it
+    was made on, the recorded backward would make that stream wait for the recording, and the recording's end would end the
+    process.  (A mark says that a recording on the stream has the leaf's node.)"""
+    if any(_accumulator(t).metadata.get(_RECORDING) != stream and _elsewhere(t) for t in leaves):
+        raise RuntimeError("a training pass cannot be recorded while a graph made before holds one of its leaves: let go of "
+                           "that graph's outputs first")
 
 
 def _own_operands(operands, stream):

@@ -703,3 +703,44 @@ def test_recording_with_views_of_held_leaves_is_refused():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_recordings_whose_leaves_have_nodes_of_their_own():
+    """What a recording's leaves are used for before in the same recording, on the same stream before it, or on a stream that it forks
+    onto does not keep a training pass from being recorded."""
+    F = fh()
+    x, w = make((2, 64, 12, 12), F32, 33).cuda().requires_grad_(True), make((32, 64), F32, 34).cuda().requires_grad_(True)
+    gy = torch.randn(2, 32, 12, 12, device="cuda")
+    side, fork = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def penalty():
+        p = 0.5 * w.square().sum(1)
+        y = F.conv1x1_mxfp4_train(x * 2.0, w.view(32, 64, 1, 1))
+        return torch.autograd.grad((y, p), (x, w), (gy, torch.ones_like(p)))
+
+    def forked():
+        fork.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(fork):
+            v = w * 2.0
+        torch.cuda.current_stream().wait_stream(fork)
+        grads = torch.autograd.grad(F.conv1x1_mxfp4_train(x, v), (x, w), gy)
+        torch.cuda.current_stream().wait_stream(fork)
+        return grads
+
+    def again():
+        return torch.autograd.grad(F.conv1x1_mxfp4_train(x, w), (x, w), gy)
+
+    for step, held in ((penalty, False), (forked, False), (again, True)):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = step()
+            alive = [x * 2.0, w * 2.0] if held else None  # nodes on the recording's stream
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got = step()
+        for _ in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del alive
