@@ -279,9 +279,12 @@ class Conv1x1MXFP4(nn.Conv2d):
 
     @classmethod
     def of(cls, conv):
-        """An MXFP4 convolution with a 1x1 nn.Conv2d's parameters (the same tensors)."""
-        if conv.kernel_size != (1, 1) or conv.stride != (1, 1) or conv.padding != (0, 0) or conv.groups != 1:
-            raise ValueError("not a 1x1 convolution")
+        """An MXFP4 convolution with a 1x1 nn.Conv2d's parameters (the same tensors).  What the convolution has beside them would
+        be lost, and is refused; use_mxfp4 keeps it."""
+        _check_1x1(conv)
+        if type(conv.weight) is not nn.Parameter or set(conv._parameters) != {"weight", "bias"} or conv._buffers or conv._modules \
+                or any(v for k, v in conv.__dict__.items() if k.endswith("_hooks")):
+            raise ValueError("a convolution with hooks, or whose weight is made of other parameters, is no plain one")
         new = cls(conv.in_channels, conv.out_channels, conv.bias is not None, device="meta")
         new.weight, new.bias = conv.weight, conv.bias
         new.train(conv.training)
@@ -298,15 +301,25 @@ class Conv1x1MXFP4(nn.Conv2d):
         return functional.conv1x1_mxfp4(x, self.weight, self.bias)
 
 
+def _check_1x1(conv):
+    """Refuses what Conv1x1MXFP4.forward would not compute."""
+    if conv.kernel_size != (1, 1) or conv.stride != (1, 1) or conv.padding not in ((0, 0), "same", "valid") or conv.groups != 1:
+        raise ValueError("not a 1x1 convolution")
+    if "forward" in conv.__dict__ or conv._compiled_call_impl is not None:
+        raise ValueError("a convolution with a forward of its own (set on it, or compiled) does not run in MXFP4")
+
+
 def use_mxfp4(model):
-    """Runs the 1x1 convolutions of a model's ConverseBlocks in MXFP4, for evaluation and training: each becomes a
-    Conv1x1MXFP4 of the same parameters.  Returns the model, whose state dict stays as it was."""
-    for blk in model.modules():
-        if isinstance(blk, (ConverseBlock, ConverseBlockAlphaVariant)):
-            for seq in (blk.conv1, blk.conv2):
-                for name, m in seq.named_children():
-                    if type(m) is nn.Conv2d and m.kernel_size == (1, 1):
-                        setattr(seq, name, Conv1x1MXFP4.of(m))
+    """Runs the 1x1 convolutions of a model's ConverseBlocks in MXFP4, for evaluation and training: each nn.Conv2d becomes a
+    Conv1x1MXFP4 and stays the same object, with its parameters, hooks and what else it has (one that computes its weight in a
+    hook goes on doing so).  Those of other classes, parametrised ones among them, stay what they are.  Returns the model, whose
+    state dict stays as it was; ValueError leaves it as it was."""
+    convs = [m for blk in model.modules() if isinstance(blk, (ConverseBlock, ConverseBlockAlphaVariant))
+             for seq in (blk.conv1, blk.conv2) for m in seq.children() if type(m) is nn.Conv2d and m.kernel_size == (1, 1)]
+    for m in convs:
+        _check_1x1(m)
+    for m in convs:
+        m.__class__ = Conv1x1MXFP4
     return model
 
 

@@ -207,3 +207,52 @@ def test_graphs_are_walked():
     assert _lib.graph_streams(w) == []
     with pytest.raises(RuntimeError, match="not a tensor"):
         _lib.graph_streams(None)
+
+
+def test_use_mxfp4_keeps_what_convolutions_carry():
+    """Hooks, weights made in hooks, shared convolutions and the state dict; all or nothing."""
+    torch.manual_seed(0)
+    blk = ConverseBlock(8, 8, kernel_size=3, padding=2, padding_mode="circular")
+    x = torch.randn(2, 8, 6, 7)
+    seen, conv = [], blk.conv2[3]
+    handle = conv.register_forward_hook(lambda m, args, out: seen.append(out))
+    with pytest.warns(FutureWarning):
+        torch.nn.utils.weight_norm(blk.conv1[1])
+    blk.conv2.append(conv), blk.conv2.insert(3, torch.nn.Conv2d(16, 16, 1, padding="same"))
+    blk.conv2[5] = torch.nn.Conv2d(8, 8, 1, padding="valid")
+    keys = list(blk.state_dict())
+    assert use_mxfp4(blk) is blk and list(blk.state_dict()) == keys and blk.conv2[4] is conv
+    assert all(type(blk.conv1[i]) is Conv1x1MXFP4 for i in (1, 5)) and all(type(blk.conv2[i]) is Conv1x1MXFP4 for i in (1, 3, 4, 5))
+    with torch.no_grad():
+        blk.conv1[1].weight_g.mul_(3.0)
+        n = blk.conv1[0](x)
+        w = torch._weight_norm(blk.conv1[1].weight_v, blk.conv1[1].weight_g, 0)
+        assert torch.equal(blk.conv1[1](n), composite.conv1x1_mxfp4(n, w, blk.conv1[1].bias))
+        blk(x)
+    assert len(seen) == 1
+    handle.remove()
+    blk(x).sum().backward()
+    assert len(seen) == 1 and blk.conv1[1].weight_g.grad is not None and blk.conv1[1].weight_v.grad is not None
+
+    for spoil in (lambda c: setattr(c, "forward", c.forward), lambda c: setattr(c, "stride", (2, 2)), lambda c: c.compile()):
+        blk = ConverseBlockAlphaVariant(8, 8, kernel_size=3, padding=2, padding_mode="circular")
+        spoil(blk.conv2[3])
+        with pytest.raises(ValueError):
+            use_mxfp4(blk)
+        assert all(type(m) is not Conv1x1MXFP4 for m in blk.modules())
+
+
+def test_convolutions_that_would_lose_something_are_refused():
+    c = lambda: torch.nn.Conv2d(4, 6, 1)  # noqa: E731
+    hooked, pre, late = c(), c(), c()
+    hooked.register_forward_hook(lambda *a: None), pre.register_forward_pre_hook(lambda *a: None)
+    late.register_full_backward_hook(lambda *a: None)
+    with pytest.warns(FutureWarning):
+        normed = torch.nn.utils.weight_norm(c())
+    bad = [hooked, pre, late, normed, torch.nn.utils.parametrizations.weight_norm(c()), torch.nn.utils.spectral_norm(c())]
+    buffer, child = c(), c()
+    buffer.register_buffer("mask", torch.ones(1)), child.add_module("extra", torch.nn.Identity())
+    for conv in (*bad, buffer, child):
+        with pytest.raises(ValueError):
+            Conv1x1MXFP4.of(conv)
+    assert Conv1x1MXFP4.of(torch.nn.Conv2d(4, 6, 1, padding="same", bias=False)).bias is None
