@@ -292,7 +292,7 @@ class Conv1x1MXFP4(nn.Conv2d):
 
     def forward(self, x):
         if x.dim() == 3:  # one sample
-            return self(x.unsqueeze(0)).squeeze(0)
+            return self.forward(x.unsqueeze(0)).squeeze(0)
         if not _mxfp4_eligible(x, self.weight, self.bias) or x.dim() != 4:
             return composite.conv1x1_mxfp4(x, self.weight, self.bias)
         if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad

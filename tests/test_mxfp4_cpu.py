@@ -256,3 +256,12 @@ def test_convolutions_that_would_lose_something_are_refused():
         with pytest.raises(ValueError):
             Conv1x1MXFP4.of(conv)
     assert Conv1x1MXFP4.of(torch.nn.Conv2d(4, 6, 1, padding="same", bias=False)).bias is None
+
+
+def test_hooks_see_a_single_sample_once():
+    conv = Conv1x1MXFP4(8, 4)
+    seen = []
+    conv.register_forward_pre_hook(lambda m, args: seen.append(args[0].shape))
+    conv.register_forward_hook(lambda m, args, out: seen.append(out.shape))
+    conv(torch.randn(8, 3, 5))
+    assert seen == [(8, 3, 5), (4, 3, 5)]
