@@ -415,8 +415,12 @@ def _fused_block_forward(blk, x, alpha1=None, alpha2=None):
 
 
 def _all_mxfp4(blk) -> bool:
+    """True when _mxfp4_block_forward computes what the block's modules would: theirs are its classes' forwards, with no hooks
+    (one may make a convolution's weight)."""
     return len(blk.conv1) == 6 and len(blk.conv2) == 4 and all(
-        type(m) is Conv1x1MXFP4 for m in (blk.conv1[1], blk.conv1[5], blk.conv2[1], blk.conv2[3]))
+        type(m) is Conv1x1MXFP4 for m in (blk.conv1[1], blk.conv1[5], blk.conv2[1], blk.conv2[3])) and all(
+        type(m) is nn.GELU and m.approximate == "none" for m in (blk.conv1[2], blk.conv1[4], blk.conv2[2])) and _plain(
+        blk.conv1, *blk.conv1, blk.conv2, *blk.conv2)
 
 
 def _mxfp4_block_forward(blk, x, alpha1, alpha2):

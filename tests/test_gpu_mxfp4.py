@@ -744,3 +744,27 @@ def test_recordings_whose_leaves_have_nodes_of_their_own():
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
         del alive
+
+
+def test_evaluation_of_blocks_with_hooks():
+    """Hooks of a block's convolutions run in evaluation, and a weight that a hook makes is the current one."""
+    F = fh()
+    blk = block("ConverseBlockAlphaVariant", seed=3)
+    x = make((2, 64, 16, 18), F32, 36).cuda()
+    with torch.no_grad():
+        seen = []
+        handle = blk.conv2[3].register_forward_hook(lambda m, args, out: seen.append(out))
+        y = blk(x)
+        assert len(seen) == 1
+        handle.remove()
+        t = blk.alpha1 * blk.conv1(x) + x
+        assert torch.equal(y, blk.alpha2 * blk.conv2(t) + t)
+        with pytest.warns(FutureWarning):
+            conv = torch.nn.utils.weight_norm(blk.conv2[1])
+        n = make((2, 64, 16, 18), F32, 37).cuda()
+        args = {}
+        conv.register_forward_hook(lambda m, a, out: args.update(x=a[0], y=out))
+        conv.weight_g.mul_(3.0)
+        blk(x)
+        w = torch._weight_norm(conv.weight_v, conv.weight_g, 0)
+        assert torch.equal(args["y"], F.conv1x1_mxfp4(args["x"], w, conv.bias))

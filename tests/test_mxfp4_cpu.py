@@ -265,3 +265,27 @@ def test_hooks_see_a_single_sample_once():
     conv.register_forward_hook(lambda m, args, out: seen.append(out.shape))
     conv(torch.randn(8, 3, 5))
     assert seen == [(8, 3, 5), (4, 3, 5)]
+
+
+def test_blocks_whose_modules_are_observed_run_them():
+    """The joint forward of a block is for plain modules."""
+    from conversenet_amd import util_converse as U
+    make = lambda: use_mxfp4(ConverseBlock(8, 8, kernel_size=3, padding=2, padding_mode="circular"))  # noqa: E731
+    assert U._all_mxfp4(make())
+    for i in (0, 1, 2, 3, 4, 5):
+        blk = make()
+        handle = blk.conv1[i].register_forward_hook(lambda *a: None)
+        assert not U._all_mxfp4(blk)
+        handle.remove()
+        assert U._all_mxfp4(blk)
+    blk = make()
+    blk.conv2[3].register_forward_pre_hook(lambda *a: None)
+    assert not U._all_mxfp4(blk)
+    for i, m in ((2, torch.nn.ReLU()), (4, torch.nn.GELU("tanh")), (1, torch.nn.Conv2d(8, 16, 1))):
+        blk = make()
+        blk.conv1[i] = m
+        assert not U._all_mxfp4(blk)
+    blk = make()
+    with pytest.warns(FutureWarning):
+        torch.nn.utils.weight_norm(blk.conv2[1])
+    assert not U._all_mxfp4(blk)
