@@ -9,6 +9,8 @@ so gradients and CPU results follow the reference exactly.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 import torch.nn.functional as F
 
@@ -147,5 +149,18 @@ def _straight(x):
 
 def conv1x1_mxfp4(x, weight, bias=None):
     """1x1 convolution of the values that MXFP4 gives x (B,C,H,W) and weight (N,C,1,1), differentiable straight through
-    both roundings."""
-    return F.conv2d(_straight(x), _straight(weight), bias)
+    both roundings.  The result has x's type, under autocast too; of arguments of different types it is computed in the wider one,
+    float32 at least, and rounded."""
+    with _no_autocast(x.device.type):
+        x_values, w_values = _straight(x), _straight(weight)
+        if x.dtype == weight.dtype and (bias is None or bias.dtype == x.dtype):
+            return F.conv2d(x_values, w_values, bias)
+        wide = torch.promote_types(torch.promote_types(x.dtype, weight.dtype), torch.float32)
+        return F.conv2d(x_values.to(wide), w_values.to(wide), None if bias is None else bias.to(wide)).to(x.dtype)
+
+
+def _no_autocast(kind):
+    """A context of a device type's in which torch's operations compute in their arguments' types."""
+    if kind in ("cpu", "cuda") and torch.is_autocast_enabled(kind):
+        return torch.autocast(kind, enabled=False)
+    return contextlib.nullcontext()

@@ -272,7 +272,8 @@ def _mxfp4_eligible(x, *params) -> bool:
 
 class Conv1x1MXFP4(nn.Conv2d):
     """nn.Conv2d(in_channels, out_channels, 1) whose product runs on MXFP4 values of its input and weight, quantised in every
-    call; gradients pass the quantisation unchanged.  The parameters stay as they are, with nn.Conv2d's names."""
+    call; gradients pass the quantisation unchanged.  The parameters stay as they are, with nn.Conv2d's names.  The result has the
+    input's type; parameters may be of another, and autocast, whose types are wider than the operands', changes nothing."""
 
     def __init__(self, in_channels, out_channels, bias=True, device=None, dtype=None):
         super().__init__(in_channels, out_channels, 1, bias=bias, device=device, dtype=dtype)

@@ -768,3 +768,26 @@ def test_evaluation_of_blocks_with_hooks():
         blk(x)
         w = torch._weight_norm(conv.weight_v, conv.weight_g, 0)
         assert torch.equal(args["y"], F.conv1x1_mxfp4(args["x"], w, conv.bias))
+
+
+def test_autocast_changes_nothing():
+    """The kernels and the composition that stands in for them give the input's type under autocast, forward and backward."""
+    from conversenet_amd import composite
+    from conversenet_amd.util_converse import Conv1x1MXFP4
+    conv = Conv1x1MXFP4(40, 8).cuda()
+    x = make((2, 40, 5, 6), F32, 38).cuda()
+    params = list(conv.parameters())
+    y = conv(x)
+    grads = torch.autograd.grad(y.square().sum(), params)
+    mag = O.conv1x1(O.rounded(flat(x)), O.rounded(flat(conv.weight))[:, :, 0], np64(conv.bias))[1]
+    for t in (torch.bfloat16, torch.float16):
+        with torch.autocast("cuda", dtype=t):
+            z = conv(x)
+            assert z.dtype is F32 and torch.equal(z, y)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(z.square().sum(), params), grads))
+            with torch.no_grad():
+                assert torch.equal(conv(x), y)
+                c = composite.conv1x1_mxfp4(x, conv.weight, conv.bias)
+                assert c.dtype is F32 and torch.allclose(c, y, rtol=0, atol=2 * 42 * 2.0 ** -23 * mag.max())
+                h = conv(x.to(t))  # what a convolution under autocast hands on
+                assert h.dtype is t and torch.equal(h, fh().conv1x1_mxfp4(x.to(t), conv.weight, conv.bias))

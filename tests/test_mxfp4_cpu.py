@@ -289,3 +289,30 @@ def test_blocks_whose_modules_are_observed_run_them():
     with pytest.warns(FutureWarning):
         torch.nn.utils.weight_norm(blk.conv2[1])
     assert not U._all_mxfp4(blk)
+
+
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16])
+def test_autocast_changes_nothing_on_the_cpu(cast):
+    conv = Conv1x1MXFP4(40, 8)
+    x = torch.randn(2, 40, 5, 6)
+    y = conv(x)
+    with torch.autocast("cpu", dtype=cast):
+        z = conv(x)
+        assert torch.is_autocast_enabled("cpu")
+    assert z.dtype is torch.float32 and torch.equal(y, z)
+
+
+@pytest.mark.parametrize("tx", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tw", [torch.float32, torch.bfloat16, torch.float16])
+def test_types_of_a_convolution_on_the_cpu(tx, tw):
+    """Parameters of another type than the input: the result has the input's, and gradients are of the parameters'."""
+    conv = Conv1x1MXFP4(40, 8).to(tw)
+    x = torch.randn(2, 40, 5, 6).to(tx).requires_grad_()
+    y = conv(x)
+    n = lambda t: t.detach().double().numpy().reshape(t.shape[0], t.shape[1], -1)  # noqa: E731
+    want, mag = O.conv1x1(O.rounded(n(x)), O.rounded(n(conv.weight))[:, :, 0], conv.bias.detach().double().numpy())
+    # sums of 41 terms in float32, then the rounding of a result of x's type (fp16: also of numbers below its smallest normal one)
+    lim = 43 * 2.0 ** -24 * mag + torch.finfo(tx).eps / 2 * np.abs(want) + 2.0 ** -25
+    assert y.dtype is tx and (np.abs(n(y) - want) <= lim).all()
+    y.float().sum().backward()
+    assert x.grad.dtype is tx and conv.weight.grad.dtype is tw and conv.bias.grad.dtype is tw
