@@ -261,13 +261,17 @@ def _mxfp4_eligible(x, *params) -> bool:
     """True when an MXFP4 convolution runs on the library's kernels: HIP tensors of its types, and no transform, tracer or mode
     that looks into torch's operations (those see the composition)."""
     ts = [t for t in (x, *params) if t is not None]
-    if not all(t.is_cuda and t.dtype in _lib.TYPES for t in ts) or type(x) not in _TENSORS:
+    if not all(t.is_cuda and t.dtype in _lib.TYPES for t in ts) or type(x) not in _TENSORS or any(
+            type(p).__torch_dispatch__ is not _NO_DISPATCH for p in ts):
         return False
     if torch._C._are_functorch_transforms_active() or fwAD._current_level >= 0 or torch.compiler.is_compiling() \
             or torch.jit.is_tracing() or functional.observed():
         return False
     _lib.load()
     return True
+
+
+_NO_DISPATCH = torch._C._disabled_torch_dispatch_impl  # (a class with one of its own stands for other tensors)
 
 
 class Conv1x1MXFP4(nn.Conv2d):

@@ -791,3 +791,34 @@ def test_autocast_changes_nothing():
                 assert c.dtype is F32 and torch.allclose(c, y, rtol=0, atol=2 * 42 * 2.0 ** -23 * mag.max())
                 h = conv(x.to(t))  # what a convolution under autocast hands on
                 assert h.dtype is t and torch.equal(h, fh().conv1x1_mxfp4(x.to(t), conv.weight, conv.bias))
+
+
+class Holder(torch.Tensor):
+    """A tensor that stands for another one and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device,
+                                                   requires_grad=inner.requires_grad)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        from torch.utils._pytree import tree_map
+        return func(*tree_map(lambda t: t.inner if isinstance(t, cls) else t, args), **(kwargs or {}))
+
+
+def test_parameters_that_stand_for_others():
+    from conversenet_amd.util_converse import Conv1x1MXFP4
+    conv = Conv1x1MXFP4(40, 8).cuda().requires_grad_(False)
+    x = make((2, 40, 5, 6), F32, 39).cuda()
+    y = conv(x)
+    mag = O.conv1x1(O.rounded(flat(x)), O.rounded(flat(conv.weight))[:, :, 0], np64(conv.bias))[1]
+    for name in ("weight", "bias"):
+        other = copy.deepcopy(conv)
+        delattr(other, name)
+        setattr(other, name, Holder(getattr(conv, name).detach()))
+        # (the composition: both sides' sums of 41 terms)
+        assert torch.allclose(other(x), y, rtol=0, atol=2 * 42 * 2.0 ** -23 * mag.max())
