@@ -646,7 +646,10 @@ def _param32(keep, t, C, index, what):
     if t.dtype is not torch.float32 or not t.is_contiguous():
         t = t.to(torch.float32).contiguous()
         keep.append(t)
-    return t.data_ptr()
+    at = t.data_ptr()
+    if not at and C:  # (the library would take it for none)
+        raise RuntimeError(f"{what} stands for other tensors: it has no memory to compute on")
+    return at
 
 
 def _gate_kind(h, gate):
@@ -1152,7 +1155,11 @@ def _values(t):
     if t is None:
         return None
     t = t if t.is_contiguous() else t.contiguous()
-    return t.resolve_neg() if t.is_neg() else t
+    if t.is_neg():
+        t = t.resolve_neg()
+    if not t.data_ptr() and t.numel():  # (the library would take it for none)
+        raise RuntimeError("a tensor that stands for others has no memory to compute on")
+    return t
 
 
 def _mx_parts(q, what):

@@ -822,3 +822,25 @@ def test_parameters_that_stand_for_others():
         setattr(other, name, Holder(getattr(conv, name).detach()))
         # (the composition: both sides' sums of 41 terms)
         assert torch.allclose(other(x), y, rtol=0, atol=2 * 42 * 2.0 ** -23 * mag.max())
+
+
+def test_tensors_without_memory_are_refused():
+    """An operand that stands for another tensor is not taken for one that is not there."""
+    F = fh()
+    x, w = make((2, 40, 3, 4), F32, 40).cuda(), make((8, 40), F32, 41).cuda()
+    q, wm, v = F.quantize_mxfp4(x), F.quantize_mxfp4(w), torch.ones(8, device="cuda")
+    r = torch.ones(2, 8, 3, 4, device="cuda")
+    H = Holder
+    for call in (lambda: F.quantize_mxfp4(H(x)), lambda: F.conv1x1_mxfp4(H(x), w), lambda: F.conv1x1_mxfp4(x, H(w)),
+                 lambda: F.conv1x1_mxfp4(x, w, H(v)), lambda: F.conv1x1_mxfp4(x, w, res_scale=H(v)),
+                 lambda: F.conv1x1_mxfp4(x, w, residual=H(r)), lambda: F.conv1x1_mxfp4(x, w, out=H(r)),
+                 lambda: F.conv1x1_mxfp4(F.MXFP4(H(q.codes), q.scales, 40), w),
+                 lambda: F.conv1x1_mxfp4(q, F.MXFP4(wm.codes, H(wm.scales), 40)),
+                 lambda: F.dequantize_mxfp4(F.MXFP4(q.codes, H(q.scales), 40)),
+                 lambda: F.conv1x1_mxfp4_backward(H(r), q, wm),
+                 lambda: F.conv1x1_mxfp4_backward(r, F.MXFP4(H(q.codes), q.scales, 40), wm),
+                 lambda: F.conv1x1_mxfp4_backward(r, q, F.MXFP4(wm.codes, H(wm.scales), 40)),
+                 lambda: F.conv1x1_mxfp4_train(H(x), w.requires_grad_()), lambda: F.conv1x1_mxfp4_train(x.requires_grad_(), H(w)),
+                 lambda: F.conv1x1_mxfp4_train(x, w, H(v))):
+        with pytest.raises(RuntimeError, match="no memory|null pointer"):
+            call()

@@ -316,3 +316,17 @@ def test_types_of_a_convolution_on_the_cpu(tx, tw):
     assert y.dtype is tx and (np.abs(n(y) - want) <= lim).all()
     y.float().sum().backward()
     assert x.grad.dtype is tx and conv.weight.grad.dtype is tw and conv.bias.grad.dtype is tw
+
+
+def test_tensors_without_memory_are_no_operands():
+    class Holder(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError
+
+    held = torch.Tensor._make_wrapper_subclass(Holder, (3, 4))
+    with pytest.raises(RuntimeError, match="no memory"):
+        F._values(held)
+    with pytest.raises(RuntimeError, match="no memory"):
+        F._param32([], held, 12, -1, "bias")
+    assert F._values(torch.empty(0, 4)).numel() == 0 and F._values(None) is None
