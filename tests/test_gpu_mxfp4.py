@@ -844,3 +844,59 @@ def test_tensors_without_memory_are_refused():
                  lambda: F.conv1x1_mxfp4_train(x, w, H(v))):
         with pytest.raises(RuntimeError, match="no memory|null pointer"):
             call()
+
+
+EXACT = [((1, 64, 129, 131), 64), ((1, 200, 130, 131), 40), ((2, 40, 131, 65), 9), ((3, 300, 67, 71), 130), ((17003, 200), 33),
+         ((5003, 64), 130), ((1, 64, 401, 503), 128), ((7, 33, 1, 3), 257), ((2, 130, 257), 1)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", EXACT, ids=str)
+def test_sums_that_are_exact(case, dtype):
+    """Whole numbers whose sums float32 holds: every term counts, to the last pixel of the last split, and none is counted twice.
+    x and w are MXFP4 values in steps of 1/2 (each block's scale reaches them), grad_y whole numbers of up to 9 bits (8 in
+    bfloat16): products in steps of 1/4 and 1/2, the sums of their magnitudes below 2^24 steps."""
+    shape, N = case
+    F = fh()
+    g = gen(shape[0] + shape[1])
+    values = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.5, -1, -1.5, -2, -3, -4, -6])
+    pick = lambda *s: values[torch.randint(0, 15, s, generator=g)]  # noqa: E731
+    P = shape[0] * int(np.prod(shape[2:]))
+    most = min(200 if dtype is BF16 else 300, 5000000 // P)
+    x, w, bias = pick(*shape), pick(N, shape[1]), torch.randint(-9, 10, (N,), generator=g).float()
+    gy = torch.randint(-most, most + 1, (shape[0], N) + shape[2:], generator=g).float()
+    gy.view(shape[0], N, -1)[-1, :, -1], x.view(*shape[:2], -1)[-1, :, -1] = most, 6.0  # a lost last pixel shows everywhere
+    xs, ws, gs, bs = (t.to(d).cuda() for t, d in ((x, dtype), (w, F32), (gy, dtype), (bias, F32)))
+    for t in (xs, ws, bs):
+        t.requires_grad_(True)
+    y = F.conv1x1_mxfp4_train(xs, ws, bs)
+    gx, gw, gb = torch.autograd.grad(y, (xs, ws, bs), gs)
+    xc, gc, wd = by_channels(x).double(), by_channels(gy).double(), w.double()
+    for got, a, b, steps, t, extra in ((by_channels(y), wd, xc, 4, dtype, bias[:, None].double()), (by_channels(gx), wd.t(), gc, 2, dtype, 0),
+                                       (gw, gc, xc.t(), 2, F32, 0), (gb[:, None], gc, torch.ones(P, 1, dtype=torch.float64), 1, F32, 0)):
+        assert steps * ((a.abs() @ b.abs()).max() + 9) < 2 ** 24
+        want = a @ b + extra
+        assert t is not F16 or want.abs().max() < 65504
+        assert torch.equal(got.detach().cpu().double().view(want.shape), want.to(t).double())
+    q, m = F.quantize_mxfp4(xs.detach()), F.quantize_mxfp4(ws.detach())
+    again = F.conv1x1_mxfp4_backward(gs, q, m)
+    assert torch.equal(again[0], gx) and torch.equal(again[1], gw) and torch.equal(again[2], gb)
+    assert torch.equal(F.conv1x1_mxfp4(q, m, bs.detach(), dtype=dtype), y)
+    assert torch.equal(F.conv1x1_mxfp4_backward(gs, q, m, (True, False, True))[2], gb)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [((1, 64, 129, 131), 64), ((1, 200, 130, 131), 40), ((17003, 70), 33), ((3, 40, 80, 71), 130)], ids=str)
+def test_bias_gradients_are_sums_in_64_bits(case, dtype):
+    """grad_bias is summed in float64 and rounded once, with the matrix' gradient and without it."""
+    shape, N = case
+    F = fh()
+    x, w = F.quantize_mxfp4(make(shape, dtype, 53).cuda()), F.quantize_mxfp4(make((N, shape[1]), F32, 54).cuda())
+    gy = torch.randn((shape[0], N) + shape[2:], generator=gen(55)).to(dtype)
+    g = by_channels(gy).double()
+    want, mag, P = g.sum(1), g.abs().sum(1), g.shape[1]
+    assert (g[:, -1].abs() > 2.0 ** -23 * want.abs() + 2 * P * 2.0 ** -52 * mag).float().mean() > 0.9  # a lost pixel shows
+    for need in ((True, True, True), (False, True, True), (True, False, True), (False, False, True)):
+        gb = F.conv1x1_mxfp4_backward(gy.cuda(), x, w, need)[2].cpu().double()
+        # both sides' sums of P terms in float64, one rounding to float32
+        assert ((gb - want).abs() <= 2.0 ** -24 * want.abs() + 2 * P * 2.0 ** -53 * mag).all()
