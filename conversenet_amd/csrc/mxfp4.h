@@ -72,10 +72,10 @@ __device__ __forceinline__ mx_i32x8 mx_operand(mx_i32x4 q) { return mx_i32x8{q.x
 constexpr int kMxFp4 = 4;  // the builtins' number of the type
 
 // GELU(x) = max(x, 0) - |x| Q(|x|), Q the upper tail of the normal distribution: log2 Q is smooth, so Q = 2^p(|x|) with a polynomial p
-// whose largest error a |2^p(a) - Q(a)| over 0 .. 6 is least for its degree (7e-9 for 8; a linear program over 3000 points found
-// it) and which falls beyond.  14 issue slots, four of them the exponential's, against 20 of gelu_fast, whose reciprocal takes
-// four more: 8 x 64 x 256 x 256 bfloat16 to 128 channels 50 us, 53 with that.  The largest error in float32 is 1.3e-7 for |x| < 3.9 and
-// 6.1e-8 |x| beyond (gelu_fast: 3.3e-7).  Infinities are the caller's.
+// whose largest error a |2^p(a) - Q(a)| over 0 .. 6 is near the least for its degree (9.5e-9, at 1.69; a linear program over 3000
+// points found it) and which falls beyond.  14 issue slots, four of them the exponential's, against 20 of gelu_fast, whose reciprocal takes
+// four more: 8 x 64 x 256 x 256 bfloat16 to 128 channels 50 us, 53 with that.  The largest error in float32 is 1.4e-7 for |x| < 3.9 and
+// 6.0e-8 |x| beyond (gelu_fast: 3.3e-7).  Infinities are the caller's.
 __device__ __forceinline__ float mx_gelu(float x) {
   const float a = fabsf(x);
   float p = fmaf(-1.690395606601669e-06f, a, 2.5083225409616716e-05f);

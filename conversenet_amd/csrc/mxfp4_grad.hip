@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_mx_grads(MxGradArgs x, MxGradAr
 }
 
 // The sum over the splits, in the same order on every call: R threads an element take every R-th of them.  (One thread an
-// element leaves few to wait for long chains of loads: 288 splits of 8192 elements take 134 us that way, 8 threads an element
-// 11.6, 16 threads 7.4; 8 splits of a million elements take 9 with one thread, 16 with eight.)
+// element leaves few to wait for long chains of loads: 256 splits of 8192 elements take 70 us that way, 16 threads 6.6; 64 of 65536
+// 19 and 7.6; but 16 of 262144, where one thread takes over, 7.1 and 9.6, and 4 of a million 6.4 and 28.6.)
 template <int R>
 __global__ void __launch_bounds__(kThreads) k_mx_grad_join(const float* __restrict__ part, int64_t n,
                                                            const double* __restrict__ gbp, int64_t nb, int splits,

@@ -132,8 +132,8 @@ __device__ __forceinline__ void mx_store_pixels(const MxOut& o, const MxPixels<V
 // ------------------------------------------------------------------------------------------------
 // Many pixels of many channels: both operands in MXFP4, tiles staged through LDS.
 // ------------------------------------------------------------------------------------------------
-// 16384 pixels, 2048 to 4096 channels: 119 us behind the quantisation, 2.3 PFLOP/s (150 us call after call, where the card's
-// clock falls; a library's 8192^3 product: 3.1 PFLOP/s), bound by the wait for each step's fetch; the matrix units are busy a fifth
+// 16384 pixels, 2048 to 4096 channels: 136 us behind the quantisation, 2.0 PFLOP/s (137 to 152 us call after call; a library's
+// 8192^3 product: 3.1 PFLOP/s), bound by the wait for each step's fetch; the matrix units are busy a fifth
 // of the time, LDS an eighth.  Another order of the tiles, two patches of the longer side, changes nothing.
 // A step takes 256 channels: 128 bytes of codes a row, which a wave fetches 8 rows at a time straight into LDS.  A row's
 // 16-byte pieces are stored in an order that depends on the row (piece ^ (row / 2 & 7)), so that 16 lanes which read the
@@ -362,8 +362,9 @@ int gemm_tile(const MxIn& in, const MxOut& o, hipStream_t st) {
 
 template <class T, bool MAP>
 int gemm(const MxIn& in, const MxOut& o, hipStream_t st) {
-  // Tiles of 128 from one for every CU on, 64 below.  (16384 pixels, 2048 to 4096 channels: 131 us, 64: 208, 256 x 256 with
-  // eight waves 133; 8192 pixels, 1024 to 1024: 14.7, 64: 19, 256 x 256: 16.5; 256 pixels, 2048 to 2048: 14.7, 64: 12.5.)
+  // Tiles of 128 from one for every CU on, 64 below.  (16384 pixels, 2048 to 4096 channels: 136 us, 64: 230; 8192 pixels, 1024 to
+  // 1024: 14.3, 64: 22.8; 4092 pixels, 1024 to 1024, where the rule begins: 14.3, 64: 12.1; 256 pixels, 2048 to 2048: 12.6, 64:
+  // 9.3; 17 vectors, 4096 to 4096: 17.4, 64: 10.8.)
   if ((o.N + 127) / 128 * ((o.rows + 127) / 128) >= 256)
     return o.lines ? gemm_tile<T, MAP, true, 128, 128, 64, 64>(in, o, st) : gemm_tile<T, MAP, false, 128, 128, 64, 64>(in, o, st);
   return gemm_tile<T, MAP, false, 64, 64, 32, 32>(in, o, st);
