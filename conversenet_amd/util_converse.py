@@ -308,6 +308,8 @@ class Conv1x1MXFP4(nn.Conv2d):
 
 def _check_1x1(conv):
     """Refuses what Conv1x1MXFP4.forward would not compute."""
+    if not isinstance(conv, nn.Conv2d) or type(conv).forward not in (nn.Conv2d.forward, Conv1x1MXFP4.forward):
+        raise ValueError("not an nn.Conv2d")  # (a transposed one has its weight the other way round)
     if conv.kernel_size != (1, 1) or conv.stride != (1, 1) or conv.padding not in ((0, 0), "same", "valid") or conv.groups != 1:
         raise ValueError("not a 1x1 convolution")
     if "forward" in conv.__dict__ or conv._compiled_call_impl is not None:

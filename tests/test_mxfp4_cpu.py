@@ -330,3 +330,17 @@ def test_tensors_without_memory_are_no_operands():
     with pytest.raises(RuntimeError, match="no memory"):
         F._param32([], held, 12, -1, "bias")
     assert F._values(torch.empty(0, 4)).numel() == 0 and F._values(None) is None
+
+
+def test_only_convolutions_become_mxfp4_ones():
+    class Own(torch.nn.Conv2d):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Plain(torch.nn.Conv2d):
+        pass
+
+    for m in (torch.nn.ConvTranspose2d(4, 4, 1), Own(4, 6, 1), torch.nn.Linear(4, 6)):
+        with pytest.raises(ValueError):
+            Conv1x1MXFP4.of(m)
+    assert Conv1x1MXFP4.of(Plain(4, 6, 1)).out_channels == Conv1x1MXFP4.of(Conv1x1MXFP4(4, 6)).out_channels == 6
