@@ -30,6 +30,20 @@ inline unsigned mx_grid(int64_t blocks, int threads) {
   return (unsigned)(blocks < most ? blocks : most);
 }
 
+// Memory of a call, and whether the first `written` pieces of n share any with each other or with the rest.
+struct MxMem {
+  const void* p;  // or null
+  int64_t n;      // bytes
+};
+inline bool mx_shared(const MxMem* m, int written, int n) {
+  for (int i = 0; i < written; ++i)
+    for (int k = i + 1; k < n; ++k) {
+      const uintptr_t x = (uintptr_t)m[i].p, y = (uintptr_t)m[k].p;
+      if (x && y && x < y + (uintptr_t)m[k].n && y < x + (uintptr_t)m[i].n) return true;
+    }
+  return false;
+}
+
 inline int mx_type_size(int type) { return type == CVN_F32 ? 4 : type == CVN_BF16 || type == CVN_F16 ? 2 : 0; }
 
 // The bits of a magnitude as float32: ordered as integers, with infinities and NaNs above all numbers.

@@ -197,6 +197,9 @@ extern "C" int cvn_mxfp4_quantize(const void* x, int x_type, int64_t B, int64_t 
   if (rc != CVN_OK) return rc;
   if (B * HW == 0) return CVN_OK;
   if (!x || !codes || !scales) return fail(CVN_ERR_ARG, "null pointer");
+  const int64_t blocks = B * HW * mx_blocks(C);
+  const MxMem mem[] = {{codes, 16 * blocks}, {scales, blocks}, {x, B * HW * C * mx_type_size(x_type)}};
+  if (mx_shared(mem, 2, 3)) return fail(CVN_ERR_ARG, "an output shares memory with the input or another output");
   return mx_quantize(x, x_type, B, C, HW, codes, scales, (hipStream_t)stream);
 }
 
@@ -206,6 +209,9 @@ extern "C" int cvn_mxfp4_dequantize(const void* codes, const void* scales, int64
   if (rc != CVN_OK) return rc;
   if (B * HW == 0) return CVN_OK;
   if (!y || !codes || !scales) return fail(CVN_ERR_ARG, "null pointer");
+  const int64_t blocks = B * HW * mx_blocks(C);
+  const MxMem mem[] = {{y, B * HW * C * mx_type_size(y_type)}, {codes, 16 * blocks}, {scales, blocks}};
+  if (mx_shared(mem, 1, 3)) return fail(CVN_ERR_ARG, "the output shares memory with an input");
   if (y_type == CVN_F32) return dequantize<float>(codes, scales, B, C, HW, y, (hipStream_t)stream);
   if (y_type == CVN_BF16) return dequantize<__bf16>(codes, scales, B, C, HW, y, (hipStream_t)stream);
   return dequantize<_Float16>(codes, scales, B, C, HW, y, (hipStream_t)stream);

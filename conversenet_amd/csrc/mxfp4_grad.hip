@@ -523,6 +523,16 @@ extern "C" int cvn_conv1x1_mxfp4_bwd(const void* grad_y, int type, const void* x
   if (!grad_y || (grad_x && (!w_codes || !w_scales)) || (grad_w && (!x_codes || !x_scales)))
     return fail(CVN_ERR_ARG, "null pointer");
   if (((uintptr_t)w_codes | (uintptr_t)x_codes) & 15) return fail(CVN_ERR_ARG, "codes must be aligned to 16 bytes");
+  const int64_t es = mx_type_size(type), KB = mx_blocks(C);
+  const MxMem mem[] = {{grad_x, rows * C * es},
+                       {grad_w, N * C * 4},
+                       {grad_bias, N * 4},  // written up to here
+                       {grad_y, rows * N * es},
+                       {grad_w ? x_codes : nullptr, rows * KB * 16},
+                       {grad_w ? x_scales : nullptr, rows * KB},
+                       {grad_x ? w_codes : nullptr, N * KB * 16},
+                       {grad_x ? w_scales : nullptr, N * KB}};
+  if (mx_shared(mem, 3, 8)) return fail(CVN_ERR_ARG, "an output shares memory with an input or another output");
   if (grad_w && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < cvn_conv1x1_mxfp4_bwd_workspace(B, C, HW, N)))
     return fail(CVN_ERR_WORKSPACE, "workspace missing, too small or not aligned to 16 bytes");
   if (type == CVN_F32)

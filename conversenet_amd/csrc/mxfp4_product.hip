@@ -637,11 +637,6 @@ int mx_check_product(int64_t B, int64_t C, int64_t HW, int64_t N, int type) {
   return CVN_OK;
 }
 
-bool mx_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return a && b && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
-}
-
 template <class T>
 int product(const MxIn& in, const MxOut& o, int type, bool keep, hipStream_t st) {
   // (the tiled kernel reads scales by words of four)
@@ -687,27 +682,21 @@ extern "C" int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, i
     return fail(CVN_ERR_ARG, "null pointer");
   if (((uintptr_t)w_codes | (uintptr_t)x_codes) & 15) return fail(CVN_ERR_ARG, "codes must be aligned to 16 bytes");
   // What is written is apart from all else, but y may be the residual.
-  const struct {
-    const void* p;
-    int64_t n;
-  } mem[] = {{y, rows * N * es},
-             {x ? x_codes : nullptr, rows * KB * 16},
-             {x ? x_scales : nullptr, rows * KB},
-             {w ? w_codes : nullptr, N * KB * 16},
-             {w ? w_scales : nullptr, N * KB},  // written up to here
-             {x, rows * C * es},
-             {w, w ? N * C * mx_type_size(w_type) : 0},
-             {x ? nullptr : x_codes, rows * KB * 16},
-             {x ? nullptr : x_scales, rows * KB},
-             {w ? nullptr : w_codes, N * KB * 16},
-             {w ? nullptr : w_scales, N * KB},
-             {residual == y ? nullptr : residual, rows * N * es},
-             {bias, N * 4},
-             {res_scale, N * 4}};
-  for (int i = 0; i < 5; ++i)
-    for (int k = i + 1; k < 14; ++k)
-      if (mx_overlap(mem[i].p, mem[i].n, mem[k].p, mem[k].n))
-        return fail(CVN_ERR_ARG, "an output shares memory with an input or another output");
+  const MxMem mem[] = {{y, rows * N * es},
+                       {x ? x_codes : nullptr, rows * KB * 16},
+                       {x ? x_scales : nullptr, rows * KB},
+                       {w ? w_codes : nullptr, N * KB * 16},
+                       {w ? w_scales : nullptr, N * KB},  // written up to here
+                       {x, rows * C * es},
+                       {w, w ? N * C * mx_type_size(w_type) : 0},
+                       {x ? nullptr : x_codes, rows * KB * 16},
+                       {x ? nullptr : x_scales, rows * KB},
+                       {w ? nullptr : w_codes, N * KB * 16},
+                       {w ? nullptr : w_scales, N * KB},
+                       {residual == y ? nullptr : residual, rows * N * es},
+                       {bias, N * 4},
+                       {res_scale, N * 4}};
+  if (mx_shared(mem, 5, 14)) return fail(CVN_ERR_ARG, "an output shares memory with an input or another output");
   const bool keep = x_codes != nullptr;
   const size_t need = cvn_conv1x1_mxfp4_workspace(keep, w_codes != nullptr, B, C, HW, N);
   if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))

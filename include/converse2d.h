@@ -312,7 +312,8 @@ int cvn_clip_grads(const void* const* grads, void* const* out, const int64_t* nu
  * code is the nearest to x / 2^(s - 127), ties to the even code, at most 6.  A block with an infinity or a NaN has
  * s = 255: each of its values is NaN.  x: (B,C,HW) of x_type, or a matrix (B,C) with HW 1.  codes: (B HW, KB, 16) bytes
  * aligned to 16, KB = ceil(C / 32), the even channel of a byte in its lower half; scales: (B HW, KB) bytes.  Channels
- * past C are zeros.  Here and below up to 65536 channels and 2^31 - 256 pixels. */
+ * past C are zeros.  Here and below up to 65536 channels and 2^31 - 256 pixels; what is written shares no memory with anything
+ * else (CVN_ERR_ARG). */
 int cvn_mxfp4_quantize(const void* x, int x_type, int64_t B, int64_t C, int64_t HW, void* codes, void* scales,
                        cvn_stream_t stream);
 /* The values, rounded to y_type: y (B,C,HW). */
@@ -322,7 +323,7 @@ int cvn_mxfp4_dequantize(const void* codes, const void* scales, int64_t B, int64
  * residual[b,n,p]: cvn_conv1x1_f32 of MXFP4 operands, summed in fp32 and rounded once.  x: (B,C,HW) of type, quantised in
  * the call, its MXFP4 form written to x_codes and x_scales unless they are NULL; or x NULL and its MXFP4 form given there.
  * w: (N,C) of w_type, likewise.  y, residual: (B,N,HW) of type; bias, res_scale: fp32 (N).  bias, residual and res_scale may be
- * NULL.  y may be the residual itself; what is written shares no other memory with anything else (CVN_ERR_ARG).
+ * NULL.  y may be the residual itself.
  * _workspace: x_given, w_given: x_codes, w_codes will be given (read or written). */
 size_t cvn_conv1x1_mxfp4_workspace(int x_given, int w_given, int64_t B, int64_t C, int64_t HW, int64_t N);
 int cvn_conv1x1_mxfp4(const void* x, void* x_codes, void* x_scales, int64_t B, int64_t C, int64_t HW, const void* w,

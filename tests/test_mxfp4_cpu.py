@@ -344,3 +344,30 @@ def test_only_convolutions_become_mxfp4_ones():
         with pytest.raises(ValueError):
             Conv1x1MXFP4.of(m)
     assert Conv1x1MXFP4.of(Plain(4, 6, 1)).out_channels == Conv1x1MXFP4.of(Conv1x1MXFP4(4, 6)).out_channels == 6
+
+
+def test_outputs_that_share_memory_are_refused():
+    """By the C entry points, whose callers choose every address; a byte beside is another matter for the device to run."""
+    lib = _lib.load()
+
+    def refused(rc):
+        return rc == _lib.CVN_ERR_ARG and b"shares memory" in lib.cvn_last_error()
+
+    # 64 channels of 4 pixels: 1024 bytes of float32, 128 of codes, 8 of scales
+    x, codes, scales = D << 20, D << 21, D << 22
+    q, d, g = lib.cvn_mxfp4_quantize, lib.cvn_mxfp4_dequantize, lib.cvn_conv1x1_mxfp4_bwd
+    for c, s in ((x, scales), (x + 1008, scales), (x - 112, scales), (codes, x + 1023), (codes, x - 7), (codes, codes + 127),
+                 (codes, codes - 7)):
+        assert refused(q(x, 0, 1, 64, 4, c, s, None)), (c, s)
+    for y in (codes, codes + 112, codes - 1020, scales + 4, scales - 1020):
+        assert refused(d(codes, scales, 1, 64, 4, y, 0, None)), y
+    # and to 8 channels: grad_y 128 bytes, the matrix 256 of codes and 16 of scales, its gradient 2048, the bias' 32
+    gy, wc, ws, gx, gw, gb = D << 23, D << 24, D << 25, D << 26, D << 27, D << 28
+
+    def bwd(gx=gx, gw=gw, gb=gb):
+        return g(gy, 0, codes, scales, wc, ws, 1, 64, 4, 8, gx, gw, gb, D << 29, 1 << 24, None)
+
+    for bad in (dict(gx=gy), dict(gx=gy - 1020), dict(gx=wc + 240), dict(gx=ws), dict(gx=codes), dict(gx=scales), dict(gx=gw + 2044),
+                dict(gx=gb), dict(gw=gy), dict(gw=codes), dict(gw=scales - 2044), dict(gw=wc), dict(gw=gb + 28), dict(gb=gy + 124),
+                dict(gb=gw - 28), dict(gb=gx + 1020), dict(gx=gy, gw=None, gb=None), dict(gx=None, gb=None, gw=codes + 124)):
+        assert refused(bwd(**bad)), bad
