@@ -1,5 +1,6 @@
-// Where the nodes of an autograd graph were made: torch runs a node's backward on the stream that was current when the node was made, and
-// tells Python nothing of that stream.  Host code only; a library of its own (libcvn_autograd.so), since it is bound to torch's C++ interface.
+// Where the nodes of an autograd graph were made: torch runs a node's backward on the stream that was current when the node was
+// made, and tells Python nothing of that stream.  Host code only; a library of its own (libcvn_autograd.so), since it is bound to
+// torch's C++ interface.
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
